@@ -26,9 +26,10 @@ COMMON = ["-std=c++17", "-O3", "-lineinfo", "--fmad=false", "-Xcompiler", "-fPIC
           "-I" + str(INCLUDE), "-I" + str(CSRC)]
 
 
-# Compiled with contraction on, as the reference's nonlinear kernels are: the
-# pointwise functions then round exactly as the reference's do.
-FMAD_DEFAULT = {"nonlinear.cu"}
+# Compiled with contraction on: the nonlinear kernels as the reference's are (the
+# pointwise functions then round exactly as the reference's do), the block
+# operators because nothing asks for separately rounded products there.
+FMAD_DEFAULT = {"nonlinear.cu", "block_norm.cu", "matvec_w4.cu", "paged_attention.cu"}
 
 
 def nvcc() -> str:

@@ -1,0 +1,555 @@
+"""The block operators on the GPU against their plain 64-bit statements (tests/block_cases.py).
+
+Tolerances count roundings: half a step of the output's type, plus a number of
+32-bit roundings of the magnitude of the terms.  A sum of w terms over t
+threads carries at most w / t + 16 of them (sequential in a thread, then a
+tree), a norm's square root halves its sum's, and each product adds one.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import block_cases as R
+from powermodeling_b200 import blocks
+
+pytestmark = pytest.mark.gpu
+BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def randn(gen, *shape, dtype=F32, scale=1.0, shift=0.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale + shift).to(dtype)
+
+
+@pytest.fixture
+def gen(gpu_ready):
+    return torch.Generator(device="cuda").manual_seed(20)
+
+
+def check(what, got, pair, steps):
+    bad, worst = R.within(got, *pair, steps)
+    assert not bad, f"{what}: {bad} of {got.numel()} beyond the tolerance, worst {worst:.3g} of it"
+
+
+# ---------------------------------------------------------------- norms around a block
+def norm_inputs(gen, rows, width, dtype, *, post=True, gate_rows=1, weights=None, gate_dtype=None):
+    w = weights or dtype
+    return dict(residual=randn(gen, rows, width, dtype=dtype, scale=2.0), block=randn(gen, rows, width, dtype=dtype),
+                pre=randn(gen, width, dtype=w, scale=0.1, shift=1.0),
+                post=randn(gen, width, dtype=w, scale=0.1, shift=1.0) if post else None,
+                gate=randn(gen, gate_rows, width, dtype=gate_dtype or w, scale=0.5, shift=0.5) if gate_rows else None)
+
+
+def norm_both(t, gen, scale=0.75, eps=1e-5, use=("hidden", "normed")):
+    """Forward and backward of the inputs `t`, each output checked."""
+    rows, width = t["residual"].shape
+    steps = width / 32 + 64                      # two norms' sums and about a dozen products
+    hidden, normed, stats = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"],
+                                              scale=scale, eps=eps, return_stats=True)
+    args = (t["residual"], t["block"], t["pre"], t["post"], t["gate"], scale, eps)
+    want = R.norm(*args)
+    check("hidden", hidden, want["hidden"], steps)
+    check("normed", normed, want["normed"], steps)
+    gh = randn(gen, rows, width, dtype=hidden.dtype, scale=0.3) if "hidden" in use else None
+    gy = randn(gen, rows, width, dtype=hidden.dtype) if "normed" in use else None
+    grads = blocks.block_norm_backward(gh, gy, t["residual"], t["block"], t["pre"], stats, post_weight=t["post"],
+                                       gate=t["gate"], scale=scale)
+    want = R.norm_grads(gh, gy, *args)
+    for name, got in zip(("residual", "block", "pre", "post", "gate"), grads):
+        if got is None:
+            assert name not in want
+            continue
+        # sums over rows: the rows of one CTA one after the other, then its partial sums
+        more = rows + 600 if name in ("pre", "post", "gate") else 0
+        check("grad " + name, got, want[name], 3 * steps + more)
+    again = blocks.block_norm_backward(gh, gy, t["residual"], t["block"], t["pre"], stats, post_weight=t["post"],
+                                       gate=t["gate"], scale=scale)
+    for a, b in zip(grads, again):
+        assert (a is None and b is None) or torch.equal(a, b)
+    return hidden, normed, grads
+
+
+WIDTHS = [1, 2, 7, 8, 31, 64, 100, 255, 256, 520, 1023, 1024, 1032, 2048, 4096, 5120, 8192, 8200, 12288, 16384, 20000, 33001]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, FP])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_norm_widths(gen, width, dtype):
+    for rows in (1, 3, 37):
+        norm_both(norm_inputs(gen, rows, width, dtype), gen)
+
+
+@pytest.mark.parametrize("rows,gate_rows", [(1, 1), (6, 6), (6, 2), (6, 3), (300, 1), (300, 300), (900, 9), (1200, 400),
+                                            (2048, 1), (2048, 2), (1500, 500)])
+@pytest.mark.parametrize("dtype,weights,gate_dtype", [(BF, BF, BF), (BF, F32, BF), (FP, F32, F32), (F32, F32, F32)])
+def test_norm_gates_and_types(gen, rows, gate_rows, dtype, weights, gate_dtype):
+    for width in (96, 1000, 99):
+        norm_both(norm_inputs(gen, rows, width, dtype, gate_rows=gate_rows, weights=weights, gate_dtype=gate_dtype), gen)
+
+
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("gate_rows", [0, 1, 64])
+@pytest.mark.parametrize("use", [("hidden",), ("normed",), ("hidden", "normed")])
+def test_norm_parts_left_out(gen, post, gate_rows, use):
+    for dtype, width in ((BF, 768), (F32, 77)):
+        norm_both(norm_inputs(gen, 64, width, dtype, post=post, gate_rows=gate_rows), gen, use=use)
+
+
+def test_norm_many_rows(gen):
+    norm_both(norm_inputs(gen, 20011, 256, BF), gen)
+    norm_both(norm_inputs(gen, 5003, 4096, BF, weights=F32), gen)
+    norm_both(norm_inputs(gen, 5000, 1024, FP, gate_rows=5000), gen)
+
+
+def test_norm_row_strides_and_alignment(gen):
+    for dtype in (BF, F32):
+        for width, pad in ((512, 64), (512, 3), (1024, 8), (333, 5)):
+            wide = {k: randn(gen, 40, width + pad, dtype=dtype) for k in ("residual", "block", "gh", "gy")}
+            for shift in (0, pad, 1):
+                if shift > pad:
+                    continue
+                part = {k: v[:, shift:shift + width] for k, v in wide.items()}
+                t = norm_inputs(gen, 40, width, dtype)
+                base = norm_inputs(gen, 40, width, dtype)
+                t.update(residual=part["residual"], block=part["block"])
+                args = dict(post_weight=t["post"], gate=t["gate"], scale=0.75)
+                h, y, st = blocks.block_norm(t["residual"], t["block"], t["pre"], return_stats=True, **args)
+                want = R.norm(t["residual"], t["block"], t["pre"], t["post"], t["gate"], 0.75, 1e-5)
+                check("hidden", h, want["hidden"], 200)
+                check("normed", y, want["normed"], 200)
+                g = blocks.block_norm_backward(part["gh"], part["gy"], t["residual"], t["block"], t["pre"], st, **args)
+                gw = R.norm_grads(part["gh"], part["gy"], t["residual"], t["block"], t["pre"], t["post"], t["gate"], 0.75, 1e-5)
+                for name, got in zip(("residual", "block", "pre", "post", "gate"), g):
+                    check("grad " + name, got, gw[name], 900)
+                # a weight that starts off a 16-byte boundary
+                off = torch.cat((base["pre"][:1], base["pre"]))[1:]
+                h2, y2 = blocks.block_norm(base["residual"], base["block"], off, post_weight=base["post"], gate=base["gate"])
+                h3, y3 = blocks.block_norm(base["residual"], base["block"], base["pre"], post_weight=base["post"], gate=base["gate"])
+                check("normed, shifted weight", y2, R.norm(base["residual"], base["block"], off, base["post"], base["gate"], 1.0, 1e-5)["normed"], 200)
+                assert torch.equal(h2.isnan(), h3.isnan())
+
+
+def test_norm_no_rows(gen):
+    t = norm_inputs(gen, 0, 64, BF, gate_rows=1)
+    h, y, st = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"], return_stats=True)
+    assert h.shape == y.shape == (0, 64) and st.shape == (0, 2)
+    g = blocks.block_norm_backward(h, y, t["residual"], t["block"], t["pre"], st, post_weight=t["post"], gate=t["gate"])
+    assert g[0].shape == (0, 64) and all(not x.any() for x in g[2:])
+
+
+def test_norm_zero_rows_and_extreme_values(gen):
+    z = torch.zeros(5, 512, device="cuda", dtype=BF)
+    one = torch.ones(512, device="cuda", dtype=BF)
+    h, y = blocks.block_norm(z, z, one, post_weight=one)
+    assert not h.any() and not y.any()
+    # values whose squares stay within 32 bits, at both ends; a row with a NaN spoils itself alone
+    t = norm_inputs(gen, 6, 512, F32)
+    t["residual"][1] *= 1e15
+    t["block"][1] *= 1e15
+    t["block"][2] *= 1e-15
+    norm_both(t, gen)
+    t["block"][3, 7] = float("nan")
+    t["residual"][4, 9] = float("inf")
+    h, y = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"])
+    assert y[3].isnan().all() and y[4].isnan().any()
+    assert y[[0, 1, 2, 5]].isfinite().all() and h[[0, 1, 2, 5]].isfinite().all()
+
+
+def test_norm_gradient_against_differences(gen):
+    """The formula's gradients and central differences of the 64-bit forward agree, so the kernel's do."""
+    t = norm_inputs(gen, 4, 24, F32, gate_rows=2)
+    names = ("residual", "block", "pre", "post", "gate")
+    gh, gy = randn(gen, 4, 24), randn(gen, 4, 24)
+    _, _, stats = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"], scale=0.75,
+                                    return_stats=True)
+    grads = dict(zip(names, blocks.block_norm_backward(gh, gy, t["residual"], t["block"], t["pre"], stats,
+                                                       post_weight=t["post"], gate=t["gate"], scale=0.75)))
+
+    def loss(v):
+        f = R.norm(v["residual"], v["block"], v["pre"], v["post"], v["gate"], 0.75, 1e-5)
+        return float((f["hidden"][0] * gh.double()).sum() + (f["normed"][0] * gy.double()).sum())
+
+    wide = {k: v.double() for k, v in t.items()}
+    for name in names:
+        direction = torch.randn(wide[name].shape, generator=gen, device="cuda", dtype=torch.float64)
+        step = 1e-5
+        up = loss({**wide, name: wide[name] + step * direction})
+        down = loss({**wide, name: wide[name] - step * direction})
+        slope = float((grads[name].double() * direction).sum())
+        # a third derivative of order 100 leaves 1e-8, the loss's 64-bit rounding 1e-9, the kernel's 32 bits 1e-5
+        assert math.isclose((up - down) / (2 * step), slope, rel_tol=1e-4, abs_tol=1e-3), name
+
+
+def test_norm_autograd(gen):
+    t = norm_inputs(gen, 60, 384, BF, gate_rows=3, weights=F32, gate_dtype=BF)
+    leaves = [x.clone().requires_grad_() for x in t.values()]
+    hidden, normed = blocks.block_norm(*leaves[:3], post_weight=leaves[3], gate=leaves[4], scale=0.75)
+    assert hidden.requires_grad and normed.requires_grad
+    gh, gy = randn(gen, 60, 384, dtype=BF), randn(gen, 60, 384, dtype=BF)
+    got = torch.autograd.grad((hidden, normed), leaves, (gh, gy))
+    want = R.norm_grads(gh, gy, *t.values(), 0.75, 1e-5)
+    for name, g in zip(("residual", "block", "pre", "post", "gate"), got):
+        check("grad " + name, g, want[name], 3 * (384 / 32 + 64) + 660)
+    # one output used, an expanded incoming gradient, part of the leaves
+    hidden, normed = blocks.block_norm(*leaves[:3], post_weight=leaves[3], gate=leaves[4], scale=0.75)
+    (g,) = torch.autograd.grad(normed.sum(), [leaves[1]])
+    want = R.norm_grads(None, torch.ones_like(normed), *t.values(), 0.75, 1e-5)
+    check("grad block", g, want["block"], 3 * (384 / 32 + 64))
+    with torch.no_grad():
+        assert not blocks.block_norm(*leaves[:3])[0].requires_grad
+
+
+def test_norm_captured_backward(gen):
+    """Forward and backward in one graph, replayed on new inputs; the autograd engine's call under capture is refused."""
+    t = norm_inputs(gen, 50, 1024, BF, weights=F32)
+    gh, gy = randn(gen, 50, 1024, dtype=BF), randn(gen, 50, 1024, dtype=BF)
+
+    def step():
+        h, y, st = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"],
+                                     return_stats=True)
+        return (h, y) + blocks.block_norm_backward(gh, gy, t["residual"], t["block"], t["pre"], st,
+                                                   post_weight=t["post"], gate=t["gate"])
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in (1, 2):
+        t["block"].copy_(randn(gen, 50, 1024, dtype=BF))
+        gy.copy_(randn(gen, 50, 1024, dtype=BF))
+        graph.replay()
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- 4-bit weights
+def w4_inputs(gen, tokens, n, k, dtype, group, zeros, scales=None):
+    groups = -(-k // group)
+    q = torch.randint(0, 16, (n, k), generator=gen, device="cuda")
+    return dict(x=randn(gen, tokens, k, dtype=dtype), q=q, weight=R.pack(q),
+                scales=randn(gen, n, groups, scale=0.01, shift=0.0, dtype=scales or dtype),
+                zeros=torch.randint(0, 16, (n, groups), generator=gen, device="cuda").to(torch.uint8) if zeros else None)
+
+
+def w4_check(t, group, got=None):
+    if got is None:
+        got = blocks.matvec_w4(t["x"], t["weight"], t["scales"], t["zeros"], group_size=group)
+    k = t["x"].shape[1]
+    # 32 products to a matrix instruction, each accumulation truncated once, a few roundings per group
+    check("y", got, R.matvec(t["x"], t["q"], t["scales"], t["zeros"], group), k / 8 + 64)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("k", [1, 2, 31, 32, 33, 64, 100, 126, 128, 256, 500, 1000, 1024, 2048 + 32, 4090, 4096, 8192, 11008, 16384 + 64])
+def test_w4_depths(gen, k, dtype):
+    for group in (32, 64, 128):
+        for tokens, n in ((1, 48), (5, 17), (16, 130)):
+            w4_check(w4_inputs(gen, tokens, n, k, dtype, group, zeros=group == 64), group)
+
+
+@pytest.mark.parametrize("n", [1, 2, 8, 15, 16, 17, 63, 64, 100, 128, 1001, 4096, 20000])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 16])
+def test_w4_rows_and_tokens(gen, n, tokens):
+    w4_check(w4_inputs(gen, tokens, n, 512, BF, 128, zeros=True), 128)
+    w4_check(w4_inputs(gen, tokens, n, 2048, FP, 64, zeros=False), 64)
+
+
+@pytest.mark.parametrize("group", [32, 64, 96, 128, 160, 256, 512, 1024, 4096])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_w4_groups_and_scale_types(gen, group, zeros):
+    for k in (1024, 2600):
+        for scales in (BF, F32):
+            w4_check(w4_inputs(gen, 3, 200, k, BF, group, zeros, scales), group)
+
+
+@pytest.mark.parametrize("tokens", [17, 33, 64])
+def test_w4_more_tokens_than_one_pass(gen, tokens):
+    w4_check(w4_inputs(gen, tokens, 333, 768, BF, 64, True), 64)
+
+
+def test_w4_strides_and_alignment(gen):
+    for k, pad_x, pad_w, shift in ((512, 8, 16, 0), (512, 1, 16, 0), (512, 3, 1, 1), (512, 8, 4, 4), (1000, 24, 12, 4), (1001, 5, 7, 3)):
+        t = w4_inputs(gen, 6, 77, k, BF, 64, True)
+        xs = torch.full((6, k + pad_x), float("nan"), device="cuda", dtype=BF)
+        ws = torch.full((77, t["weight"].shape[1] + pad_w + shift), 255, device="cuda", dtype=torch.uint8)
+        xs[:, min(shift, pad_x):min(shift, pad_x) + k] = t["x"]
+        ws[:, shift:shift + t["weight"].shape[1]] = t["weight"]
+        t["x"], t["weight"] = xs[:, min(shift, pad_x):min(shift, pad_x) + k], ws[:, shift:shift + t["weight"].shape[1]]
+        w4_check(t, 64)
+
+
+def test_w4_values_that_are_not_numbers(gen):
+    """A token with an infinity or a NaN spoils its own row of the result and no other."""
+    t = w4_inputs(gen, 4, 64, 300, BF, 32, False)
+    t["x"][1, 299] = float("inf")
+    t["x"][2, 0] = float("nan")
+    y = blocks.matvec_w4(t["x"], t["weight"], t["scales"], group_size=32)
+    assert y[0].isfinite().all() and y[3].isfinite().all()
+    assert y[2].isnan().all() and not y[1].isfinite().any()
+
+
+# ---------------------------------------------------------------- paged attention
+def cache(gen, lens, hk, d, page, dtype, layout="NHD", columns=None, spare=2, fill=float("nan")):
+    """Caches whose pages lie in no order; everything that is not live holds `fill`."""
+    b = len(lens)
+    used = [-(-max(n, 0) // page) for n in lens]
+    columns = max(used + [1]) if columns is None else columns
+    pages = sum(used) + spare
+    mix = torch.randperm(pages, generator=gen, device="cuda").tolist()
+    table = torch.full((b, columns), -1, dtype=torch.int32)
+    kc = torch.full((pages, page, hk, d), fill, device="cuda", dtype=dtype)
+    vc = kc.clone()
+    for i, n in enumerate(lens):
+        for c in range(min(used[i], columns)):
+            p = mix.pop()
+            table[i, c] = p
+            m = min(page, n - c * page)
+            kc[p, :m] = randn(gen, m, hk, d, dtype=dtype)
+            vc[p, :m] = randn(gen, m, hk, d, dtype=dtype)
+    if layout == "HND":
+        kc, vc = kc.transpose(1, 2).contiguous(), vc.transpose(1, 2).contiguous()
+    return kc, vc, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def attend(gen, lens, hk, share, d, page, dtype, *, layout="NHD", window=0, new=True, scale=None, q=None, made=None):
+    kc, vc, table, lengths = made or cache(gen, lens, hk, d, page, dtype, layout)
+    b = len(lens)
+    q = randn(gen, b, hk * share, d, dtype=dtype) if q is None else q
+    nk, nv = (randn(gen, b, hk, d, dtype=dtype), randn(gen, b, hk, d, dtype=dtype)) if new else (None, None)
+    want = R.attention(q, kc, vc, table, lengths, nk, nv, d ** -0.5 if scale is None else scale, window, layout)
+    out, lse = blocks.paged_attention(q, kc, vc, table, lengths, new_k=nk, new_v=nv, scale=scale, window=window,
+                                      layout=layout, return_lse=True)
+    # a score's sum of d products and its scaling, twice in a weight; a weight held in two 16-bit halves is off by
+    # 2^-16; the sums over the live positions and the joins
+    check("out", out, want[:2], d / 8 + 600)
+    empty = torch.isinf(want[2])
+    assert torch.equal(torch.isinf(lse) & (lse < 0), empty) and not out[empty].any()
+    off = (lse.double() - want[2])[~empty].abs()
+    assert bool((off <= (d / 8 + 100) * 2.0 ** -24 * want[3][~empty]).all()), float(off.max())
+    assert torch.equal(kc.view(torch.int16), want[4].view(torch.int16))
+    assert torch.equal(vc.view(torch.int16), want[5].view(torch.int16))
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("d", [8, 16, 40, 64, 72, 80, 96, 112, 128, 136, 160, 192, 200, 256])
+def test_attention_head_sizes(gen, d, dtype):
+    attend(gen, [1, 65, 130, 0, 300], 2, 4, d, 16, dtype)
+    attend(gen, [17, 1], 3, 1, d, 8, dtype, layout="HND", new=False)
+
+
+@pytest.mark.parametrize("share", [1, 2, 3, 4, 5, 7, 8, 9, 12, 16, 17, 32, 40])
+def test_attention_shared_heads(gen, share):
+    for hk in (1, 3):
+        attend(gen, [100, 1, 0, 513], hk, share, 64, 16, BF)
+        attend(gen, [260], hk, share, 128, 32, FP)
+
+
+@pytest.mark.parametrize("page", [1, 2, 3, 8, 16, 17, 48, 64, 100, 128, 1024])
+def test_attention_pages(gen, page):
+    for layout in ("NHD", "HND"):
+        attend(gen, [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 0, 400], 2, 2, 64, page, BF, layout=layout)
+
+
+@pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 64, 100, 129, 1000, 5000])
+def test_attention_windows(gen, window):
+    attend(gen, [1, 16, 17, 100, 130, 1001, 0, 2000], 2, 4, 64, 16, FP, window=window)
+    attend(gen, [700, 64], 1, 1, 80, 32, BF, window=window, layout="HND")
+
+
+def test_attention_long_and_ragged(gen):
+    attend(gen, [20000], 2, 4, 128, 64, BF)
+    attend(gen, [9000, 3, 0, 1, 777, 4096, 8191], 4, 8, 128, 16, FP)
+    attend(gen, [0, 0, 0], 2, 4, 64, 16, BF)
+    attend(gen, [1] * 300, 2, 4, 64, 16, BF)
+    attend(gen, [33 * (i % 7) for i in range(200)], 8, 1, 64, 16, BF)
+
+
+def test_attention_absent_pages_and_short_tables(gen):
+    lens = [200, 150, 64, 100]
+    kc, vc, table, lengths = cache(gen, lens, 2, 64, 16, BF)
+    table[0, 3] = -1                              # a hole inside
+    table[1, 0] = kc.shape[0]                     # just beyond the pool
+    table[2] = -7                                 # nothing left
+    table[3, 6] = 2 ** 31 - 1                     # the last page, the new token's
+    attend(gen, lens, 2, 4, 64, 16, BF, made=(kc, vc, table, lengths))
+    attend(gen, lens, 2, 4, 64, 16, BF, made=(kc, vc, table, lengths), window=40)
+    # lengths beyond the table's columns, below zero, and as long as they get
+    kc, vc, table, _ = cache(gen, lens, 2, 64, 16, BF)
+    odd = torch.tensor([2 ** 31 - 1, -5, 10000, -(2 ** 31)], dtype=torch.int32, device="cuda")
+    nan = torch.isnan(kc)
+    kc[nan], vc[nan] = 0.5, 0.25                   # every entry of the table's pages is live now
+    kc2, vc2 = kc.clone(), vc.clone()
+    q = randn(gen, 4, 8, 64, dtype=BF)
+    nk = randn(gen, 4, 2, 64, dtype=BF)
+    out = blocks.paged_attention(q, kc, vc, table, odd, new_k=nk, new_v=nk)
+    capped = torch.tensor([table.shape[1] * 16, 0, table.shape[1] * 16, 0], dtype=torch.int32, device="cuda")
+    want = R.attention(q, kc2, vc2, table, capped, None, None, 64 ** -0.5, 0, "NHD")
+    check("out", out, want[:2], 700)
+    assert torch.equal(kc, kc2) and torch.equal(vc, vc2)       # no entry for the new token
+    # a table without columns, a pool without pages
+    none = torch.zeros(4, 0, dtype=torch.int32, device="cuda")
+    out, lse = blocks.paged_attention(q, kc, vc, none, capped, return_lse=True)
+    assert not out.any() and torch.isinf(lse).all()
+    out = blocks.paged_attention(q, kc[:0], vc[:0], table, capped, new_k=nk, new_v=nk)
+    assert not out.any()
+    assert blocks.paged_attention(q[:0], kc, vc, table[:0], capped[:0]).shape == (0, 8, 64)
+
+
+def test_attention_strides(gen):
+    """Cuts of wider tensors, heads and tokens in other orders, keys and values in one tensor."""
+    lens = [77, 5, 130]
+    kc, vc, table, lengths = cache(gen, lens, 2, 64, 16, BF)
+    both = torch.stack((kc, vc), 1)               # [pages, 2, page, heads, d]
+    k, v = both[:, 0], both[:, 1]
+    wide = randn(gen, 3, 3, 8, 64, dtype=BF)      # q, k and v of a fused projection
+    q = wide[:, 0]
+    nk, nv = wide[:, 1, :2], wide[:, 2, 3:5]
+    table2 = torch.cat((table, table), 1)[:, :table.shape[1]]
+    assert not table2.is_contiguous()
+    want = R.attention(q, k, v, table, lengths, nk, nv, 64 ** -0.5, 0, "NHD")
+    out = blocks.paged_attention(q, k, v, table2, lengths, new_k=nk, new_v=nv)
+    check("out", out, want[:2], 700)
+    assert torch.equal(k.contiguous().view(torch.int16), want[4].view(torch.int16))
+    order = randn(gen, 8, 3, 64, dtype=BF).transpose(0, 1)
+    want = R.attention(order, k, v, table, lengths, None, None, 0.2, 50, "NHD")
+    check("out", blocks.paged_attention(order, k, v, table2, lengths, scale=0.2, window=50), want[:2], 700)
+
+
+def test_attention_scores_far_apart(gen):
+    """Large scores: weights of one and of nothing; a large negative scale; equal scores."""
+    lens = [300, 40]
+    q = randn(gen, 2, 8, 64, dtype=BF, scale=30.0)
+    attend(gen, lens, 2, 4, 64, 16, BF, q=q)
+    attend(gen, lens, 2, 4, 64, 16, BF, q=q, scale=-0.5)
+    attend(gen, lens, 2, 4, 64, 16, FP, q=torch.zeros(2, 8, 64, dtype=FP, device="cuda"))
+
+
+def test_attention_values_that_are_not_numbers(gen):
+    """A live NaN spoils the rows that attend to it and no others; entries that are not live may hold anything
+    (every other test's caches are NaN there)."""
+    lens = [100, 100]
+    kc, vc, table, lengths = cache(gen, lens, 2, 64, 16, BF)
+    q = randn(gen, 2, 8, 64, dtype=BF)
+    kc[table[0, 2], 3, 1] = float("nan")
+    out = blocks.paged_attention(q, kc, vc, table, lengths)
+    assert out[0, 4:].isnan().all() and out[0, :4].isfinite().all() and out[1].isfinite().all()
+
+
+def test_attention_offsets_beyond_32_bits(gen):
+    """A pool whose last pages lie more than 2^32 elements in."""
+    page, hk, d = 64, 8, 128
+    pages = (1 << 32) // (page * hk * d) + 40
+    kc = torch.zeros(pages, page, hk, d, dtype=BF, device="cuda")
+    vc = torch.zeros(pages, page, hk, d, dtype=BF, device="cuda")
+    table = torch.arange(pages - 8, pages, dtype=torch.int32, device="cuda").reshape(2, 4)
+    kc[-8:], vc[-8:] = randn(gen, 8, page, hk, d, dtype=BF), randn(gen, 8, page, hk, d, dtype=BF)
+    lengths = torch.tensor([256, 130], dtype=torch.int32, device="cuda")
+    q, nk, nv = randn(gen, 2, 32, d, dtype=BF), randn(gen, 2, hk, d, dtype=BF), randn(gen, 2, hk, d, dtype=BF)
+    small = table - (pages - 8)
+    want = R.attention(q, kc[-8:].clone(), vc[-8:].clone(), small, lengths, nk, nv, d ** -0.5, 0, "NHD")
+    out = blocks.paged_attention(q, kc, vc, table, lengths, new_k=nk, new_v=nv)
+    check("out", out, want[:2], 700)
+    assert torch.equal(kc[-8:], want[4]) and torch.equal(vc[-8:], want[5])
+    del kc, vc
+    torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------- together, on streams, in graphs
+def test_decode_layer(gen):
+    """A decode layer as it is used: norm, the projections, attention over the cache with its append, norm; three
+    tokens one after the other, against the same layer in 64 bits."""
+    b, hk, share, d, page, group = 5, 2, 4, 64, 16, 64
+    width, heads = 512, 8
+    lens = [40, 1, 16, 63, 200]
+    kc, vc, table, lengths = cache(gen, [n + 3 for n in lens], hk, d, page, BF)
+    lengths = lengths - 3
+    pre, post = randn(gen, width, scale=0.1, shift=1.0), randn(gen, width, scale=0.1, shift=1.0)
+    gate = randn(gen, width, scale=0.5)
+    wqkv = w4_inputs(gen, 1, (heads + 2 * hk) * d, width, BF, group, True)
+    wo = w4_inputs(gen, 1, width, heads * d, BF, group, False)
+    kr, vr = kc.clone(), vc.clone()
+
+    def weights(t):
+        s = t["scales"].double().repeat_interleave(group, 1)
+        z = t["zeros"].double().repeat_interleave(group, 1) if t["zeros"] is not None else 8.0
+        return (t["q"].double() - z) * s
+
+    for _ in range(3):
+        x, blk = randn(gen, b, width, dtype=BF), randn(gen, b, width, dtype=BF)
+        lengths = lengths + 1
+        h, y = blocks.block_norm(x, blk, pre, post_weight=post, gate=gate)
+        qkv = blocks.matvec_w4(y, wqkv["weight"], wqkv["scales"], wqkv["zeros"], group_size=group).view(b, heads + 2 * hk, d)
+        att = blocks.paged_attention(qkv[:, :heads], kc, vc, table, lengths, new_k=qkv[:, heads:heads + hk],
+                                     new_v=qkv[:, heads + hk:])
+        o = blocks.matvec_w4(att.view(b, -1), wo["weight"], wo["scales"], group_size=group)
+        h2, y2 = blocks.block_norm(h, o, pre, post_weight=post, gate=gate)
+        # in 64 bits from the same inputs, the 16-bit tensors between the operators rounded as they are
+        f = R.norm(x, blk, pre, post, gate, 1.0, 1e-5)
+        check("hidden", h, f["hidden"], 80)
+        check("normed", y, f["normed"], 80)
+        qkv64 = (y.double() @ weights(wqkv).t()).view(b, heads + 2 * hk, d)
+        assert torch.allclose(qkv.double(), qkv64, rtol=2.0 ** -7, atol=2e-3)
+        a64 = R.attention(qkv[:, :heads], kr, vr, table, lengths, qkv[:, heads:heads + hk], qkv[:, heads + hk:],
+                          d ** -0.5, 0, "NHD")
+        check("attention", att, a64[:2], 700)
+        kr, vr = a64[4], a64[5]
+        assert torch.equal(kc.view(torch.int16), kr.view(torch.int16)) and torch.equal(vc.view(torch.int16), vr.view(torch.int16))
+        check("o", o, R.matvec(att.view(b, -1), wo["q"], wo["scales"], None, group), 128)
+        f = R.norm(h, o, pre, post, gate, 1.0, 1e-5)
+        check("hidden 2", h2, f["hidden"], 80)
+        check("normed 2", y2, f["normed"], 80)
+
+
+def layer(s):
+    h, y = blocks.block_norm(s["x"], s["b"], s["pre"], gate=s["gate"])
+    qkv = blocks.matvec_w4(y, s["w"]["weight"], s["w"]["scales"], group_size=64).view(-1, 12, 64)
+    att = blocks.paged_attention(qkv[:, :8], s["kc"], s["vc"], s["table"], s["lengths"], new_k=qkv[:, 8:10], new_v=qkv[:, 10:])
+    return h, y, qkv, att
+
+
+def layer_inputs(gen, lens):
+    kc, vc, table, lengths = cache(gen, lens, 2, 64, 16, BF, fill=0.0)
+    b = len(lens)
+    return dict(x=randn(gen, b, 512, dtype=BF), b=randn(gen, b, 512, dtype=BF), pre=randn(gen, 512, dtype=BF),
+                gate=randn(gen, 512, dtype=BF), w=w4_inputs(gen, 1, 768, 512, BF, 64, False), kc=kc, vc=vc, table=table,
+                lengths=lengths)
+
+
+def test_graphs_streams_and_repeats(gen):
+    """Two captured layers replayed in turn and on two streams at once give what eager calls give, bit for bit."""
+    states = [layer_inputs(gen, [700, 3, 0, 129]), layer_inputs(gen, [5000])]
+    want = [[x.clone() for x in layer(s)] for s in states]
+    for s, w in zip(states, want):
+        for _ in range(3):
+            for a, b in zip(layer(s), w):
+                assert torch.equal(a, b)
+    graphs, outs = [], []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(layer(s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        for a, b in zip(o, w):
+            assert torch.equal(a, b)
+    # eager calls on two streams at once
+    got = []
+    for _ in range(5):
+        for s, st in zip(states, streams):
+            with torch.cuda.stream(st):
+                got.append((s, layer(s)))
+    torch.cuda.synchronize()
+    for s, o in got:
+        for a, b in zip(o, want[0 if s is states[0] else 1]):
+            assert torch.equal(a, b)
