@@ -1,5 +1,29 @@
 // Attention of one query token per sequence over a paged key-value cache:
 //   out = softmax(scale q K^T) V over the live positions.
+//
+// The cache is read once and everything else is small, so the bytes of K and
+// V over the memory's rate bound it; what the kernel has to do is to keep
+// enough bytes in flight on every SM whatever the lengths are.
+//  * Work is counted in tiles of 64 positions of one (sequence, key head).
+//    All tiles of all sequences form one line that is cut into as many equal
+//    runs as CTAs are resident: the CTAs read the lengths and find their run
+//    themselves, so neither a long sequence nor a ragged batch leaves SMs
+//    idle and the host needs no lengths.  A run that ends inside a sequence
+//    leaves (maximum, sum, weighted values) in scratch, at most two such
+//    pieces a CTA, and a second kernel joins them in the order of the runs.
+//  * A warp takes 16 positions of a tile and has its own ring of 16-byte
+//    asynchronous copies into shared memory, its own running maximum and sum:
+//    no barrier inside a run.  Positions that are not live are filled with
+//    zeros instead of being read, so nothing there (NaN included) counts.
+//  * The query heads of one key head are the 8 columns of the matrix
+//    instruction: S^T[16 positions x 8 heads] = K Q^T, and O^T[16 dims x 8
+//    heads] += V^T P^T, K and V^T being the row operands straight from shared
+//    memory.  A group of 8 costs no padding, and its keys are read once.
+//    mma.sync serves because 8 columns are all there is: the tensor core is
+//    idle most of the time and tcgen05's 128-row tiles would be mostly empty.
+//  * A weight p enters the product as two 16-bit halves, p = hi + lo, which
+//    keeps 2^-16 of it (16 bits alone would round the output twice); sums
+//    and the running output are 32-bit.
 #include <climits>
 #include <cmath>
 
@@ -9,81 +33,508 @@ namespace pm {
 namespace blk {
 namespace {
 
-// Writes the new token's key and value to its entry of the cache.
-template <class T>
-__global__ void __launch_bounds__(128) append_kernel(pm_paged_attention j) {
-  const int b = blockIdx.x / j.kv_heads, g = blockIdx.x % j.kv_heads;
-  const int pos = j.lengths[b] - 1;
-  if (pos < 0 || pos / j.page_size >= j.table_columns) return;
-  const int page = j.table[b * j.table_stride + pos / j.page_size];
-  if (page < 0 || page >= j.n_pages) return;
-  const int off = pos % j.page_size;
-  T* k = static_cast<T*>(j.k_cache) + page * j.k_page_stride + off * j.k_token_stride + g * j.k_head_stride;
-  T* v = static_cast<T*>(j.v_cache) + page * j.v_page_stride + off * j.v_token_stride + g * j.v_head_stride;
-  const T* nk = static_cast<const T*>(j.new_k) + b * j.new_k_stride + g * j.new_k_head_stride;
-  const T* nv = static_cast<const T*>(j.new_v) + b * j.new_v_stride + g * j.new_v_head_stride;
-  for (int c = threadIdx.x; c < j.head_dim; c += blockDim.x) {
-    k[c] = nk[c];
-    v[c] = nv[c];
-  }
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kSlice = 16, kTile = kSlice * kWarps;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnArgs {
+  pm_paged_attention j;
+  int share, blocks;                     // query heads per key head; groups of them that one pass serves
+  float* part;                           // [2 * CTAs, kHeads, head_dim] weighted values of split segments
+  float2* stat;                          // [2 * CTAs, kHeads] (maximum, sum), base 2
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_groups() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <class T> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<bf16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<fp16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two floats as packed 16-bit values and what their rounding left.
+__device__ __forceinline__ void halves(bf16*, float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(x - __bfloat162float(h.x), y - __bfloat162float(h.y));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void halves(fp16*, float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// One CTA per sequence and query head; each warp takes every fourth position,
-// with its own running maximum and sum.
-template <class T>
-__global__ void __launch_bounds__(128) attention_kernel(pm_paged_attention j) {
-  __shared__ float tops[4], sums[4], acc[4][256];
-  const int b = blockIdx.x / j.q_heads, h = blockIdx.x % j.q_heads, g = h / (j.q_heads / j.kv_heads);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* q = static_cast<const T*>(j.q) + b * j.q_stride + h * j.q_head_stride;
-  float qf[8], o[8];
-  for (int i = 0; i < 8; ++i) {
-    qf[i] = lane + 32 * i < j.head_dim ? to_float(q[lane + 32 * i]) : 0.0f;
-    o[i] = 0.0f;
-  }
+// Positions [from, to) of a sequence and the tiles that they touch.
+struct Span {
+  uint32_t from, to, first;              // first: index of the first tile
+  int tiles;
+};
+__device__ __forceinline__ Span span_of(const pm_paged_attention& j, int b) {
+  Span s;
+  const int length = max(j.lengths[b], 0);
   const int64_t room = int64_t(j.table_columns) * j.page_size;
-  const int64_t length = j.lengths[b] < 0 ? 0 : j.lengths[b];
-  const int64_t from = j.window && length > j.window ? length - j.window : 0;
-  const int64_t to = length < room ? length : room;
-  float top = -INFINITY, sum = 0.0f;
-  for (int64_t pos = from + warp; pos < to; pos += 4) {
-    const int page = j.table[b * j.table_stride + pos / j.page_size];
-    if (page < 0 || page >= j.n_pages) continue;
-    const int off = int(pos % j.page_size);
-    const T* k = static_cast<const T*>(j.k_cache) + page * j.k_page_stride + off * j.k_token_stride + g * j.k_head_stride;
-    const T* v = static_cast<const T*>(j.v_cache) + page * j.v_page_stride + off * j.v_token_stride + g * j.v_head_stride;
-    float s = 0.0f;
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < j.head_dim) s += qf[i] * to_float(k[lane + 32 * i]);
-    s = warp_sum(s) * j.scale;
-    const float next = fmaxf(top, s), base = next == -INFINITY ? 0.0f : next;
-    const float keep = expf(top - base), w = expf(s - base);
-    sum = sum * keep + w;
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < j.head_dim) o[i] = o[i] * keep + w * to_float(v[lane + 32 * i]);
-    top = next;
+  s.from = j.window && length > j.window ? length - j.window : 0;
+  s.to = j.n_pages == 0 ? 0u : uint32_t(min(int64_t(length), room));
+  s.first = s.from / kTile;
+  s.tiles = s.to > s.from ? int((s.to + kTile - 1) / kTile - s.first) : 0;
+  return s;
+}
+
+// Tiles per sequence summed over the batch: thread t has the sum over the
+// sequences before its `per` consecutive ones, prefix[kThreads] all of them.
+__device__ __forceinline__ int64_t scan_tiles(const pm_paged_attention& j, int per, int64_t* prefix) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  int64_t own = 0;
+  for (int b = t * per; b < min(j.batch, (t + 1) * per); ++b) own += span_of(j, b).tiles;
+  int64_t sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
   }
-  if (lane == 0) { tops[warp] = top; sums[warp] = sum; }
-  for (int i = 0; i < 8; ++i) acc[warp][lane + 32 * i] = o[i];
+  __shared__ int64_t warp_sums[kWarps];
+  if (lane == 31) warp_sums[warp] = sum;
   __syncthreads();
-  float best = -INFINITY, total = 0.0f;
-  for (int w = 0; w < 4; ++w) best = fmaxf(best, tops[w]);
-  const float base = best == -INFINITY ? 0.0f : best;
-  for (int w = 0; w < 4; ++w) total += sums[w] * expf(tops[w] - base);
-  T* out = static_cast<T*>(j.out) + (int64_t(b) * j.q_heads + h) * j.head_dim;
-  for (int c = threadIdx.x; c < j.head_dim; c += 128) {
-    float v = 0.0f;
-    for (int w = 0; w < 4; ++w) v += acc[w][c] * expf(tops[w] - base);
-    out[c] = from_float<T>(total == 0.0f ? 0.0f : v / total);
+  int64_t before = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) before += w < warp ? warp_sums[w] : 0;
+  prefix[t] = before + sum - own;
+  if (t == kThreads - 1) prefix[kThreads] = before + sum;
+  __syncthreads();
+  return prefix[kThreads];
+}
+
+// ---------------------------------------------------------------- the runs
+// DP: head_dim rounded up to 64; NT: groups of 8 query heads served at once.
+template <class T, int DP, int NT>
+struct Shape {
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kSliceBytes = 2 * kSlice * DP * 2;                       // K, then V
+  static constexpr int kStages = DP == 64 ? 4 : 3;
+  static constexpr int kWarpBytes = kStages * kSliceBytes;
+  static constexpr int kOutStride = DP + 4;                                     // floats; 8t + g: no two lanes in a bank
+  static constexpr size_t kSmem = size_t(kWarps) * kWarpBytes;
+  static_assert(kHeads * kOutStride * 4 <= kWarpBytes, "a warp's output fits in its ring");
+};
+
+template <class T, int DP, int NT>
+__global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_constant__ AttnArgs a) {
+  using S = Shape<T, DP, NT>;
+  constexpr int kChunks = DP / 8;                        // 16-byte pieces of a row
+  constexpr int kCopies = kSlice * kChunks / 32;         // per lane, for K and for V
+  constexpr float kLift = sizeof(T) == 2 && std::is_same<T, fp16>::value ? 8.0f : 0.0f;   // fp16 halves: weights up to 2^8
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ int64_t prefix[kThreads + 1];
+  __shared__ int64_t found_before;
+  __shared__ int found_b;
+  __shared__ uint32_t live_of[kWarps][S::kStages];
+  __shared__ float2 warp_stat[kWarps][S::kHeads];
+  __shared__ float factor[kWarps][S::kHeads];
+  __shared__ float total_of[S::kHeads];
+
+  const pm_paged_attention& j = a.j;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int D = j.head_dim, heads = j.kv_heads * a.blocks;
+  const int per = (j.batch + kThreads - 1) / kThreads;
+  const int64_t total = scan_tiles(j, per, prefix) * heads;
+
+  // sequences without a live position: zeros
+  for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
+    if (span_of(j, b).tiles) continue;
+    T* out = static_cast<T*>(j.out) + int64_t(b) * j.q_heads * D;
+    for (int i = threadIdx.x; i < j.q_heads * D; i += kThreads) out[i] = from_float<T>(0.0f);
+    if (j.lse)
+      for (int i = threadIdx.x; i < j.q_heads; i += kThreads) j.lse[int64_t(b) * j.q_heads + i] = -INFINITY;
   }
-  if (j.lse && threadIdx.x == 0) j.lse[int64_t(b) * j.q_heads + h] = base + logf(total);
+
+  const int64_t runs = min(int64_t(gridDim.x), total);   // no run is empty
+  if (blockIdx.x >= runs) return;
+  int64_t cur = total * blockIdx.x / runs;
+  const int64_t end = total * (blockIdx.x + 1) / runs;
+  if (prefix[threadIdx.x] * heads <= cur && cur < prefix[threadIdx.x + 1] * heads) {
+    int64_t before = prefix[threadIdx.x];
+    int b = threadIdx.x * per;
+    for (;; ++b) {
+      const int n = span_of(j, b).tiles;
+      if (cur < (before + n) * heads) break;
+      before += n;
+    }
+    found_b = b;
+    found_before = before;
+  }
+  __syncthreads();
+  int b = found_b;
+  Span sp = span_of(j, b);
+  int64_t base = found_before * heads;                   // the sequence's first tile on the line
+
+  uint8_t* mine = ring + warp * S::kWarpBytes;
+  const uint32_t mine_addr = smem_addr(mine);
+  const float scale2 = j.scale * kLog2e;
+
+  while (cur < end) {
+    const int which = int((cur - base) / sp.tiles);      // key head and group of query heads
+    const int kvh = which / a.blocks, hb = which - kvh * a.blocks;
+    const int t0 = int(cur - base - int64_t(which) * sp.tiles);
+    const int t1 = int(min(int64_t(sp.tiles), t0 + (end - cur)));
+    const int h0 = kvh * a.share + hb * S::kHeads, nh = min(S::kHeads, a.share - hb * S::kHeads);
+    const int n_slices = t1 - t0;                        // one slice of this warp in each tile
+    const uint32_t pos0 = (sp.first + t0) * uint32_t(kTile) + warp * kSlice;
+    const int32_t* table = j.table + b * j.table_stride;
+    const T* kc = static_cast<const T*>(j.k_cache) + kvh * j.k_head_stride;
+    const T* vc = static_cast<const T*>(j.v_cache) + kvh * j.v_head_stride;
+    const T* nk = static_cast<const T*>(j.new_k) + b * j.new_k_stride + kvh * j.new_k_head_stride;
+    const T* nv = static_cast<const T*>(j.new_v) + b * j.new_v_stride + kvh * j.new_v_head_stride;
+    const uint32_t newest = j.new_k ? uint32_t(max(j.lengths[b], 0)) - 1u : 0xffffffffu;
+
+    // the page of this lane's position (lanes 0-15) in slice i, -1 where it is not live
+    auto page_of = [&](int i) {
+      const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
+      int page = -1;
+      if (i < n_slices && lane < kSlice && pos >= sp.from && pos < sp.to) {
+        page = table[pos / uint32_t(j.page_size)];
+        if (page >= j.n_pages) page = -1;
+      }
+      return page;
+    };
+    auto fetch = [&](int i, int page) {
+      if (i < n_slices) {
+        const int stage = i % S::kStages;
+        const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
+        const int off = int(pos % uint32_t(j.page_size));
+        const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+        if (lane == 0) live_of[warp][stage] = live;
+        const uint32_t kdst = mine_addr + stage * S::kSliceBytes, vdst = kdst + kSlice * DP * 2;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
+          const int row_page = __shfl_sync(0xffffffffu, page, row), row_off = __shfl_sync(0xffffffffu, off, row);
+          const bool read = row_page >= 0 && chunk * 8 < D;
+          const T* ks = kc;
+          const T* vs = vc;
+          if (read) {
+            ks += row_page * j.k_page_stride + row_off * j.k_token_stride + chunk * 8;
+            vs += row_page * j.v_page_stride + row_off * j.v_token_stride + chunk * 8;
+            if (pos0 + uint32_t(i) * kTile + row == newest) {
+              // the new token: read from its own tensors, and written to the cache by the first group
+              if (hb == 0) {
+                *reinterpret_cast<uint4*>(const_cast<T*>(ks)) = *reinterpret_cast<const uint4*>(nk + chunk * 8);
+                *reinterpret_cast<uint4*>(const_cast<T*>(vs)) = *reinterpret_cast<const uint4*>(nv + chunk * 8);
+              }
+              ks = nk + chunk * 8;
+              vs = nv + chunk * 8;
+            }
+          }
+          const uint32_t at = uint32_t(row * kChunks + (chunk ^ (row & 7))) * 16;
+          copy16(kdst + at, ks, read);
+          copy16(vdst + at, vs, read);
+        }
+      }
+      commit();
+    };
+
+    // queries as the column operand: head g, dims 2t, 2t+1 and 2t+8, 2t+9 of each 16
+    uint32_t q[NT][DP / 16][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool have = n * 8 + g < nh;
+      const T* qp = static_cast<const T*>(j.q) + b * j.q_stride + (h0 + (have ? n * 8 + g : 0)) * j.q_head_stride;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = k * 16 + e * 8 + 2 * t;
+          q[n][k][e] = have && d < D ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
+        }
+    }
+
+    float o[NT][DP / 16][4] = {};
+    float top[NT][2], sum[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
+
+    int page = page_of(0);
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      const int ahead = page_of(i + 1);
+      fetch(i, page);
+      page = ahead;
+    }
+    for (int i = 0; i < n_slices; ++i) {
+      // the page index of the slice after the next fetch travels while this slice is computed
+      const int ahead = page_of(i + S::kStages);
+      fetch(i + S::kStages - 1, page);
+      page = ahead;
+      wait_groups<S::kStages - 1>();
+      __syncwarp();
+      const int stage = i % S::kStages;
+      const uint32_t live = live_of[warp][stage];
+      if (live) {
+        const uint32_t kbase = mine_addr + stage * S::kSliceBytes, vbase = kbase + kSlice * DP * 2;
+        float s[NT][4] = {};
+        {
+          const int row = lane & 15, half = lane >> 4;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            uint32_t ka[4];
+            ldsm(ka, kbase + uint32_t(row * kChunks + ((2 * k + half) ^ (row & 7))) * 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<T>(s[n], ka, q[n][k][0], q[n][k][1]);
+          }
+        }
+        const bool live_a = live >> g & 1, live_b = live >> (g + 8) & 1;
+        uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[n][0] = live_a ? s[n][0] * scale2 : -INFINITY;
+          s[n][1] = live_a ? s[n][1] * scale2 : -INFINITY;
+          s[n][2] = live_b ? s[n][2] * scale2 : -INFINITY;
+          s[n][3] = live_b ? s[n][3] * scale2 : -INFINITY;
+          float m0 = fmaxf(s[n][0], s[n][2]), m1 = fmaxf(s[n][1], s[n][3]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
+            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
+          }
+          m0 = fmaxf(m0, top[n][0]);
+          m1 = fmaxf(m1, top[n][1]);
+          const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+          if (__any_sync(0xffffffffu, m0 != top[n][0] || m1 != top[n][1])) {
+            const float c0 = exp2_fast(top[n][0] - b0), c1 = exp2_fast(top[n][1] - b1);
+            sum[n][0] *= c0;
+            sum[n][1] *= c1;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+              o[n][k][0] *= c0; o[n][k][1] *= c1; o[n][k][2] *= c0; o[n][k][3] *= c1;
+            }
+            top[n][0] = m0;
+            top[n][1] = m1;
+          }
+          const float p0 = exp2_fast(s[n][0] - b0 + kLift), p1 = exp2_fast(s[n][1] - b1 + kLift);
+          const float p2 = exp2_fast(s[n][2] - b0 + kLift), p3 = exp2_fast(s[n][3] - b1 + kLift);
+          sum[n][0] += p0 + p2;
+          sum[n][1] += p1 + p3;
+          halves(static_cast<T*>(nullptr), p0, p1, hi[n][0], lo[n][0]);
+          halves(static_cast<T*>(nullptr), p2, p3, hi[n][1], lo[n][1]);
+          hi[n][0] = transpose8(hi[n][0]);
+          hi[n][1] = transpose8(hi[n][1]);
+          lo[n][0] = transpose8(lo[n][0]);
+          lo[n][1] = transpose8(lo[n][1]);
+        }
+        {
+          const int row = (lane & 7) + (lane >> 4) * 8, half = lane >> 3 & 1;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            uint32_t va[4];
+            ldsm_t(va, vbase + uint32_t(row * kChunks + ((2 * k + half) ^ (row & 7))) * 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma<T>(o[n][k], va, hi[n][0], hi[n][1]);
+              mma<T>(o[n][k], va, lo[n][0], lo[n][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();                                      // the slice is read before its place is filled again
+    }
+    wait_groups<0>();
+    __syncwarp();
+
+    // the warps' results through shared memory, each in its own ring
+    float* ow = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        sum[n][0] += __shfl_xor_sync(0xffffffffu, sum[n][0], x);
+        sum[n][1] += __shfl_xor_sync(0xffffffffu, sum[n][1], x);
+      }
+      if (g == 0) {
+        warp_stat[warp][n * 8 + 2 * t] = make_float2(top[n][0], sum[n][0]);
+        warp_stat[warp][n * 8 + 2 * t + 1] = make_float2(top[n][1], sum[n][1]);
+      }
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        float* at = ow + (n * 8 + 2 * t) * S::kOutStride + k * 16 + g;
+        at[0] = o[n][k][0];
+        at[S::kOutStride] = o[n][k][1];
+        at[8] = o[n][k][2];
+        at[S::kOutStride + 8] = o[n][k][3];
+      }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == sp.tiles;
+    const int64_t slot = 2 * int64_t(blockIdx.x) + (t0 == 0 ? 1 : 0);
+    if (threadIdx.x < S::kHeads) {
+      const int h = threadIdx.x;
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[w][h].x);
+      const float mb = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = exp2_fast(warp_stat[w][h].x - mb);
+        factor[w][h] = f;
+        l += warp_stat[w][h].y * f;
+      }
+      total_of[h] = l;
+      if (h < nh) {
+        if (!whole) a.stat[slot * S::kHeads + h] = make_float2(m, l);
+        else if (j.lse) j.lse[int64_t(b) * j.q_heads + h0 + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+      }
+    }
+    __syncthreads();
+    for (int h = 0; h < nh; ++h) {
+      const float l = total_of[h];
+      for (int d = threadIdx.x; d < D; d += kThreads) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+          v += reinterpret_cast<const float*>(ring + w * S::kWarpBytes)[h * S::kOutStride + d] * factor[w][h];
+        if (whole) static_cast<T*>(j.out)[(int64_t(b) * j.q_heads + h0 + h) * D + d] = from_float<T>(l == 0.0f ? 0.0f : v / l);
+        else a.part[(slot * S::kHeads + h) * D + d] = v;
+      }
+    }
+    __syncthreads();
+
+    cur += t1 - t0;
+    if (cur < end && cur == base + int64_t(sp.tiles) * heads) {
+      base = cur;
+      do sp = span_of(j, ++b);                           // the line goes on: a later sequence has tiles
+      while (!sp.tiles);
+    }
+  }
+}
+
+// Joins the pieces of each segment that was cut: one CTA per query head.
+template <class T, int NT>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+  constexpr int kHeads = 8 * NT;
+  constexpr float kLift = std::is_same<T, fp16>::value ? 8.0f : 0.0f;
+  __shared__ int64_t prefix[kThreads + 1];
+  const pm_paged_attention& j = a.j;
+  const int b = blockIdx.x / j.q_heads, h = blockIdx.x - b * j.q_heads;
+  const int heads = j.kv_heads * a.blocks, D = j.head_dim;
+  const int per = (j.batch + kThreads - 1) / kThreads;
+  const int64_t total = scan_tiles(j, per, prefix) * heads;
+  const int tiles = span_of(j, b).tiles;
+  asm volatile("griddepcontrol.wait;" ::: "memory");    // in every CTA: this kernel's end has to mean the first one's
+  if (!tiles) return;
+  int64_t before = prefix[b / per];
+  for (int i = b / per * per; i < b; ++i) before += span_of(j, i).tiles;
+  const int kvh = h / a.share, within = h - kvh * a.share, hb = within / kHeads, row = within - hb * kHeads;
+  const int64_t s0 = before * heads + int64_t(kvh * a.blocks + hb) * tiles, s1 = s0 + tiles;
+  // run c holds tiles [total c / runs, total (c + 1) / runs)
+  const int64_t runs = min(int64_t(ctas), total);
+  const int c0 = int(((s0 + 1) * runs - 1) / total), c1 = int((s1 * runs - 1) / total);
+  if (c0 == c1) return;
+  auto slot_of = [&](int c) { return 2 * int64_t(c) + (total * c / runs <= s0 ? 1 : 0); };
+  float m = -INFINITY;
+  for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(&a.stat[slot_of(c) * kHeads + row]).x);
+  const float mb = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
+  const int d = threadIdx.x;
+  for (int c = c0; c <= c1; ++c) {
+    const int64_t at = slot_of(c) * kHeads + row;
+    const float2 st = __ldcg(&a.stat[at]);
+    const float f = exp2_fast(st.x - mb);
+    l += st.y * f;
+    if (d < D) v0 += __ldcg(&a.part[at * D + d]) * f;
+    if (d + kThreads < D) v1 += __ldcg(&a.part[at * D + d + kThreads]) * f;
+  }
+  T* out = static_cast<T*>(j.out) + (int64_t(b) * j.q_heads + h) * D;
+  if (d < D) out[d] = from_float<T>(l == 0.0f ? 0.0f : v0 / l);
+  if (d + kThreads < D) out[d + kThreads] = from_float<T>(l == 0.0f ? 0.0f : v1 / l);
+  if (j.lse && d == 0) j.lse[int64_t(b) * j.q_heads + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+}
+
+// ---------------------------------------------------------------- launch
+// Query heads in groups of 8, two groups at once where more than 8 share a
+// key head and their registers allow it (head_dim up to 128).
+int tiles_of_heads(int share, int head_dim) { return share > 8 && head_dim <= 128 ? 2 : 1; }
+constexpr int kMaxRuns = 148 * 4;        // CTAs of the first kernel at most: sizes the scratch
+
+std::atomic<int> g_occupancy[kMaxDevices][2][4][2];
+std::atomic<int> g_smem_limit[2][4][2][kMaxDevices];
+
+template <class T, int DP, int NT>
+cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s) {
+  using S = Shape<T, DP, NT>;
+  constexpr int ti = std::is_same<T, fp16>::value ? 1 : 0;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const auto kernel = attention_runs_kernel<T, DP, NT>;
+  std::atomic<int>& known = g_occupancy[device][ti][DP / 64 - 1][NT - 1];
+  int occ = known.load(std::memory_order_relaxed);
+  if (!occ) {
+    ensure_dynamic_smem(kernel, 4096, S::kSmem, g_smem_limit[ti][DP / 64 - 1][NT - 1]);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, kThreads, S::kSmem);
+    if (e != cudaSuccess) return e;
+    if (occ < 1) return cudaErrorInvalidConfiguration;
+    known.store(occ, std::memory_order_relaxed);
+  }
+  const pm_paged_attention& j = a.j;
+  a.blocks = (a.share + S::kHeads - 1) / S::kHeads;
+  // no more runs than tiles at the tables' full length, which bounds the lengths
+  const int64_t room = (int64_t(j.table_columns) * j.page_size + kTile - 1) / kTile;
+  const int64_t most = int64_t(j.batch) * j.kv_heads * a.blocks * (room < (1 << 20) ? (room > 1 ? room : 1) : (1 << 20));
+  int64_t runs = int64_t(sms) * occ;
+  if (runs > kMaxRuns) runs = kMaxRuns;
+  if (runs > most) runs = most;
+  a.stat = reinterpret_cast<float2*>(scratch);
+  a.part = reinterpret_cast<float*>(scratch + size_t(2) * kMaxRuns * S::kHeads * sizeof(float2));
+  kernel<<<unsigned(runs), kThreads, S::kSmem, s>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || room <= 1) return e;           // one tile at most: nothing is ever cut
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(j.batch * j.q_heads));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, NT>, a, int(runs));
 }
 
 template <class T>
-cudaError_t launch(const pm_paged_attention& j, cudaStream_t s) {
-  if (j.new_k) append_kernel<T><<<j.batch * j.kv_heads, 128, 0, s>>>(j);
-  attention_kernel<T><<<j.batch * j.q_heads, 128, 0, s>>>(j);
-  return cudaGetLastError();
+cudaError_t launch(const pm_paged_attention& j, void* scratch, int sms, cudaStream_t s) {
+  AttnArgs a{};
+  a.j = j;
+  a.share = j.q_heads / j.kv_heads;
+  uint8_t* f = static_cast<uint8_t*>(scratch);
+  const int nt = tiles_of_heads(a.share, j.head_dim);
+  if (j.head_dim <= 64) return nt == 2 ? launch_shape<T, 64, 2>(a, f, sms, s) : launch_shape<T, 64, 1>(a, f, sms, s);
+  if (j.head_dim <= 128) return nt == 2 ? launch_shape<T, 128, 2>(a, f, sms, s) : launch_shape<T, 128, 1>(a, f, sms, s);
+  return j.head_dim <= 192 ? launch_shape<T, 192, 1>(a, f, sms, s) : launch_shape<T, 256, 1>(a, f, sms, s);
 }
 
 }  // namespace
@@ -94,8 +545,9 @@ using namespace pm;
 using namespace pm::blk;
 
 extern "C" size_t pm_paged_attention_scratch_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
-  if (batch < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1) return 0;
-  return 256;
+  if (batch < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || q_heads % kv_heads) return 0;
+  const size_t rows = size_t(2) * kMaxRuns * 8 * tiles_of_heads(q_heads / kv_heads, head_dim);
+  return rows * sizeof(float2) + rows * size_t(head_dim) * sizeof(float);
 }
 
 extern "C" int pm_paged_attention_device(const pm_paged_attention* j, void* scratch, size_t scratch_bytes, void* stream) {
@@ -132,6 +584,6 @@ extern "C" int pm_paged_attention_device(const pm_paged_attention* j, void* scra
   const int rc = sm_count(&sms);
   if (rc != PM_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(*j, s) : launch<fp16>(*j, s);
+  const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(*j, scratch, sms, s) : launch<fp16>(*j, scratch, sms, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_paged_attention_device launch");
 }
