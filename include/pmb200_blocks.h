@@ -90,7 +90,7 @@ int pm_block_norm_backward_device(const pm_block_norm* forward, const pm_block_n
  * y[m, n] = sum_k x[m, k] * scales[n, k / group] * (q[n, k] - zero[n, k / group])
  * with q the 4-bit weights of row n, two to a byte, the even k in the low
  * half (an odd k leaves the last high half unread), and zero = zeros[n, k / group]
- * (0..255) or 8 where zeros is NULL.  dtype (x and y) is PM_DT_BF16 or
+ * (0..15, the high half of the byte unread) or 8 where zeros is NULL.  dtype (x and y) is PM_DT_BF16 or
  * PM_DT_F16; scales are of that type or PM_DT_F32, [n, ceil(k / group)]
  * contiguous, as are zeros.  group is a multiple of 32; the last may be
  * partial.  y is contiguous [tokens, n].  tokens 0 is allowed and does

@@ -257,7 +257,7 @@ def matvec_w4(x, weight, scales, zeros=None, *, group_size=128):
 
     ``weight`` is [n, ceil(k / 2)] uint8 (any row stride), the even k in the
     low half of a byte; ``scales`` [n, ceil(k / group_size)] of x's type or
-    float32; ``zeros`` the same shape in uint8, or None for 8 everywhere.
+    float32; ``zeros`` the same shape in uint8 (0..15), or None for 8 everywhere.
     Meant for single tokens and small batches: the weights are read once for
     every 16 tokens.
     """
