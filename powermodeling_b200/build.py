@@ -6,6 +6,7 @@ are recompiled only when they or a header changed.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -47,6 +48,9 @@ PACKER = PACKAGE / ("_packnative" + (sysconfig.get_config_var("EXT_SUFFIX") or "
 # The record assembly helpers: a second CPython extension (host C++).
 RECORDS_SRC = CSRC / "python" / "records.cpp"
 RECORDS = PACKAGE / ("_recordnative" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+# The block operators on torch tensors: a CPython extension over libpmb200 and torch's C++ API (host C++).
+BLOCKS_SRC = CSRC / "python" / "blocks.cpp"
+BLOCKS = PACKAGE / ("_blocksnative" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
 def _sources() -> list[Path]:
@@ -101,7 +105,24 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
             if verbose:
                 print(" ".join(ext), file=sys.stderr)
             _drain(subprocess.Popen(ext, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    if _stale(BLOCKS, BLOCKS_SRC, [INCLUDE / "pmb200.h", INCLUDE / "pmb200_blocks.h"]):
+        ext = _blocks_command()
+        if verbose:
+            print(" ".join(ext), file=sys.stderr)
+        _drain(subprocess.Popen(ext, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
     return LIBRARY
+
+
+def _blocks_command() -> list[str]:
+    """g++ for the block operators' extension, against the installed torch (found without importing it)."""
+    torch = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    include = torch / "include"
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    return [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden",
+            "-I" + sysconfig.get_paths()["include"], "-I" + str(INCLUDE), "-isystem", str(include), "-isystem",
+            str(include / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda), str(BLOCKS_SRC), "-o", str(BLOCKS),
+            "-L" + str(PACKAGE), "-lpmb200", "-Wl,-rpath,$ORIGIN", "-L" + str(torch / "lib"), "-lc10", "-lc10_cuda",
+            "-ltorch_cpu", "-ltorch_python"]
 
 
 def _drain(proc: subprocess.Popen) -> None:

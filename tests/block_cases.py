@@ -6,9 +6,12 @@ within (number of roundings) x 2^-24 x magnitude of the value.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 import torch
+
+from powermodeling_b200 import _native as N
 
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 # the smallest half step: below it a rounding is off by an absolute amount
@@ -133,3 +136,51 @@ def attention(q, k_cache, v_cache, table, lengths, new_k, new_v, scale, window, 
         # every weight is off by the roundings of its score and of the largest, besides its own
         mag[i] = (w[:, :, None] * v.abs() * (1 + 2 * S.amax(0))[None, :, None]).sum(0)
     return out, mag, lse, lmag, kc, vc
+
+
+# ---------------------------------------------------------------- the C entries (include/pmb200_blocks.h)
+_p = C.c_void_p
+
+
+class BlockNorm(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("gate_rows", C.c_int64), ("residual_stride", C.c_int64),
+                ("block_stride", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32), ("pre_dtype", C.c_int32),
+                ("post_dtype", C.c_int32), ("gate_dtype", C.c_int32), ("scale", C.c_float), ("eps", C.c_float),
+                ("residual", _p), ("block", _p), ("pre_weight", _p), ("post_weight", _p), ("gate", _p),
+                ("hidden", _p), ("normed", _p), ("stats", _p)]
+
+
+class BlockNormGrads(C.Structure):
+    _fields_ = [("grad_hidden_stride", C.c_int64), ("grad_normed_stride", C.c_int64), ("grad_hidden", _p),
+                ("grad_normed", _p), ("grad_residual", _p), ("grad_block", _p), ("grad_pre", _p), ("grad_post", _p),
+                ("grad_gate", _p)]
+
+
+class MatvecW4(C.Structure):
+    _fields_ = [("tokens", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32), ("dtype", C.c_int32),
+                ("scales_dtype", C.c_int32), ("x_stride", C.c_int64), ("weight_stride", C.c_int64), ("x", _p),
+                ("weight", _p), ("scales", _p), ("zeros", _p), ("y", _p)]
+
+
+class PagedAttention(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_size", C.c_int32), ("n_pages", C.c_int32), ("table_columns", C.c_int32), ("dtype", C.c_int32),
+                ("window", C.c_int32), ("scale", C.c_float), ("q_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("new_k_stride", C.c_int64), ("new_k_head_stride", C.c_int64), ("new_v_stride", C.c_int64),
+                ("new_v_head_stride", C.c_int64), ("table_stride", C.c_int64), ("q", _p), ("k_cache", _p),
+                ("v_cache", _p), ("table", _p), ("lengths", _p), ("new_k", _p), ("new_v", _p), ("out", _p), ("lse", _p)]
+
+
+def library():
+    lib = N.library()
+    lib.pm_block_norm_device.argtypes = [_p, _p]
+    lib.pm_block_norm_backward_scratch_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int32]
+    lib.pm_block_norm_backward_scratch_bytes.restype = C.c_size_t
+    lib.pm_block_norm_backward_device.argtypes = [_p, _p, _p, C.c_size_t, _p]
+    lib.pm_matvec_w4_device.argtypes = [_p, _p]
+    lib.pm_paged_attention_scratch_bytes.argtypes = [C.c_int32] * 4
+    lib.pm_paged_attention_scratch_bytes.restype = C.c_size_t
+    lib.pm_paged_attention_device.argtypes = [_p, _p, C.c_size_t, _p]
+    return lib

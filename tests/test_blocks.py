@@ -7,6 +7,7 @@ import re
 import pytest
 import torch
 
+import block_cases as K
 from conftest import ROOT
 from powermodeling_b200 import _native as N
 from powermodeling_b200 import blocks
@@ -52,8 +53,13 @@ def test_block_norm_refusals(kw, message):
 
 def test_block_norm_backward_refusals():
     x, w, st = z(4, 32), z(32), z(4, 2, dtype=torch.float32)
-    for args, message in (((None, None, x, x, w, st), "CUDA device"),      # the inputs' place comes first
-                          ((x, x, x, z(4, 31), w, st), "must be")):
+    for args, message in (((None, None, x, x, w, st), "no incoming gradient"),
+                          ((x, None, x, x, w, z(4, 2)), "stats"),
+                          ((x, None, x, x, w, z(3, 2, dtype=torch.float32)), "stats"),
+                          ((z(4, 32, dtype=torch.float32), None, x, x, w, st), "grad_hidden"),
+                          ((None, z(4, 31), x, x, w, st), "grad_normed"),
+                          ((x, x, x, z(4, 31), w, st), "must be"),
+                          ((x, x, x, x, w, st), "CUDA device")):
         with pytest.raises(ValueError, match=message):
             blocks.block_norm_backward(*args)
 
@@ -78,6 +84,7 @@ def matvec(**kw):
     (dict(scales=z(8, 1, dtype=torch.float16)), "scales"),
     (dict(zeros=z(8, 1)), "zeros"),
     (dict(zeros=z(8, 2, dtype=torch.uint8)), "zeros"),
+    (dict(x=z(2, 64).requires_grad_()), "no backward"),
     (dict(), "CUDA device"),
 ])
 def test_matvec_refusals(kw, message):
@@ -117,6 +124,8 @@ def attention(**kw):
     (dict(page_table=z(2, 4, dtype=torch.int32)[:, ::2]), "page_table"),
     (dict(lengths=z(2, dtype=torch.int64)), "lengths"),
     (dict(lengths=z(4, dtype=torch.int32)[::2]), "lengths"),
+    (dict(new_k=z(2, 2, 64).requires_grad_(), new_v=z(2, 2, 64)), "no backward"),
+    (dict(q="q"), "must be a tensor"),
     (dict(), "CUDA device"),
 ])
 def test_attention_refusals(kw, message):
@@ -133,7 +142,7 @@ def c_norm(**kw):
              gate_dtype=0, scale=1.0, eps=1e-5, residual=A, block=A, pre_weight=A, post_weight=None, gate=None,
              hidden=A, normed=A, stats=None)
     a.update(kw)
-    return blocks._BlockNorm(**a)
+    return K.BlockNorm(**a)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -145,20 +154,20 @@ def c_norm(**kw):
     (dict(hidden=None), INVALID), (dict(pre_weight=None), INVALID), (dict(block=A + 1), INVALID),
     (dict(pre_weight=A + 2, pre_dtype=0), INVALID), (dict(stats=A + 2), INVALID)])
 def test_c_block_norm_refusals(kw, code):
-    lib = blocks._lib()
+    lib = K.library()
     assert lib.pm_block_norm_device(C.byref(c_norm(**kw)), None) == code
     assert "pm_block_norm_device" in N.last_error()
 
 
 def test_c_block_norm_backward_refusals():
-    lib = blocks._lib()
+    lib = K.library()
     job = c_norm(stats=A, hidden=None, normed=None)
     need = lib.pm_block_norm_backward_scratch_bytes(4, 0, 32)
     assert need > 0 and lib.pm_block_norm_backward_scratch_bytes(4, 3, 32) == 0
     full = dict(grad_hidden_stride=32, grad_normed_stride=32, grad_hidden=A, grad_normed=A, grad_residual=A, grad_block=A)
 
     def call(job=job, scratch=A, size=need, **kw):
-        return lib.pm_block_norm_backward_device(C.byref(job), C.byref(blocks._BlockNormGrads(**{**full, **kw})), scratch, size, None)
+        return lib.pm_block_norm_backward_device(C.byref(job), C.byref(K.BlockNormGrads(**{**full, **kw})), scratch, size, None)
     assert call(job=c_norm(stats=None)) == INVALID
     assert call(grad_residual=None) == INVALID
     assert call(grad_hidden_stride=31) == INVALID
@@ -173,7 +182,7 @@ def c_w4(**kw):
     a = dict(tokens=2, n=8, k=64, group=64, dtype=1, scales_dtype=1, x_stride=64, weight_stride=32, x=A, weight=A, scales=A,
              zeros=None, y=A)
     a.update(kw)
-    return blocks._MatvecW4(**a)
+    return K.MatvecW4(**a)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -182,7 +191,7 @@ def c_w4(**kw):
     (dict(dtype=0), INVALID), (dict(scales_dtype=2), INVALID), (dict(x_stride=63), INVALID), (dict(weight_stride=31), INVALID),
     (dict(x=None), INVALID), (dict(y=None), INVALID), (dict(scales=A + 1), INVALID), (dict(x=A + 1), INVALID)])
 def test_c_matvec_refusals(kw, code):
-    assert blocks._lib().pm_matvec_w4_device(C.byref(c_w4(**kw)), None) == code
+    assert K.library().pm_matvec_w4_device(C.byref(c_w4(**kw)), None) == code
     assert "pm_matvec_w4_device" in N.last_error()
 
 
@@ -193,7 +202,7 @@ def c_attention(**kw):
              new_v_head_stride=0, table_stride=2, q=A, k_cache=A, v_cache=A, table=A, lengths=A, new_k=None, new_v=None, out=A,
              lse=None)
     a.update(kw)
-    return blocks._PagedAttention(**a)
+    return K.PagedAttention(**a)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -204,21 +213,21 @@ def c_attention(**kw):
     (dict(k_cache=A + 8), INVALID), (dict(out=A + 8), INVALID), (dict(lengths=A + 2), INVALID), (dict(k_token_stride=65), INVALID),
     (dict(q_stride=-8), INVALID), (dict(table_stride=-1), INVALID)])
 def test_c_attention_refusals(kw, code):
-    lib = blocks._lib()
+    lib = K.library()
     need = lib.pm_paged_attention_scratch_bytes(2, 4, 2, 64)
     assert lib.pm_paged_attention_device(C.byref(c_attention(**kw)), A, need, None) == code
     assert "pm_paged_attention_device" in N.last_error()
 
 
 def test_c_attention_scratch():
-    lib = blocks._lib()
+    lib = K.library()
     need = lib.pm_paged_attention_scratch_bytes(2, 4, 2, 64)
     for scratch, size in ((None, need), (A + 16, need), (A, need - 1)):
         assert lib.pm_paged_attention_device(C.byref(c_attention()), scratch, size, None) == INVALID
 
 
 def test_empty_calls_need_no_device():
-    lib = blocks._lib()
+    lib = K.library()
     assert lib.pm_block_norm_device(C.byref(c_norm(rows=0)), None) == 0
     assert lib.pm_matvec_w4_device(C.byref(c_w4(tokens=0)), None) == 0
     assert lib.pm_paged_attention_device(C.byref(c_attention(batch=0)), None, 0, None) == 0
@@ -227,8 +236,8 @@ def test_empty_calls_need_no_device():
 def test_structs_follow_the_header():
     """Field names and order of every job struct are the header's."""
     text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "pmb200_blocks.h").read_text(), flags=re.S)
-    for name, struct in (("pm_block_norm", blocks._BlockNorm), ("pm_block_norm_grads", blocks._BlockNormGrads),
-                         ("pm_matvec_w4", blocks._MatvecW4), ("pm_paged_attention", blocks._PagedAttention)):
+    for name, struct in (("pm_block_norm", K.BlockNorm), ("pm_block_norm_grads", K.BlockNormGrads),
+                         ("pm_matvec_w4", K.MatvecW4), ("pm_paged_attention", K.PagedAttention)):
         body = re.search(r"typedef struct \{([^}]*)\} " + name + ";", text).group(1)
         fields = [f.strip().split()[-1].lstrip("*") for line in body.split(";") for f in line.split(",") if f.strip()]
         assert fields == [f for f, _ in struct._fields_], name
