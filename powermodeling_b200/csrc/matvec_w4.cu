@@ -3,11 +3,13 @@
 //   y[m, n] = sum_g s[n, g] sum_{k in g} x[m, k] (q[n, k] - z[n, g]).
 //
 // The weights are read once and bound it.
-//  * A warp owns 16 rows of weights and 256 values of k at a time, 2 KB that
+//  * A warp owns 32 rows of weights and 128 values of k at a time, 2 KB that
 //    it copies into shared memory asynchronously, four stages deep.  The 8
 //    warps of a CTA stand side by side along n or along k, so a stage is 16 KB
 //    whatever the matrix's shape: enough bytes in flight with two CTAs an SM.
-//    The tokens' values for a stage are copied beside it, for all warps.
+//    The tokens' values for a stage are copied beside it, for all warps, and
+//    each serves two tiles of 16 rows in registers: unpacking has to keep up
+//    with the memory on the integer pipe, where every other instruction counts.
 //  * q - z is an integer that 16-bit floats hold exactly: four nibbles are
 //    masked into the mantissas of 128 (bf16) or 1024 (fp16) and the same
 //    number plus z is subtracted.  The matrix instruction multiplies 16 rows
@@ -32,8 +34,9 @@ namespace blk {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 256, kStages = 4;
-constexpr int kWarpK = 256;                              // k of a warp's tile
-constexpr int kTileBytes = 16 * kWarpK / 2;              // 16 rows
+constexpr int kRows = 32, kTileK = 128;                  // of a warp's tile
+constexpr int kPitch = kTileK / 2;                       // bytes of a tile's row: four pieces, in an order of the row's own
+constexpr int kTileBytes = kRows * kPitch;
 constexpr int kWeightBytes = kWarps * kTileBytes;        // a stage
 constexpr int kXPad = 64;                                // bytes after a token's values: neighbours in other banks
 
@@ -46,28 +49,53 @@ struct W4Args {
   const uint8_t* zeros;
   void* y;
   int warps_n;                                           // warps along n; the others along k
+  int vector_scales;                                     // scales 16-byte, zeros 4-byte aligned
+  int x_shift;                                           // log2 of the 16-byte pieces of a token in a stage
+  int group_shift;                                       // log2 of the 32-k blocks of a group, -1: no power of two
   int slice;                                             // k of one CTA of the cluster, a multiple of the stage's
 };
 
-template <class T> struct Magic;
-template <> struct Magic<bf16> { static constexpr uint32_t value = 0x43004300u; };   // 128
-template <> struct Magic<fp16> { static constexpr uint32_t value = 0x64006400u; };   // 1024
-
-__device__ __forceinline__ uint32_t sub2(bf16*, uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// (a & b) | c in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
-__device__ __forceinline__ uint32_t sub2(fp16*, uint32_t a, uint32_t b) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-// The pairs (0,4), (1,5), (2,6), (3,7) of a word's nibbles, less the zero point.
-template <class T>
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
+// A zero point as the pair that unpacking subtracts, and the pairs
+// (0,4), (1,5), (2,6), (3,7) of a word's nibbles, less the zero point.
+template <class T> struct Nibbles;
+template <> struct Nibbles<bf16> {
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x43004300u | z * 0x10001u; }   // 128 + z
+  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
+    const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zero);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = sub2(static_cast<T*>(nullptr), ((w >> (4 * i)) & 0x000f000fu) | Magic<T>::value, zero);
-}
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z);
+      p[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+  }
+};
+// fp16's longer mantissa takes a nibble four bits further up as well: 1024 +
+// 16 q, which one fused multiply-add brings to q - z exactly.  One shift a word.
+template <> struct Nibbles<fp16> {
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | z * 0x10001u; }   // 1024 + z
+  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
+    const __half2 z = *reinterpret_cast<const __half2*>(&zero);
+    const uint32_t high = and_or(zero << 4, 0x00f000f0u, 0xd400d400u);                                  // -(64 + z)
+    const uint32_t sixteenth = 0x2c002c00u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t u = i ? w >> 8 : w;
+      const uint32_t a = and_or(u, 0x000f000fu, 0x64006400u), b = and_or(u, 0x00f000f0u, 0x64006400u);
+      const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), z);
+      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&sixteenth),
+                                *reinterpret_cast<const __half2*>(&high));
+      p[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+      p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+  }
+};
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -105,121 +133,164 @@ __device__ __forceinline__ uint4 keep(uint4 v, int count) {
   return make_uint4(word(v.x, 0), word(v.y, 1), word(v.z, 2), word(v.w, 3));
 }
 
-// GB: blocks of 32 k per scale within a warp's 256 (1, 2, 4, 8); 1 also serves
-// the group sizes that 256 is no multiple of, or no divisor.
+// GB: blocks of 32 k per scale within a tile's 128 (1, 2, 4); 1 also serves the
+// group sizes that 128 is no multiple of, or no divisor.
 // Aligned: rows of weights and tokens start on 16-byte boundaries.
 template <class T, int NT, int GB, bool Aligned>
-__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__ W4Args a) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __grid_constant__ W4Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kGroups = 8 / GB;                        // scales of a row in a warp's tile
-  constexpr int kRegs = GB == 1 ? 2 : 1;                 // ... of which each of four lanes holds this many
+  constexpr int kGroups = 4 / GB;                        // scales of a row in a tile
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
-  const int stage_k = warps_k * kWarpK;
+  const int stage_k = warps_k * kTileK;
   const int m0 = blockIdx.z * 8 * NT, tokens = min(a.tokens - m0, 8 * NT);
   const int x_row = stage_k * 2 + kXPad;
   const int stage_bytes = kWeightBytes + min(a.tokens, 8 * NT) * x_row;
   const int k_first = blockIdx.x * a.slice, k_last = min(a.k, k_first + a.slice);
   const int n_stages = k_last > k_first ? (k_last - k_first + stage_k - 1) / stage_k : 0;
-  const int n0 = (blockIdx.y * a.warps_n + wn) * 16;
+  const int n0 = (blockIdx.y * a.warps_n + wn) * kRows;
   const uint32_t ring = smem_addr(smem);
-  const T* xs = static_cast<const T*>(a.x) + int64_t(m0) * a.x_stride;
 
-  auto fetch = [&](int i) {
-    if (i < n_stages) {
-      const uint32_t stage = ring + (i % kStages) * stage_bytes;
-      // this warp's tile: 16 rows of 128 bytes, the row's 16-byte pieces in an order of its own (piece ^ row)
-      const int k0 = k_first + i * stage_k + wk * kWarpK;
-      const uint32_t dst = stage + warp * kTileBytes;
+  // This lane's copies of its warp's tile, 32 rows of 64 bytes: four rows, 8
+  // apart, one 16-byte piece each.  The sources move on by a stage at a time.
+  const int piece_k = k_first + wk * kTileK + (lane & 3) * 32;
+  const uint8_t* w_src = a.weight + int64_t(min(n0 + (lane >> 2), a.n - 1)) * a.weight_stride + (piece_k >> 1);
+  const int64_t w_step = 8 * a.weight_stride;
+  const int w_rows = a.n - n0 - (lane >> 2);             // rows 8 c below it that there are
+  const uint32_t w_dst = ring + warp * kTileBytes + (lane >> 2) * kPitch + ((lane & 3) ^ (lane >> 3)) * 16;   // piece ^ (row / 2) mod 4
+  int w_left = a.k - piece_k;                            // k from here on
+  // ... and of the tokens' values of the whole stage, 8 at a time
+  const int lg = a.x_shift, x_tokens = kThreads >> lg;   // pieces of a token: 2^lg; tokens that one round of copies serves
+  const int x_piece = threadIdx.x & ((1 << lg) - 1), x_m = threadIdx.x >> lg;
+  const T* x_src = static_cast<const T*>(a.x) + (int64_t(m0) + min(x_m, tokens - 1)) * a.x_stride + k_first + x_piece * 8;
+  const uint32_t x_dst = ring + kWeightBytes + x_m * x_row + x_piece * 16;
+  int x_left = a.k - k_first - x_piece * 8;
+  int next = 0;                                          // the next copies' stage
+
+  auto fetch = [&](bool some) {
+    if (some) {
+      const uint32_t at = next * stage_bytes;
+      const int bytes = min(max((w_left + 1) >> 1, 0), 16);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int row = c * 4 + (lane >> 3), piece = lane & 7;
-        const int k = k0 + piece * 32;
-        const int bytes = n0 + row < a.n ? min(max((a.k - k + 1) >> 1, 0), 16) : 0;
-        const uint8_t* src = a.weight + int64_t(bytes ? n0 + row : 0) * a.weight_stride + (bytes ? k >> 1 : 0);
-        const uint32_t at = dst + row * 128 + ((piece ^ (row & 7)) << 4);
-        if constexpr (Aligned) copy16(at, src, bytes);
-        else sts128(at, load_any(src, bytes));
+        const int n = 8 * c < w_rows ? bytes : 0;
+        const uint8_t* src = n ? w_src + c * w_step : a.weight;
+        if constexpr (Aligned) copy16(w_dst + at + c * 8 * kPitch, src, n);
+        else sts128(w_dst + at + c * 8 * kPitch, load_any(src, n));
       }
-      // the tokens' values of the whole stage, zeros beyond k
-      const int pieces = stage_k / 8;
-      for (int p = threadIdx.x; p < tokens * pieces; p += kThreads) {
-        const int m = p / pieces, piece = p - m * pieces;
-        const int k = k_first + i * stage_k + piece * 8;
-        const int bytes = 2 * min(max(a.k - k, 0), 8);
-        const T* src = xs + m * a.x_stride + (bytes ? k : 0);
-        const uint32_t at = stage + kWeightBytes + m * x_row + piece * 16;
-        if constexpr (Aligned) copy16(at, src, bytes);
-        else sts128(at, keep(load_any(reinterpret_cast<const uint8_t*>(src), bytes), bytes >> 1));
+      const int x_bytes = 2 * min(max(x_left, 0), 8);    // zeros beyond k
+      for (int m = x_m; m < tokens; m += x_tokens) {
+        const T* src = x_bytes ? x_src + (m - x_m) * a.x_stride : static_cast<const T*>(a.x);
+        if constexpr (Aligned) copy16(x_dst + at + (m - x_m) * x_row, src, x_bytes);
+        else sts128(x_dst + at + (m - x_m) * x_row, keep(load_any(reinterpret_cast<const uint8_t*>(src), x_bytes), x_bytes >> 1));
       }
+      w_src += stage_k / 2;
+      x_src += stage_k;
+      w_left -= stage_k;
+      x_left -= stage_k;
+      next = next == kStages - 1 ? 0 : next + 1;
     }
     commit();
   };
 
-  // scales (and zero points) of rows g and g + 8, one stage ahead of their use
-  float scale_next[2][kRegs];
-  uint32_t zero_next[2][kRegs];
+  // Scales and zero points of row `lane`, one stage ahead of their use and as
+  // they are in memory: converting them here would wait for them here.  A
+  // tile's lie side by side, one access where that is aligned.
+  uint32_t scale_next[kGroups], zero_next[kGroups];
+  const int per = a.group / 32;
+  const int64_t scale_row = int64_t(min(n0 + lane, a.n - 1)) * a.groups;
+  const bool side_by_side = kGroups > 1 && per == GB && a.groups % kGroups == 0 && a.vector_scales;
   auto fetch_scales = [&](int i) {
-    const int block0 = (k_first + i * stage_k + wk * kWarpK) / 32, per = a.group / 32;
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int e = 0; e < kRegs; ++e) {
-        const int block = block0 + (GB == 1 ? t + 4 * e : min(t, kGroups - 1) * GB);
-        const int64_t at = int64_t(min(n0 + g + 8 * r, a.n - 1)) * a.groups + min(block / per, a.groups - 1);
-        scale_next[r][e] = a.scales32 ? __ldg(static_cast<const float*>(a.scales) + at)
-                                      : to_float(static_cast<const T*>(a.scales)[at]);
-        zero_next[r][e] = Magic<T>::value | (a.zeros ? uint32_t(__ldg(a.zeros + at) & 15) * 0x10001u : 0x00080008u);
+    const int block0 = (k_first + i * stage_k + wk * kTileK) / 32;
+    if (side_by_side) {
+      const int64_t at = scale_row + min(block0 / GB, a.groups - kGroups);
+      if (a.scales32) {
+        const float* p = static_cast<const float*>(a.scales) + at;
+        if constexpr (kGroups == 4) *reinterpret_cast<uint4*>(scale_next) = __ldg(reinterpret_cast<const uint4*>(p));
+        else if constexpr (kGroups == 2) *reinterpret_cast<uint2*>(scale_next) = __ldg(reinterpret_cast<const uint2*>(p));
+      } else {
+        const T* p = static_cast<const T*>(a.scales) + at;
+        if constexpr (kGroups == 4) *reinterpret_cast<uint2*>(scale_next) = __ldg(reinterpret_cast<const uint2*>(p));
+        else if constexpr (kGroups == 2) scale_next[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
       }
+      if (a.zeros) zero_next[0] = kGroups == 4 ? __ldg(reinterpret_cast<const uint32_t*>(a.zeros + at)) : __ldg(reinterpret_cast<const uint16_t*>(a.zeros + at));
+    } else {
+#pragma unroll
+      for (int e = 0; e < kGroups; ++e) {
+        const int block = block0 + e * GB, group = a.group_shift >= 0 ? block >> a.group_shift : block / per;
+        const int64_t at = scale_row + min(group, a.groups - 1);
+        scale_next[e] = a.scales32 ? __ldg(static_cast<const uint32_t*>(a.scales) + at) : __ldg(static_cast<const uint16_t*>(a.scales) + at);
+        if (a.zeros) zero_next[e] = __ldg(a.zeros + at);
+      }
+    }
+  };
+  auto take_scales = [&](float (&scale)[kGroups], uint32_t (&zero)[kGroups]) {
+#pragma unroll
+    for (int e = 0; e < kGroups; ++e) {
+      const uint16_t half = uint16_t(side_by_side ? scale_next[e / 2] >> (16 * (e & 1)) : scale_next[e]);
+      scale[e] = a.scales32 ? __uint_as_float(scale_next[e]) : to_float(*reinterpret_cast<const T*>(&half));
+      zero[e] = a.zeros ? (side_by_side ? zero_next[0] >> (8 * e) : zero_next[e]) & 15u : 8u;
+    }
   };
 
-  float acc[NT][4] = {};
+  float acc[2][NT][4] = {};
   if (n_stages) fetch_scales(0);
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  for (int i = 0; i < kStages - 1; ++i) fetch(i < n_stages);
   for (int i = 0; i < n_stages; ++i) {
     wait_groups<kStages - 2>();
     __syncthreads();                                     // stage i is there for all; stage i - 1 is read by all
-    fetch(i + kStages - 1);
-    float scale[2][kRegs];
-    uint32_t zero[2][kRegs];
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int e = 0; e < kRegs; ++e) scale[r][e] = scale_next[r][e], zero[r][e] = zero_next[r][e];
+    fetch(i + kStages - 1 < n_stages);
+    float scale[kGroups];
+    uint32_t zero[kGroups];
+    take_scales(scale, zero);
     if (i + 1 < n_stages) fetch_scales(i + 1);
     const uint32_t stage = ring + (i % kStages) * stage_bytes;
-    const uint32_t w_at = stage + warp * kTileBytes + g * 128 + t * 4;
-    const uint32_t x_at = stage + kWeightBytes + wk * (kWarpK * 2) + t * 16;
-    float part[NT][4];
+    const uint32_t w_at = stage + warp * kTileBytes + g * kPitch + (g >> 1) * 16 + t * 4;
+    const uint32_t x_at = stage + kWeightBytes + wk * (kTileK * 2) + t * 16;
+    uint32_t x_of[NT];                                   // columns beyond the tokens repeat the last one: nothing reads their sums
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      if (b % GB == 0) {
+    for (int n = 0; n < NT; ++n) x_of[n] = x_at + min(n * 8 + g, tokens - 1) * x_row;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.0f;
-      }
-      const int from = (lane & ~3) | (GB == 1 ? b & 3 : b / GB);
-      const int e = GB == 1 ? b >> 2 : 0;
-      const uint32_t z0 = __shfl_sync(0xffffffffu, zero[0][e], from), z1 = __shfl_sync(0xffffffffu, zero[1][e], from);
-      uint32_t p0[4], p1[4];
-      unpack<T>(lds32(w_at + ((b ^ g) << 4)), z0, p0);
-      unpack<T>(lds32(w_at + 8 * 128 + ((b ^ g) << 4)), z1, p1);
-      const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+    for (int e = 0; e < kGroups; ++e) {
+      float part[2][NT][4];
+      uint32_t z[4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        // columns beyond the tokens repeat the last one: nothing reads their sums
-        const uint4 x = lds128(x_at + min(n * 8 + g, tokens - 1) * x_row + b * 64);
-        mma<T>(part[n], a0, __byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632));
-        mma<T>(part[n], a1, __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-      }
-      if (b % GB == GB - 1) {
-        const float s0 = __shfl_sync(0xffffffffu, scale[0][e], from), s1 = __shfl_sync(0xffffffffu, scale[1][e], from);
+      for (int r = 0; r < 4; ++r) z[r] = Nibbles<T>::zero(a.zeros ? __shfl_sync(0xffffffffu, zero[e], g + 8 * r) : 8u);
+#pragma unroll
+      for (int b = e * GB; b < (e + 1) * GB; ++b) {
+        uint32_t x[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          acc[n][0] += s0 * part[n][0];
-          acc[n][1] += s0 * part[n][1];
-          acc[n][2] += s1 * part[n][2];
-          acc[n][3] += s1 * part[n][3];
+          const uint4 v = lds128(x_of[n] + b * 64);
+          x[n][0] = __byte_perm(v.x, v.z, 0x5410);
+          x[n][1] = __byte_perm(v.x, v.z, 0x7632);
+          x[n][2] = __byte_perm(v.y, v.w, 0x5410);
+          x[n][3] = __byte_perm(v.y, v.w, 0x7632);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint32_t p0[4], p1[4];
+          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r) * kPitch), z[2 * r], p0);
+          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r + 8) * kPitch), z[2 * r + 1], p1);
+          const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (b == e * GB) mma_first<T>(part[r][n], a0, x[n][0], x[n][1]);
+            else mma<T>(part[r][n], a0, x[n][0], x[n][1]);
+            mma<T>(part[r][n], a1, x[n][2], x[n][3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float s0 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r), s1 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r + 8);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          acc[r][n][0] += s0 * part[r][n][0];
+          acc[r][n][1] += s0 * part[r][n][1];
+          acc[r][n][2] += s1 * part[r][n][2];
+          acc[r][n][3] += s1 * part[r][n][3];
         }
       }
     }
@@ -230,15 +301,17 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
   // sums of the warps along k, then of the cluster's CTAs: [wk][row][token] in shared memory
   constexpr int kCols = 8 * NT;
   float* red = reinterpret_cast<float*>(smem);
-  const int rows = a.warps_n * 16;
+  const int rows = a.warps_n * kRows;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float* at = red + ((wk * rows + wn * 16 + g) * kCols + n * 8 + 2 * t);
-    at[0] = acc[n][0];
-    at[1] = acc[n][1];
-    at[8 * kCols] = acc[n][2];
-    at[8 * kCols + 1] = acc[n][3];
-  }
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float* at = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
+      at[0] = acc[r][n][0];
+      at[1] = acc[r][n][1];
+      at[8 * kCols] = acc[r][n][2];
+      at[8 * kCols + 1] = acc[r][n][3];
+    }
   __syncthreads();
   const int cells = rows * kCols;
   if (warps_k > 1) {
@@ -266,26 +339,30 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------- launch
-std::atomic<int> g_smem[2][2][4][2][kMaxDevices];
+std::atomic<int> g_smem[2][2][3][2][kMaxDevices];
 
 template <class T, int NT, int GB, bool Aligned>
 cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
-  // Rows of a CTA (16 to 128): as many as leave a CTA per SM, but at least 8
+  // Rows of a CTA (32 to 256): as many as leave a CTA per SM, but at least 8
   // per token, so that the tokens' values, read again by every CTA, stay
   // within half of the weights' bytes.  Then the cluster's share of k: enough
-  // CTAs for the SMs, each with at least 4 stages' worth of its warps' k.
+  // CTAs for the SMs, each with at least two stages.
   const int held = a.tokens < 8 * NT ? a.tokens : 8 * NT;
+  auto blocks_of = [&](int w) { return (a.n + kRows * w - 1) / (kRows * w); };
   int warps_n = 8;
-  while (warps_n > 1 && (a.n + 16 * warps_n - 1) / (16 * warps_n) < sms && 16 * (warps_n / 2) >= 8 * held) warps_n /= 2;
-  const int row_blocks = (a.n + 16 * warps_n - 1) / (16 * warps_n), stage_k = kWarps / warps_n * kWarpK;
+  while (warps_n > 1 && blocks_of(warps_n) < sms && kRows * (warps_n / 2) >= 8 * held) warps_n /= 2;
+  const int row_blocks = blocks_of(warps_n), stage_k = kWarps / warps_n * kTileK;
   int ranks = 1;
   while (ranks < 8 && row_blocks * ranks < sms && a.k > 2 * ranks * stage_k) ranks *= 2;
   const int stages = (a.k + stage_k - 1) / stage_k;
   a.warps_n = warps_n;
+  a.x_shift = 31 - __builtin_clz(unsigned(stage_k / 8));
+  const unsigned per = unsigned(a.group / 32);
+  a.group_shift = per & (per - 1) ? -1 : 31 - __builtin_clz(per);
   a.slice = (stages + ranks - 1) / ranks * stage_k;
   const size_t bytes = size_t(kStages) * (kWeightBytes + size_t(held) * (stage_k * 2 + kXPad));
   const auto kernel = w4_kernel<T, NT, GB, Aligned>;
-  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB == 1 ? 0 : GB == 2 ? 1 : GB == 4 ? 2 : 3][Aligned]);
+  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB / 2][Aligned]);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ranks, row_blocks, (a.tokens + 8 * NT - 1) / (8 * NT));
   cfg.blockDim = dim3(kThreads);
@@ -304,8 +381,7 @@ cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
 template <class T, int NT, bool Aligned>
 cudaError_t launch_group(const W4Args& a, int sms, cudaStream_t s) {
   if (a.group == 64) return launch_shape<T, NT, 2, Aligned>(a, sms, s);
-  if (a.group == 128) return launch_shape<T, NT, 4, Aligned>(a, sms, s);
-  if (a.group % 256 == 0) return launch_shape<T, NT, 8, Aligned>(a, sms, s);
+  if (a.group % 128 == 0) return launch_shape<T, NT, 4, Aligned>(a, sms, s);
   return launch_shape<T, NT, 1, Aligned>(a, sms, s);
 }
 
@@ -343,7 +419,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* stream) {
   const int rc = sm_count(&sms);
   if (rc != PM_OK) return rc;
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, 0};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->scales, 16) && aligned(j->zeros, 4), 0, 0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, sms, s) : launch<fp16>(a, sms, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");
