@@ -100,7 +100,7 @@ typedef struct {
   int32_t tokens, n, k, group;
   int32_t dtype, scales_dtype;
   int64_t x_stride;                        /* elements between tokens, >= k */
-  int64_t weight_stride;                   /* bytes between weight rows, >= (k + 1) / 2 */
+  int64_t weight_stride;                   /* bytes between weight rows, >= (k + 1) / 2, at most 2^23 */
   const void* x;
   const uint8_t* weight;
   const void* scales;

@@ -3,18 +3,17 @@
 //   y[m, n] = sum_g s[n, g] sum_{k in g} x[m, k] (q[n, k] - z[n, g]).
 //
 // The weights are read once and bound it.
-//  * A warp owns 32 rows of weights and 128 values of k at a time, 2 KB that
-//    it copies into shared memory asynchronously, four stages deep.  The 8
-//    warps of a CTA stand side by side along n or along k, so a stage is 16 KB
-//    whatever the matrix's shape: enough bytes in flight with two CTAs an SM.
+//  * A warp owns 32 rows of weights and 256 (128) values of k at a time, 4 KB
+//    that it copies into shared memory asynchronously, three stages deep.  The
+//    8 warps of a CTA stand side by side along n or along k, so a stage is 32
+//    KB whatever the matrix's shape: enough bytes in flight with two CTAs an SM.
 //    The tokens' values for a stage are copied beside it, for all warps, and
 //    each serves two tiles of 16 rows in registers: unpacking has to keep up
 //    with the memory on the integer pipe, where every other instruction counts.
-//  * q - z is an integer that 16-bit floats hold exactly: four nibbles are
-//    masked into the mantissas of 128 (bf16) or 1024 (fp16) and the same
-//    number plus z is subtracted.  The matrix instruction multiplies 16 rows
-//    by 8 tokens with exact products and 32-bit sums; the scale enters once a
-//    group, in 32 bits.  So nothing is rounded before the output.
+//  * A nibble is masked into a 16-bit float's mantissa, exactly.  The matrix
+//    instruction multiplies 16 rows by 8 tokens with exact products and 32-bit
+//    sums; the scale enters once a group, in 32 bits.  So nothing is rounded
+//    to 16 bits before the output.
 //  * k is summed in an order that suits the nibbles: a lane's word holds k =
 //    0..7 of its eight, and the pairs (0,4), (1,5), (2,6), (3,7) are the
 //    instruction's neighbours, for the weights and for the tokens alike.
@@ -33,12 +32,25 @@ namespace pm {
 namespace blk {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 256, kStages = 4;
-constexpr int kRows = 32, kTileK = 128;                  // of a warp's tile
-constexpr int kPitch = kTileK / 2;                       // bytes of a tile's row: four pieces, in an order of the row's own
-constexpr int kTileBytes = kRows * kPitch;
-constexpr int kWeightBytes = kWarps * kTileBytes;        // a stage
+constexpr int kWarps = 8, kThreads = 256, kRows = 32;    // rows of a warp's tile
 constexpr int kXPad = 64;                                // bytes after a token's values: neighbours in other banks
+
+// Up to 8 tokens: tiles of 256 k, which halves what a stage costs besides its
+// products; up to 16: of 128 k, as the tokens' values take the room.
+template <int NT>
+struct Tile {
+  static constexpr int kK = NT == 1 ? 256 : 128, kStages = NT == 1 ? 3 : 4;
+  static constexpr int kPitch = kK / 2, kPieces = kPitch / 16;                 // a row, in 16-byte pieces
+  static constexpr int kBytes = kRows * kPitch, kStageBytes = kWarps * kBytes;
+  // Pieces lie in an order of the row's own, so that 8 rows x 4 words meet all 32 banks.
+  static __device__ __forceinline__ int turn(int row) { return kPieces == 8 ? row & 7 : row >> 1 & 3; }
+};
+
+// Bytes of a stage with the values of `tokens` tokens, a multiple of the 128 in which rows take turns.
+template <int NT>
+__host__ __device__ inline int stage_size(int tokens, int stage_k) {
+  return Tile<NT>::kStageBytes + (tokens * (stage_k * 2 + kXPad) + 127) / 128 * 128;
+}
 
 struct W4Args {
   int tokens, n, k, group, groups, scales32;
@@ -55,30 +67,35 @@ struct W4Args {
   int slice;                                             // k of one CTA of the cluster, a multiple of the stage's
 };
 
+constexpr uint32_t kOnes = 0x3f803f80u;                  // two bf16 ones
+
 // (a & b) | c in one instruction.
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// A zero point as the pair that unpacking subtracts, and the pairs
-// (0,4), (1,5), (2,6), (3,7) of a word's nibbles, less the zero point.
+// The pairs (0,4), (1,5), (2,6), (3,7) of a word's nibbles as 16-bit floats.
+// bf16: the mantissa takes a nibble as 128 + q; what is 128 + z too much of
+// every product is taken off a group's sum, where the tokens' sums come from
+// a matrix instruction with ones.  (Subtracting in the pairs costs 8
+// instructions per 512 weights more, and issue slots are what is short.)
+// The offset costs 32-bit sums of 2^5 times the size, 2^-19 of a result that
+// is rounded to 2^-9.
+// fp16: a mantissa holds a nibble as 1024 + q, and four bits further up as
+// 1024 + 16 q; one subtraction and one fused multiply-add bring both to q - z
+// exactly.  The offset would cost 2^-16 here, too near the output's 2^-12.
 template <class T> struct Nibbles;
 template <> struct Nibbles<bf16> {
-  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x43004300u | z * 0x10001u; }   // 128 + z
-  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
-    const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zero);
+  static constexpr bool kOffset = true;
+  static __device__ __forceinline__ uint32_t zero(uint32_t) { return 0; }
+  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t (&p)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
-      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z);
-      p[i] = *reinterpret_cast<const uint32_t*>(&d);
-    }
+    for (int i = 0; i < 4; ++i) p[i] = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
   }
 };
-// fp16's longer mantissa takes a nibble four bits further up as well: 1024 +
-// 16 q, which one fused multiply-add brings to q - z exactly.  One shift a word.
 template <> struct Nibbles<fp16> {
+  static constexpr bool kOffset = false;
   static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | z * 0x10001u; }   // 1024 + z
   static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
     const __half2 z = *reinterpret_cast<const __half2*>(&zero);
@@ -133,37 +150,44 @@ __device__ __forceinline__ uint4 keep(uint4 v, int count) {
   return make_uint4(word(v.x, 0), word(v.y, 1), word(v.z, 2), word(v.w, 3));
 }
 
-// GB: blocks of 32 k per scale within a tile's 128 (1, 2, 4); 1 also serves the
-// group sizes that 128 is no multiple of, or no divisor.
+// GB: blocks of 32 k per scale within a tile (1 to all of them); 1 also serves
+// the group sizes that the tile's k is no multiple of, or no divisor.
 // Aligned: rows of weights and tokens start on 16-byte boundaries.
 template <class T, int NT, int GB, bool Aligned>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __grid_constant__ W4Args a) {
+__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__ W4Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int kGroups = 4 / GB;                        // scales of a row in a tile
+  using L = Tile<NT>;
+  constexpr int kStages = L::kStages, kGroups = L::kK / 32 / GB;               // scales of a row in a tile
+  constexpr int kRowLanes = 32 / L::kPieces, kCopies = kRows / kRowLanes;      // rows that one round of copies takes
+  constexpr bool kOffset = Nibbles<T>::kOffset;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
-  const int stage_k = warps_k * kTileK;
+  const int stage_k = warps_k * L::kK;
   const int m0 = blockIdx.z * 8 * NT, tokens = min(a.tokens - m0, 8 * NT);
   const int x_row = stage_k * 2 + kXPad;
-  const int stage_bytes = kWeightBytes + min(a.tokens, 8 * NT) * x_row;
+  const int stage_bytes = stage_size<NT>(min(a.tokens, 8 * NT), stage_k);
   const int k_first = blockIdx.x * a.slice, k_last = min(a.k, k_first + a.slice);
   const int n_stages = k_last > k_first ? (k_last - k_first + stage_k - 1) / stage_k : 0;
   const int n0 = (blockIdx.y * a.warps_n + wn) * kRows;
   const uint32_t ring = smem_addr(smem);
 
-  // This lane's copies of its warp's tile, 32 rows of 64 bytes: four rows, 8
-  // apart, one 16-byte piece each.  The sources move on by a stage at a time.
-  const int piece_k = k_first + wk * kTileK + (lane & 3) * 32;
-  const uint8_t* w_src = a.weight + int64_t(min(n0 + (lane >> 2), a.n - 1)) * a.weight_stride + (piece_k >> 1);
-  const int64_t w_step = 8 * a.weight_stride;
-  const int w_rows = a.n - n0 - (lane >> 2);             // rows 8 c below it that there are
-  const uint32_t w_dst = ring + warp * kTileBytes + (lane >> 2) * kPitch + ((lane & 3) ^ (lane >> 3)) * 16;   // piece ^ (row / 2) mod 4
+  // This lane's copies of its warp's tile: every kRowLanes-th row, one piece
+  // each.  The sources move on by a stage at a time.
+  const int w_row = lane / L::kPieces, w_piece = lane % L::kPieces;
+  const int piece_k = k_first + wk * L::kK + w_piece * 32;
+  const uint8_t* w_base = a.weight + int64_t(blockIdx.y) * a.warps_n * kRows * a.weight_stride;   // this CTA's rows: offsets of 32 bits
+  uint32_t w_off = uint32_t(wn * kRows + w_row) * uint32_t(a.weight_stride) + uint32_t(piece_k >> 1);
+  const uint32_t w_step = kRowLanes * uint32_t(a.weight_stride);
+  const int w_rows = a.n - n0 - w_row;                   // rows below this one that there are
+  uint32_t w_dst[2];                                     // the place in the ring, by the row's turn
+#pragma unroll
+  for (int c = 0; c < 2; ++c) w_dst[c] = ring + warp * L::kBytes + w_row * L::kPitch + ((w_piece ^ L::turn(w_row + c * kRowLanes)) * 16);
   int w_left = a.k - piece_k;                            // k from here on
   // ... and of the tokens' values of the whole stage, 8 at a time
   const int lg = a.x_shift, x_tokens = kThreads >> lg;   // pieces of a token: 2^lg; tokens that one round of copies serves
   const int x_piece = threadIdx.x & ((1 << lg) - 1), x_m = threadIdx.x >> lg;
   const T* x_src = static_cast<const T*>(a.x) + (int64_t(m0) + min(x_m, tokens - 1)) * a.x_stride + k_first + x_piece * 8;
-  const uint32_t x_dst = ring + kWeightBytes + x_m * x_row + x_piece * 16;
+  const uint32_t x_dst = ring + L::kStageBytes + x_m * x_row + x_piece * 16;
   int x_left = a.k - k_first - x_piece * 8;
   int next = 0;                                          // the next copies' stage
 
@@ -171,12 +195,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
     if (some) {
       const uint32_t at = next * stage_bytes;
       const int bytes = min(max((w_left + 1) >> 1, 0), 16);
+      if (Aligned && __all_sync(0xffffffffu, bytes == 16 && w_rows > (kCopies - 1) * kRowLanes)) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = 8 * c < w_rows ? bytes : 0;
-        const uint8_t* src = n ? w_src + c * w_step : a.weight;
-        if constexpr (Aligned) copy16(w_dst + at + c * 8 * kPitch, src, n);
-        else sts128(w_dst + at + c * 8 * kPitch, load_any(src, n));
+        for (int c = 0; c < kCopies; ++c) copy16(w_dst[c & 1] + at + c * kRowLanes * L::kPitch, w_base + (w_off + c * w_step), 16);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          const int n = kRowLanes * c < w_rows ? bytes : 0;
+          const uint8_t* src = n ? w_base + (w_off + c * w_step) : a.weight;
+          const uint32_t dst = w_dst[c & 1] + at + c * kRowLanes * L::kPitch;
+          if constexpr (Aligned) copy16(dst, src, n);
+          else sts128(dst, load_any(src, n));
+        }
       }
       const int x_bytes = 2 * min(max(x_left, 0), 8);    // zeros beyond k
       for (int m = x_m; m < tokens; m += x_tokens) {
@@ -184,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
         if constexpr (Aligned) copy16(x_dst + at + (m - x_m) * x_row, src, x_bytes);
         else sts128(x_dst + at + (m - x_m) * x_row, keep(load_any(reinterpret_cast<const uint8_t*>(src), x_bytes), x_bytes >> 1));
       }
-      w_src += stage_k / 2;
+      w_off += stage_k / 2;
       x_src += stage_k;
       w_left -= stage_k;
       x_left -= stage_k;
@@ -196,24 +226,32 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
   // Scales and zero points of row `lane`, one stage ahead of their use and as
   // they are in memory: converting them here would wait for them here.  A
   // tile's lie side by side, one access where that is aligned.
+  constexpr int kZeroWords = kGroups > 4 ? 2 : 1;
   uint32_t scale_next[kGroups], zero_next[kGroups];
   const int per = a.group / 32;
   const int64_t scale_row = int64_t(min(n0 + lane, a.n - 1)) * a.groups;
   const bool side_by_side = kGroups > 1 && per == GB && a.groups % kGroups == 0 && a.vector_scales;
   auto fetch_scales = [&](int i) {
-    const int block0 = (k_first + i * stage_k + wk * kTileK) / 32;
+    const int block0 = (k_first + i * stage_k + wk * L::kK) / 32;
     if (side_by_side) {
       const int64_t at = scale_row + min(block0 / GB, a.groups - kGroups);
-      if (a.scales32) {
-        const float* p = static_cast<const float*>(a.scales) + at;
-        if constexpr (kGroups == 4) *reinterpret_cast<uint4*>(scale_next) = __ldg(reinterpret_cast<const uint4*>(p));
-        else if constexpr (kGroups == 2) *reinterpret_cast<uint2*>(scale_next) = __ldg(reinterpret_cast<const uint2*>(p));
-      } else {
-        const T* p = static_cast<const T*>(a.scales) + at;
-        if constexpr (kGroups == 4) *reinterpret_cast<uint2*>(scale_next) = __ldg(reinterpret_cast<const uint2*>(p));
-        else if constexpr (kGroups == 2) scale_next[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-      }
-      if (a.zeros) zero_next[0] = kGroups == 4 ? __ldg(reinterpret_cast<const uint32_t*>(a.zeros + at)) : __ldg(reinterpret_cast<const uint16_t*>(a.zeros + at));
+      auto words = [&](const void* from, uint32_t* to, int bytes) {
+        if (bytes == 32) {
+          *reinterpret_cast<uint4*>(to) = __ldg(static_cast<const uint4*>(from));
+          *reinterpret_cast<uint4*>(to + 4) = __ldg(static_cast<const uint4*>(from) + 1);
+        } else if (bytes == 16) {
+          *reinterpret_cast<uint4*>(to) = __ldg(static_cast<const uint4*>(from));
+        } else if (bytes == 8) {
+          *reinterpret_cast<uint2*>(to) = __ldg(static_cast<const uint2*>(from));
+        } else if (bytes == 4) {
+          *to = __ldg(static_cast<const uint32_t*>(from));
+        } else {
+          *to = __ldg(static_cast<const uint16_t*>(from));
+        }
+      };
+      if (a.scales32) words(static_cast<const float*>(a.scales) + at, scale_next, 4 * kGroups);
+      else words(static_cast<const T*>(a.scales) + at, scale_next, 2 * kGroups);
+      if (a.zeros) words(a.zeros + at, zero_next, kGroups);
     } else {
 #pragma unroll
       for (int e = 0; e < kGroups; ++e) {
@@ -224,39 +262,40 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
       }
     }
   };
-  auto take_scales = [&](float (&scale)[kGroups], uint32_t (&zero)[kGroups]) {
-#pragma unroll
-    for (int e = 0; e < kGroups; ++e) {
-      const uint16_t half = uint16_t(side_by_side ? scale_next[e / 2] >> (16 * (e & 1)) : scale_next[e]);
-      scale[e] = a.scales32 ? __uint_as_float(scale_next[e]) : to_float(*reinterpret_cast<const T*>(&half));
-      zero[e] = a.zeros ? (side_by_side ? zero_next[0] >> (8 * e) : zero_next[e]) & 15u : 8u;
-    }
-  };
 
   float acc[2][NT][4] = {};
   if (n_stages) fetch_scales(0);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i < n_stages);
+  int stage_now = 0;
   for (int i = 0; i < n_stages; ++i) {
     wait_groups<kStages - 2>();
     __syncthreads();                                     // stage i is there for all; stage i - 1 is read by all
     fetch(i + kStages - 1 < n_stages);
     float scale[kGroups];
     uint32_t zero[kGroups];
-    take_scales(scale, zero);
+#pragma unroll
+    for (int e = 0; e < kGroups; ++e) {
+      const uint16_t half = uint16_t(side_by_side ? scale_next[e / 2] >> (16 * (e & 1)) : scale_next[e]);
+      scale[e] = a.scales32 ? __uint_as_float(scale_next[e]) : to_float(*reinterpret_cast<const T*>(&half));
+      zero[e] = a.zeros ? (side_by_side ? zero_next[kZeroWords == 2 ? e / 4 : 0] >> (8 * (e & 3)) : zero_next[e]) & 15u : 8u;
+    }
     if (i + 1 < n_stages) fetch_scales(i + 1);
-    const uint32_t stage = ring + (i % kStages) * stage_bytes;
-    const uint32_t w_at = stage + warp * kTileBytes + g * kPitch + (g >> 1) * 16 + t * 4;
-    const uint32_t x_at = stage + kWeightBytes + wk * (kTileK * 2) + t * 16;
+    const uint32_t stage = ring + stage_now * stage_bytes;
+    stage_now = stage_now == kStages - 1 ? 0 : stage_now + 1;
+    const uint32_t w_at = stage + warp * L::kBytes + g * L::kPitch + L::turn(g) * 16 + t * 4;
+    const uint32_t x_at = stage + L::kStageBytes + wk * (L::kK * 2) + t * 16;
     uint32_t x_of[NT];                                   // columns beyond the tokens repeat the last one: nothing reads their sums
 #pragma unroll
     for (int n = 0; n < NT; ++n) x_of[n] = x_at + min(n * 8 + g, tokens - 1) * x_row;
 #pragma unroll
     for (int e = 0; e < kGroups; ++e) {
-      float part[2][NT][4];
+      float part[2][NT][4], x_sum[NT][4];
       uint32_t z[4];
+      if constexpr (!kOffset) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) z[r] = Nibbles<T>::zero(a.zeros ? __shfl_sync(0xffffffffu, zero[e], g + 8 * r) : 8u);
+        for (int r = 0; r < 4; ++r) z[r] = Nibbles<T>::zero(a.zeros ? __shfl_sync(0xffffffffu, zero[e], g + 8 * r) : 8u);
+      }
 #pragma unroll
       for (int b = e * GB; b < (e + 1) * GB; ++b) {
         uint32_t x[NT][4];
@@ -267,12 +306,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
           x[n][1] = __byte_perm(v.x, v.z, 0x7632);
           x[n][2] = __byte_perm(v.y, v.w, 0x5410);
           x[n][3] = __byte_perm(v.y, v.w, 0x7632);
+          if constexpr (kOffset) {
+            const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
+            if (b == e * GB) mma_first<T>(x_sum[n], ones, x[n][0], x[n][1]);
+            else mma<T>(x_sum[n], ones, x[n][0], x[n][1]);
+            mma<T>(x_sum[n], ones, x[n][2], x[n][3]);
+          }
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           uint32_t p0[4], p1[4];
-          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r) * kPitch), z[2 * r], p0);
-          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r + 8) * kPitch), z[2 * r + 1], p1);
+          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r) * L::kPitch), z[2 * r], p0);
+          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r + 8) * L::kPitch), z[2 * r + 1], p1);
           const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -282,11 +327,23 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
           }
         }
       }
+      const float offset = 128.0f + float(zero[e]);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float s0 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r), s1 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r + 8);
+        float o0 = 136.0f, o1 = 136.0f;
+        if (kOffset && a.zeros) {
+          o0 = __shfl_sync(0xffffffffu, offset, g + 16 * r);
+          o1 = __shfl_sync(0xffffffffu, offset, g + 16 * r + 8);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          if constexpr (kOffset) {
+            part[r][n][0] -= o0 * x_sum[n][0];
+            part[r][n][1] -= o0 * x_sum[n][1];
+            part[r][n][2] -= o1 * x_sum[n][2];
+            part[r][n][3] -= o1 * x_sum[n][3];
+          }
           acc[r][n][0] += s0 * part[r][n][0];
           acc[r][n][1] += s0 * part[r][n][1];
           acc[r][n][2] += s1 * part[r][n][2];
@@ -339,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) w4_kernel(const __g
 }
 
 // ---------------------------------------------------------------- launch
-std::atomic<int> g_smem[2][2][3][2][kMaxDevices];
+std::atomic<int> g_smem[2][2][4][2][kMaxDevices];
 
 template <class T, int NT, int GB, bool Aligned>
 cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
@@ -351,7 +408,7 @@ cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
   auto blocks_of = [&](int w) { return (a.n + kRows * w - 1) / (kRows * w); };
   int warps_n = 8;
   while (warps_n > 1 && blocks_of(warps_n) < sms && kRows * (warps_n / 2) >= 8 * held) warps_n /= 2;
-  const int row_blocks = blocks_of(warps_n), stage_k = kWarps / warps_n * kTileK;
+  const int row_blocks = blocks_of(warps_n), stage_k = kWarps / warps_n * Tile<NT>::kK;
   int ranks = 1;
   while (ranks < 8 && row_blocks * ranks < sms && a.k > 2 * ranks * stage_k) ranks *= 2;
   const int stages = (a.k + stage_k - 1) / stage_k;
@@ -360,9 +417,9 @@ cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
   const unsigned per = unsigned(a.group / 32);
   a.group_shift = per & (per - 1) ? -1 : 31 - __builtin_clz(per);
   a.slice = (stages + ranks - 1) / ranks * stage_k;
-  const size_t bytes = size_t(kStages) * (kWeightBytes + size_t(held) * (stage_k * 2 + kXPad));
+  const size_t bytes = size_t(Tile<NT>::kStages) * stage_size<NT>(held, stage_k);
   const auto kernel = w4_kernel<T, NT, GB, Aligned>;
-  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB / 2][Aligned]);
+  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB == 8 ? 3 : GB / 2][Aligned]);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ranks, row_blocks, (a.tokens + 8 * NT - 1) / (8 * NT));
   cfg.blockDim = dim3(kThreads);
@@ -381,7 +438,8 @@ cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
 template <class T, int NT, bool Aligned>
 cudaError_t launch_group(const W4Args& a, int sms, cudaStream_t s) {
   if (a.group == 64) return launch_shape<T, NT, 2, Aligned>(a, sms, s);
-  if (a.group % 128 == 0) return launch_shape<T, NT, 4, Aligned>(a, sms, s);
+  if (NT == 1 && a.group % 256 == 0) return launch_shape<T, NT, NT == 1 ? 8 : 4, Aligned>(a, sms, s);
+  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_shape<T, NT, 4, Aligned>(a, sms, s);
   return launch_shape<T, NT, 1, Aligned>(a, sms, s);
 }
 
@@ -410,6 +468,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* stream) {
   if (j->scales_dtype != j->dtype && j->scales_dtype != PM_DT_F32)
     return fail(PM_E_INVALID, "%s: scales are of the activations' type or 32-bit floats", who);
   if (!j->tokens) return PM_OK;
+  if (j->weight_stride > (1 << 23)) return fail(PM_E_LIMIT, "%s: weight rows lie at most 2^23 bytes apart", who);
   if (j->x_stride < j->k || j->weight_stride < (int64_t(j->k) + 1) / 2)
     return fail(PM_E_INVALID, "%s: strides must be at least a row", who);
   if (!j->x || !j->weight || !j->scales || !j->y) return fail(PM_E_INVALID, "%s: NULL buffer", who);
