@@ -108,7 +108,9 @@ typedef struct {
   void* y;
 } pm_matvec_w4;
 
-int pm_matvec_w4_device(const pm_matvec_w4* job, void* stream);
+/* Scratch for the current device: 0 where the product needs none (scratch may then be NULL). */
+size_t pm_matvec_w4_scratch_bytes(int32_t tokens, int32_t n, int32_t k);
+int pm_matvec_w4_device(const pm_matvec_w4* job, void* scratch, size_t scratch_bytes, void* stream);
 
 /*
  * Attention of one query token per sequence over a paged cache:

@@ -61,13 +61,13 @@ struct W4Args {
   const uint8_t* zeros;
   void* y;
   int warps_n;                                           // warps along n; the others along k
-  int vector_scales;                                     // scales 16-byte, zeros 4-byte aligned
+  int vector_scales;                                     // scales 16-byte, zeros 8-byte aligned
   int x_shift;                                           // log2 of the 16-byte pieces of a token in a stage
   int group_shift;                                       // log2 of the 32-k blocks of a group, -1: no power of two
-  int slice;                                             // k of one CTA of the cluster, a multiple of the stage's
+  int stages;                                            // stages of a row block: its k over the stage's
+  int ranks;                                             // CTAs of a cluster, which share each row block's stages
+  float* part;                                           // ranks == 1: sums of cut row blocks, [2 * CTAs][rows][8 NT]
 };
-
-constexpr uint32_t kOnes = 0x3f803f80u;                  // two bf16 ones
 
 // (a & b) | c in one instruction.
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
@@ -75,27 +75,37 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-// The pairs (0,4), (1,5), (2,6), (3,7) of a word's nibbles as 16-bit floats.
-// bf16: the mantissa takes a nibble as 128 + q; what is 128 + z too much of
-// every product is taken off a group's sum, where the tokens' sums come from
-// a matrix instruction with ones.  (Subtracting in the pairs costs 8
-// instructions per 512 weights more, and issue slots are what is short.)
-// The offset costs 32-bit sums of 2^5 times the size, 2^-19 of a result that
-// is rounded to 2^-9.
-// fp16: a mantissa holds a nibble as 1024 + q, and four bits further up as
-// 1024 + 16 q; one subtraction and one fused multiply-add bring both to q - z
-// exactly.  The offset would cost 2^-16 here, too near the output's 2^-12.
+// The pairs (0,4), (1,5), (2,6), (3,7) of a word's nibbles, less the zero
+// point and over kScale, as exact 16-bit floats.  Integer instructions are
+// what the kernel has least of, so two nibble positions of a half are taken
+// where they lie and one shift brings the other two: five and four fused
+// multiply-adds a word.
+// bf16: the bits of an integer below 256 are that integer times 2^-133 (the
+// subnormals and the first binade are one even grid), so a nibble at bit 0 or
+// bit 4 is n 2^-133 or n 2^-129, and n - z over 64 is one fma away.
+// fp16: a nibble at bit 0 of 1024's mantissa is 1024 + n, at bit 4 1024 + 16 n.
 template <class T> struct Nibbles;
 template <> struct Nibbles<bf16> {
-  static constexpr bool kOffset = true;
-  static __device__ __forceinline__ uint32_t zero(uint32_t) { return 0; }
-  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t (&p)[4]) {
+  static constexpr float kScale = 64.0f;
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) {
+    const __nv_bfloat162 v = __float2bfloat162_rn(float(z) * -0.015625f);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
+    const uint32_t low = 0x7f007f00u, high = 0x7d007d00u;                      // 2^127, 2^123
+    const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zero);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t u = i ? w >> 8 : w, a = u & 0x000f000fu, b = u & 0x00f000f0u;
+      const __nv_bfloat162 x = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&low), z);
+      const __nv_bfloat162 y = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&high), z);
+      p[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+      p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    }
   }
 };
 template <> struct Nibbles<fp16> {
-  static constexpr bool kOffset = false;
+  static constexpr float kScale = 1.0f;
   static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | z * 0x10001u; }   // 1024 + z
   static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
     const __half2 z = *reinterpret_cast<const __half2*>(&zero);
@@ -113,16 +123,6 @@ template <> struct Nibbles<fp16> {
     }
   }
 };
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -159,40 +159,58 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
   using L = Tile<NT>;
   constexpr int kStages = L::kStages, kGroups = L::kK / 32 / GB;               // scales of a row in a tile
   constexpr int kRowLanes = 32 / L::kPieces, kCopies = kRows / kRowLanes;      // rows that one round of copies takes
-  constexpr bool kOffset = Nibbles<T>::kOffset;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
   const int stage_k = warps_k * L::kK;
   const int m0 = blockIdx.z * 8 * NT, tokens = min(a.tokens - m0, 8 * NT);
   const int x_row = stage_k * 2 + kXPad;
   const int stage_bytes = stage_size<NT>(min(a.tokens, 8 * NT), stage_k);
-  const int k_first = blockIdx.x * a.slice, k_last = min(a.k, k_first + a.slice);
-  const int n_stages = k_last > k_first ? (k_last - k_first + stage_k - 1) / stage_k : 0;
-  const int n0 = (blockIdx.y * a.warps_n + wn) * kRows;
+  // The work is a line of stages, row block after row block.  A cluster's CTAs
+  // each take a share of one block's; without clusters the line is cut into
+  // equal runs.
+  const int rank = blockIdx.x % a.ranks, rows = a.warps_n * kRows;
+  int64_t first;
+  int count;                                             // stages of this CTA: [first, first + count) of the line
+  if (a.ranks > 1) {
+    const int from = a.stages * rank / a.ranks;
+    first = int64_t(blockIdx.x / a.ranks) * a.stages + from;
+    count = a.stages * (rank + 1) / a.ranks - from;
+  } else {
+    const int64_t total = int64_t((a.n + rows - 1) / rows) * a.stages;
+    first = total * blockIdx.x / gridDim.x;
+    count = int(total * (blockIdx.x + 1) / gridDim.x - first);
+  }
+  int block = int(first / a.stages), s = int(first - int64_t(block) * a.stages), s_first = s;
   const uint32_t ring = smem_addr(smem);
 
   // This lane's copies of its warp's tile: every kRowLanes-th row, one piece
-  // each.  The sources move on by a stage at a time.
+  // each, and of the tokens' values of the whole stage, 8 at a time.  The
+  // sources move on by a stage at a time, and to the next row block's start.
   const int w_row = lane / L::kPieces, w_piece = lane % L::kPieces;
-  const int piece_k = k_first + wk * L::kK + w_piece * 32;
-  const uint8_t* w_base = a.weight + int64_t(blockIdx.y) * a.warps_n * kRows * a.weight_stride;   // this CTA's rows: offsets of 32 bits
-  uint32_t w_off = uint32_t(wn * kRows + w_row) * uint32_t(a.weight_stride) + uint32_t(piece_k >> 1);
   const uint32_t w_step = kRowLanes * uint32_t(a.weight_stride);
-  const int w_rows = a.n - n0 - w_row;                   // rows below this one that there are
   uint32_t w_dst[2];                                     // the place in the ring, by the row's turn
 #pragma unroll
   for (int c = 0; c < 2; ++c) w_dst[c] = ring + warp * L::kBytes + w_row * L::kPitch + ((w_piece ^ L::turn(w_row + c * kRowLanes)) * 16);
-  int w_left = a.k - piece_k;                            // k from here on
-  // ... and of the tokens' values of the whole stage, 8 at a time
   const int lg = a.x_shift, x_tokens = kThreads >> lg;   // pieces of a token: 2^lg; tokens that one round of copies serves
   const int x_piece = threadIdx.x & ((1 << lg) - 1), x_m = threadIdx.x >> lg;
-  const T* x_src = static_cast<const T*>(a.x) + (int64_t(m0) + min(x_m, tokens - 1)) * a.x_stride + k_first + x_piece * 8;
   const uint32_t x_dst = ring + L::kStageBytes + x_m * x_row + x_piece * 16;
-  int x_left = a.k - k_first - x_piece * 8;
-  int next = 0;                                          // the next copies' stage
-
-  auto fetch = [&](bool some) {
-    if (some) {
+  const uint8_t* w_base;                                 // the row block's first row: offsets of 32 bits from there
+  const T* x_src;
+  uint32_t w_off;
+  int w_rows, w_left, x_left;                            // rows below this one and k from here on that there are
+  int next_block = block, next_s = s, next_left = count, next = 0;             // the next copies' stage, and its place in the ring
+  auto start_at = [&](int at_block, int at_s) {
+    const int k = at_s * stage_k, piece_k = k + wk * L::kK + w_piece * 32;
+    w_base = a.weight + int64_t(at_block) * rows * a.weight_stride;
+    w_off = uint32_t(wn * kRows + w_row) * uint32_t(a.weight_stride) + uint32_t(piece_k >> 1);
+    w_rows = min(a.n - at_block * rows, rows) - wn * kRows - w_row;
+    w_left = a.k - piece_k;
+    x_src = static_cast<const T*>(a.x) + (int64_t(m0) + min(x_m, tokens - 1)) * a.x_stride + k + x_piece * 8;
+    x_left = a.k - k - x_piece * 8;
+  };
+  start_at(block, s);
+  auto fetch = [&]() {
+    if (next_left > 0) {
       const uint32_t at = next * stage_bytes;
       const int bytes = min(max((w_left + 1) >> 1, 0), 16);
       if (Aligned && __all_sync(0xffffffffu, bytes == 16 && w_rows > (kCopies - 1) * kRowLanes)) {
@@ -219,6 +237,11 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
       w_left -= stage_k;
       x_left -= stage_k;
       next = next == kStages - 1 ? 0 : next + 1;
+      --next_left;
+      if (++next_s == a.stages) {
+        next_s = 0;
+        start_at(++next_block, 0);
+      }
     }
     commit();
   };
@@ -229,10 +252,10 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
   constexpr int kZeroWords = kGroups > 4 ? 2 : 1;
   uint32_t scale_next[kGroups], zero_next[kGroups];
   const int per = a.group / 32;
-  const int64_t scale_row = int64_t(min(n0 + lane, a.n - 1)) * a.groups;
   const bool side_by_side = kGroups > 1 && per == GB && a.groups % kGroups == 0 && a.vector_scales;
-  auto fetch_scales = [&](int i) {
-    const int block0 = (k_first + i * stage_k + wk * L::kK) / 32;
+  auto fetch_scales = [&](int at_block, int at_s) {
+    const int block0 = (at_s * stage_k + wk * L::kK) / 32;
+    const int64_t scale_row = int64_t(min(at_block * rows + wn * kRows + lane, a.n - 1)) * a.groups;
     if (side_by_side) {
       const int64_t at = scale_row + min(block0 / GB, a.groups - kGroups);
       auto words = [&](const void* from, uint32_t* to, int bytes) {
@@ -263,61 +286,59 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
     }
   };
 
+  constexpr int kCols = 8 * NT;
   float acc[2][NT][4] = {};
-  if (n_stages) fetch_scales(0);
+  if (count) fetch_scales(block, s);
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i < n_stages);
+  for (int i = 0; i < kStages - 1; ++i) fetch();
   int stage_now = 0;
-  for (int i = 0; i < n_stages; ++i) {
+  float* red = nullptr;                                  // [wk][row][token], in the place of a row block's last stage
+  for (int left = count; left > 0; --left) {
     wait_groups<kStages - 2>();
-    __syncthreads();                                     // stage i is there for all; stage i - 1 is read by all
-    fetch(i + kStages - 1 < n_stages);
+    __syncthreads();                                     // this stage is there for all; the one before is read by all
+    fetch();
     float scale[kGroups];
     uint32_t zero[kGroups];
 #pragma unroll
     for (int e = 0; e < kGroups; ++e) {
       const uint16_t half = uint16_t(side_by_side ? scale_next[e / 2] >> (16 * (e & 1)) : scale_next[e]);
-      scale[e] = a.scales32 ? __uint_as_float(scale_next[e]) : to_float(*reinterpret_cast<const T*>(&half));
+      scale[e] = Nibbles<T>::kScale * (a.scales32 ? __uint_as_float(scale_next[e]) : to_float(*reinterpret_cast<const T*>(&half)));
       zero[e] = a.zeros ? (side_by_side ? zero_next[kZeroWords == 2 ? e / 4 : 0] >> (8 * (e & 3)) : zero_next[e]) & 15u : 8u;
     }
-    if (i + 1 < n_stages) fetch_scales(i + 1);
-    const uint32_t stage = ring + stage_now * stage_bytes;
+    const bool last = s + 1 == a.stages || left == 1;    // of this CTA in this row block
+    if (left > 1) fetch_scales(s + 1 == a.stages ? block + 1 : block, s + 1 == a.stages ? 0 : s + 1);
+    const int stage = stage_now * stage_bytes;
     stage_now = stage_now == kStages - 1 ? 0 : stage_now + 1;
-    const uint32_t w_at = stage + warp * L::kBytes + g * L::kPitch + L::turn(g) * 16 + t * 4;
-    const uint32_t x_at = stage + L::kStageBytes + wk * (L::kK * 2) + t * 16;
-    uint32_t x_of[NT];                                   // columns beyond the tokens repeat the last one: nothing reads their sums
+    const int w_at = stage + warp * L::kBytes + g * L::kPitch + L::turn(g) * 16 + t * 4;
+    const int x_at = stage + L::kStageBytes + wk * (L::kK * 2) + t * 16;
+    int x_of[NT];                                        // columns beyond the tokens repeat the last one: nothing reads their sums
 #pragma unroll
     for (int n = 0; n < NT; ++n) x_of[n] = x_at + min(n * 8 + g, tokens - 1) * x_row;
 #pragma unroll
     for (int e = 0; e < kGroups; ++e) {
-      float part[2][NT][4], x_sum[NT][4];
+      float part[2][NT][4];
       uint32_t z[4];
-      if constexpr (!kOffset) {
+      {
+        const uint32_t own = Nibbles<T>::zero(zero[e]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = Nibbles<T>::zero(a.zeros ? __shfl_sync(0xffffffffu, zero[e], g + 8 * r) : 8u);
+        for (int r = 0; r < 4; ++r) z[r] = a.zeros ? __shfl_sync(0xffffffffu, own, g + 8 * r) : own;
       }
 #pragma unroll
       for (int b = e * GB; b < (e + 1) * GB; ++b) {
         uint32_t x[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint4 v = lds128(x_of[n] + b * 64);
+          const uint4 v = *reinterpret_cast<const uint4*>(smem + x_of[n] + b * 64);
           x[n][0] = __byte_perm(v.x, v.z, 0x5410);
           x[n][1] = __byte_perm(v.x, v.z, 0x7632);
           x[n][2] = __byte_perm(v.y, v.w, 0x5410);
           x[n][3] = __byte_perm(v.y, v.w, 0x7632);
-          if constexpr (kOffset) {
-            const uint32_t ones[4] = {kOnes, kOnes, kOnes, kOnes};
-            if (b == e * GB) mma_first<T>(x_sum[n], ones, x[n][0], x[n][1]);
-            else mma<T>(x_sum[n], ones, x[n][0], x[n][1]);
-            mma<T>(x_sum[n], ones, x[n][2], x[n][3]);
-          }
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           uint32_t p0[4], p1[4];
-          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r) * L::kPitch), z[2 * r], p0);
-          Nibbles<T>::unpack(lds32((w_at ^ (b * 16)) + (16 * r + 8) * L::kPitch), z[2 * r + 1], p1);
+          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(smem + (w_at ^ (b * 16)) + (16 * r) * L::kPitch), z[2 * r], p0);
+          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(smem + (w_at ^ (b * 16)) + (16 * r + 8) * L::kPitch), z[2 * r + 1], p1);
           const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -327,23 +348,11 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
           }
         }
       }
-      const float offset = 128.0f + float(zero[e]);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float s0 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r), s1 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r + 8);
-        float o0 = 136.0f, o1 = 136.0f;
-        if (kOffset && a.zeros) {
-          o0 = __shfl_sync(0xffffffffu, offset, g + 16 * r);
-          o1 = __shfl_sync(0xffffffffu, offset, g + 16 * r + 8);
-        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if constexpr (kOffset) {
-            part[r][n][0] -= o0 * x_sum[n][0];
-            part[r][n][1] -= o0 * x_sum[n][1];
-            part[r][n][2] -= o1 * x_sum[n][2];
-            part[r][n][3] -= o1 * x_sum[n][3];
-          }
           acc[r][n][0] += s0 * part[r][n][0];
           acc[r][n][1] += s0 * part[r][n][1];
           acc[r][n][2] += s1 * part[r][n][2];
@@ -351,103 +360,180 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
         }
       }
     }
+    ++s;
+    if (!last) continue;
+
+    // the row block's sums over the warps along k, where nobody reads the stage any more; the copies that go there next
+    // are issued after the next barrier
+    __syncthreads();
+    red = reinterpret_cast<float*>(smem + stage);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* at = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
+        at[0] = acc[r][n][0];
+        at[1] = acc[r][n][1];
+        at[8 * kCols] = acc[r][n][2];
+        at[8 * kCols + 1] = acc[r][n][3];
+        acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.0f;
+      }
+    __syncthreads();
+    if (a.ranks == 1) {
+      // a whole block to y, a cut one to scratch: at most one that this run ends within and one that it starts within
+      const bool whole = s_first == 0 && s == a.stages;
+      float* part = a.part + ((int64_t(blockIdx.z) * gridDim.x + blockIdx.x) * 2 + (s_first == 0 ? 1 : 0)) * rows * kCols;
+      T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + int64_t(block) * rows;
+      const int there = min(rows, a.n - block * rows);
+      for (int c = threadIdx.x; c < rows * tokens; c += kThreads) {
+        const int m = c / rows, row = c - m * rows;
+        float v = 0.0f;
+        for (int w = 0; w < warps_k; ++w) v += red[(w * rows + row) * kCols + m];
+        if (!whole) part[m * rows + row] = v;
+        else if (row < there) y[int64_t(m) * a.n + row] = from_float<T>(v);
+      }
+      if (s == a.stages) s = 0, ++block;
+      s_first = s;
+    }
   }
   wait_groups<0>();
-  __syncthreads();
+  if (a.ranks == 1) return;
 
-  // sums of the warps along k, then of the cluster's CTAs: [wk][row][token] in shared memory
-  constexpr int kCols = 8 * NT;
-  float* red = reinterpret_cast<float*>(smem);
-  const int rows = a.warps_n * kRows;
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* at = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
-      at[0] = acc[r][n][0];
-      at[1] = acc[r][n][1];
-      at[8 * kCols] = acc[r][n][2];
-      at[8 * kCols + 1] = acc[r][n][3];
-    }
-  __syncthreads();
-  const int cells = rows * kCols;
-  if (warps_k > 1) {
-    for (int c = threadIdx.x; c < cells; c += kThreads) {
-      float v = red[c];
-      for (int w = 1; w < warps_k; ++w) v += red[w * cells + c];
-      red[c] = v;
-    }
+  // a cluster's sums, through distributed shared memory, in the ranks' order
+  float* sums = reinterpret_cast<float*>(smem);          // one place for all ranks; red's own, or where no copy is under way
+  for (int c = threadIdx.x; c < rows * kCols; c += kThreads) {
+    float v = red[c];
+    for (int w = 1; w < warps_k; ++w) v += red[w * rows * kCols + c];
+    sums[c] = v;
   }
-  const int ranks = gridDim.x;
-  if (ranks > 1) cg::this_cluster().sync();
-  else __syncthreads();
-  if (blockIdx.x == 0) {
-    T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n;
-    const int first = blockIdx.y * rows;
+  cg::this_cluster().sync();
+  if (rank == 0) {
+    const int64_t first = int64_t(blockIdx.x / a.ranks) * rows;
+    T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + first;
     for (int c = threadIdx.x; c < rows * tokens; c += kThreads) {
       const int m = c / rows, row = c - m * rows;
       if (first + row >= a.n) continue;
-      float v = red[row * kCols + m];
-      for (int r = 1; r < ranks; ++r) v += cg::this_cluster().map_shared_rank(red, r)[row * kCols + m];
-      y[int64_t(m) * a.n + first + row] = from_float<T>(v);
+      float v = sums[row * kCols + m];
+      for (int r = 1; r < a.ranks; ++r) v += cg::this_cluster().map_shared_rank(sums, r)[row * kCols + m];
+      y[int64_t(m) * a.n + row] = from_float<T>(v);
     }
   }
-  if (ranks > 1) cg::this_cluster().sync();              // a CTA's sums stay until rank 0 has them
+  cg::this_cluster().sync();                             // a CTA's sums stay until rank 0 has them
+}
+
+// Joins the pieces of the row blocks that runs were cut within: CTA c takes
+// the block in which run c starts, unless an earlier run starts there too.
+template <class T, int NT>
+__global__ void __launch_bounds__(kThreads) w4_join_kernel(const __grid_constant__ W4Args a, int runs) {
+  constexpr int kCols = 8 * NT;
+  const int rows = a.warps_n * kRows, c = blockIdx.x + 1;
+  const int64_t total = int64_t((a.n + rows - 1) / rows) * a.stages;
+  auto start = [&](int run) { return total * run / runs; };
+  const int64_t block = start(c) / a.stages;
+  asm volatile("griddepcontrol.wait;" ::: "memory");    // in every CTA: this kernel's end has to mean the first one's
+  if (start(c) % a.stages == 0 || (start(c - 1) > block * a.stages)) return;
+  const int m0 = blockIdx.z * kCols, tokens = min(a.tokens - m0, kCols);
+  const float* part = a.part + int64_t(blockIdx.z) * runs * 2 * rows * kCols;
+  T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + block * rows;
+  const int there = int(min(int64_t(rows), a.n - block * rows));
+  const int i = blockIdx.y * kThreads + threadIdx.x, m = i / rows, row = i - m * rows;
+  if (m >= tokens || row >= there) return;
+  float v = __ldcg(part + (int64_t(c - 1) * 2 + 1) * rows * kCols + i);
+  int last = c;
+  while (last < runs && start(last) < (block + 1) * a.stages) ++last;
+#pragma unroll 4
+  for (int k = c; k < last; ++k) v += __ldcg(part + int64_t(k) * 2 * rows * kCols + i);
+  y[int64_t(m) * a.n + row] = from_float<T>(v);
 }
 
 // ---------------------------------------------------------------- launch
 std::atomic<int> g_smem[2][2][4][2][kMaxDevices];
 
+// How a product is shared out.
+struct Plan {
+  int nt, warps_n, ranks, stages;
+  int64_t ctas;
+  bool cut;                              // runs end within row blocks: scratch and the second kernel
+};
+
+template <int NT>
+Plan plan_for(int tokens, int n, int k, int sms) {
+  constexpr int kK = Tile<NT>::kK;
+  Plan p{NT, 8, 1, 0, 0, false};
+  const int held = tokens < 8 * NT ? tokens : 8 * NT;
+  // Rows of a CTA (32 to 256): few, as long as the warps along k all have some
+  // and there are 8 rows per token: the tokens' values, read again by every
+  // CTA, then stay within half of the weights' bytes.
+  while (p.warps_n > 1 && kRows * (p.warps_n / 2) >= 8 * held && kWarps / (p.warps_n / 2) * kK < k + kK) p.warps_n /= 2;
+  const int rows = kRows * p.warps_n, stage_k = kWarps / p.warps_n * kK;
+  const int64_t blocks = (int64_t(n) + rows - 1) / rows;
+  p.stages = (k + stage_k - 1) / stage_k;
+  const int64_t slots = 2 * int64_t(sms);                // CTAs resident at once
+  if (blocks * p.stages >= 4 * slots) {
+    // enough for every CTA to have four stages or more: equal runs
+    p.ctas = slots;
+    p.cut = blocks * p.stages % slots != 0 || blocks * p.stages / slots % p.stages != 0;
+  } else {
+    // a cluster for each row block, as long as the SMs hold more and every CTA has a stage
+    while (p.ranks < 8 && blocks * p.ranks * 2 <= slots && p.ranks * 2 <= p.stages) p.ranks *= 2;
+    p.ctas = p.ranks > 1 ? blocks * p.ranks : blocks;
+  }
+  return p;
+}
+Plan plan_of(int tokens, int n, int k, int sms) { return tokens <= 8 ? plan_for<1>(tokens, n, k, sms) : plan_for<2>(tokens, n, k, sms); }
+size_t plan_scratch(const Plan& p, int tokens) {
+  return p.cut ? size_t((tokens + 8 * p.nt - 1) / (8 * p.nt)) * p.ctas * 2 * (kRows * p.warps_n) * (8 * p.nt) * sizeof(float) : 0;
+}
+
 template <class T, int NT, int GB, bool Aligned>
-cudaError_t launch_shape(W4Args a, int sms, cudaStream_t s) {
-  // Rows of a CTA (32 to 256): as many as leave a CTA per SM, but at least 8
-  // per token, so that the tokens' values, read again by every CTA, stay
-  // within half of the weights' bytes.  Then the cluster's share of k: enough
-  // CTAs for the SMs, each with at least two stages.
-  const int held = a.tokens < 8 * NT ? a.tokens : 8 * NT;
-  auto blocks_of = [&](int w) { return (a.n + kRows * w - 1) / (kRows * w); };
-  int warps_n = 8;
-  while (warps_n > 1 && blocks_of(warps_n) < sms && kRows * (warps_n / 2) >= 8 * held) warps_n /= 2;
-  const int row_blocks = blocks_of(warps_n), stage_k = kWarps / warps_n * Tile<NT>::kK;
-  int ranks = 1;
-  while (ranks < 8 && row_blocks * ranks < sms && a.k > 2 * ranks * stage_k) ranks *= 2;
-  const int stages = (a.k + stage_k - 1) / stage_k;
-  a.warps_n = warps_n;
+cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
+  const int held = a.tokens < 8 * NT ? a.tokens : 8 * NT, stage_k = kWarps / p.warps_n * Tile<NT>::kK;
+  a.warps_n = p.warps_n;
+  a.stages = p.stages;
+  a.ranks = p.ranks;
   a.x_shift = 31 - __builtin_clz(unsigned(stage_k / 8));
   const unsigned per = unsigned(a.group / 32);
   a.group_shift = per & (per - 1) ? -1 : 31 - __builtin_clz(per);
-  a.slice = (stages + ranks - 1) / ranks * stage_k;
   const size_t bytes = size_t(Tile<NT>::kStages) * stage_size<NT>(held, stage_k);
   const auto kernel = w4_kernel<T, NT, GB, Aligned>;
   ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB == 8 ? 3 : GB / 2][Aligned]);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ranks, row_blocks, (a.tokens + 8 * NT - 1) / (8 * NT));
+  cfg.gridDim = dim3(unsigned(p.ctas), 1, (a.tokens + 8 * NT - 1) / (8 * NT));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  if (p.ranks > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess || !p.cut) return e;
+  cfg.gridDim.x = unsigned(p.ctas - 1);
+  cfg.gridDim.y = unsigned((kRows * p.warps_n * held + kThreads - 1) / kThreads);
+  cfg.dynamicSmemBytes = 0;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, w4_join_kernel<T, NT>, a, int(p.ctas));
 }
 
 template <class T, int NT, bool Aligned>
-cudaError_t launch_group(const W4Args& a, int sms, cudaStream_t s) {
-  if (a.group == 64) return launch_shape<T, NT, 2, Aligned>(a, sms, s);
-  if (NT == 1 && a.group % 256 == 0) return launch_shape<T, NT, NT == 1 ? 8 : 4, Aligned>(a, sms, s);
-  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_shape<T, NT, 4, Aligned>(a, sms, s);
-  return launch_shape<T, NT, 1, Aligned>(a, sms, s);
+cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
+  if (a.group == 64) return launch_shape<T, NT, 2, Aligned>(a, p, s);
+  if (NT == 1 && a.group % 256 == 0) return launch_shape<T, NT, NT == 1 ? 8 : 4, Aligned>(a, p, s);
+  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_shape<T, NT, 4, Aligned>(a, p, s);
+  return launch_shape<T, NT, 1, Aligned>(a, p, s);
 }
 
 template <class T>
-cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
+cudaError_t launch(const W4Args& a, const Plan& p, cudaStream_t s) {
   const bool aligned_rows = aligned(a.weight, 16) && a.weight_stride % 16 == 0 && aligned(a.x, 16) && (a.x_stride % 8 == 0 || a.tokens == 1);
-  if (a.tokens <= 8) return aligned_rows ? launch_group<T, 1, true>(a, sms, s) : launch_group<T, 1, false>(a, sms, s);
-  return aligned_rows ? launch_group<T, 2, true>(a, sms, s) : launch_group<T, 2, false>(a, sms, s);
+  if (a.tokens <= 8) return aligned_rows ? launch_group<T, 1, true>(a, p, s) : launch_group<T, 1, false>(a, p, s);
+  return aligned_rows ? launch_group<T, 2, true>(a, p, s) : launch_group<T, 2, false>(a, p, s);
 }
 
 }  // namespace
@@ -457,7 +543,13 @@ cudaError_t launch(const W4Args& a, int sms, cudaStream_t s) {
 using namespace pm;
 using namespace pm::blk;
 
-extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* stream) {
+extern "C" size_t pm_matvec_w4_scratch_bytes(int32_t tokens, int32_t n, int32_t k) {
+  int sms = 0;
+  if (tokens < 1 || n < 1 || k < 1 || tokens > (1 << 16) || n > (1 << 24) || k > (1 << 24) || sm_count(&sms) != PM_OK) return 0;
+  return plan_scratch(plan_of(tokens, n, k, sms), tokens);
+}
+
+extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t scratch_bytes, void* stream) {
   const char* who = "pm_matvec_w4_device";
   if (!j) return fail(PM_E_INVALID, "%s: NULL job", who);
   if (j->tokens < 0 || j->n < 1 || j->k < 1) return fail(PM_E_INVALID, "%s: tokens must be >= 0, n and k >= 1", who);
@@ -477,9 +569,13 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* stream) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc != PM_OK) return rc;
+  const Plan plan = plan_of(j->tokens, j->n, j->k, sms);
+  const size_t need = plan_scratch(plan, j->tokens);
+  if (need && (!scratch || !aligned(scratch, 256) || scratch_bytes < need))
+    return fail(PM_E_INVALID, "%s: needs %zu bytes of scratch, 256-byte aligned", who, need);
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->scales, 16) && aligned(j->zeros, 4), 0, 0, 0};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->scales, 16) && aligned(j->zeros, 8), 0, 0, 0, 0, static_cast<float*>(scratch)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, sms, s) : launch<fp16>(a, sms, s);
+  const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, plan, s) : launch<fp16>(a, plan, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");
 }

@@ -284,7 +284,10 @@ PyObject* matvec_w4(PyObject* const* args) {
     j.scales = scales.const_data_ptr();
     j.zeros = zeros.defined() ? static_cast<const uint8_t*>(zeros.const_data_ptr()) : nullptr;
     j.y = y.mutable_data_ptr();
-    check(pm_matvec_w4_device(&j, stream_of(place.device)), "pm_matvec_w4_device");
+    const size_t need = pm_matvec_w4_scratch_bytes(j.tokens, j.n, j.k);
+    at::Tensor scratch;
+    if (need) scratch = scratch_of(need, x);
+    check(pm_matvec_w4_device(&j, need ? scratch.mutable_data_ptr() : nullptr, need, stream_of(place.device)), "pm_matvec_w4_device");
   }
   return wrap(y);
 }

@@ -179,7 +179,9 @@ def library():
     lib.pm_block_norm_backward_scratch_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int32]
     lib.pm_block_norm_backward_scratch_bytes.restype = C.c_size_t
     lib.pm_block_norm_backward_device.argtypes = [_p, _p, _p, C.c_size_t, _p]
-    lib.pm_matvec_w4_device.argtypes = [_p, _p]
+    lib.pm_matvec_w4_scratch_bytes.argtypes = [C.c_int32] * 3
+    lib.pm_matvec_w4_scratch_bytes.restype = C.c_size_t
+    lib.pm_matvec_w4_device.argtypes = [_p, _p, C.c_size_t, _p]
     lib.pm_paged_attention_scratch_bytes.argtypes = [C.c_int32] * 4
     lib.pm_paged_attention_scratch_bytes.restype = C.c_size_t
     lib.pm_paged_attention_device.argtypes = [_p, _p, C.c_size_t, _p]

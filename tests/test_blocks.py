@@ -188,10 +188,10 @@ def c_w4(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(tokens=-1), INVALID), (dict(n=0), INVALID), (dict(k=0), INVALID), (dict(tokens=1 << 17), LIMIT),
     (dict(n=1 << 25), LIMIT), (dict(k=1 << 25), LIMIT), (dict(group=0), INVALID), (dict(group=40), INVALID),
-    (dict(dtype=0), INVALID), (dict(scales_dtype=2), INVALID), (dict(x_stride=63), INVALID), (dict(weight_stride=31), INVALID),
+    (dict(dtype=0), INVALID), (dict(scales_dtype=2), INVALID), (dict(x_stride=63), INVALID), (dict(weight_stride=31), INVALID), (dict(weight_stride=(1 << 23) + 16), LIMIT),
     (dict(x=None), INVALID), (dict(y=None), INVALID), (dict(scales=A + 1), INVALID), (dict(x=A + 1), INVALID)])
 def test_c_matvec_refusals(kw, code):
-    assert K.library().pm_matvec_w4_device(C.byref(c_w4(**kw)), None) == code
+    assert K.library().pm_matvec_w4_device(C.byref(c_w4(**kw)), None, 0, None) == code
     assert "pm_matvec_w4_device" in N.last_error()
 
 
@@ -229,7 +229,7 @@ def test_c_attention_scratch():
 def test_empty_calls_need_no_device():
     lib = K.library()
     assert lib.pm_block_norm_device(C.byref(c_norm(rows=0)), None) == 0
-    assert lib.pm_matvec_w4_device(C.byref(c_w4(tokens=0)), None) == 0
+    assert lib.pm_matvec_w4_device(C.byref(c_w4(tokens=0)), None, 0, None) == 0
     assert lib.pm_paged_attention_device(C.byref(c_attention(batch=0)), None, 0, None) == 0
 
 
