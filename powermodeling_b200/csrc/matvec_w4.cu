@@ -3,13 +3,14 @@
 //   y[m, n] = sum_g s[n, g] sum_{k in g} x[m, k] (q[n, k] - z[n, g]).
 //
 // The weights are read once and bound it.
-//  * A warp owns 32 rows of weights and 256 (128) values of k at a time, 4 KB
-//    that it copies into shared memory asynchronously, three stages deep.  The
-//    8 warps of a CTA stand side by side along n or along k, so a stage is 32
-//    KB whatever the matrix's shape: enough bytes in flight with two CTAs an SM.
-//    The tokens' values for a stage are copied beside it, for all warps, and
-//    each serves two tiles of 16 rows in registers: unpacking has to keep up
-//    with the memory on the integer pipe, where every other instruction counts.
+//  * A warp owns 32 rows of weights and 256 (128) values of k at a time, a
+//    tile of 4 KB.  8 such warps stand side by side along n or along k, so a
+//    stage is 32 KB whatever the matrix's shape: with three stages and two
+//    CTAs an SM enough bytes are in flight.  A ninth warp fills the stages by
+//    tensor copies, the tokens' values beside the weights (rows that start at
+//    any byte: four warps that shift words into place), so the others do
+//    nothing but unpack and multiply: issue slots, not bytes, are short.
+//  * Each token pair serves two tiles of 16 rows in registers.
 //  * A nibble is masked into a 16-bit float's mantissa, exactly.  The matrix
 //    instruction multiplies 16 rows by 8 tokens with exact products and 32-bit
 //    sums; the scale enters once a group, in 32 bits.  So nothing is rounded
@@ -23,6 +24,9 @@
 //  * Few rows: the CTAs of a cluster share k and add their sums through
 //    distributed shared memory, in rank order, so results do not vary.
 #include <cooperative_groups.h>
+#include <cuda.h>
+
+#include <cmath>
 
 #include "blocks.cuh"
 
@@ -32,8 +36,8 @@ namespace pm {
 namespace blk {
 namespace {
 
-constexpr int kWarps = 8, kThreads = 256, kRows = 32;    // rows of a warp's tile
-constexpr int kXPad = 64;                                // bytes after a token's values: neighbours in other banks
+constexpr int kWarps = 8, kRows = 32;                    // warps that multiply; rows of a warp's tile
+constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait; a result that it poisons is NaN
 
 // Up to 8 tokens: tiles of 256 k, which halves what a stage costs besides its
 // products; up to 16: of 128 k, as the tokens' values take the room.
@@ -46,10 +50,11 @@ struct Tile {
   static __device__ __forceinline__ int turn(int row) { return kPieces == 8 ? row & 7 : row >> 1 & 3; }
 };
 
-// Bytes of a stage with the values of `tokens` tokens, a multiple of the 128 in which rows take turns.
+// Bytes of a stage with the values of `tokens` tokens, a multiple of the
+// swizzle's 1 KB: per warp along k its weights, then per warp along k its tokens' values.
 template <int NT>
-__host__ __device__ inline int stage_size(int tokens, int stage_k) {
-  return Tile<NT>::kStageBytes + (tokens * (stage_k * 2 + kXPad) + 127) / 128 * 128;
+__host__ __device__ inline int stage_size(int tokens, int warps_k) {
+  return Tile<NT>::kStageBytes + (warps_k * tokens * Tile<NT>::kK * 2 + 1023) / 1024 * 1024;
 }
 
 struct W4Args {
@@ -62,7 +67,6 @@ struct W4Args {
   void* y;
   int warps_n;                                           // warps along n; the others along k
   int vector_scales;                                     // scales 16-byte, zeros 8-byte aligned
-  int x_shift;                                           // log2 of the 16-byte pieces of a token in a stage
   int group_shift;                                       // log2 of the 32-k blocks of a group, -1: no power of two
   int stages;                                            // stages of a row block: its k over the stage's
   int ranks;                                             // CTAs of a cluster, which share each row block's stages
@@ -150,102 +154,133 @@ __device__ __forceinline__ uint4 keep(uint4 v, int count) {
   return make_uint4(word(v.x, 0), word(v.y, 1), word(v.z, 2), word(v.w, 3));
 }
 
+__device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// False when the wait runs out.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+  if (barrier_try(bar, parity)) return true;
+  const uint64_t deadline = nanoseconds() + kWaitNs;
+  while (!barrier_try(bar, parity))
+    if (nanoseconds() > deadline) return false;
+  return true;
+}
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void multipliers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
 // GB: blocks of 32 k per scale within a tile (1 to all of them); 1 also serves
 // the group sizes that the tile's k is no multiple of, or no divisor.
-// Aligned: rows of weights and tokens start on 16-byte boundaries.
-template <class T, int NT, int GB, bool Aligned>
-__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__ W4Args a) {
-  extern __shared__ __align__(128) uint8_t smem[];
+// Copies: rows of weights and tokens start on 16-byte boundaries, and one lane
+// of one warp copies boxes; else four warps copy words.
+constexpr int kBoxThreads = 32, kWordThreads = 128;
+template <class T, int NT, int GB, bool Boxes>
+__global__ void __launch_bounds__(32 * kWarps + (Boxes ? kBoxThreads : kWordThreads), Boxes ? 2 : 1)
+w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+  extern __shared__ uint8_t smem_raw[];
   using L = Tile<NT>;
-  constexpr int kStages = L::kStages, kGroups = L::kK / 32 / GB;               // scales of a row in a tile
-  constexpr int kRowLanes = 32 / L::kPieces, kCopies = kRows / kRowLanes;      // rows that one round of copies takes
+  constexpr int kStages = L::kStages, kGroups = L::kK / 32 / GB, kCols = 8 * NT;
+  __shared__ __align__(8) uint64_t bars[2 * kStages];    // a stage is full; it is read
+  uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
-  const int stage_k = warps_k * L::kK;
-  const int m0 = blockIdx.z * 8 * NT, tokens = min(a.tokens - m0, 8 * NT);
-  const int x_row = stage_k * 2 + kXPad;
-  const int stage_bytes = stage_size<NT>(min(a.tokens, 8 * NT), stage_k);
+  const int stage_k = warps_k * L::kK, rows = a.warps_n * kRows;
+  const int m0 = blockIdx.z * kCols, held = min(a.tokens, kCols), tokens = min(a.tokens - m0, kCols);
+  const int stage_bytes = stage_size<NT>(held, warps_k);
   // The work is a line of stages, row block after row block.  A cluster's CTAs
   // each take a share of one block's; without clusters the line is cut into
   // equal runs.
-  const int rank = blockIdx.x % a.ranks, rows = a.warps_n * kRows;
+  const int rank = blockIdx.x % a.ranks;
   int64_t first;
   int count;                                             // stages of this CTA: [first, first + count) of the line
   if (a.ranks > 1) {
-    const int from = a.stages * rank / a.ranks;
+    const int from = int(int64_t(a.stages) * rank / a.ranks);
     first = int64_t(blockIdx.x / a.ranks) * a.stages + from;
-    count = a.stages * (rank + 1) / a.ranks - from;
+    count = int(int64_t(a.stages) * (rank + 1) / a.ranks) - from;
   } else {
     const int64_t total = int64_t((a.n + rows - 1) / rows) * a.stages;
     first = total * blockIdx.x / gridDim.x;
     count = int(total * (blockIdx.x + 1) / gridDim.x - first);
   }
-  int block = int(first / a.stages), s = int(first - int64_t(block) * a.stages), s_first = s;
-  const uint32_t ring = smem_addr(smem);
+  int block = int(first / a.stages), s = int(first - int64_t(block) * a.stages);
+  const uint32_t ring = smem_addr(smem), full = smem_addr(bars), read = full + 8 * kStages;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      barrier_init(full + 8 * i, Boxes ? 1 : kWordThreads);
+      barrier_init(read + 8 * i, kWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
 
-  // This lane's copies of its warp's tile: every kRowLanes-th row, one piece
-  // each, and of the tokens' values of the whole stage, 8 at a time.  The
-  // sources move on by a stage at a time, and to the next row block's start.
-  const int w_row = lane / L::kPieces, w_piece = lane % L::kPieces;
-  const uint32_t w_step = kRowLanes * uint32_t(a.weight_stride);
-  uint32_t w_dst[2];                                     // the place in the ring, by the row's turn
-#pragma unroll
-  for (int c = 0; c < 2; ++c) w_dst[c] = ring + warp * L::kBytes + w_row * L::kPitch + ((w_piece ^ L::turn(w_row + c * kRowLanes)) * 16);
-  const int lg = a.x_shift, x_tokens = kThreads >> lg;   // pieces of a token: 2^lg; tokens that one round of copies serves
-  const int x_piece = threadIdx.x & ((1 << lg) - 1), x_m = threadIdx.x >> lg;
-  const uint32_t x_dst = ring + L::kStageBytes + x_m * x_row + x_piece * 16;
-  const uint8_t* w_base;                                 // the row block's first row: offsets of 32 bits from there
-  const T* x_src;
-  uint32_t w_off;
-  int w_rows, w_left, x_left;                            // rows below this one and k from here on that there are
-  int next_block = block, next_s = s, next_left = count, next = 0;             // the next copies' stage, and its place in the ring
-  auto start_at = [&](int at_block, int at_s) {
-    const int k = at_s * stage_k, piece_k = k + wk * L::kK + w_piece * 32;
-    w_base = a.weight + int64_t(at_block) * rows * a.weight_stride;
-    w_off = uint32_t(wn * kRows + w_row) * uint32_t(a.weight_stride) + uint32_t(piece_k >> 1);
-    w_rows = min(a.n - at_block * rows, rows) - wn * kRows - w_row;
-    w_left = a.k - piece_k;
-    x_src = static_cast<const T*>(a.x) + (int64_t(m0) + min(x_m, tokens - 1)) * a.x_stride + k + x_piece * 8;
-    x_left = a.k - k - x_piece * 8;
-  };
-  start_at(block, s);
-  auto fetch = [&]() {
-    if (next_left > 0) {
-      const uint32_t at = next * stage_bytes;
-      const int bytes = min(max((w_left + 1) >> 1, 0), 16);
-      if (Aligned && __all_sync(0xffffffffu, bytes == 16 && w_rows > (kCopies - 1) * kRowLanes)) {
-#pragma unroll
-        for (int c = 0; c < kCopies; ++c) copy16(w_dst[c & 1] + at + c * kRowLanes * L::kPitch, w_base + (w_off + c * w_step), 16);
-      } else {
-#pragma unroll
-        for (int c = 0; c < kCopies; ++c) {
-          const int n = kRowLanes * c < w_rows ? bytes : 0;
-          const uint8_t* src = n ? w_base + (w_off + c * w_step) : a.weight;
-          const uint32_t dst = w_dst[c & 1] + at + c * kRowLanes * L::kPitch;
-          if constexpr (Aligned) copy16(dst, src, n);
-          else sts128(dst, load_any(src, n));
+  if (warp >= kWarps) {
+    // ------------------------------------------------ the copies
+    const int me = threadIdx.x - 32 * kWarps;
+    bool ok = true;
+    for (int i = 0; i < count && ok; ++i) {
+      const int place = i % kStages;
+      const uint32_t stage = ring + place * stage_bytes, bar = full + 8 * place;
+      const int k0 = s * stage_k;
+      if (Boxes ? me == 0 : true) {
+        if (i >= kStages) ok = barrier_wait(read + 8 * place, (i / kStages - 1) & 1);
+        if (!ok) break;
+        if constexpr (Boxes) {
+          barrier_expect(bar, L::kStageBytes + warps_k * held * L::kK * 2);
+          for (int w = 0; w < warps_k; ++w) {
+            copy_box(stage + w * rows * L::kPitch, &map_w, (k0 + w * L::kK) / 2, block * rows, bar);
+            copy_box(stage + L::kStageBytes + w * held * L::kK * 2, &map_x, k0 + w * L::kK, m0, bar);
+          }
+        } else {
+          constexpr int kPieces = L::kStageBytes / 16 / kWordThreads;          // of a thread
+#pragma unroll 4
+          for (int c = 0; c < kPieces; ++c) {
+            const int p = c * kWordThreads + me, tile = p / (kRows * L::kPieces), row = p / L::kPieces % kRows, piece = p % L::kPieces;
+            const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * L::kK + piece * 32;
+            const int bytes = n < a.n ? min(max((a.k - k + 1) >> 1, 0), 16) : 0;
+            const uint8_t* src = a.weight + (bytes ? int64_t(n) * a.weight_stride + (k >> 1) : 0);
+            sts128(stage + tile * L::kBytes + row * L::kPitch + ((piece ^ L::turn(row)) * 16), load_any(src, bytes));
+          }
+          for (int p = me; p < warps_k * tokens * (L::kK / 8); p += kWordThreads) {
+            const int piece = p % (L::kK / 8), m = p / (L::kK / 8) % tokens, w = p / (L::kK / 8) / tokens;
+            const int k = k0 + w * L::kK + piece * 8, left = min(max(a.k - k, 0), 8);
+            const T* src = static_cast<const T*>(a.x) + (left ? int64_t(m0 + m) * a.x_stride + k : 0);
+            sts128(stage + L::kStageBytes + ((w * held + m) * (L::kK / 8) + piece) * 16,
+                   keep(load_any(reinterpret_cast<const uint8_t*>(src), 2 * left), left));
+          }
+          barrier_arrive(bar);
         }
       }
-      const int x_bytes = 2 * min(max(x_left, 0), 8);    // zeros beyond k
-      for (int m = x_m; m < tokens; m += x_tokens) {
-        const T* src = x_bytes ? x_src + (m - x_m) * a.x_stride : static_cast<const T*>(a.x);
-        if constexpr (Aligned) copy16(x_dst + at + (m - x_m) * x_row, src, x_bytes);
-        else sts128(x_dst + at + (m - x_m) * x_row, keep(load_any(reinterpret_cast<const uint8_t*>(src), x_bytes), x_bytes >> 1));
-      }
-      w_off += stage_k / 2;
-      x_src += stage_k;
-      w_left -= stage_k;
-      x_left -= stage_k;
-      next = next == kStages - 1 ? 0 : next + 1;
-      --next_left;
-      if (++next_s == a.stages) {
-        next_s = 0;
-        start_at(++next_block, 0);
-      }
+      if (++s == a.stages) s = 0, ++block;
     }
-    commit();
-  };
+    if (Boxes && me == 0 && !ok)                         // copies under way land before the CTA goes
+      for (int i = 0; i < kStages; ++i) barrier_wait(full + 8 * i, 0), barrier_wait(full + 8 * i, 1);
+    if (a.ranks > 1) {
+      cg::this_cluster().sync();
+      cg::this_cluster().sync();
+    }
+    return;
+  }
 
+  // -------------------------------------------------- the products
   // Scales and zero points of row `lane`, one stage ahead of their use and as
   // they are in memory: converting them here would wait for them here.  A
   // tile's lie side by side, one access where that is aligned.
@@ -278,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
     } else {
 #pragma unroll
       for (int e = 0; e < kGroups; ++e) {
-        const int block = block0 + e * GB, group = a.group_shift >= 0 ? block >> a.group_shift : block / per;
+        const int at_k = block0 + e * GB, group = a.group_shift >= 0 ? at_k >> a.group_shift : at_k / per;
         const int64_t at = scale_row + min(group, a.groups - 1);
         scale_next[e] = a.scales32 ? __ldg(static_cast<const uint32_t*>(a.scales) + at) : __ldg(static_cast<const uint16_t*>(a.scales) + at);
         if (a.zeros) zero_next[e] = __ldg(a.zeros + at);
@@ -286,17 +321,19 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
     }
   };
 
-  constexpr int kCols = 8 * NT;
   float acc[2][NT][4] = {};
-  if (count) fetch_scales(block, s);
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch();
-  int stage_now = 0;
+  bool ok = true;
+  int s_first = s, place = 0;
+  uint32_t parity = 0;
   float* red = nullptr;                                  // [wk][row][token], in the place of a row block's last stage
+  // this lane's words of its tile (rows g + 8 r), and its tokens' values; columns beyond the tokens repeat the last one:
+  // nothing reads their sums
+  const int w_lane = warp * L::kBytes + g * L::kPitch + L::turn(g) * 16 + t * 4;
+  int x_lane[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) x_lane[n] = L::kStageBytes + (wk * held + min(n * 8 + g, tokens - 1)) * (L::kK * 2) + t * 16;
+  if (count) fetch_scales(block, s);
   for (int left = count; left > 0; --left) {
-    wait_groups<kStages - 2>();
-    __syncthreads();                                     // this stage is there for all; the one before is read by all
-    fetch();
     float scale[kGroups];
     uint32_t zero[kGroups];
 #pragma unroll
@@ -307,13 +344,9 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
     }
     const bool last = s + 1 == a.stages || left == 1;    // of this CTA in this row block
     if (left > 1) fetch_scales(s + 1 == a.stages ? block + 1 : block, s + 1 == a.stages ? 0 : s + 1);
-    const int stage = stage_now * stage_bytes;
-    stage_now = stage_now == kStages - 1 ? 0 : stage_now + 1;
-    const int w_at = stage + warp * L::kBytes + g * L::kPitch + L::turn(g) * 16 + t * 4;
-    const int x_at = stage + L::kStageBytes + wk * (L::kK * 2) + t * 16;
-    int x_of[NT];                                        // columns beyond the tokens repeat the last one: nothing reads their sums
-#pragma unroll
-    for (int n = 0; n < NT; ++n) x_of[n] = x_at + min(n * 8 + g, tokens - 1) * x_row;
+    ok = ok && barrier_wait(full + 8 * place, parity);
+    const int stage = place * stage_bytes;
+    const int w_at = stage + w_lane;
 #pragma unroll
     for (int e = 0; e < kGroups; ++e) {
       float part[2][NT][4];
@@ -328,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
         uint32_t x[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint4 v = *reinterpret_cast<const uint4*>(smem + x_of[n] + b * 64);
+          const uint4 v = *reinterpret_cast<const uint4*>(smem + stage + x_lane[n] + b * 64);
           x[n][0] = __byte_perm(v.x, v.z, 0x5410);
           x[n][1] = __byte_perm(v.x, v.z, 0x7632);
           x[n][2] = __byte_perm(v.y, v.w, 0x5410);
@@ -337,8 +370,9 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           uint32_t p0[4], p1[4];
-          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(smem + (w_at ^ (b * 16)) + (16 * r) * L::kPitch), z[2 * r], p0);
-          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(smem + (w_at ^ (b * 16)) + (16 * r + 8) * L::kPitch), z[2 * r + 1], p1);
+          const uint8_t* at = smem + (w_at ^ (b * 16)) + 16 * r * L::kPitch;
+          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(at), z[2 * r], p0);
+          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(at + 8 * L::kPitch), z[2 * r + 1], p1);
           const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -361,58 +395,60 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
       }
     }
     ++s;
-    if (!last) continue;
-
-    // the row block's sums over the warps along k, where nobody reads the stage any more; the copies that go there next
-    // are issued after the next barrier
-    __syncthreads();
-    red = reinterpret_cast<float*>(smem + stage);
+    if (last) {
+      // the row block's sums over the warps along k, where nobody reads the stage any more
+      multipliers_sync();
+      red = reinterpret_cast<float*>(smem + stage);
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float* at = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
-        at[0] = acc[r][n][0];
-        at[1] = acc[r][n][1];
-        at[8 * kCols] = acc[r][n][2];
-        at[8 * kCols + 1] = acc[r][n][3];
-        acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.0f;
+        for (int n = 0; n < NT; ++n) {
+          float* at = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
+          at[0] = ok ? acc[r][n][0] : NAN;
+          at[1] = ok ? acc[r][n][1] : NAN;
+          at[8 * kCols] = ok ? acc[r][n][2] : NAN;
+          at[8 * kCols + 1] = ok ? acc[r][n][3] : NAN;
+          acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.0f;
+        }
+      multipliers_sync();
+      if (a.ranks == 1) {
+        // a whole block to y, a cut one to scratch: at most one that this run ends within and one that it starts within
+        const bool whole = s_first == 0 && s == a.stages;
+        float* part = a.part + ((int64_t(blockIdx.z) * gridDim.x + blockIdx.x) * 2 + (s_first == 0 ? 1 : 0)) * rows * kCols;
+        T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + int64_t(block) * rows;
+        const int there = min(rows, a.n - block * rows);
+        for (int c = threadIdx.x; c < rows * tokens; c += 32 * kWarps) {
+          const int m = c / rows, row = c - m * rows;
+          float v = 0.0f;
+          for (int w = 0; w < warps_k; ++w) v += red[(w * rows + row) * kCols + m];
+          if (!whole) part[m * rows + row] = v;
+          else if (row < there) y[int64_t(m) * a.n + row] = from_float<T>(v);
+        }
       }
-    __syncthreads();
-    if (a.ranks == 1) {
-      // a whole block to y, a cut one to scratch: at most one that this run ends within and one that it starts within
-      const bool whole = s_first == 0 && s == a.stages;
-      float* part = a.part + ((int64_t(blockIdx.z) * gridDim.x + blockIdx.x) * 2 + (s_first == 0 ? 1 : 0)) * rows * kCols;
-      T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + int64_t(block) * rows;
-      const int there = min(rows, a.n - block * rows);
-      for (int c = threadIdx.x; c < rows * tokens; c += kThreads) {
-        const int m = c / rows, row = c - m * rows;
-        float v = 0.0f;
-        for (int w = 0; w < warps_k; ++w) v += red[(w * rows + row) * kCols + m];
-        if (!whole) part[m * rows + row] = v;
-        else if (row < there) y[int64_t(m) * a.n + row] = from_float<T>(v);
-      }
+      asm volatile("fence.proxy.async;" ::: "memory");   // these writes come before the copies that go there next
       if (s == a.stages) s = 0, ++block;
       s_first = s;
     }
+    __syncwarp();
+    if (lane == 0) barrier_arrive(read + 8 * place);
+    if (++place == kStages) place = 0, parity ^= 1;
   }
-  wait_groups<0>();
   if (a.ranks == 1) return;
 
   // a cluster's sums, through distributed shared memory, in the ranks' order
   float* sums = reinterpret_cast<float*>(smem);          // one place for all ranks; red's own, or where no copy is under way
-  for (int c = threadIdx.x; c < rows * kCols; c += kThreads) {
+  for (int c = threadIdx.x; c < rows * kCols; c += 32 * kWarps) {
     float v = red[c];
     for (int w = 1; w < warps_k; ++w) v += red[w * rows * kCols + c];
     sums[c] = v;
   }
   cg::this_cluster().sync();
   if (rank == 0) {
-    const int64_t first = int64_t(blockIdx.x / a.ranks) * rows;
-    T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + first;
-    for (int c = threadIdx.x; c < rows * tokens; c += kThreads) {
+    const int64_t first_row = int64_t(blockIdx.x / a.ranks) * rows;
+    T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + first_row;
+    for (int c = threadIdx.x; c < rows * tokens; c += 32 * kWarps) {
       const int m = c / rows, row = c - m * rows;
-      if (first + row >= a.n) continue;
+      if (first_row + row >= a.n) continue;
       float v = sums[row * kCols + m];
       for (int r = 1; r < a.ranks; ++r) v += cg::this_cluster().map_shared_rank(sums, r)[row * kCols + m];
       y[int64_t(m) * a.n + row] = from_float<T>(v);
@@ -423,8 +459,9 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const __grid_constant__
 
 // Joins the pieces of the row blocks that runs were cut within: CTA c takes
 // the block in which run c starts, unless an earlier run starts there too.
+constexpr int kJoinThreads = 256;
 template <class T, int NT>
-__global__ void __launch_bounds__(kThreads) w4_join_kernel(const __grid_constant__ W4Args a, int runs) {
+__global__ void __launch_bounds__(kJoinThreads) w4_join_kernel(const __grid_constant__ W4Args a, int runs) {
   constexpr int kCols = 8 * NT;
   const int rows = a.warps_n * kRows, c = blockIdx.x + 1;
   const int64_t total = int64_t((a.n + rows - 1) / rows) * a.stages;
@@ -436,7 +473,7 @@ __global__ void __launch_bounds__(kThreads) w4_join_kernel(const __grid_constant
   const float* part = a.part + int64_t(blockIdx.z) * runs * 2 * rows * kCols;
   T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + block * rows;
   const int there = int(min(int64_t(rows), a.n - block * rows));
-  const int i = blockIdx.y * kThreads + threadIdx.x, m = i / rows, row = i - m * rows;
+  const int i = blockIdx.y * kJoinThreads + threadIdx.x, m = i / rows, row = i - m * rows;
   if (m >= tokens || row >= there) return;
   float v = __ldcg(part + (int64_t(c - 1) * 2 + 1) * rows * kCols + i);
   int last = c;
@@ -462,9 +499,10 @@ Plan plan_for(int tokens, int n, int k, int sms) {
   Plan p{NT, 8, 1, 0, 0, false};
   const int held = tokens < 8 * NT ? tokens : 8 * NT;
   // Rows of a CTA (32 to 256): few, as long as the warps along k all have some
-  // and there are 8 rows per token: the tokens' values, read again by every
-  // CTA, then stay within half of the weights' bytes.
-  while (p.warps_n > 1 && kRows * (p.warps_n / 2) >= 8 * held && kWarps / (p.warps_n / 2) * kK < k + kK) p.warps_n /= 2;
+  // and the tokens' values, read again by every CTA, stay within 4 (8) KB of a
+  // stage: a quarter (half) of the weights' bytes, and two CTAs to an SM.
+  const int need = NT == 1 ? held : 4;
+  while (p.warps_n > 1 && p.warps_n / 2 >= need && kWarps / (p.warps_n / 2) * kK < k + kK) p.warps_n /= 2;
   const int rows = kRows * p.warps_n, stage_k = kWarps / p.warps_n * kK;
   const int64_t blocks = (int64_t(n) + rows - 1) / rows;
   p.stages = (k + stage_k - 1) / stage_k;
@@ -485,21 +523,52 @@ size_t plan_scratch(const Plan& p, int tokens) {
   return p.cut ? size_t((tokens + 8 * p.nt - 1) / (8 * p.nt)) * p.ctas * 2 * (kRows * p.warps_n) * (8 * p.nt) * sizeof(float) : 0;
 }
 
-template <class T, int NT, int GB, bool Aligned>
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<EncodeTiled>(p) : nullptr;
+  }();
+  return fn;
+}
+// A matrix of rows x columns and boxes of it; what lies beyond reads as zeros.
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, int64_t columns, int64_t rows,
+              int64_t stride_bytes, int box_columns, int box_rows) {
+  const EncodeTiled encode = encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {cuuint64_t(columns), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride_bytes)};
+  const cuuint32_t box[2] = {cuuint32_t(box_columns), cuuint32_t(box_rows)}, step[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int NT, int GB, bool Boxes>
 cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
-  const int held = a.tokens < 8 * NT ? a.tokens : 8 * NT, stage_k = kWarps / p.warps_n * Tile<NT>::kK;
+  using L = Tile<NT>;
+  const int held = a.tokens < 8 * NT ? a.tokens : 8 * NT, warps_k = kWarps / p.warps_n;
   a.warps_n = p.warps_n;
   a.stages = p.stages;
   a.ranks = p.ranks;
-  a.x_shift = 31 - __builtin_clz(unsigned(stage_k / 8));
   const unsigned per = unsigned(a.group / 32);
   a.group_shift = per & (per - 1) ? -1 : 31 - __builtin_clz(per);
-  const size_t bytes = size_t(Tile<NT>::kStages) * stage_size<NT>(held, stage_k);
-  const auto kernel = w4_kernel<T, NT, GB, Aligned>;
-  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB == 8 ? 3 : GB / 2][Aligned]);
+  CUtensorMap map_w{}, map_x{};
+  if (Boxes) {
+    const int64_t x_stride = a.tokens == 1 ? (int64_t(a.k) + 7) / 8 * 8 : a.x_stride;   // one token has no stride
+    if (!make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, L::kPitch == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  a.weight, (int64_t(a.k) + 1) / 2, a.n, a.weight_stride, L::kPitch, kRows * p.warps_n) ||
+        !make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_NONE, a.x, a.k, a.tokens, x_stride * 2, L::kK, held))
+      return cudaErrorInvalidValue;
+  }
+  const size_t bytes = size_t(L::kStages) * stage_size<NT>(held, warps_k) + 1024;
+  const auto kernel = w4_kernel<T, NT, GB, Boxes>;
+  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB == 8 ? 3 : GB / 2][Boxes]);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(p.ctas), 1, (a.tokens + 8 * NT - 1) / (8 * NT));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(32 * kWarps + (Boxes ? kBoxThreads : kWordThreads));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -510,10 +579,11 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, map_w, map_x);
   if (e != cudaSuccess || !p.cut) return e;
   cfg.gridDim.x = unsigned(p.ctas - 1);
-  cfg.gridDim.y = unsigned((kRows * p.warps_n * held + kThreads - 1) / kThreads);
+  cfg.gridDim.y = unsigned((kRows * p.warps_n * held + kJoinThreads - 1) / kJoinThreads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -521,12 +591,12 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, w4_join_kernel<T, NT>, a, int(p.ctas));
 }
 
-template <class T, int NT, bool Aligned>
+template <class T, int NT, bool Boxes>
 cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
-  if (a.group == 64) return launch_shape<T, NT, 2, Aligned>(a, p, s);
-  if (NT == 1 && a.group % 256 == 0) return launch_shape<T, NT, NT == 1 ? 8 : 4, Aligned>(a, p, s);
-  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_shape<T, NT, 4, Aligned>(a, p, s);
-  return launch_shape<T, NT, 1, Aligned>(a, p, s);
+  if (a.group == 64) return launch_shape<T, NT, 2, Boxes>(a, p, s);
+  if (NT == 1 && a.group % 256 == 0) return launch_shape<T, NT, NT == 1 ? 8 : 4, Boxes>(a, p, s);
+  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_shape<T, NT, 4, Boxes>(a, p, s);
+  return launch_shape<T, NT, 1, Boxes>(a, p, s);
 }
 
 template <class T>
@@ -574,7 +644,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t 
   if (need && (!scratch || !aligned(scratch, 256) || scratch_bytes < need))
     return fail(PM_E_INVALID, "%s: needs %zu bytes of scratch, 256-byte aligned", who, need);
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->scales, 16) && aligned(j->zeros, 8), 0, 0, 0, 0, static_cast<float*>(scratch)};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->scales, 16) && aligned(j->zeros, 8), 0, 0, 0, static_cast<float*>(scratch)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, plan, s) : launch<fp16>(a, plan, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");
