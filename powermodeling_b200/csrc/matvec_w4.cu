@@ -251,7 +251,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
           }
         } else {
           constexpr int kPieces = L::kStageBytes / 16 / kWordThreads;          // of a thread
-#pragma unroll 4
+#pragma unroll 16
           for (int c = 0; c < kPieces; ++c) {
             const int p = c * kWordThreads + me, tile = p / (kRows * L::kPieces), row = p / L::kPieces % kRows, piece = p % L::kPieces;
             const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * L::kK + piece * 32;
