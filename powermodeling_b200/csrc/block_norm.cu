@@ -6,21 +6,23 @@
 // Both directions are bound by the rows' bytes (forward: two arrays read, two
 // written; backward: four read, two written), so each row is read once and
 // kept on chip between its reductions.
-//  * Forward: a warp (rows of up to 64 16-byte pieces) or a CTA per row, two
-//    pieces of each array per thread in registers (four for 32-bit rows of
-//    more than 2048 pieces).
+//  * Persistent CTAs take runs of consecutive rows, each thread the same
+//    columns of every row: the parameters stay in registers, and the next rows
+//    arrive meanwhile in a ring of thread-private 16-byte asynchronous copies
+//    (each thread reads what it copied: no barrier but the reductions').  512
+//    threads an SM hold rows of up to 1024 pieces; wider ones are shared by a
+//    cluster (backward) or read by a CTA each (forward), and rows of up to 64
+//    pieces go by warps.
 //  * Backward: h is recomputed from r, b and the two saved statistics, which
 //    costs no bytes (b is needed anyway) and no rounding.  With gp = scale
 //    gate w_post and bu = b r1 the sums over rows that the parameters need are
 //    only P = sum dy u and, per gate row, A = sum dh bu: dw_pre = P, dgate =
-//    scale w_post A, dw_post = sum scale gate A.  Persistent CTAs take runs of
-//    consecutive rows, each thread the same columns of every row, P and A in
-//    registers; the next rows arrive meanwhile in a ring of thread-private
-//    asynchronous copies (each thread reads what it copied: no barrier but
-//    the reductions').  Rows beyond 1024 pieces are shared by a cluster.
-//    A second kernel adds the CTAs' partial sums in order.
-//  * Any other width, stride or alignment: the loop kernels, which read a row
-//    again in each pass.
+//    scale w_post A, dw_post = sum scale gate A; they too stay in registers,
+//    and a second kernel adds the CTAs' in order.
+//  * Rows that 16-byte pieces do not fit (odd widths, strides, addresses): the
+//    same with single elements, neighbours in neighbouring lanes, the next
+//    row's loaded ahead into registers.  What is wider than that reads its
+//    rows again in each pass (the loop kernels).
 #include <cooperative_groups.h>
 
 #include "blocks.cuh"
@@ -76,63 +78,113 @@ struct GradArgs {
   int slice;                             // 16-byte pieces of a row that one CTA of the cluster takes
 };
 
-// 16 bytes of T.
-template <class T> struct Vec {
-  static constexpr int n = 16 / sizeof(T);
+// N neighbouring elements: 16 bytes of them, or one.
+template <class T, int N> struct Raw {
   uint4 q;
-  __device__ __forceinline__ float at(int i) const { return to_float(reinterpret_cast<const T*>(&q)[i]); }
-};
-template <class T>
-__device__ __forceinline__ uint4 pack(const float (&v)[Vec<T>::n]) {
-  uint4 q;
-  T* t = reinterpret_cast<T*>(&q);
+  __device__ __forceinline__ void unpack(float (&v)[N]) const {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < Vec<T>::n; ++i) t[i] = from_float<T>(v[i]);
-  return q;
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
+template <class T> struct Raw<T, 1> {
+  T q;
+  __device__ __forceinline__ void unpack(float (&v)[1]) const { v[0] = to_float(q); }
+};
+template <class T> constexpr int kWide = 16 / sizeof(T);
+template <class T, int N>
+__device__ __forceinline__ Raw<T, N> load_raw(const T* p) {
+  if constexpr (N == 1) return {__ldcs(p)};
+  else return {__ldcs(reinterpret_cast<const uint4*>(p))};
 }
-template <class T>
-__device__ __forceinline__ Vec<T> load_stream(const T* p) {
-  return {__ldcs(reinterpret_cast<const uint4*>(p))};
+template <class T, int N>
+__device__ __forceinline__ void store(T* p, const float (&v)[N]) {
+  if constexpr (N == 1) {
+    __stcs(p, from_float<T>(v[0]));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(v[i]);
+      } else if constexpr (std::is_same<T, bf16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+  }
 }
-template <class T>
-__device__ __forceinline__ void param_piece(const Param<T>& w, int64_t at, float (&v)[Vec<T>::n]) {
-  constexpr int n = Vec<T>::n;
-  if (w.f32) {
+template <int N>
+__device__ __forceinline__ void store32(float* p, const float (&v)[N]) {
+  if constexpr (N == 1) p[0] = v[0];
+  else
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+template <class T, int N>
+__device__ __forceinline__ void param_piece(const Param<T>& w, int64_t at, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = w.at(at);
+  } else if (w.f32) {
     const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w.p) + at);
 #pragma unroll
-    for (int i = 0; i < n / 4; ++i) {
+    for (int i = 0; i < N / 4; ++i) {
       const float4 q = __ldg(p + i);
       v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
     }
   } else {
-    const Vec<T> q{__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w.p) + at))};
-#pragma unroll
-    for (int i = 0; i < n; ++i) v[i] = q.at(i);
+    Raw<T, N>{__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w.p) + at))}.unpack(v);
   }
 }
+// scale gate w_post of N columns; parts that are not there count as one.
+template <class T, int N>
+__device__ __forceinline__ void factor_piece(const NormArgs<T>& f, int64_t segment, int col, float (&v)[N]) {
+  float g[N];
+  if (f.post.p) param_piece<T, N>(f.post, col, v);
+  if (f.gate_rows) param_piece<T, N>(f.gate, segment * f.width + col, g);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (f.post.p ? v[i] : 1.0f) * (f.gate_rows ? g[i] * f.scale : f.scale);
+}
 
-// ---------------------------------------------------------------- forward, rows in registers
-// C 16-byte pieces per thread; WarpRow: one warp per row, else one CTA.
-template <class T, int C, bool WarpRow>
+// ---------------------------------------------------------------- forward, a row at a time
+// C pieces of N elements per thread, in registers; WarpRow: one warp per row, else one CTA.
+template <class T, int N, int C, bool WarpRow>
 __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ NormArgs<T> a) {
-  constexpr int n = Vec<T>::n;
   __shared__ float red[2][32];
   const int64_t row = WarpRow ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.rows) return;                             // whole warps of the last CTA, which has no barrier
   const int first = WarpRow ? threadIdx.x & 31 : threadIdx.x, step = WarpRow ? 32 : blockDim.x;
-  const int pieces = a.width / n;
+  const int pieces = a.width / N;
   const T* r = a.residual + row * a.residual_stride;
   const T* b = a.block + row * a.block_stride;
-  const int64_t g = a.gate_rows ? row / a.rows_per_gate * a.width : 0;
-  Vec<T> rv[C], bv[C];
+  const int64_t segment = a.gate_rows ? row / a.rows_per_gate : 0;
+  float h[C][N], x[C][N];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int p = first + c * step;
     if (p < pieces) {
-      bv[c] = load_stream(b + p * n);
-      rv[c] = load_stream(r + p * n);
-    } else {
-      bv[c].q = rv[c].q = make_uint4(0, 0, 0, 0);
+      const Raw<T, N> bv = load_raw<T, N>(b + p * N), rv = load_raw<T, N>(r + p * N);
+      bv.unpack(x[c]);
+      rv.unpack(h[c]);
     }
   }
   auto total = [&](float v, float* where) { return WarpRow ? warp_sum(v) : cta_sum(v, where); };
@@ -141,26 +193,24 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ 
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
+      if (first + c * step < pieces)
 #pragma unroll
-      for (int i = 0; i < n; ++i) s += bv[c].at(i) * bv[c].at(i);
+        for (int i = 0; i < N; ++i) s += x[c][i] * x[c][i];
     r1 = rsqrtf(total(s, red[0]) / float(a.width) + a.eps);
   }
-  float h[C][n], s = 0.0f;
+  float s = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int p = first + c * step;
     if (p < pieces) {
-      float w[n], v[n];
-      if (a.post.p) param_piece(a.post, p * n, w);
-      if (a.gate_rows) param_piece(a.gate, g + p * n, v);
+      float w[N];
+      factor_piece<T, N>(a, segment, p * N, w);
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        float x = bv[c].at(i) * r1;
-        if (a.post.p) x *= w[i];
-        h[c][i] = rv[c].at(i) + (a.gate_rows ? v[i] * a.scale : a.scale) * x;
+      for (int i = 0; i < N; ++i) {
+        h[c][i] += w[i] * (x[c][i] * r1);
         s += h[c][i] * h[c][i];
       }
-      __stcs(reinterpret_cast<uint4*>(a.hidden + row * a.width + p * n), pack<T>(h[c]));
+      store<T, N>(a.hidden + row * a.width + p * N, h[c]);
     }
   }
   const float r2 = rsqrtf(total(s, red[1]) / float(a.width) + a.eps);
@@ -168,16 +218,144 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ 
   for (int c = 0; c < C; ++c) {
     const int p = first + c * step;
     if (p < pieces) {
-      float w[n];
-      param_piece(a.pre, p * n, w);
+      float w[N];
+      param_piece<T, N>(a.pre, p * N, w);
 #pragma unroll
-      for (int i = 0; i < n; ++i) h[c][i] *= r2 * w[i];
-      __stcs(reinterpret_cast<uint4*>(a.normed + row * a.width + p * n), pack<T>(h[c]));
+      for (int i = 0; i < N; ++i) h[c][i] *= r2 * w[i];
+      store<T, N>(a.normed + row * a.width + p * N, h[c]);
     }
   }
   if (a.stats && first == 0) {
     a.stats[2 * row] = r1;
     a.stats[2 * row + 1] = r2;
+  }
+}
+
+// Sum over the CTA in one barrier; `red` alternates between two buffers.
+__device__ __forceinline__ float cta_total(float v, float (&red)[2][32], int& parity) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) red[parity][threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.0f;
+  const int warps = blockDim.x >> 5;
+  for (int w = 0; w < warps; ++w) s += red[parity][w];
+  parity ^= 1;
+  return s;
+}
+
+// ---------------------------------------------------------------- forward, rows streamed
+// One CTA per run of consecutive rows of at most 1024 pieces.  EachRow: the
+// gate changes with every row, and streams with them when it is of type T.
+constexpr int kNormStages = 4;
+template <class T, bool EachRow>
+__global__ void __launch_bounds__(512) norm_stream_kernel(const __grid_constant__ NormArgs<T> a) {
+  constexpr int N = kWide<T>, C = 2, kArrays = EachRow ? 3 : 2;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float red[2][32];
+  const int pieces = a.width / N, threads = blockDim.x;
+  const int64_t from = a.rows * blockIdx.x / gridDim.x, to = a.rows * (blockIdx.x + 1) / gridDim.x;
+  const float inv = 1.0f / float(a.width);
+  int col[C];
+  bool own[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int p = threadIdx.x + c * threads;
+    own[c] = p < pieces;
+    col[c] = (own[c] ? p : 0) * N;
+  }
+  uint8_t* ring = smem + threadIdx.x * 16;               // a thread's copies: [stage][array][c], threads side by side
+  const uint32_t ring_addr = smem_addr(ring);
+  const bool gate_streams = EachRow && !a.gate.f32;
+  auto slot = [&](int stage, int array, int c) { return ((stage * kArrays + array) * C + c) * threads * 16; };
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < to) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (own[c]) {
+          copy16(ring_addr + slot(stage, 0, c), a.residual + row * a.residual_stride + col[c], 16);
+          copy16(ring_addr + slot(stage, 1, c), a.block + row * a.block_stride + col[c], 16);
+          if (gate_streams) copy16(ring_addr + slot(stage, 2, c), static_cast<const T*>(a.gate.p) + row * a.width + col[c], 16);
+        }
+    }
+    commit();
+  };
+  auto piece = [&](int stage, int array, int c, float (&v)[N]) {
+    Raw<T, N>{*reinterpret_cast<const uint4*>(ring + slot(stage, array, c))}.unpack(v);
+  };
+#pragma unroll
+  for (int i = 0; i < kNormStages - 1; ++i) fetch(from + i, i);
+  float pre[C][N], gp[C][N];                             // gp: scale gate w_post (EachRow: w_post)
+  int64_t segment = EachRow || !a.gate_rows ? 0 : from / a.rows_per_gate;
+  int64_t segment_end = EachRow || !a.gate_rows ? to : (segment + 1) * a.rows_per_gate;
+  auto load_factor = [&]() {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (own[c]) {
+        if constexpr (EachRow) {
+          if (a.post.p) param_piece<T, N>(a.post, col[c], gp[c]);
+          else
+#pragma unroll
+            for (int i = 0; i < N; ++i) gp[c][i] = 1.0f;
+        } else {
+          factor_piece<T, N>(a, segment, col[c], gp[c]);
+        }
+      }
+  };
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (own[c]) param_piece<T, N>(a.pre, col[c], pre[c]);
+  load_factor();
+  int parity = 0, stage = 0;
+  for (int64_t row = from; row < to; ++row) {
+    if constexpr (!EachRow) {
+      if (row >= segment_end) {
+        ++segment;
+        segment_end += a.rows_per_gate;
+        load_factor();
+      }
+    }
+    fetch(row + kNormStages - 1, stage == 0 ? kNormStages - 1 : stage - 1);    // the place of the row before, which this thread is done with
+    wait_groups<kNormStages - 1>();
+    float r1 = 1.0f, s = 0.0f, h[C][N];
+    if (a.post.p) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (own[c]) {
+          float x[N];
+          piece(stage, 1, c, x);
+#pragma unroll
+          for (int i = 0; i < N; ++i) s += x[i] * x[i];
+        }
+      r1 = rsqrtf(cta_total(s, red, parity) * inv + a.eps);
+      s = 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (own[c]) {
+        float x[N], g[N];
+        piece(stage, 0, c, h[c]);
+        piece(stage, 1, c, x);
+        if constexpr (EachRow) {
+          if (gate_streams) piece(stage, 2, c, g);
+          else param_piece<T, N>(a.gate, row * a.width + col[c], g);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          h[c][i] += (EachRow ? g[i] * a.scale * gp[c][i] : gp[c][i]) * (x[i] * r1);
+          s += h[c][i] * h[c][i];
+        }
+        store<T, N>(a.hidden + row * a.width + col[c], h[c]);
+      }
+    const float r2 = rsqrtf(cta_total(s, red, parity) * inv + a.eps);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (own[c]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[c][i] *= r2 * pre[c][i];
+        store<T, N>(a.normed + row * a.width + col[c], h[c]);
+      }
+    if (a.stats && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(r1, r2);
+    stage = stage + 1 == kNormStages ? 0 : stage + 1;
   }
 }
 
@@ -197,15 +375,18 @@ __device__ __forceinline__ Run run_of(int64_t rows, int64_t segments, int chunks
 
 // Rows in a ring: 512 threads of an SM then hold 192 (EachRow: 160) KB of them.
 constexpr __host__ __device__ int stages_of(bool each_row) { return each_row ? 2 : 3; }
+constexpr int kSingles = 8;              // single elements of a thread
 
+// N: elements of a piece, 16 bytes of them in the ring, or one in registers.
 // Threads of a row (Warps == false: the CTA, or the cluster's CTAs; true: a
 // warp, the CTA's warps then taking rows in turn).  EachRow: a gate per row,
 // which streams with the rows; its gradient is complete with the row.
-template <class T, bool Warps, bool EachRow, bool Cluster>
+template <class T, int N, bool Warps, bool EachRow, bool Cluster>
 __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ GradArgs<T> a) {
-  constexpr int n = Vec<T>::n, C = 2, kArrays = EachRow ? 5 : 4, kStages = stages_of(EachRow);
+  constexpr bool kRing = N > 1;
+  constexpr int C = kRing ? 2 : kSingles, kArrays = EachRow ? 5 : 4, kStages = stages_of(EachRow);
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float red[2][32];
+  __shared__ float red[2][32];
   __shared__ float shared_sum[2][8];
   const NormArgs<T>& f = a.f;
   const int ranks = Cluster ? int(cg::this_cluster().num_blocks()) : 1, rank = Cluster ? int(cg::this_cluster().block_rank()) : 0;
@@ -214,7 +395,7 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int width_threads = Warps ? 32 : blockDim.x, me = Warps ? lane : threadIdx.x;
   const int row_step = Warps ? blockDim.x >> 5 : 1;
-  const int pieces = f.width / n, piece0 = rank * a.slice, slice = min(a.slice, pieces - piece0);
+  const int pieces = f.width / N, piece0 = rank * a.slice, slice = min(a.slice, pieces - piece0);
   const Run run = run_of(f.rows, a.segments, a.chunks, part, parts);
   const int64_t row_end = run.row_of(run.to);
   const float inv = 1.0f / float(f.width);
@@ -226,119 +407,124 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
   for (int c = 0; c < C; ++c) {
     const int p = me + c * width_threads;
     own[c] = p < slice;
-    col[c] = (piece0 + (own[c] ? p : 0)) * n;
+    col[c] = (piece0 + (own[c] ? p : 0)) * N;
   }
-  // a thread's copies: [stage][array][c], 16 bytes each, threads side by side
+  // a thread's copies: [stage][array][c], 16 bytes each, threads side by side.  A gradient that does not come in stays zero.
   const int row_bytes = kArrays * C * width_threads * 16;
   uint8_t* ring = smem + (Warps ? warp * kStages * row_bytes : 0) + me * 16;
   const uint32_t ring_addr = smem_addr(ring);
+  Raw<T, N> now[kRing ? 1 : 4][C], next[kRing ? 1 : 4][C];
   auto slot = [&](int stage, int array, int c) { return stage * row_bytes + (array * C + c) * width_threads * 16; };
+  if constexpr (kRing) {
+    if (!has_gh || !has_gy)
+      for (int i = 0; i < kStages; ++i)
+        for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(ring + slot(i, has_gh ? 3 : 2, c)) = make_uint4(0, 0, 0, 0);
+  }
   auto fetch = [&](int64_t row, int stage) {
-    if (row < row_end) {
+    if constexpr (kRing) {
+      if (row < row_end) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (own[c]) {
+            copy16(ring_addr + slot(stage, 0, c), f.residual + row * f.residual_stride + col[c], 16);
+            copy16(ring_addr + slot(stage, 1, c), f.block + row * f.block_stride + col[c], 16);
+            if (has_gh) copy16(ring_addr + slot(stage, 2, c), a.grad_hidden + row * a.grad_hidden_stride + col[c], 16);
+            if (has_gy) copy16(ring_addr + slot(stage, 3, c), a.grad_normed + row * a.grad_normed_stride + col[c], 16);
+            if constexpr (EachRow) {
+              if (!f.gate.f32) copy16(ring_addr + slot(stage, 4, c), static_cast<const T*>(f.gate.p) + row * f.width + col[c], 16);
+            }
+          }
+      }
+      commit();
+    } else if (row < row_end) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (own[c]) {
-          copy16(ring_addr + slot(stage, 0, c), f.residual + row * f.residual_stride + col[c], 16);
-          copy16(ring_addr + slot(stage, 1, c), f.block + row * f.block_stride + col[c], 16);
-          if (has_gh) copy16(ring_addr + slot(stage, 2, c), a.grad_hidden + row * a.grad_hidden_stride + col[c], 16);
-          if (has_gy) copy16(ring_addr + slot(stage, 3, c), a.grad_normed + row * a.grad_normed_stride + col[c], 16);
-          if constexpr (EachRow) {
-            if (!f.gate.f32) copy16(ring_addr + slot(stage, 4, c), static_cast<const T*>(f.gate.p) + row * f.width + col[c], 16);
-          }
+          next[0][c] = load_raw<T, N>(f.residual + row * f.residual_stride + col[c]);
+          next[1][c] = load_raw<T, N>(f.block + row * f.block_stride + col[c]);
+          next[2][c].q = next[3][c].q = from_float<T>(0.0f);
+          if (has_gh) next[2][c] = load_raw<T, N>(a.grad_hidden + row * a.grad_hidden_stride + col[c]);
+          if (has_gy) next[3][c] = load_raw<T, N>(a.grad_normed + row * a.grad_normed_stride + col[c]);
         }
     }
-    commit();
   };
-  auto piece = [&](int stage, int array, int c) { return Vec<T>{*reinterpret_cast<const uint4*>(ring + slot(stage, array, c))}; };
+  auto piece = [&](int stage, int array, int c, float (&v)[N]) {
+    if constexpr (kRing) Raw<T, N>{*reinterpret_cast<const uint4*>(ring + slot(stage, array, c))}.unpack(v);
+    else now[array][c].unpack(v);
+  };
 
   int parity = 0;
   auto total = [&](float v) {
     if constexpr (Warps) return warp_sum(v);
-    v = warp_sum(v);
-    if (lane == 0) red[parity][warp] = v;
-    __syncthreads();
-    const int warps = blockDim.x >> 5;
-    float s = 0.0f;
-    for (int w = 0; w < warps; ++w) s += red[parity][w];
     if constexpr (Cluster) {
-      if (threadIdx.x < ranks) cg::this_cluster().map_shared_rank(&shared_sum[parity][0], threadIdx.x)[rank] = s;
+      const int now_parity = parity;
+      const float own_sum = cta_total(v, red, parity);
+      if (threadIdx.x < ranks) cg::this_cluster().map_shared_rank(&shared_sum[now_parity][0], threadIdx.x)[rank] = own_sum;
       cg::this_cluster().sync();
-      s = 0.0f;
-      for (int k = 0; k < ranks; ++k) s += shared_sum[parity][k];
+      float s = 0.0f;
+      for (int k = 0; k < ranks; ++k) s += shared_sum[now_parity][k];
+      return s;
     }
-    parity ^= 1;
-    return s;
+    return cta_total(v, red, parity);
   };
 
   // pre, and gp = scale gate w_post of the segment (EachRow: w_post)
-  float pre[C][n], gp[C][n], sum_p[C][n] = {}, sum_a[C][n] = {};   // EachRow: sum_a is sum scale gate dh bu
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (own[c]) param_piece(f.pre, col[c], pre[c]);
+  float pre[C][N], gp[C][N], sum_p[C][N] = {}, sum_a[C][N] = {};   // EachRow: sum_a is sum scale gate dh bu
   auto load_gp = [&](int64_t segment) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (own[c]) {
-        if (has_post) param_piece(f.post, col[c], gp[c]);
-        else
+        if constexpr (EachRow) {
+          if (has_post) param_piece<T, N>(f.post, col[c], gp[c]);
+          else
 #pragma unroll
-          for (int i = 0; i < n; ++i) gp[c][i] = 1.0f;
-        if constexpr (!EachRow) {
-          float g[n];
-          if (f.gate_rows) param_piece(f.gate, segment * f.width + col[c], g);
-#pragma unroll
-          for (int i = 0; i < n; ++i) gp[c][i] *= f.gate_rows ? g[i] * f.scale : f.scale;
+            for (int i = 0; i < N; ++i) gp[c][i] = 1.0f;
+        } else {
+          factor_piece<T, N>(f, segment, col[c], gp[c]);
         }
       }
   };
-  if constexpr (EachRow) load_gp(0);
 
-  // A of a finished piece of a segment (each warp its own where rows go by warps; joined below)
+  // A of a finished piece of a segment, or the gate's gradient itself and the post weight's sum so far
   auto flush = [&](int64_t item) {
-    if (a.part_a) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (own[c]) {
-          float4* at = reinterpret_cast<float4*>(a.part_a + item * f.width + col[c]);
-#pragma unroll
-          for (int i = 0; i < n / 4; ++i) at[i] = make_float4(sum_a[c][4 * i], sum_a[c][4 * i + 1], sum_a[c][4 * i + 2], sum_a[c][4 * i + 3]);
-        }
-    } else {
-      const int64_t segment = item / a.chunks;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (own[c]) {
-          float g[n], w[n];
-          param_piece(f.gate, segment * f.width + col[c], g);
-          if (has_post) param_piece(f.post, col[c], w);
-          if (a.gate_out) {
-#pragma unroll
-            for (int i = 0; i < n; ++i) {
-              const float v = f.scale * (has_post ? w[i] : 1.0f) * sum_a[c][i];
-              const int64_t at = segment * f.width + col[c] + i;
-              if (a.gate_out32) static_cast<float*>(a.gate_out)[at] = v;
-              else static_cast<T*>(a.gate_out)[at] = from_float<T>(v);
-            }
-          }
-          if (a.part_post) {
-            float* at = a.part_post + int64_t(part) * f.width + col[c];
-            const bool fresh = item == run.from;
-#pragma unroll
-            for (int i = 0; i < n; ++i) at[i] = (fresh ? 0.0f : at[i]) + f.scale * g[i] * sum_a[c][i];
-          }
-        }
-    }
+    const int64_t segment = item / a.chunks;
 #pragma unroll
     for (int c = 0; c < C; ++c)
+      if (own[c]) {
+        if (a.part_a) {
+          store32<N>(a.part_a + item * f.width + col[c], sum_a[c]);
+        } else {
+          float g[N], w[N];
+          param_piece<T, N>(f.gate, segment * f.width + col[c], g);
+          if (has_post) param_piece<T, N>(f.post, col[c], w);
 #pragma unroll
-      for (int i = 0; i < n; ++i) sum_a[c][i] = 0.0f;
+          for (int i = 0; i < N; ++i) {
+            const int64_t at = segment * f.width + col[c] + i;
+            const float v = f.scale * (has_post ? w[i] : 1.0f) * sum_a[c][i];
+            if (a.gate_out && a.gate_out32) static_cast<float*>(a.gate_out)[at] = v;
+            else if (a.gate_out) static_cast<T*>(a.gate_out)[at] = from_float<T>(v);
+            if (a.part_post) {
+              float* post = a.part_post + int64_t(part) * f.width + col[c] + i;
+              *post = (item == run.from ? 0.0f : *post) + f.scale * g[i] * sum_a[c][i];
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum_a[c][i] = 0.0f;
+      }
   };
 
   int64_t item = run.from;
-  int64_t row = run.row_of(item) + (Warps ? warp : 0), item_end = run.row_of(item + 1);
-  if constexpr (!EachRow) load_gp(item / a.chunks);
-  int64_t ahead = row;
-  for (int i = 0; i < kStages - 1; ++i, ahead += row_step) fetch(ahead, i);
+  int64_t row = run.row_of(item) + (Warps ? warp : 0), item_end = run.row_of(item + 1), ahead = row;
+  if constexpr (kRing) {
+    for (int i = 0; i < kStages - 1; ++i, ahead += row_step) fetch(ahead, i);
+  } else {
+    fetch(ahead, 0);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (own[c]) param_piece<T, N>(f.pre, col[c], pre[c]);
+  load_gp(EachRow ? 0 : item / a.chunks);
   float2 st_next = row < row_end ? *reinterpret_cast<const float2*>(f.stats + 2 * row) : make_float2(0.0f, 0.0f);
   int stage = 0;
   for (; row < row_end; row += row_step) {
@@ -352,33 +538,39 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
     }
     const float r1 = st_next.x, r2 = st_next.y;
     if (row + row_step < row_end) st_next = *reinterpret_cast<const float2*>(f.stats + 2 * (row + row_step));
-    fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);  // the place of the row before, which this thread is done with
-    ahead += row_step;
-    if constexpr (EachRow) wait_groups<1>();
-    else wait_groups<2>();
-    float u[C][n], gate[EachRow ? C : 1][n], s = 0.0f;
+    if constexpr (kRing) {
+      fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);  // the place of the row before, which this thread is done with
+      ahead += row_step;
+      wait_groups<kStages - 1>();
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int c = 0; c < C; ++c) now[k][c] = next[k][c];
+      ahead += row_step;
+      fetch(ahead, 0);
+    }
+    float u[C][N], gate[EachRow ? C : 1][N], s = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (own[c]) {
-        const Vec<T> rv = piece(stage, 0, c), bv = piece(stage, 1, c);
-        Vec<T> gy{};
-        if (has_gy) gy = piece(stage, 3, c);
+        float x[N], gy[N];
+        piece(stage, 0, c, u[c]);
+        piece(stage, 1, c, x);
+        piece(stage, 3, c, gy);
         if constexpr (EachRow) {
-          if (f.gate.f32) {
-            param_piece(f.gate, row * f.width + col[c], gate[c]);
+          if (kRing && !f.gate.f32) {
+            if constexpr (kRing) piece(stage, 4, c, gate[c]);
           } else {
-            const Vec<T> gv = piece(stage, 4, c);
-#pragma unroll
-            for (int i = 0; i < n; ++i) gate[c][i] = gv.at(i);
+            param_piece<T, N>(f.gate, row * f.width + col[c], gate[c]);
           }
 #pragma unroll
-          for (int i = 0; i < n; ++i) gate[c][i] *= f.scale;
+          for (int i = 0; i < N; ++i) gate[c][i] *= f.scale;
         }
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
-          const float w = EachRow ? gate[c][i] * gp[c][i] : gp[c][i];
-          u[c][i] = (rv.at(i) + w * (bv.at(i) * r1)) * r2;
-          if (has_gy) s += gy.at(i) * pre[c][i] * u[c][i];
+        for (int i = 0; i < N; ++i) {
+          u[c][i] = (u[c][i] + (EachRow ? gate[c][i] * gp[c][i] : gp[c][i]) * (x[i] * r1)) * r2;
+          s += gy[i] * pre[c][i] * u[c][i];
         }
       }
     const float m2 = has_gy ? total(s) * inv : 0.0f;
@@ -386,20 +578,16 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (own[c]) {
-        const Vec<T> bv = piece(stage, 1, c);
-        Vec<T> gh{}, gy{};
-        if (has_gh) gh = piece(stage, 2, c);
-        if (has_gy) gy = piece(stage, 3, c);
-        float dr[n];
+        float x[N], gh[N], gy[N], dr[N];
+        piece(stage, 1, c, x);
+        piece(stage, 2, c, gh);
+        piece(stage, 3, c, gy);
 #pragma unroll
-        for (int i = 0; i < n; ++i) {
-          float d = has_gh ? gh.at(i) : 0.0f;
-          if (has_gy) {
-            d += r2 * (gy.at(i) * pre[c][i] - u[c][i] * m2);
-            sum_p[c][i] += gy.at(i) * u[c][i];
-          }
+        for (int i = 0; i < N; ++i) {
+          const float d = has_gy ? gh[i] + r2 * (gy[i] * pre[c][i] - u[c][i] * m2) : gh[i];
+          if (has_gy) sum_p[c][i] += gy[i] * u[c][i];
           dr[i] = d;
-          const float bu = bv.at(i) * r1;
+          const float bu = x[i] * r1;
           if constexpr (EachRow) {
             // gate holds scale gate; what the gate's gradient needs is kept in its place
             const float dgb = gate[c][i] * d;
@@ -412,33 +600,29 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
           }
           s1 += u[c][i] * bu;
         }
-        __stcs(reinterpret_cast<uint4*>(a.grad_residual + row * f.width + col[c]), pack<T>(dr));
+        store<T, N>(a.grad_residual + row * f.width + col[c], dr);
         if constexpr (EachRow) {
-          if (a.gate_out) {
-            const int64_t at = row * f.width + col[c];
-            if (a.gate_out32) {
-              float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.gate_out) + at);
-#pragma unroll
-              for (int i = 0; i < n / 4; ++i) o[i] = make_float4(gate[c][4 * i], gate[c][4 * i + 1], gate[c][4 * i + 2], gate[c][4 * i + 3]);
-            } else {
-              __stcs(reinterpret_cast<uint4*>(static_cast<T*>(a.gate_out) + at), pack<T>(gate[c]));
-            }
-          }
+          if (a.gate_out && a.gate_out32) store32<N>(static_cast<float*>(a.gate_out) + row * f.width + col[c], gate[c]);
+          else if (a.gate_out) store<T, N>(static_cast<T*>(a.gate_out) + row * f.width + col[c], gate[c]);
         }
       }
-    const float m1 = has_post ? total(s1) * inv : 0.0f;
+    if (has_post) {
+      const float m1 = total(s1) * inv;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (own[c]) {
+          float x[N];
+          piece(stage, 1, c, x);
+#pragma unroll
+          for (int i = 0; i < N; ++i) u[c][i] = r1 * (u[c][i] - x[i] * r1 * m1);
+        }
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (own[c]) {
-        const Vec<T> bv = piece(stage, 1, c);
-        float db[n];
-#pragma unroll
-        for (int i = 0; i < n; ++i) db[i] = has_post ? r1 * (u[c][i] - bv.at(i) * r1 * m1) : u[c][i];
-        __stcs(reinterpret_cast<uint4*>(a.grad_block + row * f.width + col[c]), pack<T>(db));
-      }
+      if (own[c]) store<T, N>(a.grad_block + row * f.width + col[c], u[c]);
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  wait_groups<0>();
+  if constexpr (kRing) wait_groups<0>();
 
   if constexpr (Warps) {
     // the warps' sums, in their order, through shared memory
@@ -447,12 +631,10 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
     const int warps = blockDim.x >> 5;
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (own[c])
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-          sums[warp * f.width + col[c] + i] = sum_p[c][i];
-          sums[(warps + warp) * f.width + col[c] + i] = sum_a[c][i];
-        }
+      if (own[c]) {
+        store32<N>(sums + warp * f.width + col[c], sum_p[c]);
+        store32<N>(sums + (warps + warp) * f.width + col[c], sum_a[c]);
+      }
     __syncthreads();
     float* second = EachRow ? a.part_post : a.part_a;
     const int64_t second_row = EachRow ? part : item;
@@ -466,24 +648,13 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
       if (second) second[second_row * f.width + x] = q;
     }
   } else {
-    if constexpr (EachRow) {
-      if (a.part_post) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-          if (own[c])
-#pragma unroll
-            for (int i = 0; i < n; ++i) a.part_post[int64_t(part) * f.width + col[c] + i] = sum_a[c][i];
+    for (int c = 0; c < C; ++c)
+      if (own[c]) {
+        if (EachRow && a.part_post) store32<N>(a.part_post + int64_t(part) * f.width + col[c], sum_a[c]);
+        if (a.part_pre) store32<N>(a.part_pre + int64_t(part) * f.width + col[c], sum_p[c]);
       }
-    } else {
-      flush(item);
-    }
-    if (a.part_pre) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (own[c])
-#pragma unroll
-          for (int i = 0; i < n; ++i) a.part_pre[int64_t(part) * f.width + col[c] + i] = sum_p[c][i];
-    }
+    if constexpr (!EachRow) flush(item);
     if constexpr (Cluster) cg::this_cluster().sync();    // no CTA leaves while another may still write its sums here
   }
 }
@@ -597,7 +768,8 @@ __global__ void __launch_bounds__(256) grad_loop_kernel(const __grid_constant__ 
 }
 
 // Adds the partial sums in order: 32 columns of one output row per CTA, 16
-// threads a column.  Output rows: grad_pre, grad_post, then the gate's.
+// threads a column.  Output rows: grad_pre, grad_post, then the gate's; with
+// one segment the gate's and grad_post come from the same sum.
 constexpr int kLanes = 16;
 template <class T>
 struct JoinArgs {
@@ -616,32 +788,44 @@ struct JoinArgs {
 template <class T>
 __global__ void __launch_bounds__(32 * kLanes) grad_join_kernel(const __grid_constant__ JoinArgs<T> a) {
   __shared__ float sums[kLanes][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
-  for (int64_t job = blockIdx.y; job < 2 + a.gate_rows; job += gridDim.y) {
+  const bool single = a.part_a && a.items == a.chunks;   // one segment, with or without a gate
+  const int64_t jobs = single ? 2 : 2 + a.gate_rows;
+  for (int64_t job = blockIdx.y; job < jobs; job += gridDim.y) {
     const float* part = job == 0 ? a.part_pre : job == 1 ? (a.part_post ? a.part_post : a.part_a) : a.part_a;
-    void* out = job == 0 ? a.grad_pre : job == 1 ? a.grad_post : a.grad_gate;
-    if (!out || !part) continue;
-    const bool gated = job == 1 && part == a.part_a;     // dw_post from A
-    const int count = job == 0 ? a.parts : job == 1 ? (gated ? a.items : a.parts) : a.chunks;
+    if (!part || !(job == 0 ? a.grad_pre : job == 1 ? (single && a.grad_gate ? a.grad_gate : a.grad_post) : a.grad_gate)) continue;
+    const bool gated = job == 1 && part == a.part_a && !single;                // dw_post from every segment's A
+    const int count = job == 0 ? a.parts : job == 1 ? (part == a.part_a ? a.items : a.parts) : a.chunks;
     const float* from = part + (job >= 2 ? (job - 2) * a.chunks * int64_t(a.width) : 0);
     float sum = 0.0f;
-    if (c < a.width)
-#pragma unroll 4
+    if (c < a.width) {
+#pragma unroll 10
       for (int k = y; k < count; k += kLanes) {
         float v = __ldcg(from + int64_t(k) * a.width + c);
         if (gated) v *= a.gate_rows ? a.gate.at(int64_t(k / a.chunks) * a.width + c) * a.scale : a.scale;
         sum += v;
       }
+    }
     sums[y][x] = sum;
     __syncthreads();
     if (y == 0 && c < a.width) {
       float v = 0.0f;
 #pragma unroll
       for (int k = 0; k < kLanes; ++k) v += sums[k][x];
-      if (job >= 2) v *= a.scale * (a.post.p ? a.post.at(c) : 1.0f);
-      const int64_t at = (job >= 2 ? (job - 2) * a.width : 0) + c;
-      if (job == 0 ? a.pre32 : job == 1 ? a.post32 : a.gate32) static_cast<float*>(out)[at] = v;
-      else static_cast<T*>(out)[at] = from_float<T>(v);
+      auto put = [&](void* out, int f32, int64_t at, float value) {
+        if (f32) static_cast<float*>(out)[at] = value;
+        else static_cast<T*>(out)[at] = from_float<T>(value);
+      };
+      const float to_gate = a.scale * (a.post.p ? a.post.at(c) : 1.0f);
+      if (job == 0) {
+        put(a.grad_pre, a.pre32, c, v);
+      } else if (job >= 2) {
+        put(a.grad_gate, a.gate32, (job - 2) * a.width + c, to_gate * v);
+      } else {
+        if (a.grad_post) put(a.grad_post, a.post32, c, single ? v * (a.gate_rows ? a.gate.at(c) * a.scale : a.scale) : v);
+        if (single && a.grad_gate) put(a.grad_gate, a.gate32, c, to_gate * v);
+      }
     }
     __syncthreads();
   }
@@ -694,50 +878,68 @@ NormArgs<T> forward_args(const pm_block_norm* j) {
 // Whether 16-byte accesses serve every array of the call.
 template <class T>
 bool wide(const NormArgs<T>& a, bool outputs) {
-  bool ok = a.width % Vec<T>::n == 0 && a.residual_stride % Vec<T>::n == 0 && a.block_stride % Vec<T>::n == 0 &&
+  bool ok = a.width % kWide<T> == 0 && a.residual_stride % kWide<T> == 0 && a.block_stride % kWide<T> == 0 &&
             aligned(a.residual, 16) && aligned(a.block, 16) && aligned(a.pre.p, 16) && aligned(a.post.p, 16) && aligned(a.gate.p, 16);
   if (outputs) ok = ok && aligned(a.hidden, 16) && aligned(a.normed, 16);
   return ok;
 }
+int threads_for(int pieces, int per) { return ((pieces + per - 1) / per + 31) / 32 * 32; }
+// CTAs of so many threads that share an SM's 512.
+int share_of_sm(int threads) { return 512 / threads > 4 ? 4 : 512 / threads; }
+
+std::atomic<int> g_norm_smem[3][2][kMaxDevices];         // by type, gate per row
+std::atomic<int> g_grad_smem[3][3][2][kMaxDevices];      // by type, threads of a row, gate per row
+template <class T> constexpr int kType = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 1 : 2;
 
 template <class T>
 cudaError_t launch_forward(const pm_block_norm* j, int sms, cudaStream_t s) {
   const NormArgs<T> a = forward_args<T>(j);
-  const int pieces = a.width / Vec<T>::n;
-  auto threads_for = [&](int per) { return ((pieces + per - 1) / per + 31) / 32 * 32; };
-  if (wide(a, true) && a.rows <= 0x7fffffff) {
+  const bool fits = a.rows <= 0x7fffffff, each_row = a.gate_rows == a.rows && a.rows > 1;
+  if (wide(a, true) && fits) {
+    const int pieces = a.width / kWide<T>;
     if (pieces <= 64) {
       const unsigned grid = unsigned((a.rows + 7) / 8);
-      if (pieces <= 32) norm_row_kernel<T, 1, true><<<grid, 256, 0, s>>>(a);
-      else norm_row_kernel<T, 2, true><<<grid, 256, 0, s>>>(a);
+      if (pieces <= 32) norm_row_kernel<T, kWide<T>, 1, true><<<grid, 256, 0, s>>>(a);
+      else norm_row_kernel<T, kWide<T>, 2, true><<<grid, 256, 0, s>>>(a);
+      return cudaGetLastError();
+    }
+    if (pieces <= 1024 && aligned(a.stats, 8)) {
+      const int threads = threads_for(pieces, 2), most = sms * share_of_sm(threads);
+      const unsigned grid = unsigned(a.rows < most ? a.rows : most);
+      const size_t bytes = size_t(kNormStages) * (each_row ? 3 : 2) * 2 * threads * 16;
+      if (each_row) {
+        ensure_dynamic_smem(norm_stream_kernel<T, true>, 1024, bytes, g_norm_smem[kType<T>][1]);
+        norm_stream_kernel<T, true><<<grid, threads, bytes, s>>>(a);
+      } else {
+        ensure_dynamic_smem(norm_stream_kernel<T, false>, 1024, bytes, g_norm_smem[kType<T>][0]);
+        norm_stream_kernel<T, false><<<grid, threads, bytes, s>>>(a);
+      }
       return cudaGetLastError();
     }
     if (pieces <= 2048) {
-      norm_row_kernel<T, 2, false><<<unsigned(a.rows), threads_for(2), 0, s>>>(a);
+      norm_row_kernel<T, kWide<T>, 2, false><<<unsigned(a.rows), threads_for(pieces, 2), 0, s>>>(a);
       return cudaGetLastError();
     }
-    if (pieces <= 4096 && sizeof(T) == 4) {              // 16-bit rows this wide would not fit the registers
-      norm_row_kernel<T, sizeof(T) == 4 ? 4 : 2, false><<<unsigned(a.rows), threads_for(4), 0, s>>>(a);
-      return cudaGetLastError();
-    }
+  }
+  if (fits && a.width <= 8192) {                         // single elements, 8 a thread
+    norm_row_kernel<T, 1, kSingles, false><<<unsigned(a.rows), threads_for(a.width, kSingles), 0, s>>>(a);
+    return cudaGetLastError();
   }
   const int64_t most = int64_t(sms) * 8;
   norm_loop_kernel<T><<<int(a.rows < most ? a.rows : most), 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 
-std::atomic<int> g_grad_smem[3][3][2][kMaxDevices];      // by type, threads of a row, gate per row
-
-template <class T, bool Warps, bool EachRow, bool Cluster>
+template <class T, int N, bool Warps, bool EachRow, bool Cluster>
 cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int threads, cudaStream_t s) {
-  constexpr int type = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 1 : 2;
-  const auto kernel = grad_row_kernel<T, Warps, EachRow, Cluster>;
-  size_t bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * 2 * threads * 16;
-  if (Warps) {
-    const size_t sums = size_t(2) * (threads / 32) * a.f.width * 4;
+  const auto kernel = grad_row_kernel<T, N, Warps, EachRow, Cluster>;
+  size_t bytes = 0;
+  if (N > 1) {
+    bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * 2 * threads * 16;
+    const size_t sums = Warps ? size_t(2) * (threads / 32) * a.f.width * 4 : 0;
     if (sums > bytes) bytes = sums;
+    ensure_dynamic_smem(kernel, 1024, bytes, g_grad_smem[kType<T>][Warps ? 0 : Cluster ? 1 : 2][EachRow]);
   }
-  ensure_dynamic_smem(kernel, 1024, bytes, g_grad_smem[type][Warps ? 0 : Cluster ? 1 : 2][EachRow]);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(parts * ranks));
   cfg.blockDim = dim3(threads);
@@ -754,6 +956,7 @@ cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int thr
 
 template <class T>
 cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d, float* scratch, int sms, cudaStream_t s) {
+  constexpr int N = kWide<T>;
   GradArgs<T> a{};
   a.f = forward_args<T>(j);
   a.grad_hidden = static_cast<const T*>(d->grad_hidden);
@@ -763,21 +966,19 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
   a.grad_residual = static_cast<T*>(d->grad_residual);
   a.grad_block = static_cast<T*>(d->grad_block);
   const int64_t w = j->width;
-  const int pieces = j->width / Vec<T>::n;
   const bool each_row = j->gate_rows == j->rows && j->rows > 1;
   const bool rows16 = wide(a.f, false) && aligned(a.grad_residual, 16) && aligned(a.grad_block, 16) && aligned(d->grad_gate, 16) &&
-                      aligned(a.f.stats, 8) && (!a.grad_hidden || (aligned(a.grad_hidden, 16) && a.grad_hidden_stride % Vec<T>::n == 0)) &&
-                      (!a.grad_normed || (aligned(a.grad_normed, 16) && a.grad_normed_stride % Vec<T>::n == 0));
-  const int ranks = pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8;
-  bool streamed = rows16 && pieces <= 8192;
+                      (!a.grad_hidden || (aligned(a.grad_hidden, 16) && a.grad_hidden_stride % N == 0)) &&
+                      (!a.grad_normed || (aligned(a.grad_normed, 16) && a.grad_normed_stride % N == 0));
+  // pieces of 16 bytes, or single elements
+  const int pieces = rows16 ? j->width / N : j->width, per = rows16 ? 2 : kSingles;
+  const int ranks = !rows16 || pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8;
+  bool streamed = aligned(a.f.stats, 8) && pieces <= (rows16 ? 8192 : 512 * kSingles);
   a.slice = (pieces + ranks - 1) / ranks;
-  const int row_threads = streamed ? ((a.slice + 1) / 2 + 31) / 32 * 32 : 256;
-  // rows of up to 64 pieces go by warps, 8 of them a CTA, where a warp stays in one segment or gates every row
-  const bool by_warps = streamed && pieces <= 64;
-  // CTAs that fit an SM at 128 registers a thread, and rings of at most 200 KB together
-  int per_sm = by_warps ? 2 : ranks > 1 ? 1 : 512 / row_threads;
-  if (per_sm > 4) per_sm = 4;
-  int want = streamed ? sms * per_sm / ranks : 2 * sms;
+  const int row_threads = streamed ? threads_for(a.slice, per) : 256;
+  // rows of up to 64 pieces go by warps, 8 of them a CTA, where a CTA stays in one segment or every row has its gate
+  const bool by_warps = streamed && rows16 && pieces <= 64;
+  int want = !streamed || by_warps ? 2 * sms : ranks > 1 ? sms / ranks : sms * share_of_sm(row_threads);
   if (want > kMaxParts) want = kMaxParts;
   if (want < 1) want = 1;
   const Split sp = split_rows(j->rows, j->gate_rows, want);
@@ -801,16 +1002,18 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
   if (!streamed) {
     grad_loop_kernel<T><<<sp.parts, 256, 0, s>>>(a);
     e = cudaGetLastError();
+  } else if (!rows16) {
+    e = each_row ? launch_grad_rows<T, 1, false, true, false>(a, sp.parts, 1, row_threads, s)
+                 : launch_grad_rows<T, 1, false, false, false>(a, sp.parts, 1, row_threads, s);
   } else if (by_warps) {
-    e = each_row ? launch_grad_rows<T, true, true, false>(a, sp.parts, 1, 256, s)
-                 : launch_grad_rows<T, true, false, false>(a, sp.parts, 1, 256, s);
+    e = each_row ? launch_grad_rows<T, N, true, true, false>(a, sp.parts, 1, 256, s)
+                 : launch_grad_rows<T, N, true, false, false>(a, sp.parts, 1, 256, s);
+  } else if (ranks > 1) {
+    e = each_row ? launch_grad_rows<T, N, false, true, true>(a, sp.parts, ranks, row_threads, s)
+                 : launch_grad_rows<T, N, false, false, true>(a, sp.parts, ranks, row_threads, s);
   } else {
-    if (ranks > 1)
-      e = each_row ? launch_grad_rows<T, false, true, true>(a, sp.parts, ranks, row_threads, s)
-                   : launch_grad_rows<T, false, false, true>(a, sp.parts, ranks, row_threads, s);
-    else
-      e = each_row ? launch_grad_rows<T, false, true, false>(a, sp.parts, 1, row_threads, s)
-                   : launch_grad_rows<T, false, false, false>(a, sp.parts, 1, row_threads, s);
+    e = each_row ? launch_grad_rows<T, N, false, true, false>(a, sp.parts, 1, row_threads, s)
+                 : launch_grad_rows<T, N, false, false, false>(a, sp.parts, 1, row_threads, s);
   }
   if (e != cudaSuccess) return e;
   const bool gate_joined = wants_gate && by_a;
@@ -819,10 +1022,17 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
                 gate_joined ? d->grad_gate : nullptr, a.f.post, a.f.gate, j->gate_rows, sp.parts, sp.chunks, j->width,
                 j->pre_dtype == PM_DT_F32, j->post_dtype == PM_DT_F32, j->gate_dtype == PM_DT_F32,
                 int(by_a ? sp.segments * sp.chunks : 0), j->scale};
-  const int64_t jobs = 2 + (gate_joined ? j->gate_rows : 0);
-  if (!gate_joined) q.grad_gate = nullptr;
-  grad_join_kernel<T><<<dim3(unsigned((j->width + 31) / 32), unsigned(jobs < 65535 ? jobs : 65535)), 32 * kLanes, 0, s>>>(q);
-  return cudaGetLastError();
+  const int64_t jobs = by_a && sp.segments == 1 ? 2 : 2 + (gate_joined ? j->gate_rows : 0);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned((j->width + 31) / 32), unsigned(jobs < 65535 ? jobs : 65535));
+  cfg.blockDim = dim3(32 * kLanes);
+  cfg.stream = s;
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, grad_join_kernel<T>, q);
 }
 
 int check_forward(const char* who, const pm_block_norm* j, bool backward) {
