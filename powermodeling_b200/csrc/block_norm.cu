@@ -78,6 +78,8 @@ struct GradArgs {
   int slice;                             // 16-byte pieces of a row that one CTA of the cluster takes
 };
 
+constexpr int kSingles = 8;              // single elements of a thread, where pieces do not fit
+
 // N neighbouring elements: 16 bytes of them, or one.
 template <class T, int N> struct Raw {
   uint4 q;
@@ -231,61 +233,117 @@ __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ 
   }
 }
 
-// Sum over the CTA in one barrier; `red` alternates between two buffers.
-__device__ __forceinline__ float cta_total(float v, float (&red)[2][32], int& parity) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) red[parity][threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-  const int warps = blockDim.x >> 5;
-  for (int w = 0; w < warps; ++w) s += red[parity][w];
-  parity ^= 1;
-  return s;
+// Sum over the threads of a row: a warp, a CTA or a cluster's CTAs, the same
+// on each of them.  One barrier a call; buffers alternate, so a slow thread
+// still reads the last sum's while a fast one writes this one's.
+template <bool Warps, bool Cluster>
+struct RowSum {
+  float (*red)[32];
+  float (*shared_sum)[8];
+  int ranks, rank, parity;
+  __device__ __forceinline__ float operator()(float v) {
+    v = warp_sum(v);
+    if constexpr (Warps) return v;
+    if ((threadIdx.x & 31) == 0) red[parity][threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.0f;
+    const int warps = (blockDim.x + 127) >> 7;           // in fours; those that are not there are zero
+    for (int w = 0; w < warps; ++w) {
+      const float4 q = reinterpret_cast<const float4*>(red[parity])[w];
+      s += (q.x + q.y) + (q.z + q.w);
+    }
+    if constexpr (Cluster) {
+      if (threadIdx.x < ranks) cg::this_cluster().map_shared_rank(&shared_sum[parity][0], threadIdx.x)[rank] = s;
+      cg::this_cluster().sync();
+      s = 0.0f;
+      for (int k = 0; k < ranks; ++k) s += shared_sum[parity][k];
+    }
+    parity ^= 1;
+    return s;
+  }
+};
+// The buffers' first use; in a cluster also the point from which the others' shared memory may be written.
+template <bool Warps, bool Cluster>
+__device__ __forceinline__ RowSum<Warps, Cluster> row_sum(float (&red)[2][32], float (&shared_sum)[2][8]) {
+  RowSum<Warps, Cluster> r{red, shared_sum, 1, 0, 0};
+  if constexpr (!Warps) {
+    if (threadIdx.x < 32) red[0][threadIdx.x] = red[1][threadIdx.x] = 0.0f;
+    if constexpr (Cluster) {
+      r.ranks = int(cg::this_cluster().num_blocks());
+      r.rank = int(cg::this_cluster().block_rank());
+      cg::this_cluster().sync();
+    } else {
+      __syncthreads();
+    }
+  }
+  return r;
 }
 
 // ---------------------------------------------------------------- forward, rows streamed
-// One CTA per run of consecutive rows of at most 1024 pieces.  EachRow: the
-// gate changes with every row, and streams with them when it is of type T.
+// C 16-byte pieces of each array per thread.  Warps: rows by warps, a CTA's
+// warps in turn; else a CTA, or a cluster's CTAs, per run of consecutive rows.
+// EachRow: the gate changes with every row, and streams with them when it is
+// of type T.
 constexpr int kNormStages = 4;
-template <class T, bool EachRow>
-__global__ void __launch_bounds__(512) norm_stream_kernel(const __grid_constant__ NormArgs<T> a) {
-  constexpr int N = kWide<T>, C = 2, kArrays = EachRow ? 3 : 2;
+template <class T, int C, bool Warps, bool EachRow, bool Cluster>
+__global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 1024 : 512, Warps ? (C == 1 ? 4 : 2) : 1) norm_stream_kernel(const __grid_constant__ NormArgs<T> a, int slice_pieces) {
+  constexpr int N = kWide<T>, kArrays = EachRow ? 3 : 2;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float red[2][32];
-  const int pieces = a.width / N, threads = blockDim.x;
-  const int64_t from = a.rows * blockIdx.x / gridDim.x, to = a.rows * (blockIdx.x + 1) / gridDim.x;
+  __shared__ __align__(16) float red[2][32];
+  __shared__ float shared_sum[2][8];
+  auto total = row_sum<Warps, Cluster>(red, shared_sum);
+  const int pieces = a.width / N, threads = Warps ? 32 : blockDim.x, me = Warps ? threadIdx.x & 31 : threadIdx.x;
+  const int part = blockIdx.x / total.ranks, parts = gridDim.x / total.ranks, warp = threadIdx.x >> 5;
+  const int piece0 = total.rank * slice_pieces, slice = min(slice_pieces, pieces - piece0);
+  const int row_step = Warps ? blockDim.x >> 5 : 1;
+  const int64_t from = a.rows * part / parts + (Warps ? warp : 0), to = a.rows * (part + 1) / parts;
   const float inv = 1.0f / float(a.width);
   int col[C];
   bool own[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p = threadIdx.x + c * threads;
-    own[c] = p < pieces;
-    col[c] = (own[c] ? p : 0) * N;
+    const int p = me + c * threads;
+    own[c] = p < slice;
+    col[c] = (piece0 + (own[c] ? p : 0)) * N;
   }
-  uint8_t* ring = smem + threadIdx.x * 16;               // a thread's copies: [stage][array][c], threads side by side
+  const int row_bytes = kArrays * C * threads * 16;      // a thread's copies: [stage][array][c], threads side by side
+  uint8_t* ring = smem + (Warps ? warp * kNormStages * row_bytes : 0) + me * 16;
   const uint32_t ring_addr = smem_addr(ring);
   const bool gate_streams = EachRow && !a.gate.f32;
-  auto slot = [&](int stage, int array, int c) { return ((stage * kArrays + array) * C + c) * threads * 16; };
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < to) {
+  auto slot = [&](int stage, int array, int c) { return stage * row_bytes + (array * C + c) * threads * 16; };
+  // a piece beyond the row stays zero and adds nothing: only copies, parameters and stores ask whose it is
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (!own[c])
+      for (int i = 0; i < kNormStages * kArrays; ++i) *reinterpret_cast<uint4*>(ring + slot(0, i, c)) = make_uint4(0, 0, 0, 0);
+  int left = to > from ? int((to - from + row_step - 1) / row_step) : 0, to_fetch = left, place = 0;
+  const T* next_r = a.residual + from * a.residual_stride;
+  const T* next_b = a.block + from * a.block_stride;
+  const T* next_g = static_cast<const T*>(a.gate.p) + from * a.width;
+  auto fetch = [&]() {
+    if (to_fetch > 0) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (own[c]) {
-          copy16(ring_addr + slot(stage, 0, c), a.residual + row * a.residual_stride + col[c], 16);
-          copy16(ring_addr + slot(stage, 1, c), a.block + row * a.block_stride + col[c], 16);
-          if (gate_streams) copy16(ring_addr + slot(stage, 2, c), static_cast<const T*>(a.gate.p) + row * a.width + col[c], 16);
+          copy16(ring_addr + slot(place, 0, c), next_r + col[c], 16);
+          copy16(ring_addr + slot(place, 1, c), next_b + col[c], 16);
+          if (gate_streams) copy16(ring_addr + slot(place, 2, c), next_g + col[c], 16);
         }
+      next_r += row_step * a.residual_stride;
+      next_b += row_step * a.block_stride;
+      if (EachRow) next_g += int64_t(row_step) * a.width;
+      --to_fetch;
     }
+    place = place + 1 == kNormStages ? 0 : place + 1;
     commit();
   };
   auto piece = [&](int stage, int array, int c, float (&v)[N]) {
     Raw<T, N>{*reinterpret_cast<const uint4*>(ring + slot(stage, array, c))}.unpack(v);
   };
 #pragma unroll
-  for (int i = 0; i < kNormStages - 1; ++i) fetch(from + i, i);
-  float pre[C][N], gp[C][N];                             // gp: scale gate w_post (EachRow: w_post)
-  int64_t segment = EachRow || !a.gate_rows ? 0 : from / a.rows_per_gate;
+  for (int i = 0; i < kNormStages - 1; ++i) fetch();
+  float pre[C][N] = {}, gp[C][N] = {};                   // gp: scale gate w_post (EachRow: w_post)
+  int64_t row = from, segment = EachRow || !a.gate_rows ? 0 : from / a.rows_per_gate;
   int64_t segment_end = EachRow || !a.gate_rows ? to : (segment + 1) * a.rows_per_gate;
   auto load_factor = [&]() {
 #pragma unroll
@@ -301,62 +359,67 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(const __grid_constant_
         }
       }
   };
+  if (left) {
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (own[c]) param_piece<T, N>(a.pre, col[c], pre[c]);
-  load_factor();
-  int parity = 0, stage = 0;
-  for (int64_t row = from; row < to; ++row) {
+    for (int c = 0; c < C; ++c)
+      if (own[c]) param_piece<T, N>(a.pre, col[c], pre[c]);
+    load_factor();
+  }
+  T* hidden = a.hidden + from * a.width;
+  T* normed = a.normed + from * a.width;
+  int stage = 0;
+  for (; left > 0; --left) {
     if constexpr (!EachRow) {
       if (row >= segment_end) {
-        ++segment;
-        segment_end += a.rows_per_gate;
+        segment = row / a.rows_per_gate;
+        segment_end = (segment + 1) * a.rows_per_gate;
         load_factor();
       }
     }
-    fetch(row + kNormStages - 1, stage == 0 ? kNormStages - 1 : stage - 1);    // the place of the row before, which this thread is done with
+    fetch();                                             // to the place of the row before, which this thread is done with
     wait_groups<kNormStages - 1>();
-    float r1 = 1.0f, s = 0.0f, h[C][N];
+    float r1 = 1.0f, h[C][N], s[4] = {};
     if (a.post.p) {
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (own[c]) {
-          float x[N];
-          piece(stage, 1, c, x);
+      for (int c = 0; c < C; ++c) {
+        float x[N];
+        piece(stage, 1, c, x);
 #pragma unroll
-          for (int i = 0; i < N; ++i) s += x[i] * x[i];
-        }
-      r1 = rsqrtf(cta_total(s, red, parity) * inv + a.eps);
-      s = 0.0f;
+        for (int i = 0; i < N; ++i) s[i & 3] += x[i] * x[i];
+      }
+      r1 = rsqrtf(total((s[0] + s[1]) + (s[2] + s[3])) * inv + a.eps);
+      s[0] = s[1] = s[2] = s[3] = 0.0f;
     }
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (own[c]) {
-        float x[N], g[N];
-        piece(stage, 0, c, h[c]);
-        piece(stage, 1, c, x);
-        if constexpr (EachRow) {
-          if (gate_streams) piece(stage, 2, c, g);
-          else param_piece<T, N>(a.gate, row * a.width + col[c], g);
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          h[c][i] += (EachRow ? g[i] * a.scale * gp[c][i] : gp[c][i]) * (x[i] * r1);
-          s += h[c][i] * h[c][i];
-        }
-        store<T, N>(a.hidden + row * a.width + col[c], h[c]);
+    for (int c = 0; c < C; ++c) {
+      float x[N], g[N];
+      piece(stage, 0, c, h[c]);
+      piece(stage, 1, c, x);
+      if constexpr (EachRow) {
+        if (gate_streams) piece(stage, 2, c, g);
+        else param_piece<T, N>(a.gate, row * a.width + col[c], g);
       }
-    const float r2 = rsqrtf(cta_total(s, red, parity) * inv + a.eps);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (own[c]) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) h[c][i] *= r2 * pre[c][i];
-        store<T, N>(a.normed + row * a.width + col[c], h[c]);
+      for (int i = 0; i < N; ++i) {
+        h[c][i] += (EachRow ? g[i] * a.scale * gp[c][i] : gp[c][i]) * (x[i] * r1);
+        s[i & 3] += h[c][i] * h[c][i];
       }
-    if (a.stats && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(r1, r2);
+      if (own[c]) store<T, N>(hidden + col[c], h[c]);
+    }
+    const float r2 = rsqrtf(total((s[0] + s[1]) + (s[2] + s[3])) * inv + a.eps);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[c][i] *= r2 * pre[c][i];
+      if (own[c]) store<T, N>(normed + col[c], h[c]);
+    }
+    if (a.stats && me == 0 && total.rank == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(r1, r2);
+    hidden += int64_t(row_step) * a.width;
+    normed += int64_t(row_step) * a.width;
+    row += row_step;
     stage = stage + 1 == kNormStages ? 0 : stage + 1;
   }
+  if constexpr (Cluster) cg::this_cluster().sync();      // no CTA leaves while another may still write its sums here
 }
 
 // ---------------------------------------------------------------- backward, rows streamed
@@ -375,22 +438,21 @@ __device__ __forceinline__ Run run_of(int64_t rows, int64_t segments, int chunks
 
 // Rows in a ring: 512 threads of an SM then hold 192 (EachRow: 160) KB of them.
 constexpr __host__ __device__ int stages_of(bool each_row) { return each_row ? 2 : 3; }
-constexpr int kSingles = 8;              // single elements of a thread
 
 // N: elements of a piece, 16 bytes of them in the ring, or one in registers.
 // Threads of a row (Warps == false: the CTA, or the cluster's CTAs; true: a
 // warp, the CTA's warps then taking rows in turn).  EachRow: a gate per row,
 // which streams with the rows; its gradient is complete with the row.
-template <class T, int N, bool Warps, bool EachRow, bool Cluster>
-__global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ GradArgs<T> a) {
+template <class T, int N, int C, bool Warps, bool EachRow, bool Cluster>
+__global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 1) grad_row_kernel(const __grid_constant__ GradArgs<T> a) {
   constexpr bool kRing = N > 1;
-  constexpr int C = kRing ? 2 : kSingles, kArrays = EachRow ? 5 : 4, kStages = stages_of(EachRow);
+  constexpr int kArrays = EachRow ? 5 : 4, kStages = stages_of(EachRow);
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float red[2][32];
+  __shared__ __align__(16) float red[2][32];
   __shared__ float shared_sum[2][8];
   const NormArgs<T>& f = a.f;
-  const int ranks = Cluster ? int(cg::this_cluster().num_blocks()) : 1, rank = Cluster ? int(cg::this_cluster().block_rank()) : 0;
-  if constexpr (Cluster) cg::this_cluster().sync();      // the others' shared memory is written only once they run
+  auto total = row_sum<Warps, Cluster>(red, shared_sum);
+  const int ranks = total.ranks, rank = total.rank;
   const int part = blockIdx.x / ranks, parts = gridDim.x / ranks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int width_threads = Warps ? 32 : blockDim.x, me = Warps ? lane : threadIdx.x;
@@ -409,43 +471,62 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
     own[c] = p < slice;
     col[c] = (piece0 + (own[c] ? p : 0)) * N;
   }
-  // a thread's copies: [stage][array][c], 16 bytes each, threads side by side.  A gradient that does not come in stays zero.
+  // a thread's copies: [stage][array][c], 16 bytes each, threads side by side.  A piece beyond the row, and a gradient
+  // that does not come in, stay zero and add nothing: only copies, parameters and stores ask whose a piece is.
   const int row_bytes = kArrays * C * width_threads * 16;
   uint8_t* ring = smem + (Warps ? warp * kStages * row_bytes : 0) + me * 16;
   const uint32_t ring_addr = smem_addr(ring);
   Raw<T, N> now[kRing ? 1 : 4][C], next[kRing ? 1 : 4][C];
   auto slot = [&](int stage, int array, int c) { return stage * row_bytes + (array * C + c) * width_threads * 16; };
   if constexpr (kRing) {
-    if (!has_gh || !has_gy)
-      for (int i = 0; i < kStages; ++i)
-        for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(ring + slot(i, has_gh ? 3 : 2, c)) = make_uint4(0, 0, 0, 0);
-  }
-  auto fetch = [&](int64_t row, int stage) {
-    if constexpr (kRing) {
-      if (row < row_end) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-          if (own[c]) {
-            copy16(ring_addr + slot(stage, 0, c), f.residual + row * f.residual_stride + col[c], 16);
-            copy16(ring_addr + slot(stage, 1, c), f.block + row * f.block_stride + col[c], 16);
-            if (has_gh) copy16(ring_addr + slot(stage, 2, c), a.grad_hidden + row * a.grad_hidden_stride + col[c], 16);
-            if (has_gy) copy16(ring_addr + slot(stage, 3, c), a.grad_normed + row * a.grad_normed_stride + col[c], 16);
-            if constexpr (EachRow) {
-              if (!f.gate.f32) copy16(ring_addr + slot(stage, 4, c), static_cast<const T*>(f.gate.p) + row * f.width + col[c], 16);
-            }
-          }
-      }
-      commit();
-    } else if (row < row_end) {
+    for (int c = 0; c < C; ++c)
+      for (int i = 0; i < kStages; ++i)
+        for (int k = 0; k < kArrays; ++k)
+          if (!own[c] || (k == 2 && !has_gh) || (k == 3 && !has_gy)) *reinterpret_cast<uint4*>(ring + slot(i, k, c)) = make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int c = 0; c < C; ++c) next[k][c].q = from_float<T>(0.0f);
+  }
+  int64_t item = run.from, row = run.row_of(item) + (Warps ? warp : 0), item_end = run.row_of(item + 1);
+  int left = row_end > row ? int((row_end - row + row_step - 1) / row_step) : 0, to_fetch = left, place = 0;
+  const T* next_r = f.residual + row * f.residual_stride;
+  const T* next_b = f.block + row * f.block_stride;
+  const T* next_h = a.grad_hidden + row * a.grad_hidden_stride;
+  const T* next_y = a.grad_normed + row * a.grad_normed_stride;
+  const T* next_g = static_cast<const T*>(f.gate.p) + row * f.width;
+  auto fetch = [&]() {
+    if (to_fetch > 0) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (own[c]) {
-          next[0][c] = load_raw<T, N>(f.residual + row * f.residual_stride + col[c]);
-          next[1][c] = load_raw<T, N>(f.block + row * f.block_stride + col[c]);
-          next[2][c].q = next[3][c].q = from_float<T>(0.0f);
-          if (has_gh) next[2][c] = load_raw<T, N>(a.grad_hidden + row * a.grad_hidden_stride + col[c]);
-          if (has_gy) next[3][c] = load_raw<T, N>(a.grad_normed + row * a.grad_normed_stride + col[c]);
+          if constexpr (kRing) {
+            copy16(ring_addr + slot(place, 0, c), next_r + col[c], 16);
+            copy16(ring_addr + slot(place, 1, c), next_b + col[c], 16);
+            if (has_gh) copy16(ring_addr + slot(place, 2, c), next_h + col[c], 16);
+            if (has_gy) copy16(ring_addr + slot(place, 3, c), next_y + col[c], 16);
+            if constexpr (EachRow) {
+              if (!f.gate.f32) copy16(ring_addr + slot(place, 4, c), next_g + col[c], 16);
+            }
+          } else {
+            next[0][c] = load_raw<T, N>(next_r + col[c]);
+            next[1][c] = load_raw<T, N>(next_b + col[c]);
+            if (has_gh) next[2][c] = load_raw<T, N>(next_h + col[c]);
+            if (has_gy) next[3][c] = load_raw<T, N>(next_y + col[c]);
+          }
         }
+      next_r += row_step * f.residual_stride;
+      next_b += row_step * f.block_stride;
+      next_h += row_step * a.grad_hidden_stride;
+      next_y += row_step * a.grad_normed_stride;
+      if (EachRow) next_g += int64_t(row_step) * f.width;
+      --to_fetch;
+    }
+    if constexpr (kRing) {
+      place = place + 1 == kStages ? 0 : place + 1;
+      commit();
     }
   };
   auto piece = [&](int stage, int array, int c, float (&v)[N]) {
@@ -453,23 +534,8 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
     else now[array][c].unpack(v);
   };
 
-  int parity = 0;
-  auto total = [&](float v) {
-    if constexpr (Warps) return warp_sum(v);
-    if constexpr (Cluster) {
-      const int now_parity = parity;
-      const float own_sum = cta_total(v, red, parity);
-      if (threadIdx.x < ranks) cg::this_cluster().map_shared_rank(&shared_sum[now_parity][0], threadIdx.x)[rank] = own_sum;
-      cg::this_cluster().sync();
-      float s = 0.0f;
-      for (int k = 0; k < ranks; ++k) s += shared_sum[now_parity][k];
-      return s;
-    }
-    return cta_total(v, red, parity);
-  };
-
   // pre, and gp = scale gate w_post of the segment (EachRow: w_post)
-  float pre[C][N], gp[C][N], sum_p[C][N] = {}, sum_a[C][N] = {};   // EachRow: sum_a is sum scale gate dh bu
+  float pre[C][N] = {}, gp[C][N] = {}, sum_p[C][N] = {}, sum_a[C][N] = {};   // EachRow: sum_a is sum scale gate dh bu
   auto load_gp = [&](int64_t segment) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -514,20 +580,18 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
       }
   };
 
-  int64_t item = run.from;
-  int64_t row = run.row_of(item) + (Warps ? warp : 0), item_end = run.row_of(item + 1), ahead = row;
-  if constexpr (kRing) {
-    for (int i = 0; i < kStages - 1; ++i, ahead += row_step) fetch(ahead, i);
-  } else {
-    fetch(ahead, 0);
-  }
+#pragma unroll
+  for (int i = 0; i < (kRing ? kStages - 1 : 1); ++i) fetch();
 #pragma unroll
   for (int c = 0; c < C; ++c)
     if (own[c]) param_piece<T, N>(f.pre, col[c], pre[c]);
   load_gp(EachRow ? 0 : item / a.chunks);
-  float2 st_next = row < row_end ? *reinterpret_cast<const float2*>(f.stats + 2 * row) : make_float2(0.0f, 0.0f);
+  const float2* st = reinterpret_cast<const float2*>(f.stats) + row;
+  float2 st_next = left ? *st : make_float2(0.0f, 0.0f);
+  T* grad_residual = a.grad_residual + row * f.width;
+  T* grad_block = a.grad_block + row * f.width;
   int stage = 0;
-  for (; row < row_end; row += row_step) {
+  for (; left > 0; --left) {
     if constexpr (!EachRow && !Warps) {
       if (row >= item_end) {
         flush(item);
@@ -537,89 +601,94 @@ __global__ void __launch_bounds__(512) grad_row_kernel(const __grid_constant__ G
       }
     }
     const float r1 = st_next.x, r2 = st_next.y;
-    if (row + row_step < row_end) st_next = *reinterpret_cast<const float2*>(f.stats + 2 * (row + row_step));
+    st += row_step;
+    if (left > 1) st_next = *st;
     if constexpr (kRing) {
-      fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);  // the place of the row before, which this thread is done with
-      ahead += row_step;
+      fetch();                                           // to the place of the row before, which this thread is done with
       wait_groups<kStages - 1>();
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int c = 0; c < C; ++c) now[k][c] = next[k][c];
-      ahead += row_step;
-      fetch(ahead, 0);
+      fetch();
     }
-    float u[C][N], gate[EachRow ? C : 1][N], s = 0.0f;
+    float u[C][N], gate[EachRow ? C : 1][N], s[4] = {};
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (own[c]) {
-        float x[N], gy[N];
-        piece(stage, 0, c, u[c]);
-        piece(stage, 1, c, x);
-        piece(stage, 3, c, gy);
-        if constexpr (EachRow) {
-          if (kRing && !f.gate.f32) {
-            if constexpr (kRing) piece(stage, 4, c, gate[c]);
-          } else {
-            param_piece<T, N>(f.gate, row * f.width + col[c], gate[c]);
-          }
-#pragma unroll
-          for (int i = 0; i < N; ++i) gate[c][i] *= f.scale;
+    for (int c = 0; c < C; ++c) {
+      float x[N], gy[N];
+      piece(stage, 0, c, u[c]);
+      piece(stage, 1, c, x);
+      piece(stage, 3, c, gy);
+      if constexpr (EachRow) {
+        if (kRing && !f.gate.f32) {
+          if constexpr (kRing) piece(stage, 4, c, gate[c]);
+        } else {
+          param_piece<T, N>(f.gate, row * f.width + col[c], gate[c]);
         }
 #pragma unroll
+        for (int i = 0; i < N; ++i) gate[c][i] *= f.scale;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        u[c][i] = (u[c][i] + (EachRow ? gate[c][i] * gp[c][i] : gp[c][i]) * (x[i] * r1)) * r2;
+        s[(N == 1 ? c : i) & 3] += gy[i] * pre[c][i] * u[c][i];
+      }
+    }
+    const float m2 = has_gy ? total((s[0] + s[1]) + (s[2] + s[3])) * inv * r2 : 0.0f;
+    s[0] = s[1] = s[2] = s[3] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float x[N], gy[N], dr[N];
+      piece(stage, 1, c, x);
+      piece(stage, 2, c, dr);
+      if (has_gy) {
+        piece(stage, 3, c, gy);
+#pragma unroll
         for (int i = 0; i < N; ++i) {
-          u[c][i] = (u[c][i] + (EachRow ? gate[c][i] * gp[c][i] : gp[c][i]) * (x[i] * r1)) * r2;
-          s += gy[i] * pre[c][i] * u[c][i];
+          dr[i] += pre[c][i] * (r2 * gy[i]) - u[c][i] * m2;
+          sum_p[c][i] += gy[i] * u[c][i];
         }
       }
-    const float m2 = has_gy ? total(s) * inv : 0.0f;
-    float s1 = 0.0f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (own[c]) {
-        float x[N], gh[N], gy[N], dr[N];
-        piece(stage, 1, c, x);
-        piece(stage, 2, c, gh);
-        piece(stage, 3, c, gy);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float d = has_gy ? gh[i] + r2 * (gy[i] * pre[c][i] - u[c][i] * m2) : gh[i];
-          if (has_gy) sum_p[c][i] += gy[i] * u[c][i];
-          dr[i] = d;
-          const float bu = x[i] * r1;
-          if constexpr (EachRow) {
-            // gate holds scale gate; what the gate's gradient needs is kept in its place
-            const float dgb = gate[c][i] * d;
-            sum_a[c][i] += dgb * bu;
-            u[c][i] = dgb * gp[c][i];
-            gate[c][i] = f.scale * d * gp[c][i] * bu;
-          } else {
-            sum_a[c][i] += d * bu;
-            u[c][i] = d * gp[c][i];
-          }
-          s1 += u[c][i] * bu;
+      for (int i = 0; i < N; ++i) {
+        const float bu = x[i] * r1;
+        if constexpr (EachRow) {
+          // gate holds scale gate; what the gate's gradient needs is kept in its place
+          const float dgb = gate[c][i] * dr[i];
+          sum_a[c][i] += dgb * bu;
+          u[c][i] = dgb * gp[c][i];
+          gate[c][i] = f.scale * dr[i] * gp[c][i] * bu;
+        } else {
+          sum_a[c][i] += dr[i] * bu;
+          u[c][i] = dr[i] * gp[c][i];
         }
-        store<T, N>(a.grad_residual + row * f.width + col[c], dr);
+        s[(N == 1 ? c : i) & 3] += u[c][i] * bu;
+      }
+      if (own[c]) {
+        store<T, N>(grad_residual + col[c], dr);
         if constexpr (EachRow) {
           if (a.gate_out && a.gate_out32) store32<N>(static_cast<float*>(a.gate_out) + row * f.width + col[c], gate[c]);
           else if (a.gate_out) store<T, N>(static_cast<T*>(a.gate_out) + row * f.width + col[c], gate[c]);
         }
       }
+    }
     if (has_post) {
-      const float m1 = total(s1) * inv;
+      const float m1 = total((s[0] + s[1]) + (s[2] + s[3])) * inv * r1 * r1;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (own[c]) {
-          float x[N];
-          piece(stage, 1, c, x);
+      for (int c = 0; c < C; ++c) {
+        float x[N];
+        piece(stage, 1, c, x);
 #pragma unroll
-          for (int i = 0; i < N; ++i) u[c][i] = r1 * (u[c][i] - x[i] * r1 * m1);
-        }
+        for (int i = 0; i < N; ++i) u[c][i] = r1 * u[c][i] - x[i] * m1;
+      }
     }
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (own[c]) store<T, N>(a.grad_block + row * f.width + col[c], u[c]);
+      if (own[c]) store<T, N>(grad_block + col[c], u[c]);
+    grad_residual += int64_t(row_step) * f.width;
+    grad_block += int64_t(row_step) * f.width;
+    row += row_step;
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
   if constexpr (kRing) wait_groups<0>();
@@ -782,6 +851,7 @@ struct JoinArgs {
   Param<T> post, gate;
   int64_t gate_rows;
   int parts, chunks, width, pre32, post32, gate32, items;
+  int64_t jobs;                          // output rows
   float scale;
 };
 
@@ -791,8 +861,7 @@ __global__ void __launch_bounds__(32 * kLanes) grad_join_kernel(const __grid_con
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
   const bool single = a.part_a && a.items == a.chunks;   // one segment, with or without a gate
-  const int64_t jobs = single ? 2 : 2 + a.gate_rows;
-  for (int64_t job = blockIdx.y; job < jobs; job += gridDim.y) {
+  for (int64_t job = blockIdx.y; job < a.jobs; job += gridDim.y) {
     const float* part = job == 0 ? a.part_pre : job == 1 ? (a.part_post ? a.part_post : a.part_a) : a.part_a;
     if (!part || !(job == 0 ? a.grad_pre : job == 1 ? (single && a.grad_gate ? a.grad_gate : a.grad_post) : a.grad_gate)) continue;
     const bool gated = job == 1 && part == a.part_a && !single;                // dw_post from every segment's A
@@ -884,64 +953,19 @@ bool wide(const NormArgs<T>& a, bool outputs) {
   return ok;
 }
 int threads_for(int pieces, int per) { return ((pieces + per - 1) / per + 31) / 32 * 32; }
-// CTAs of so many threads that share an SM's 512.
-int share_of_sm(int threads) { return 512 / threads > 4 ? 4 : 512 / threads; }
+// CTAs of so many threads that an SM holds, of `room` threads at most.
+int share_of_sm(int threads, int room) { return room / threads > 8 ? 8 : room / threads; }
+int ranks_for(int pieces, int most) { return pieces <= most ? 1 : pieces <= 2 * most ? 2 : pieces <= 4 * most ? 4 : 8; }
 
-std::atomic<int> g_norm_smem[3][2][kMaxDevices];         // by type, gate per row
-std::atomic<int> g_grad_smem[3][3][2][kMaxDevices];      // by type, threads of a row, gate per row
+std::atomic<int> g_norm_smem[3][2][2][2][2][kMaxDevices];   // by type, pieces of a thread, warps, gate per row, cluster
+std::atomic<int> g_grad_smem[3][2][2][2][2][kMaxDevices];
 template <class T> constexpr int kType = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 1 : 2;
 
-template <class T>
-cudaError_t launch_forward(const pm_block_norm* j, int sms, cudaStream_t s) {
-  const NormArgs<T> a = forward_args<T>(j);
-  const bool fits = a.rows <= 0x7fffffff, each_row = a.gate_rows == a.rows && a.rows > 1;
-  if (wide(a, true) && fits) {
-    const int pieces = a.width / kWide<T>;
-    if (pieces <= 64) {
-      const unsigned grid = unsigned((a.rows + 7) / 8);
-      if (pieces <= 32) norm_row_kernel<T, kWide<T>, 1, true><<<grid, 256, 0, s>>>(a);
-      else norm_row_kernel<T, kWide<T>, 2, true><<<grid, 256, 0, s>>>(a);
-      return cudaGetLastError();
-    }
-    if (pieces <= 1024 && aligned(a.stats, 8)) {
-      const int threads = threads_for(pieces, 2), most = sms * share_of_sm(threads);
-      const unsigned grid = unsigned(a.rows < most ? a.rows : most);
-      const size_t bytes = size_t(kNormStages) * (each_row ? 3 : 2) * 2 * threads * 16;
-      if (each_row) {
-        ensure_dynamic_smem(norm_stream_kernel<T, true>, 1024, bytes, g_norm_smem[kType<T>][1]);
-        norm_stream_kernel<T, true><<<grid, threads, bytes, s>>>(a);
-      } else {
-        ensure_dynamic_smem(norm_stream_kernel<T, false>, 1024, bytes, g_norm_smem[kType<T>][0]);
-        norm_stream_kernel<T, false><<<grid, threads, bytes, s>>>(a);
-      }
-      return cudaGetLastError();
-    }
-    if (pieces <= 2048) {
-      norm_row_kernel<T, kWide<T>, 2, false><<<unsigned(a.rows), threads_for(pieces, 2), 0, s>>>(a);
-      return cudaGetLastError();
-    }
-  }
-  if (fits && a.width <= 8192) {                         // single elements, 8 a thread
-    norm_row_kernel<T, 1, kSingles, false><<<unsigned(a.rows), threads_for(a.width, kSingles), 0, s>>>(a);
-    return cudaGetLastError();
-  }
-  const int64_t most = int64_t(sms) * 8;
-  norm_loop_kernel<T><<<int(a.rows < most ? a.rows : most), 256, 0, s>>>(a);
-  return cudaGetLastError();
-}
-
-template <class T, int N, bool Warps, bool EachRow, bool Cluster>
-cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int threads, cudaStream_t s) {
-  const auto kernel = grad_row_kernel<T, N, Warps, EachRow, Cluster>;
-  size_t bytes = 0;
-  if (N > 1) {
-    bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * 2 * threads * 16;
-    const size_t sums = Warps ? size_t(2) * (threads / 32) * a.f.width * 4 : 0;
-    if (sums > bytes) bytes = sums;
-    ensure_dynamic_smem(kernel, 1024, bytes, g_grad_smem[kType<T>][Warps ? 0 : Cluster ? 1 : 2][EachRow]);
-  }
+template <class... Args>
+cudaError_t launch_rows(void (*kernel)(Args...), int ctas, int ranks, int threads, size_t bytes, std::atomic<int>* limits, cudaStream_t s, Args... args) {
+  if (bytes) ensure_dynamic_smem(kernel, 1024, bytes, limits);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(parts * ranks));
+  cfg.gridDim = dim3(unsigned(ctas * ranks));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
@@ -950,8 +974,69 @@ cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int thr
   attr[0].val.clusterDim.x = ranks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = Cluster ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <class T, int C, bool Warps, bool EachRow, bool Cluster>
+cudaError_t launch_norm_stream(const NormArgs<T>& a, int ctas, int ranks, int threads, int slice, cudaStream_t s) {
+  return launch_rows(norm_stream_kernel<T, C, Warps, EachRow, Cluster>, ctas, ranks, threads,
+                     size_t(kNormStages) * (EachRow ? 3 : 2) * C * threads * 16, g_norm_smem[kType<T>][C - 1][Warps][EachRow][Cluster], s, a, slice);
+}
+template <class T, bool EachRow>
+cudaError_t launch_norm_streams(const NormArgs<T>& a, int pieces, int sms, cudaStream_t s) {
+  auto of_rows = [&](int64_t per, int most) { return int((a.rows + per - 1) / per < most ? (a.rows + per - 1) / per : most); };
+  if (pieces <= 32) return launch_norm_stream<T, 1, true, EachRow, false>(a, of_rows(8, sms * 4), 1, 256, pieces, s);
+  if (pieces <= 64) return launch_norm_stream<T, 2, true, EachRow, false>(a, of_rows(8, sms * 2), 1, 256, pieces, s);
+  // one piece a thread (64 registers, 1024 threads an SM); of more than 768, two (512 threads of 128): 4.5 against 3.6
+  // of 6.5 TB/s at 1024 pieces, where 32 warps wait for one another in every sum
+  const int ranks = ranks_for(pieces, 1024), slice = (pieces + ranks - 1) / ranks, per = slice > 768 ? 2 : 1, threads = threads_for(slice, per);
+  if (ranks > 1)
+    return per == 2 ? launch_norm_stream<T, 2, false, EachRow, true>(a, of_rows(1, sms / ranks), ranks, threads, slice, s)
+                    : launch_norm_stream<T, 1, false, EachRow, true>(a, of_rows(1, sms / ranks), ranks, threads, slice, s);
+  return per == 2 ? launch_norm_stream<T, 2, false, EachRow, false>(a, of_rows(1, sms), 1, threads, slice, s)
+                  : launch_norm_stream<T, 1, false, EachRow, false>(a, of_rows(1, sms * share_of_sm(threads, 1024)), 1, threads, slice, s);
+}
+
+template <class T>
+cudaError_t launch_forward(const pm_block_norm* j, int sms, cudaStream_t s) {
+  const NormArgs<T> a = forward_args<T>(j);
+  const bool fits = a.rows <= 0x7fffffff, each_row = a.gate_rows == a.rows && a.rows > 1;
+  const int pieces = a.width / kWide<T>;
+  if (wide(a, true) && fits && pieces <= 8192 && aligned(a.stats, 8))
+    return each_row ? launch_norm_streams<T, true>(a, pieces, sms, s) : launch_norm_streams<T, false>(a, pieces, sms, s);
+  if (fits && a.width <= 1024 * kSingles) {
+    norm_row_kernel<T, 1, kSingles, false><<<unsigned(a.rows), threads_for(a.width, kSingles), 0, s>>>(a);
+    return cudaGetLastError();
+  }
+  const int64_t most = int64_t(sms) * 8;
+  norm_loop_kernel<T><<<int(a.rows < most ? a.rows : most), 256, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <class T, int N, int C, bool Warps, bool EachRow, bool Cluster>
+cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int threads, cudaStream_t s) {
+  size_t bytes = 0;
+  if (N > 1) {
+    bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * C * threads * 16;
+    const size_t sums = Warps ? size_t(2) * (threads / 32) * a.f.width * 4 : 0;
+    if (sums > bytes) bytes = sums;
+  }
+  return launch_rows(grad_row_kernel<T, N, C, Warps, EachRow, Cluster>, parts, ranks, threads, bytes,
+                     g_grad_smem[kType<T>][C == 2][Warps][EachRow][Cluster], s, a);
+}
+template <class T, bool EachRow>
+cudaError_t launch_grad_streams(const GradArgs<T>& a, bool rows16, bool by_warps, int per, int parts, int ranks, int threads, cudaStream_t s) {
+  constexpr int N = kWide<T>;
+  if (!rows16)
+    return ranks > 1 ? launch_grad_rows<T, 1, kSingles, false, EachRow, true>(a, parts, ranks, threads, s)
+                     : launch_grad_rows<T, 1, kSingles, false, EachRow, false>(a, parts, 1, threads, s);
+  if (by_warps)
+    return per == 1 ? launch_grad_rows<T, N, 1, true, EachRow, false>(a, parts, 1, 256, s)
+                    : launch_grad_rows<T, N, 2, true, EachRow, false>(a, parts, 1, 256, s);
+  if (ranks > 1) return launch_grad_rows<T, N, 2, false, EachRow, true>(a, parts, ranks, threads, s);
+  return per == 1 ? launch_grad_rows<T, N, 1, false, EachRow, false>(a, parts, 1, threads, s)
+                  : launch_grad_rows<T, N, 2, false, EachRow, false>(a, parts, 1, threads, s);
 }
 
 template <class T>
@@ -970,15 +1055,29 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
   const bool rows16 = wide(a.f, false) && aligned(a.grad_residual, 16) && aligned(a.grad_block, 16) && aligned(d->grad_gate, 16) &&
                       (!a.grad_hidden || (aligned(a.grad_hidden, 16) && a.grad_hidden_stride % N == 0)) &&
                       (!a.grad_normed || (aligned(a.grad_normed, 16) && a.grad_normed_stride % N == 0));
-  // pieces of 16 bytes, or single elements
-  const int pieces = rows16 ? j->width / N : j->width, per = rows16 ? 2 : kSingles;
-  const int ranks = !rows16 || pieces <= 1024 ? 1 : pieces <= 2048 ? 2 : pieces <= 4096 ? 4 : 8;
-  bool streamed = aligned(a.f.stats, 8) && pieces <= (rows16 ? 8192 : 512 * kSingles);
+  // pieces of 16 bytes, or single elements; 512 threads of a CTA at most, with one or two pieces or kSingles elements each
+  const int pieces = rows16 ? j->width / N : j->width;
+  const int ranks = ranks_for(pieces, rows16 ? 1024 : 512 * kSingles);
+  bool streamed = j->rows <= 0x7fffffff && aligned(a.f.stats, 8) && pieces <= 8 * (rows16 ? 1024 : 512 * kSingles);
   a.slice = (pieces + ranks - 1) / ranks;
-  const int row_threads = streamed ? threads_for(a.slice, per) : 256;
   // rows of up to 64 pieces go by warps, 8 of them a CTA, where a CTA stays in one segment or every row has its gate
   const bool by_warps = streamed && rows16 && pieces <= 64;
-  int want = !streamed || by_warps ? 2 * sms : ranks > 1 ? sms / ranks : sms * share_of_sm(row_threads);
+  int per = rows16 ? 2 : kSingles, row_threads = 256, want = 2 * sms;
+  if (by_warps) {
+    per = pieces <= 32 ? 1 : 2;
+    want = 2 * sms;
+  } else if (streamed) {
+    row_threads = threads_for(a.slice, per);
+    int held = share_of_sm(row_threads, 512);
+    // one piece a thread where its 640 threads (of 96 registers) are more than an SM holds with two
+    const int ones = threads_for(a.slice, 1);
+    if (rows16 && ranks == 1 && ones <= 640 && ones > held * row_threads) {
+      per = 1;
+      row_threads = ones;
+      held = 1;
+    }
+    want = ranks > 1 ? sms / ranks : sms * held;
+  }
   if (want > kMaxParts) want = kMaxParts;
   if (want < 1) want = 1;
   const Split sp = split_rows(j->rows, j->gate_rows, want);
@@ -1002,27 +1101,18 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
   if (!streamed) {
     grad_loop_kernel<T><<<sp.parts, 256, 0, s>>>(a);
     e = cudaGetLastError();
-  } else if (!rows16) {
-    e = each_row ? launch_grad_rows<T, 1, false, true, false>(a, sp.parts, 1, row_threads, s)
-                 : launch_grad_rows<T, 1, false, false, false>(a, sp.parts, 1, row_threads, s);
-  } else if (by_warps) {
-    e = each_row ? launch_grad_rows<T, N, true, true, false>(a, sp.parts, 1, 256, s)
-                 : launch_grad_rows<T, N, true, false, false>(a, sp.parts, 1, 256, s);
-  } else if (ranks > 1) {
-    e = each_row ? launch_grad_rows<T, N, false, true, true>(a, sp.parts, ranks, row_threads, s)
-                 : launch_grad_rows<T, N, false, false, true>(a, sp.parts, ranks, row_threads, s);
   } else {
-    e = each_row ? launch_grad_rows<T, N, false, true, false>(a, sp.parts, 1, row_threads, s)
-                 : launch_grad_rows<T, N, false, false, false>(a, sp.parts, 1, row_threads, s);
+    e = each_row ? launch_grad_streams<T, true>(a, rows16, by_warps, per, sp.parts, ranks, row_threads, s)
+                 : launch_grad_streams<T, false>(a, rows16, by_warps, per, sp.parts, ranks, row_threads, s);
   }
   if (e != cudaSuccess) return e;
   const bool gate_joined = wants_gate && by_a;
   if (!d->grad_pre && !wants_post && !gate_joined) return cudaSuccess;
+  const int64_t jobs = by_a && sp.segments == 1 ? 2 : 2 + (gate_joined ? j->gate_rows : 0);
   JoinArgs<T> q{a.part_pre, a.part_a, a.part_post, d->grad_pre, wants_post ? d->grad_post : nullptr,
                 gate_joined ? d->grad_gate : nullptr, a.f.post, a.f.gate, j->gate_rows, sp.parts, sp.chunks, j->width,
                 j->pre_dtype == PM_DT_F32, j->post_dtype == PM_DT_F32, j->gate_dtype == PM_DT_F32,
-                int(by_a ? sp.segments * sp.chunks : 0), j->scale};
-  const int64_t jobs = by_a && sp.segments == 1 ? 2 : 2 + (gate_joined ? j->gate_rows : 0);
+                int(by_a ? sp.segments * sp.chunks : 0), jobs, j->scale};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned((j->width + 31) / 32), unsigned(jobs < 65535 ? jobs : 65535));
   cfg.blockDim = dim3(32 * kLanes);
