@@ -436,6 +436,8 @@ __device__ __forceinline__ Run run_of(int64_t rows, int64_t segments, int chunks
   return {items * part / parts, items * (part + 1) / parts, rows / segments, chunks};
 }
 
+// Whether w_pre lives in shared memory: where 640 threads or a warp with two pieces run out of registers.
+constexpr __host__ __device__ bool pre_shared(int n, int c, bool warps) { return n == 8 && (warps ? c == 2 : c == 1); }
 // Rows in a ring: 512 threads of an SM then hold 192 (EachRow: 160) KB of them.
 constexpr __host__ __device__ int stages_of(bool each_row) { return each_row ? 2 : 3; }
 
@@ -447,6 +449,7 @@ template <class T, int N, int C, bool Warps, bool EachRow, bool Cluster>
 __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 1) grad_row_kernel(const __grid_constant__ GradArgs<T> a) {
   constexpr bool kRing = N > 1;
   constexpr int kArrays = EachRow ? 5 : 4, kStages = stages_of(EachRow);
+  constexpr bool kPreShared = pre_shared(N, C, Warps);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float red[2][32];
   __shared__ float shared_sum[2][8];
@@ -474,6 +477,7 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
   // a thread's copies: [stage][array][c], 16 bytes each, threads side by side.  A piece beyond the row, and a gradient
   // that does not come in, stay zero and add nothing: only copies, parameters and stores ask whose a piece is.
   const int row_bytes = kArrays * C * width_threads * 16;
+  const int ring_bytes = kStages * kArrays * C * blockDim.x * 16;
   uint8_t* ring = smem + (Warps ? warp * kStages * row_bytes : 0) + me * 16;
   const uint32_t ring_addr = smem_addr(ring);
   Raw<T, N> now[kRing ? 1 : 4][C], next[kRing ? 1 : 4][C];
@@ -529,13 +533,28 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
       commit();
     }
   };
+  float pre_held[kPreShared ? 1 : C][N] = {};
+  // w_pre of a piece: in registers, or, where those are short, in this thread's own shared memory behind the ring
+  auto pre_place = [&](int c) { return reinterpret_cast<float*>(smem + ring_bytes + ((Warps ? warp * C : 0) + c) * width_threads * N * 4) + me * 4; };
+  auto pre_of = [&](int c, float (&w)[N]) {
+    if constexpr (kPreShared) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        const float4 q = *reinterpret_cast<const float4*>(pre_place(c) + i * width_threads * 4);
+        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = pre_held[c][i];
+    }
+  };
   auto piece = [&](int stage, int array, int c, float (&v)[N]) {
     if constexpr (kRing) Raw<T, N>{*reinterpret_cast<const uint4*>(ring + slot(stage, array, c))}.unpack(v);
     else now[array][c].unpack(v);
   };
 
-  // pre, and gp = scale gate w_post of the segment (EachRow: w_post)
-  float pre[C][N] = {}, gp[C][N] = {}, sum_p[C][N] = {}, sum_a[C][N] = {};   // EachRow: sum_a is sum scale gate dh bu
+  // gp = scale gate w_post of the segment (EachRow: w_post)
+  float gp[C][N] = {}, sum_p[C][N] = {}, sum_a[C][N] = {};   // EachRow: sum_a is sum scale gate dh bu
   auto load_gp = [&](int64_t segment) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -584,7 +603,17 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
   for (int i = 0; i < (kRing ? kStages - 1 : 1); ++i) fetch();
 #pragma unroll
   for (int c = 0; c < C; ++c)
-    if (own[c]) param_piece<T, N>(f.pre, col[c], pre[c]);
+    if (own[c]) {
+      if constexpr (kPreShared) {
+        float w[N];
+        param_piece<T, N>(f.pre, col[c], w);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i)
+          *reinterpret_cast<float4*>(pre_place(c) + i * width_threads * 4) = make_float4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      } else {
+        param_piece<T, N>(f.pre, col[c], pre_held[c]);
+      }
+    }
   load_gp(EachRow ? 0 : item / a.chunks);
   const float2* st = reinterpret_cast<const float2*>(f.stats) + row;
   float2 st_next = left ? *st : make_float2(0.0f, 0.0f);
@@ -616,10 +645,11 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
     float u[C][N], gate[EachRow ? C : 1][N], s[4] = {};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float x[N], gy[N];
+      float x[N], gy[N], pre[N];
       piece(stage, 0, c, u[c]);
       piece(stage, 1, c, x);
       piece(stage, 3, c, gy);
+      pre_of(c, pre);
       if constexpr (EachRow) {
         if (kRing && !f.gate.f32) {
           if constexpr (kRing) piece(stage, 4, c, gate[c]);
@@ -632,21 +662,24 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         u[c][i] = (u[c][i] + (EachRow ? gate[c][i] * gp[c][i] : gp[c][i]) * (x[i] * r1)) * r2;
-        s[(N == 1 ? c : i) & 3] += gy[i] * pre[c][i] * u[c][i];
+        s[(N == 1 ? c : i) & 3] += gy[i] * pre[i] * u[c][i];
       }
     }
     const float m2 = has_gy ? total((s[0] + s[1]) + (s[2] + s[3])) * inv * r2 : 0.0f;
     s[0] = s[1] = s[2] = s[3] = 0.0f;
+    asm volatile("" ::: "memory");                       // the next part's loads stay there: their registers are needed here
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float x[N], gy[N], dr[N];
       piece(stage, 1, c, x);
       piece(stage, 2, c, dr);
       if (has_gy) {
+        float pre[N];
+        pre_of(c, pre);
         piece(stage, 3, c, gy);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          dr[i] += pre[c][i] * (r2 * gy[i]) - u[c][i] * m2;
+          dr[i] += pre[i] * (r2 * gy[i]) - u[c][i] * m2;
           sum_p[c][i] += gy[i] * u[c][i];
         }
       }
@@ -675,6 +708,7 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
     }
     if (has_post) {
       const float m1 = total((s[0] + s[1]) + (s[2] + s[3])) * inv * r1 * r1;
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float x[N];
@@ -1018,7 +1052,7 @@ template <class T, int N, int C, bool Warps, bool EachRow, bool Cluster>
 cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int threads, cudaStream_t s) {
   size_t bytes = 0;
   if (N > 1) {
-    bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * C * threads * 16;
+    bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * C * threads * 16 + (pre_shared(N, C, Warps) ? size_t(C) * threads * N * 4 : 0);
     const size_t sums = Warps ? size_t(2) * (threads / 32) * a.f.width * 4 : 0;
     if (sums > bytes) bytes = sums;
   }
