@@ -285,8 +285,8 @@ __device__ __forceinline__ RowSum<Warps, Cluster> row_sum(float (&red)[2][32], f
 // EachRow: the gate changes with every row, and streams with them when it is
 // of type T.
 constexpr int kNormStages = 4;
-template <class T, int C, bool Warps, bool EachRow, bool Cluster>
-__global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 1024 : 512, Warps ? (C == 1 ? 4 : 2) : 1) norm_stream_kernel(const __grid_constant__ NormArgs<T> a, int slice_pieces) {
+template <class T, int C, bool Warps, bool EachRow, bool Cluster, int kTwo = 0>
+__global__ void __launch_bounds__(Warps ? 256 : kTwo ? 384 : C == 1 ? 1024 : 512, Warps ? (C == 1 ? 4 : 2) : kTwo ? 2 : 1) norm_stream_kernel(const __grid_constant__ NormArgs<T> a, int slice_pieces) {
   constexpr int N = kWide<T>, kArrays = EachRow ? 3 : 2;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float red[2][32];
@@ -603,16 +603,14 @@ __global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 
   for (int i = 0; i < (kRing ? kStages - 1 : 1); ++i) fetch();
 #pragma unroll
   for (int c = 0; c < C; ++c)
-    if (own[c]) {
-      if constexpr (kPreShared) {
-        float w[N];
-        param_piece<T, N>(f.pre, col[c], w);
+    if constexpr (kPreShared) {
+      float w[N] = {};                                   // zeros for a piece beyond the row
+      if (own[c]) param_piece<T, N>(f.pre, col[c], w);
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i)
-          *reinterpret_cast<float4*>(pre_place(c) + i * width_threads * 4) = make_float4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      } else {
-        param_piece<T, N>(f.pre, col[c], pre_held[c]);
-      }
+      for (int i = 0; i < N / 4; ++i)
+        *reinterpret_cast<float4*>(pre_place(c) + i * width_threads * 4) = make_float4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else {
+      if (own[c]) param_piece<T, N>(f.pre, col[c], pre_held[c]);
     }
   load_gp(EachRow ? 0 : item / a.chunks);
   const float2* st = reinterpret_cast<const float2*>(f.stats) + row;
@@ -989,11 +987,9 @@ bool wide(const NormArgs<T>& a, bool outputs) {
 int threads_for(int pieces, int per) { return ((pieces + per - 1) / per + 31) / 32 * 32; }
 // CTAs of so many threads that an SM holds, of `room` threads at most.
 int share_of_sm(int threads, int room) { return room / threads > 8 ? 8 : room / threads; }
+// CTAs of the cluster that shares a row, as few as hold it: 16384 bf16 wide, 2 take 199 us for 4096 rows and 4 take 298 us
+// (two rows an SM under way do not make up for the wider cluster's barriers).
 int ranks_for(int pieces, int most) { return pieces <= most ? 1 : pieces <= 2 * most ? 2 : pieces <= 4 * most ? 4 : 8; }
-
-std::atomic<int> g_norm_smem[3][2][2][2][2][kMaxDevices];   // by type, pieces of a thread, warps, gate per row, cluster
-std::atomic<int> g_grad_smem[3][2][2][2][2][kMaxDevices];
-template <class T> constexpr int kType = sizeof(T) == 4 ? 0 : std::is_same<T, bf16>::value ? 1 : 2;
 
 template <class... Args>
 cudaError_t launch_rows(void (*kernel)(Args...), int ctas, int ranks, int threads, size_t bytes, std::atomic<int>* limits, cudaStream_t s, Args... args) {
@@ -1012,10 +1008,11 @@ cudaError_t launch_rows(void (*kernel)(Args...), int ctas, int ranks, int thread
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <class T, int C, bool Warps, bool EachRow, bool Cluster>
+template <class T, int C, bool Warps, bool EachRow, bool Cluster, int kTwo = 0>
 cudaError_t launch_norm_stream(const NormArgs<T>& a, int ctas, int ranks, int threads, int slice, cudaStream_t s) {
-  return launch_rows(norm_stream_kernel<T, C, Warps, EachRow, Cluster>, ctas, ranks, threads,
-                     size_t(kNormStages) * (EachRow ? 3 : 2) * C * threads * 16, g_norm_smem[kType<T>][C - 1][Warps][EachRow][Cluster], s, a, slice);
+  static std::atomic<int> limits[kMaxDevices];           // of this kernel
+  return launch_rows(norm_stream_kernel<T, C, Warps, EachRow, Cluster, kTwo>, ctas, ranks, threads,
+                     size_t(kNormStages) * (EachRow ? 3 : 2) * C * threads * 16, limits, s, a, slice);
 }
 template <class T, bool EachRow>
 cudaError_t launch_norm_streams(const NormArgs<T>& a, int pieces, int sms, cudaStream_t s) {
@@ -1024,10 +1021,12 @@ cudaError_t launch_norm_streams(const NormArgs<T>& a, int pieces, int sms, cudaS
   if (pieces <= 64) return launch_norm_stream<T, 2, true, EachRow, false>(a, of_rows(8, sms * 2), 1, 256, pieces, s);
   // one piece a thread (64 registers, 1024 threads an SM); of more than 768, two (512 threads of 128): 4.5 against 3.6
   // of 6.5 TB/s at 1024 pieces, where 32 warps wait for one another in every sum
+  if (pieces > 512 && pieces <= 768) return launch_norm_stream<T, 2, false, EachRow, false, 1>(a, of_rows(1, sms * 2), 1, threads_for(pieces, 2), pieces, s);
   const int ranks = ranks_for(pieces, 1024), slice = (pieces + ranks - 1) / ranks, per = slice > 768 ? 2 : 1, threads = threads_for(slice, per);
-  if (ranks > 1)
-    return per == 2 ? launch_norm_stream<T, 2, false, EachRow, true>(a, of_rows(1, sms / ranks), ranks, threads, slice, s)
-                    : launch_norm_stream<T, 1, false, EachRow, true>(a, of_rows(1, sms / ranks), ranks, threads, slice, s);
+  if (ranks > 1) {
+    const int pairs = threads_for(slice, 2), most = sms * share_of_sm(pairs, 512) / ranks;
+    return launch_norm_stream<T, 2, false, EachRow, true>(a, of_rows(1, most > 1 ? most : 1), ranks, pairs, slice, s);
+  }
   return per == 2 ? launch_norm_stream<T, 2, false, EachRow, false>(a, of_rows(1, sms), 1, threads, slice, s)
                   : launch_norm_stream<T, 1, false, EachRow, false>(a, of_rows(1, sms * share_of_sm(threads, 1024)), 1, threads, slice, s);
 }
@@ -1056,8 +1055,8 @@ cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int thr
     const size_t sums = Warps ? size_t(2) * (threads / 32) * a.f.width * 4 : 0;
     if (sums > bytes) bytes = sums;
   }
-  return launch_rows(grad_row_kernel<T, N, C, Warps, EachRow, Cluster>, parts, ranks, threads, bytes,
-                     g_grad_smem[kType<T>][C == 2][Warps][EachRow][Cluster], s, a);
+  static std::atomic<int> limits[kMaxDevices];           // of this kernel
+  return launch_rows(grad_row_kernel<T, N, C, Warps, EachRow, Cluster>, parts, ranks, threads, bytes, limits, s, a);
 }
 template <class T, bool EachRow>
 cudaError_t launch_grad_streams(const GradArgs<T>& a, bool rows16, bool by_warps, int per, int parts, int ranks, int threads, cudaStream_t s) {
@@ -1110,7 +1109,7 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
       row_threads = ones;
       held = 1;
     }
-    want = ranks > 1 ? sms / ranks : sms * held;
+    want = sms * held / ranks;
   }
   if (want > kMaxParts) want = kMaxParts;
   if (want < 1) want = 1;

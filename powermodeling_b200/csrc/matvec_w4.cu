@@ -484,8 +484,6 @@ __global__ void __launch_bounds__(kJoinThreads) w4_join_kernel(const __grid_cons
 }
 
 // ---------------------------------------------------------------- launch
-std::atomic<int> g_smem[2][2][4][2][kMaxDevices];
-
 // How a product is shared out.
 struct Plan {
   int nt, warps_n, ranks, stages;
@@ -565,7 +563,8 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   }
   const size_t bytes = size_t(L::kStages) * stage_size<NT>(held, warps_k) + 1024;
   const auto kernel = w4_kernel<T, NT, GB, Boxes>;
-  ensure_dynamic_smem(kernel, 1024, bytes, g_smem[std::is_same<T, fp16>::value][NT - 1][GB == 8 ? 3 : GB / 2][Boxes]);
+  static std::atomic<int> limits[kMaxDevices];           // of this kernel
+  ensure_dynamic_smem(kernel, 1024, bytes, limits);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(p.ctas), 1, (a.tokens + 8 * NT - 1) / (8 * NT));
   cfg.blockDim = dim3(32 * kWarps + (Boxes ? kBoxThreads : kWordThreads));

@@ -465,21 +465,18 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
 int tiles_of_heads(int share, int head_dim) { return share > 8 && head_dim <= 128 ? 2 : 1; }
 constexpr int kMaxRuns = 148 * 4;        // CTAs of the first kernel at most: sizes the scratch
 
-std::atomic<int> g_occupancy[kMaxDevices][2][4][2];
-std::atomic<int> g_smem_limit[2][4][2][kMaxDevices];
-
 template <class T, int DP, int NT>
 cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s) {
   using S = Shape<T, DP, NT>;
-  constexpr int ti = std::is_same<T, fp16>::value ? 1 : 0;
+  static std::atomic<int> occupancy[kMaxDevices], limits[kMaxDevices];   // of this kernel
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
   const auto kernel = attention_runs_kernel<T, DP, NT>;
-  std::atomic<int>& known = g_occupancy[device][ti][DP / 64 - 1][NT - 1];
+  std::atomic<int>& known = occupancy[device];
   int occ = known.load(std::memory_order_relaxed);
   if (!occ) {
-    ensure_dynamic_smem(kernel, 4096, S::kSmem, g_smem_limit[ti][DP / 64 - 1][NT - 1]);
+    ensure_dynamic_smem(kernel, 4096, S::kSmem, limits);
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, kThreads, S::kSmem);
     if (e != cudaSuccess) return e;
     if (occ < 1) return cudaErrorInvalidConfiguration;
