@@ -33,6 +33,7 @@ namespace pm {
 namespace blk {
 namespace {
 
+constexpr int kMaxRuns = 148 * 4;        // CTAs of the first kernel at most: sizes the scratch
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kSlice = 16, kTile = kSlice * kWarps;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -92,7 +93,8 @@ __device__ __forceinline__ Span span_of(const pm_paged_attention& j, int b) {
 }
 
 // Tiles per sequence summed over the batch: thread t has the sum over the
-// sequences before its `per` consecutive ones, prefix[kThreads] all of them.
+// sequences before its `per` consecutive ones, prefix[Threads] all of them.
+template <int Threads>
 __device__ __forceinline__ int64_t scan_tiles(const pm_paged_attention& j, int per, int64_t* prefix) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   int64_t own = 0;
@@ -103,25 +105,29 @@ __device__ __forceinline__ int64_t scan_tiles(const pm_paged_attention& j, int p
     const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += v;
   }
-  __shared__ int64_t warp_sums[kWarps];
+  __shared__ int64_t warp_sums[Threads / 32];
   if (lane == 31) warp_sums[warp] = sum;
   __syncthreads();
   int64_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) before += w < warp ? warp_sums[w] : 0;
+  for (int w = 0; w < Threads / 32; ++w) before += w < warp ? warp_sums[w] : 0;
   prefix[t] = before + sum - own;
-  if (t == kThreads - 1) prefix[kThreads] = before + sum;
+  if (t == Threads - 1) prefix[Threads] = before + sum;
   __syncthreads();
-  return prefix[kThreads];
+  return prefix[Threads];
 }
 
 // ---------------------------------------------------------------- the runs
-// DP: head_dim rounded up to 64; NT: groups of 8 query heads served at once.
+// DP: the head size that the kernel is built for, at least head_dim; NT: groups
+// of 8 query heads served at once.  A row of shared memory is 16 bytes longer
+// than a head, which puts 8 rows' pieces in 32 different banks at every DP.
 template <class T, int DP, int NT>
 struct Shape {
   static constexpr int kHeads = 8 * NT;
-  static constexpr int kSliceBytes = 2 * kSlice * DP * 2;                       // K, then V
-  static constexpr int kStages = DP == 64 ? 4 : 3;
+  static constexpr int kPitch = DP * 2 + 16;
+  static constexpr int kSliceBytes = 2 * kSlice * kPitch;                       // K, then V
+  // two to three slices in flight per warp; with 12 to 16 warps an SM, 90 to 190 KB
+  static constexpr int kStages = DP <= 96 ? 3 : 2;
   static constexpr int kWarpBytes = kStages * kSliceBytes;
   static constexpr int kOutStride = DP + 4;                                     // floats; 8t + g: no two lanes in a bank
   static constexpr size_t kSmem = size_t(kWarps) * kWarpBytes;
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int D = j.head_dim, heads = j.kv_heads * a.blocks;
   const int per = (j.batch + kThreads - 1) / kThreads;
-  const int64_t total = scan_tiles(j, per, prefix) * heads;
+  const int64_t total = scan_tiles<kThreads>(j, per, prefix) * heads;
 
   // sequences without a live position: zeros
   for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
@@ -178,6 +184,13 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   int b = found_b;
   Span sp = span_of(j, b);
   int64_t base = found_before * heads;                   // the sequence's first tile on the line
+
+  // Slices that lie in one page, of heads without padding and with the same way from token to token in K and V, are
+  // copied by these offsets (elements) of a lane's pieces
+  const bool plain = D == DP && j.page_size % kSlice == 0 && j.k_token_stride == j.v_token_stride && j.k_token_stride < (1 << 26);
+  uint32_t from_row[kCopies];
+#pragma unroll
+  for (int c = 0; c < kCopies; ++c) from_row[c] = uint32_t((c * 32 + lane) / kChunks) * uint32_t(j.k_token_stride) + (c * 32 + lane) % kChunks * 8;
 
   uint8_t* mine = ring + warp * S::kWarpBytes;
   const uint32_t mine_addr = smem_addr(mine);
@@ -215,7 +228,21 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
         const int off = int(pos % uint32_t(j.page_size));
         const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
         if (lane == 0) live_of[warp][stage] = live;
-        const uint32_t kdst = mine_addr + stage * S::kSliceBytes, vdst = kdst + kSlice * DP * 2;
+        const uint32_t kdst = mine_addr + stage * S::kSliceBytes, vdst = kdst + kSlice * S::kPitch;
+        if (plain && live == 0xffffu && newest - (pos - lane) >= uint32_t(kSlice)) {
+          // the whole slice is live and in one page: rows a fixed way apart
+          const int page0 = __shfl_sync(0xffffffffu, page, 0), off0 = __shfl_sync(0xffffffffu, off, 0);
+          const T* ks = kc + page0 * j.k_page_stride + off0 * j.k_token_stride;
+          const T* vs = vc + page0 * j.v_page_stride + off0 * j.v_token_stride;
+#pragma unroll
+          for (int c = 0; c < kCopies; ++c) {
+            const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
+            copy16(kdst + row * S::kPitch + chunk * 16, ks + from_row[c], 16);
+            copy16(vdst + row * S::kPitch + chunk * 16, vs + from_row[c], 16);
+          }
+          commit();
+          return;
+        }
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
           const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
@@ -236,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
               vs = nv + chunk * 8;
             }
           }
-          const uint32_t at = uint32_t(row * kChunks + (chunk ^ (row & 7))) * 16;
+          const uint32_t at = row * S::kPitch + chunk * 16;
           copy16(kdst + at, ks, read ? 16 : 0);
           copy16(vdst + at, vs, read ? 16 : 0);
         }
@@ -281,26 +308,39 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
       const int stage = i % S::kStages;
       const uint32_t live = live_of[warp][stage];
       if (live) {
-        const uint32_t kbase = mine_addr + stage * S::kSliceBytes, vbase = kbase + kSlice * DP * 2;
-        float s[NT][4] = {};
+        const uint32_t kbase = mine_addr + stage * S::kSliceBytes, vbase = kbase + kSlice * S::kPitch;
+        float s[NT][4];
         {
-          const int row = lane & 15, half = lane >> 4;
+          // even and odd 16 dims apart: half as long a chain of sums
+          float odd[NT][4];
+          const uint32_t at = kbase + (lane & 15) * S::kPitch + (lane >> 4) * 16;
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k) {
             uint32_t ka[4];
-            ldsm(ka, kbase + uint32_t(row * kChunks + ((2 * k + half) ^ (row & 7))) * 16);
+            ldsm(ka, at + k * 32);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma<T>(s[n], ka, q[n][k][0], q[n][k][1]);
+            for (int n = 0; n < NT; ++n) {
+              if (k == 0) mma_first<T>(s[n], ka, q[n][k][0], q[n][k][1]);
+              else if (k == 1) mma_first<T>(odd[n], ka, q[n][k][0], q[n][k][1]);
+              else if (k & 1) mma<T>(odd[n], ka, q[n][k][0], q[n][k][1]);
+              else mma<T>(s[n], ka, q[n][k][0], q[n][k][1]);
+            }
           }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + odd[n][e]) * scale2;
         }
         const bool live_a = live >> g & 1, live_b = live >> (g + 8) & 1;
         uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          s[n][0] = live_a ? s[n][0] * scale2 : -INFINITY;
-          s[n][1] = live_a ? s[n][1] * scale2 : -INFINITY;
-          s[n][2] = live_b ? s[n][2] * scale2 : -INFINITY;
-          s[n][3] = live_b ? s[n][3] * scale2 : -INFINITY;
+          if (live != 0xffffu) {
+            s[n][0] = live_a ? s[n][0] : -INFINITY;
+            s[n][1] = live_a ? s[n][1] : -INFINITY;
+            s[n][2] = live_b ? s[n][2] : -INFINITY;
+            s[n][3] = live_b ? s[n][3] : -INFINITY;
+          }
           float m0 = fmaxf(s[n][0], s[n][2]), m1 = fmaxf(s[n][1], s[n][3]);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
@@ -333,11 +373,11 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
           lo[n][1] = transpose8(lo[n][1]);
         }
         {
-          const int row = (lane & 7) + (lane >> 4) * 8, half = lane >> 3 & 1;
+          const uint32_t at = vbase + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16;
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k) {
             uint32_t va[4];
-            ldsm_t(va, vbase + uint32_t(row * kChunks + ((2 * k + half) ^ (row & 7))) * 16);
+            ldsm_t(va, at + k * 32);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma<T>(o[n][k], va, hi[n][0], hi[n][1]);
@@ -417,17 +457,22 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   }
 }
 
-// Joins the pieces of each segment that was cut: one CTA per query head.
+// Joins the pieces of each segment that was cut: one CTA per query head.  A
+// thread has four neighbouring values; groups of threads take every so many
+// pieces, whose factors were computed by a thread each.
+constexpr int kJoinThreads = 256;
 template <class T, int NT>
-__global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
   constexpr int kHeads = 8 * NT;
   constexpr float kLift = std::is_same<T, fp16>::value ? 8.0f : 0.0f;
-  __shared__ int64_t prefix[kThreads + 1];
+  __shared__ int64_t prefix[kJoinThreads + 1];
+  __shared__ float factor[kMaxRuns], partial[8];
+  __shared__ float4 sums[kJoinThreads];
   const pm_paged_attention& j = a.j;
-  const int b = blockIdx.x / j.q_heads, h = blockIdx.x - b * j.q_heads;
+  const int b = blockIdx.x / j.q_heads, h = blockIdx.x - b * j.q_heads, t = threadIdx.x;
   const int heads = j.kv_heads * a.blocks, D = j.head_dim;
-  const int per = (j.batch + kThreads - 1) / kThreads;
-  const int64_t total = scan_tiles(j, per, prefix) * heads;
+  const int per = (j.batch + kJoinThreads - 1) / kJoinThreads;
+  const int64_t total = scan_tiles<kJoinThreads>(j, per, prefix) * heads;
   const int tiles = span_of(j, b).tiles;
   asm volatile("griddepcontrol.wait;" ::: "memory");    // in every CTA: this kernel's end has to mean the first one's
   if (!tiles) return;
@@ -437,33 +482,66 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const __grid_c
   const int64_t s0 = before * heads + int64_t(kvh * a.blocks + hb) * tiles, s1 = s0 + tiles;
   // run c holds tiles [total c / runs, total (c + 1) / runs)
   const int64_t runs = min(int64_t(ctas), total);
-  const int c0 = int(((s0 + 1) * runs - 1) / total), c1 = int((s1 * runs - 1) / total);
-  if (c0 == c1) return;
-  auto slot_of = [&](int c) { return 2 * int64_t(c) + (total * c / runs <= s0 ? 1 : 0); };
+  const int c0 = int(((s0 + 1) * runs - 1) / total), n = int((s1 * runs - 1) / total) - c0 + 1;
+  if (n == 1) return;
+  // the first piece may begin before the segment's run does: only that one is a run's second
+  auto slot_of = [&](int i) { return 2 * int64_t(c0 + i) + (i == 0 && total * c0 / runs <= s0 ? 1 : 0); };
   float m = -INFINITY;
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(&a.stat[slot_of(c) * kHeads + row]).x);
-  const float mb = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
-  const int d = threadIdx.x;
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t at = slot_of(c) * kHeads + row;
-    const float2 st = __ldcg(&a.stat[at]);
-    const float f = exp2_fast(st.x - mb);
-    l += st.y * f;
-    if (d < D) v0 += __ldcg(&a.part[at * D + d]) * f;
-    if (d + kThreads < D) v1 += __ldcg(&a.part[at * D + d + kThreads]) * f;
+  for (int i = t; i < n; i += kJoinThreads) {
+    const float top = __ldcg(&a.stat[slot_of(i) * kHeads + row]).x;
+    factor[i] = top;
+    m = fmaxf(m, top);
   }
-  T* out = static_cast<T*>(j.out) + (int64_t(b) * j.q_heads + h) * D;
-  if (d < D) out[d] = from_float<T>(l == 0.0f ? 0.0f : v0 / l);
-  if (d + kThreads < D) out[d + kThreads] = from_float<T>(l == 0.0f ? 0.0f : v1 / l);
-  if (j.lse && d == 0) j.lse[int64_t(b) * j.q_heads + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+#pragma unroll
+  for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  if ((t & 31) == 0) partial[t >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, partial[w]);
+  const float mb = m == -INFINITY ? 0.0f : m;
+  __syncthreads();
+  float l = 0.0f;
+  for (int i = t; i < n; i += kJoinThreads) {
+    const float f = exp2_fast(factor[i] - mb);
+    factor[i] = f;
+    l += __ldcg(&a.stat[slot_of(i) * kHeads + row]).y * f;
+  }
+  l = warp_sum(l);
+  if ((t & 31) == 0) partial[t >> 5] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) l += partial[w];
+  const int quads = D / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, lane = t % lanes, groups = kJoinThreads / lanes;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (lane < quads) {
+#pragma unroll 8
+    for (int i = t / lanes; i < n; i += groups) {
+      const float4 p = __ldcg(reinterpret_cast<const float4*>(a.part + (slot_of(i) * kHeads + row) * D) + lane);
+      const float f = factor[i];
+      v.x += p.x * f; v.y += p.y * f; v.z += p.z * f; v.w += p.w * f;
+    }
+  }
+  sums[t] = v;
+  __syncthreads();
+  if (t < quads) {
+    for (int g = 1; g < groups; ++g) {
+      const float4 p = sums[g * lanes + t];
+      v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+    }
+    T* out = static_cast<T*>(j.out) + (int64_t(b) * j.q_heads + h) * D + 4 * t;
+    out[0] = from_float<T>(l == 0.0f ? 0.0f : v.x / l);
+    out[1] = from_float<T>(l == 0.0f ? 0.0f : v.y / l);
+    out[2] = from_float<T>(l == 0.0f ? 0.0f : v.z / l);
+    out[3] = from_float<T>(l == 0.0f ? 0.0f : v.w / l);
+  }
+  if (j.lse && t == 0) j.lse[int64_t(b) * j.q_heads + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
 }
 
 // ---------------------------------------------------------------- launch
 // Query heads in groups of 8, two groups at once where more than 8 share a
 // key head and their registers allow it (head_dim up to 128).
 int tiles_of_heads(int share, int head_dim) { return share > 8 && head_dim <= 128 ? 2 : 1; }
-constexpr int kMaxRuns = 148 * 4;        // CTAs of the first kernel at most: sizes the scratch
 
 template <class T, int DP, int NT>
 cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s) {
@@ -497,7 +575,7 @@ cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s)
   if (e != cudaSuccess || room <= 1) return e;           // one tile at most: nothing is ever cut
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(j.batch * j.q_heads));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -514,6 +592,8 @@ cudaError_t launch(const pm_paged_attention& j, void* scratch, int sms, cudaStre
   a.share = j.q_heads / j.kv_heads;
   uint8_t* f = static_cast<uint8_t*>(scratch);
   const int nt = tiles_of_heads(a.share, j.head_dim);
+  if (j.head_dim > 64 && j.head_dim <= 80) return nt == 2 ? launch_shape<T, 80, 2>(a, f, sms, s) : launch_shape<T, 80, 1>(a, f, sms, s);
+  if (j.head_dim > 80 && j.head_dim <= 96) return nt == 2 ? launch_shape<T, 96, 2>(a, f, sms, s) : launch_shape<T, 96, 1>(a, f, sms, s);
   if (j.head_dim <= 64) return nt == 2 ? launch_shape<T, 64, 2>(a, f, sms, s) : launch_shape<T, 64, 1>(a, f, sms, s);
   if (j.head_dim <= 128) return nt == 2 ? launch_shape<T, 128, 2>(a, f, sms, s) : launch_shape<T, 128, 1>(a, f, sms, s);
   return j.head_dim <= 192 ? launch_shape<T, 192, 1>(a, f, sms, s) : launch_shape<T, 256, 1>(a, f, sms, s);
