@@ -5,8 +5,10 @@
 // V over the memory's rate bound it; what the kernel has to do is to keep
 // enough bytes in flight on every SM whatever the lengths are.
 //  * Work is counted in tiles of 64 positions of one (sequence, key head).
-//    All tiles of all sequences form one line that is cut into as many equal
-//    runs as CTAs are resident: the CTAs read the lengths and find their run
+//    All tiles of all sequences form one line, on which the start of each
+//    (sequence, key head) counts as two tiles more (filling and draining the
+//    copies takes about as long), and the line is cut into as many equal runs
+//    as CTAs are resident: the CTAs read the lengths and find their run
 //    themselves, so neither a long sequence nor a ragged batch leaves SMs
 //    idle and the host needs no lengths.  A run that ends inside a sequence
 //    leaves (maximum, sum, weighted values) in scratch, at most two such
@@ -34,6 +36,7 @@ namespace blk {
 namespace {
 
 constexpr int kMaxRuns = 148 * 4;        // CTAs of the first kernel at most: sizes the scratch
+constexpr int kSeam = 2;                 // what the start of a segment counts for, in tiles
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kSlice = 16, kTile = kSlice * kWarps;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -42,6 +45,12 @@ struct AttnArgs {
   int share, blocks;                     // query heads per key head; groups of them that one pass serves
   float* part;                           // [2 * CTAs, kHeads, head_dim] weighted values of split segments
   float2* stat;                          // [2 * CTAs, kHeads] (maximum, sum), base 2
+  struct Cut* cuts;                      // [CTAs]
+};
+// A segment that was cut, noted by the second run that has a piece of it.
+struct Cut {
+  int pieces, first_run;                 // 0 pieces: this run is no segment's second
+  int row, rows;                         // query rows, from the start of out
 };
 
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
@@ -91,14 +100,16 @@ __device__ __forceinline__ Span span_of(const pm_paged_attention& j, int b) {
   s.tiles = s.to > s.from ? int((s.to + kTile - 1) / kTile - s.first) : 0;
   return s;
 }
+// What one key head of a sequence takes on the line.
+__device__ __forceinline__ int length_of(int tiles) { return tiles ? tiles + kSeam : 0; }
 
-// Tiles per sequence summed over the batch: thread t has the sum over the
+// The sequences' lengths on the line, of one key head each, summed over the batch: thread t has the sum over the
 // sequences before its `per` consecutive ones, prefix[Threads] all of them.
 template <int Threads>
-__device__ __forceinline__ int64_t scan_tiles(const pm_paged_attention& j, int per, int64_t* prefix) {
+__device__ __forceinline__ int64_t scan_line(const pm_paged_attention& j, int per, int64_t* prefix) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   int64_t own = 0;
-  for (int b = t * per; b < min(j.batch, (t + 1) * per); ++b) own += span_of(j, b).tiles;
+  for (int b = t * per; b < min(j.batch, (t + 1) * per); ++b) own += length_of(span_of(j, b).tiles);
   int64_t sum = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -154,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int D = j.head_dim, heads = j.kv_heads * a.blocks;
   const int per = (j.batch + kThreads - 1) / kThreads;
-  const int64_t total = scan_tiles<kThreads>(j, per, prefix) * heads;
+  const int64_t total = scan_line<kThreads>(j, per, prefix) * heads;
 
   // sequences without a live position: zeros
   for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
@@ -166,6 +177,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   }
 
   const int64_t runs = min(int64_t(gridDim.x), total);   // no run is empty
+  if (threadIdx.x == 0) a.cuts[blockIdx.x].pieces = 0;
   if (blockIdx.x >= runs) return;
   int64_t cur = total * blockIdx.x / runs;
   const int64_t end = total * (blockIdx.x + 1) / runs;
@@ -173,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
     int64_t before = prefix[threadIdx.x];
     int b = threadIdx.x * per;
     for (;; ++b) {
-      const int n = span_of(j, b).tiles;
+      const int n = length_of(span_of(j, b).tiles);
       if (cur < (before + n) * heads) break;
       before += n;
     }
@@ -183,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   __syncthreads();
   int b = found_b;
   Span sp = span_of(j, b);
-  int64_t base = found_before * heads;                   // the sequence's first tile on the line
+  int64_t base = found_before * heads;                   // where the sequence starts on the line
 
   // Slices that lie in one page, of heads without padding and with the same way from token to token in K and V, are
   // copied by these offsets (elements) of a lane's pieces
@@ -197,259 +209,270 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   const float scale2 = j.scale * kLog2e;
 
   while (cur < end) {
-    const int which = int((cur - base) / sp.tiles);      // key head and group of query heads
+    const int length = length_of(sp.tiles);
+    const int which = int((cur - base) / length);        // key head and group of query heads
     const int kvh = which / a.blocks, hb = which - kvh * a.blocks;
-    const int t0 = int(cur - base - int64_t(which) * sp.tiles);
-    const int t1 = int(min(int64_t(sp.tiles), t0 + (end - cur)));
+    const int64_t s0 = base + int64_t(which) * length;   // the segment, and this run's part of it
+    const int part0 = int(cur - s0), part1 = int(min(int64_t(length), part0 + (end - cur)));
+    const int t0 = max(part0 - kSeam, 0), t1 = max(part1 - kSeam, 0);
     const int h0 = kvh * a.share + hb * S::kHeads, nh = min(S::kHeads, a.share - hb * S::kHeads);
-    const int n_slices = t1 - t0;                        // one slice of this warp in each tile
-    const uint32_t pos0 = (sp.first + t0) * uint32_t(kTile) + warp * kSlice;
-    const int32_t* table = j.table + b * j.table_stride;
-    const T* kc = static_cast<const T*>(j.k_cache) + kvh * j.k_head_stride;
-    const T* vc = static_cast<const T*>(j.v_cache) + kvh * j.v_head_stride;
-    const T* nk = static_cast<const T*>(j.new_k) + b * j.new_k_stride + kvh * j.new_k_head_stride;
-    const T* nv = static_cast<const T*>(j.new_v) + b * j.new_v_stride + kvh * j.new_v_head_stride;
-    const uint32_t newest = j.new_k ? uint32_t(max(j.lengths[b], 0)) - 1u : 0xffffffffu;
+    if (t1 > t0) {
+      const int n_slices = t1 - t0;                        // one slice of this warp in each tile
+      const uint32_t pos0 = (sp.first + t0) * uint32_t(kTile) + warp * kSlice;
+      const int32_t* table = j.table + b * j.table_stride;
+      const T* kc = static_cast<const T*>(j.k_cache) + kvh * j.k_head_stride;
+      const T* vc = static_cast<const T*>(j.v_cache) + kvh * j.v_head_stride;
+      const T* nk = static_cast<const T*>(j.new_k) + b * j.new_k_stride + kvh * j.new_k_head_stride;
+      const T* nv = static_cast<const T*>(j.new_v) + b * j.new_v_stride + kvh * j.new_v_head_stride;
+      const uint32_t newest = j.new_k ? uint32_t(max(j.lengths[b], 0)) - 1u : 0xffffffffu;
 
-    // the page of this lane's position (lanes 0-15) in slice i, -1 where it is not live
-    auto page_of = [&](int i) {
-      const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
-      int page = -1;
-      if (i < n_slices && lane < kSlice && pos >= sp.from && pos < sp.to) {
-        page = table[pos / uint32_t(j.page_size)];
-        if (page >= j.n_pages) page = -1;
-      }
-      return page;
-    };
-    auto fetch = [&](int i, int page) {
-      if (i < n_slices) {
-        const int stage = i % S::kStages;
+      // the page of this lane's position (lanes 0-15) in slice i, -1 where it is not live
+      auto page_of = [&](int i) {
         const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
-        const int off = int(pos % uint32_t(j.page_size));
-        const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-        if (lane == 0) live_of[warp][stage] = live;
-        const uint32_t kdst = mine_addr + stage * S::kSliceBytes, vdst = kdst + kSlice * S::kPitch;
-        if (plain && live == 0xffffu && newest - (pos - lane) >= uint32_t(kSlice)) {
-          // the whole slice is live and in one page: rows a fixed way apart
-          const int page0 = __shfl_sync(0xffffffffu, page, 0), off0 = __shfl_sync(0xffffffffu, off, 0);
-          const T* ks = kc + page0 * j.k_page_stride + off0 * j.k_token_stride;
-          const T* vs = vc + page0 * j.v_page_stride + off0 * j.v_token_stride;
+        int page = -1;
+        if (i < n_slices && lane < kSlice && pos >= sp.from && pos < sp.to) {
+          page = table[pos / uint32_t(j.page_size)];
+          if (page >= j.n_pages) page = -1;
+        }
+        return page;
+      };
+      auto fetch = [&](int i, int page) {
+        if (i < n_slices) {
+          const int stage = i % S::kStages;
+          const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
+          const int off = int(pos % uint32_t(j.page_size));
+          const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+          if (lane == 0) live_of[warp][stage] = live;
+          const uint32_t kdst = mine_addr + stage * S::kSliceBytes, vdst = kdst + kSlice * S::kPitch;
+          if (plain && live == 0xffffu && newest - (pos - lane) >= uint32_t(kSlice)) {
+            // the whole slice is live and in one page: rows a fixed way apart
+            const int page0 = __shfl_sync(0xffffffffu, page, 0), off0 = __shfl_sync(0xffffffffu, off, 0);
+            const T* ks = kc + page0 * j.k_page_stride + off0 * j.k_token_stride;
+            const T* vs = vc + page0 * j.v_page_stride + off0 * j.v_token_stride;
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+              const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
+              copy16(kdst + row * S::kPitch + chunk * 16, ks + from_row[c], 16);
+              copy16(vdst + row * S::kPitch + chunk * 16, vs + from_row[c], 16);
+            }
+            commit();
+            return;
+          }
 #pragma unroll
           for (int c = 0; c < kCopies; ++c) {
             const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
-            copy16(kdst + row * S::kPitch + chunk * 16, ks + from_row[c], 16);
-            copy16(vdst + row * S::kPitch + chunk * 16, vs + from_row[c], 16);
-          }
-          commit();
-          return;
-        }
-#pragma unroll
-        for (int c = 0; c < kCopies; ++c) {
-          const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
-          const int row_page = __shfl_sync(0xffffffffu, page, row), row_off = __shfl_sync(0xffffffffu, off, row);
-          const bool read = row_page >= 0 && chunk * 8 < D;
-          const T* ks = kc;
-          const T* vs = vc;
-          if (read) {
-            ks += row_page * j.k_page_stride + row_off * j.k_token_stride + chunk * 8;
-            vs += row_page * j.v_page_stride + row_off * j.v_token_stride + chunk * 8;
-            if (pos0 + uint32_t(i) * kTile + row == newest) {
-              // the new token: read from its own tensors, and written to the cache by the first group
-              if (hb == 0) {
-                *reinterpret_cast<uint4*>(const_cast<T*>(ks)) = *reinterpret_cast<const uint4*>(nk + chunk * 8);
-                *reinterpret_cast<uint4*>(const_cast<T*>(vs)) = *reinterpret_cast<const uint4*>(nv + chunk * 8);
+            const int row_page = __shfl_sync(0xffffffffu, page, row), row_off = __shfl_sync(0xffffffffu, off, row);
+            const bool read = row_page >= 0 && chunk * 8 < D;
+            const T* ks = kc;
+            const T* vs = vc;
+            if (read) {
+              ks += row_page * j.k_page_stride + row_off * j.k_token_stride + chunk * 8;
+              vs += row_page * j.v_page_stride + row_off * j.v_token_stride + chunk * 8;
+              if (pos0 + uint32_t(i) * kTile + row == newest) {
+                // the new token: read from its own tensors, and written to the cache by the first group
+                if (hb == 0) {
+                  *reinterpret_cast<uint4*>(const_cast<T*>(ks)) = *reinterpret_cast<const uint4*>(nk + chunk * 8);
+                  *reinterpret_cast<uint4*>(const_cast<T*>(vs)) = *reinterpret_cast<const uint4*>(nv + chunk * 8);
+                }
+                ks = nk + chunk * 8;
+                vs = nv + chunk * 8;
               }
-              ks = nk + chunk * 8;
-              vs = nv + chunk * 8;
             }
+            const uint32_t at = row * S::kPitch + chunk * 16;
+            copy16(kdst + at, ks, read ? 16 : 0);
+            copy16(vdst + at, vs, read ? 16 : 0);
           }
-          const uint32_t at = row * S::kPitch + chunk * 16;
-          copy16(kdst + at, ks, read ? 16 : 0);
-          copy16(vdst + at, vs, read ? 16 : 0);
         }
+        commit();
+      };
+
+      // queries as the column operand: head g, dims 2t, 2t+1 and 2t+8, 2t+9 of each 16
+      uint32_t q[NT][DP / 16][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bool have = n * 8 + g < nh;
+        const T* qp = static_cast<const T*>(j.q) + b * j.q_stride + (h0 + (have ? n * 8 + g : 0)) * j.q_head_stride;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = k * 16 + e * 8 + 2 * t;
+            q[n][k][e] = have && d < D ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
+          }
       }
-      commit();
-    };
 
-    // queries as the column operand: head g, dims 2t, 2t+1 and 2t+8, 2t+9 of each 16
-    uint32_t q[NT][DP / 16][2];
+      float o[NT][DP / 16][4] = {};
+      float top[NT][2], sum[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool have = n * 8 + g < nh;
-      const T* qp = static_cast<const T*>(j.q) + b * j.q_stride + (h0 + (have ? n * 8 + g : 0)) * j.q_head_stride;
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = k * 16 + e * 8 + 2 * t;
-          q[n][k][e] = have && d < D ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
-        }
-    }
+      for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
 
-    float o[NT][DP / 16][4] = {};
-    float top[NT][2], sum[NT][2];
+      int page = page_of(0);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.0f;
-
-    int page = page_of(0);
-#pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-      const int ahead = page_of(i + 1);
-      fetch(i, page);
-      page = ahead;
-    }
-    for (int i = 0; i < n_slices; ++i) {
-      // the page index of the slice after the next fetch travels while this slice is computed
-      const int ahead = page_of(i + S::kStages);
-      fetch(i + S::kStages - 1, page);
-      page = ahead;
-      wait_groups<S::kStages - 1>();
-      __syncwarp();
-      const int stage = i % S::kStages;
-      const uint32_t live = live_of[warp][stage];
-      if (live) {
-        const uint32_t kbase = mine_addr + stage * S::kSliceBytes, vbase = kbase + kSlice * S::kPitch;
-        float s[NT][4];
-        {
-          // even and odd 16 dims apart: half as long a chain of sums
-          float odd[NT][4];
-          const uint32_t at = kbase + (lane & 15) * S::kPitch + (lane >> 4) * 16;
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            uint32_t ka[4];
-            ldsm(ka, at + k * 32);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if (k == 0) mma_first<T>(s[n], ka, q[n][k][0], q[n][k][1]);
-              else if (k == 1) mma_first<T>(odd[n], ka, q[n][k][0], q[n][k][1]);
-              else if (k & 1) mma<T>(odd[n], ka, q[n][k][0], q[n][k][1]);
-              else mma<T>(s[n], ka, q[n][k][0], q[n][k][1]);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + odd[n][e]) * scale2;
-        }
-        const bool live_a = live >> g & 1, live_b = live >> (g + 8) & 1;
-        uint32_t hi[NT][2], lo[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (live != 0xffffu) {
-            s[n][0] = live_a ? s[n][0] : -INFINITY;
-            s[n][1] = live_a ? s[n][1] : -INFINITY;
-            s[n][2] = live_b ? s[n][2] : -INFINITY;
-            s[n][3] = live_b ? s[n][3] : -INFINITY;
-          }
-          float m0 = fmaxf(s[n][0], s[n][2]), m1 = fmaxf(s[n][1], s[n][3]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
-            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
-          }
-          m0 = fmaxf(m0, top[n][0]);
-          m1 = fmaxf(m1, top[n][1]);
-          const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
-          if (__any_sync(0xffffffffu, m0 != top[n][0] || m1 != top[n][1])) {
-            const float c0 = exp2_fast(top[n][0] - b0), c1 = exp2_fast(top[n][1] - b1);
-            sum[n][0] *= c0;
-            sum[n][1] *= c1;
+      for (int i = 0; i < S::kStages - 1; ++i) {
+        const int ahead = page_of(i + 1);
+        fetch(i, page);
+        page = ahead;
+      }
+      for (int i = 0; i < n_slices; ++i) {
+        // the page index of the slice after the next fetch travels while this slice is computed
+        const int ahead = page_of(i + S::kStages);
+        fetch(i + S::kStages - 1, page);
+        page = ahead;
+        wait_groups<S::kStages - 1>();
+        __syncwarp();
+        const int stage = i % S::kStages;
+        const uint32_t live = live_of[warp][stage];
+        if (live) {
+          const uint32_t kbase = mine_addr + stage * S::kSliceBytes, vbase = kbase + kSlice * S::kPitch;
+          float s[NT][4];
+          {
+            // even and odd 16 dims apart: half as long a chain of sums
+            float odd[NT][4];
+            const uint32_t at = kbase + (lane & 15) * S::kPitch + (lane >> 4) * 16;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
-              o[n][k][0] *= c0; o[n][k][1] *= c1; o[n][k][2] *= c0; o[n][k][3] *= c1;
+              uint32_t ka[4];
+              ldsm(ka, at + k * 32);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                if (k == 0) mma_first<T>(s[n], ka, q[n][k][0], q[n][k][1]);
+                else if (k == 1) mma_first<T>(odd[n], ka, q[n][k][0], q[n][k][1]);
+                else if (k & 1) mma<T>(odd[n], ka, q[n][k][0], q[n][k][1]);
+                else mma<T>(s[n], ka, q[n][k][0], q[n][k][1]);
+              }
             }
-            top[n][0] = m0;
-            top[n][1] = m1;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + odd[n][e]) * scale2;
           }
-          const float p0 = exp2_fast(s[n][0] - b0 + kLift), p1 = exp2_fast(s[n][1] - b1 + kLift);
-          const float p2 = exp2_fast(s[n][2] - b0 + kLift), p3 = exp2_fast(s[n][3] - b1 + kLift);
-          sum[n][0] += p0 + p2;
-          sum[n][1] += p1 + p3;
-          halves(static_cast<T*>(nullptr), p0, p1, hi[n][0], lo[n][0]);
-          halves(static_cast<T*>(nullptr), p2, p3, hi[n][1], lo[n][1]);
-          hi[n][0] = transpose8(hi[n][0]);
-          hi[n][1] = transpose8(hi[n][1]);
-          lo[n][0] = transpose8(lo[n][0]);
-          lo[n][1] = transpose8(lo[n][1]);
-        }
-        {
-          const uint32_t at = vbase + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16;
+          const bool live_a = live >> g & 1, live_b = live >> (g + 8) & 1;
+          uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            uint32_t va[4];
-            ldsm_t(va, at + k * 32);
+          for (int n = 0; n < NT; ++n) {
+            if (live != 0xffffu) {
+              s[n][0] = live_a ? s[n][0] : -INFINITY;
+              s[n][1] = live_a ? s[n][1] : -INFINITY;
+              s[n][2] = live_b ? s[n][2] : -INFINITY;
+              s[n][3] = live_b ? s[n][3] : -INFINITY;
+            }
+            float m0 = fmaxf(s[n][0], s[n][2]), m1 = fmaxf(s[n][1], s[n][3]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma<T>(o[n][k], va, hi[n][0], hi[n][1]);
-              mma<T>(o[n][k], va, lo[n][0], lo[n][1]);
+            for (int x = 4; x < 32; x <<= 1) {
+              m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
+              m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
+            }
+            m0 = fmaxf(m0, top[n][0]);
+            m1 = fmaxf(m1, top[n][1]);
+            const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+            if (__any_sync(0xffffffffu, m0 != top[n][0] || m1 != top[n][1])) {
+              const float c0 = exp2_fast(top[n][0] - b0), c1 = exp2_fast(top[n][1] - b1);
+              sum[n][0] *= c0;
+              sum[n][1] *= c1;
+#pragma unroll
+              for (int k = 0; k < DP / 16; ++k) {
+                o[n][k][0] *= c0; o[n][k][1] *= c1; o[n][k][2] *= c0; o[n][k][3] *= c1;
+              }
+              top[n][0] = m0;
+              top[n][1] = m1;
+            }
+            const float p0 = exp2_fast(s[n][0] - b0 + kLift), p1 = exp2_fast(s[n][1] - b1 + kLift);
+            const float p2 = exp2_fast(s[n][2] - b0 + kLift), p3 = exp2_fast(s[n][3] - b1 + kLift);
+            sum[n][0] += p0 + p2;
+            sum[n][1] += p1 + p3;
+            halves(static_cast<T*>(nullptr), p0, p1, hi[n][0], lo[n][0]);
+            halves(static_cast<T*>(nullptr), p2, p3, hi[n][1], lo[n][1]);
+            hi[n][0] = transpose8(hi[n][0]);
+            hi[n][1] = transpose8(hi[n][1]);
+            lo[n][0] = transpose8(lo[n][0]);
+            lo[n][1] = transpose8(lo[n][1]);
+          }
+          {
+            const uint32_t at = vbase + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+              uint32_t va[4];
+              ldsm_t(va, at + k * 32);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma<T>(o[n][k], va, hi[n][0], hi[n][1]);
+                mma<T>(o[n][k], va, lo[n][0], lo[n][1]);
+              }
             }
           }
         }
+        __syncwarp();                                      // the slice is read before its place is filled again
       }
-      __syncwarp();                                      // the slice is read before its place is filled again
-    }
-    wait_groups<0>();
-    __syncwarp();
+      wait_groups<0>();
+      __syncwarp();
 
-    // the warps' results through shared memory, each in its own ring
-    float* ow = reinterpret_cast<float*>(mine);
+      // the warps' results through shared memory, each in its own ring
+      float* ow = reinterpret_cast<float*>(mine);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) {
-        sum[n][0] += __shfl_xor_sync(0xffffffffu, sum[n][0], x);
-        sum[n][1] += __shfl_xor_sync(0xffffffffu, sum[n][1], x);
-      }
-      if (g == 0) {
-        warp_stat[warp][n * 8 + 2 * t] = make_float2(top[n][0], sum[n][0]);
-        warp_stat[warp][n * 8 + 2 * t + 1] = make_float2(top[n][1], sum[n][1]);
-      }
+        for (int x = 4; x < 32; x <<= 1) {
+          sum[n][0] += __shfl_xor_sync(0xffffffffu, sum[n][0], x);
+          sum[n][1] += __shfl_xor_sync(0xffffffffu, sum[n][1], x);
+        }
+        if (g == 0) {
+          warp_stat[warp][n * 8 + 2 * t] = make_float2(top[n][0], sum[n][0]);
+          warp_stat[warp][n * 8 + 2 * t + 1] = make_float2(top[n][1], sum[n][1]);
+        }
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        float* at = ow + (n * 8 + 2 * t) * S::kOutStride + k * 16 + g;
-        at[0] = o[n][k][0];
-        at[S::kOutStride] = o[n][k][1];
-        at[8] = o[n][k][2];
-        at[S::kOutStride + 8] = o[n][k][3];
+        for (int k = 0; k < DP / 16; ++k) {
+          float* at = ow + (n * 8 + 2 * t) * S::kOutStride + k * 16 + g;
+          at[0] = o[n][k][0];
+          at[S::kOutStride] = o[n][k][1];
+          at[8] = o[n][k][2];
+          at[S::kOutStride + 8] = o[n][k][3];
+        }
       }
+      __syncthreads();
+      const bool whole = t0 == 0 && t1 == sp.tiles;
+      const int64_t slot = 2 * int64_t(blockIdx.x) + (t0 == 0 ? 1 : 0);
+      if (threadIdx.x < S::kHeads) {
+        const int h = threadIdx.x;
+        if (h == 0 && t0 > 0) {
+          // the run with the segment's first tile; the one after it notes the cut
+          const int c0 = int(((s0 + kSeam + 1) * runs - 1) / total), c1 = int(((s0 + length) * runs - 1) / total);
+          if (c0 + 1 == blockIdx.x) {
+            a.cuts[blockIdx.x] = {c1 - c0 + 1, c0, b * j.q_heads + h0, nh};
+          }
+        }
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[w][h].x);
+        const float mb = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = exp2_fast(warp_stat[w][h].x - mb);
+          factor[w][h] = f;
+          l += warp_stat[w][h].y * f;
+        }
+        total_of[h] = l;
+        if (h < nh) {
+          if (!whole) a.stat[slot * S::kHeads + h] = make_float2(m, l);
+          else if (j.lse) j.lse[int64_t(b) * j.q_heads + h0 + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+        }
+      }
+      __syncthreads();
+      for (int h = 0; h < nh; ++h) {
+        const float l = total_of[h];
+        for (int d = threadIdx.x; d < D; d += kThreads) {
+          float v = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w)
+            v += reinterpret_cast<const float*>(ring + w * S::kWarpBytes)[h * S::kOutStride + d] * factor[w][h];
+          if (whole) static_cast<T*>(j.out)[(int64_t(b) * j.q_heads + h0 + h) * D + d] = from_float<T>(l == 0.0f ? 0.0f : v / l);
+          else a.part[(slot * S::kHeads + h) * D + d] = v;
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == sp.tiles;
-    const int64_t slot = 2 * int64_t(blockIdx.x) + (t0 == 0 ? 1 : 0);
-    if (threadIdx.x < S::kHeads) {
-      const int h = threadIdx.x;
-      float m = -INFINITY, l = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[w][h].x);
-      const float mb = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_fast(warp_stat[w][h].x - mb);
-        factor[w][h] = f;
-        l += warp_stat[w][h].y * f;
-      }
-      total_of[h] = l;
-      if (h < nh) {
-        if (!whole) a.stat[slot * S::kHeads + h] = make_float2(m, l);
-        else if (j.lse) j.lse[int64_t(b) * j.q_heads + h0 + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
-      }
-    }
-    __syncthreads();
-    for (int h = 0; h < nh; ++h) {
-      const float l = total_of[h];
-      for (int d = threadIdx.x; d < D; d += kThreads) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w)
-          v += reinterpret_cast<const float*>(ring + w * S::kWarpBytes)[h * S::kOutStride + d] * factor[w][h];
-        if (whole) static_cast<T*>(j.out)[(int64_t(b) * j.q_heads + h0 + h) * D + d] = from_float<T>(l == 0.0f ? 0.0f : v / l);
-        else a.part[(slot * S::kHeads + h) * D + d] = v;
-      }
-    }
-    __syncthreads();
 
-    cur += t1 - t0;
-    if (cur < end && cur == base + int64_t(sp.tiles) * heads) {
+    cur += part1 - part0;
+    if (cur < end && cur == base + int64_t(length) * heads) {
       base = cur;
       do sp = span_of(j, ++b);                           // the line goes on: a later sequence has tiles
       while (!sp.tiles);
@@ -462,30 +485,19 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
 // pieces, whose factors were computed by a thread each.
 constexpr int kJoinThreads = 256;
 template <class T, int NT>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kHeads = 8 * NT;
   constexpr float kLift = std::is_same<T, fp16>::value ? 8.0f : 0.0f;
-  __shared__ int64_t prefix[kJoinThreads + 1];
   __shared__ float factor[kMaxRuns], partial[8];
   __shared__ float4 sums[kJoinThreads];
   const pm_paged_attention& j = a.j;
-  const int b = blockIdx.x / j.q_heads, h = blockIdx.x - b * j.q_heads, t = threadIdx.x;
-  const int heads = j.kv_heads * a.blocks, D = j.head_dim;
-  const int per = (j.batch + kJoinThreads - 1) / kJoinThreads;
-  const int64_t total = scan_tiles<kJoinThreads>(j, per, prefix) * heads;
-  const int tiles = span_of(j, b).tiles;
+  const int t = threadIdx.x, D = j.head_dim, row = blockIdx.y;
   asm volatile("griddepcontrol.wait;" ::: "memory");    // in every CTA: this kernel's end has to mean the first one's
-  if (!tiles) return;
-  int64_t before = prefix[b / per];
-  for (int i = b / per * per; i < b; ++i) before += span_of(j, i).tiles;
-  const int kvh = h / a.share, within = h - kvh * a.share, hb = within / kHeads, row = within - hb * kHeads;
-  const int64_t s0 = before * heads + int64_t(kvh * a.blocks + hb) * tiles, s1 = s0 + tiles;
-  // run c holds tiles [total c / runs, total (c + 1) / runs)
-  const int64_t runs = min(int64_t(ctas), total);
-  const int c0 = int(((s0 + 1) * runs - 1) / total), n = int((s1 * runs - 1) / total) - c0 + 1;
-  if (n == 1) return;
-  // the first piece may begin before the segment's run does: only that one is a run's second
-  auto slot_of = [&](int i) { return 2 * int64_t(c0 + i) + (i == 0 && total * c0 / runs <= s0 ? 1 : 0); };
+  const int4 c = __ldcg(reinterpret_cast<const int4*>(&a.cuts[blockIdx.x + 1]));
+  const int n = c.x;
+  if (!n || row >= c.w) return;
+  // a run's slots: first the piece that it starts within, then the one that it ends within, which is a segment's first
+  auto slot_of = [&](int i) { return 2 * int64_t(c.y + i) + (i == 0 ? 1 : 0); };
   float m = -INFINITY;
   for (int i = t; i < n; i += kJoinThreads) {
     const float top = __ldcg(&a.stat[slot_of(i) * kHeads + row]).x;
@@ -529,13 +541,13 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
       const float4 p = sums[g * lanes + t];
       v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
     }
-    T* out = static_cast<T*>(j.out) + (int64_t(b) * j.q_heads + h) * D + 4 * t;
+    T* out = static_cast<T*>(j.out) + int64_t(c.z + row) * D + 4 * t;
     out[0] = from_float<T>(l == 0.0f ? 0.0f : v.x / l);
     out[1] = from_float<T>(l == 0.0f ? 0.0f : v.y / l);
     out[2] = from_float<T>(l == 0.0f ? 0.0f : v.z / l);
     out[3] = from_float<T>(l == 0.0f ? 0.0f : v.w / l);
   }
-  if (j.lse && t == 0) j.lse[int64_t(b) * j.q_heads + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+  if (j.lse && t == 0) j.lse[c.z + row] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
 }
 
 // ---------------------------------------------------------------- launch
@@ -568,13 +580,14 @@ cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s)
   int64_t runs = int64_t(sms) * occ;
   if (runs > kMaxRuns) runs = kMaxRuns;
   if (runs > most) runs = most;
-  a.stat = reinterpret_cast<float2*>(scratch);
-  a.part = reinterpret_cast<float*>(scratch + size_t(2) * kMaxRuns * S::kHeads * sizeof(float2));
+  a.cuts = reinterpret_cast<Cut*>(scratch);
+  a.stat = reinterpret_cast<float2*>(scratch + kMaxRuns * sizeof(Cut));
+  a.part = reinterpret_cast<float*>(scratch + kMaxRuns * sizeof(Cut) + size_t(2) * kMaxRuns * S::kHeads * sizeof(float2));
   kernel<<<unsigned(runs), kThreads, S::kSmem, s>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || room <= 1) return e;           // one tile at most: nothing is ever cut
+  if (e != cudaSuccess || room <= 1 || runs <= 1) return e;   // one tile at most, or one run: nothing is ever cut
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(j.batch * j.q_heads));
+  cfg.gridDim = dim3(unsigned(runs - 1), unsigned(a.share < S::kHeads ? a.share : S::kHeads));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute early[1];
@@ -582,7 +595,7 @@ cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s)
   early[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = early;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, NT>, a, int(runs));
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, NT>, a);
 }
 
 template <class T>
@@ -609,7 +622,7 @@ using namespace pm::blk;
 extern "C" size_t pm_paged_attention_scratch_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (batch < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || q_heads % kv_heads) return 0;
   const size_t rows = size_t(2) * kMaxRuns * 8 * tiles_of_heads(q_heads / kv_heads, head_dim);
-  return rows * sizeof(float2) + rows * size_t(head_dim) * sizeof(float);
+  return kMaxRuns * sizeof(Cut) + rows * sizeof(float2) + rows * size_t(head_dim) * sizeof(float);
 }
 
 extern "C" int pm_paged_attention_device(const pm_paged_attention* j, void* scratch, size_t scratch_bytes, void* stream) {
