@@ -42,6 +42,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
   pm_paged_attention j;
+  int page_shift;                        // log2 of the page size, -1: no power of two
   int share, blocks;                     // query heads per key head; groups of them that one pass serves
   float* part;                           // [2 * CTAs, kHeads, head_dim] weighted values of split segments
   float2* stat;                          // [2 * CTAs, kHeads] (maximum, sum), base 2
@@ -197,6 +198,9 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   Span sp = span_of(j, b);
   int64_t base = found_before * heads;                   // where the sequence starts on the line
 
+  // page and entry of a position
+  auto page_at = [&](uint32_t pos) { return a.page_shift >= 0 ? pos >> a.page_shift : pos / uint32_t(j.page_size); };
+  auto entry_of = [&](uint32_t pos) { return int(a.page_shift >= 0 ? pos & uint32_t(j.page_size - 1) : pos % uint32_t(j.page_size)); };
   // Slices that lie in one page, of heads without padding and with the same way from token to token in K and V, are
   // copied by these offsets (elements) of a lane's pieces
   const bool plain = D == DP && j.page_size % kSlice == 0 && j.k_token_stride == j.v_token_stride && j.k_token_stride < (1 << 26);
@@ -210,7 +214,9 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
 
   while (cur < end) {
     const int length = length_of(sp.tiles);
-    const int which = int((cur - base) / length);        // key head and group of query heads
+    const uint64_t into = uint64_t(cur - base);
+    // key head and group of query heads; a 64-bit division only where it takes one
+    const int which = into >> 32 ? int(into / uint64_t(length)) : int(uint32_t(into) / uint32_t(length));
     const int kvh = which / a.blocks, hb = which - kvh * a.blocks;
     const int64_t s0 = base + int64_t(which) * length;   // the segment, and this run's part of it
     const int part0 = int(cur - s0), part1 = int(min(int64_t(length), part0 + (end - cur)));
@@ -231,57 +237,69 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
         const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
         int page = -1;
         if (i < n_slices && lane < kSlice && pos >= sp.from && pos < sp.to) {
-          page = table[pos / uint32_t(j.page_size)];
+          page = table[page_at(pos)];
           if (page >= j.n_pages) page = -1;
         }
         return page;
       };
       auto fetch = [&](int i, int page) {
-        if (i < n_slices) {
-          const int stage = i % S::kStages;
-          const uint32_t pos = pos0 + uint32_t(i) * kTile + lane;
-          const int off = int(pos % uint32_t(j.page_size));
-          const uint32_t live = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+        const uint32_t live = i < n_slices ? __ballot_sync(0xffffffffu, page >= 0) & 0xffffu : 0u;
+        if (live) {
+          const uint32_t first_pos = pos0 + uint32_t(i) * kTile;
+          const int off = entry_of(first_pos + lane), stage = i % S::kStages;
           if (lane == 0) live_of[warp][stage] = live;
           const uint32_t kdst = mine_addr + stage * S::kSliceBytes, vdst = kdst + kSlice * S::kPitch;
-          if (plain && live == 0xffffu && newest - (pos - lane) >= uint32_t(kSlice)) {
-            // the whole slice is live and in one page: rows a fixed way apart
-            const int page0 = __shfl_sync(0xffffffffu, page, 0), off0 = __shfl_sync(0xffffffffu, off, 0);
+          // the new token's row, if it is here: read from its own tensors, and written to the cache by the first group
+          const int new_row = newest - first_pos < uint32_t(kSlice) && live >> (newest - first_pos) & 1u ? int(newest - first_pos) : -1;
+          if (new_row >= 0 && hb == 0) {
+            const int new_page = __shfl_sync(0xffffffffu, page, new_row), new_off = __shfl_sync(0xffffffffu, off, new_row);
+            if (lane * 8 < D) {
+              T* ks = const_cast<T*>(kc) + new_page * j.k_page_stride + new_off * j.k_token_stride + lane * 8;
+              T* vs = const_cast<T*>(vc) + new_page * j.v_page_stride + new_off * j.v_token_stride + lane * 8;
+              *reinterpret_cast<uint4*>(ks) = *reinterpret_cast<const uint4*>(nk + lane * 8);
+              *reinterpret_cast<uint4*>(vs) = *reinterpret_cast<const uint4*>(nv + lane * 8);
+            }
+          }
+          if (plain) {
+            // the slice is in one page: rows a fixed way apart
+            const int some = __ffs(live) - 1;
+            const int page0 = __shfl_sync(0xffffffffu, page, some), off0 = __shfl_sync(0xffffffffu, off, 0);
             const T* ks = kc + page0 * j.k_page_stride + off0 * j.k_token_stride;
             const T* vs = vc + page0 * j.v_page_stride + off0 * j.v_token_stride;
+            if (live == 0xffffu && new_row < 0) {
+#pragma unroll
+              for (int c = 0; c < kCopies; ++c) {
+                const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
+                copy16(kdst + row * S::kPitch + chunk * 16, ks + from_row[c], 16);
+                copy16(vdst + row * S::kPitch + chunk * 16, vs + from_row[c], 16);
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < kCopies; ++c) {
+                const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
+                const int bytes = live >> row & 1u ? 16 : 0;
+                copy16(kdst + row * S::kPitch + chunk * 16, row == new_row ? nk + chunk * 8 : ks + from_row[c], bytes);
+                copy16(vdst + row * S::kPitch + chunk * 16, row == new_row ? nv + chunk * 8 : vs + from_row[c], bytes);
+              }
+            }
+          } else {
 #pragma unroll
             for (int c = 0; c < kCopies; ++c) {
               const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
-              copy16(kdst + row * S::kPitch + chunk * 16, ks + from_row[c], 16);
-              copy16(vdst + row * S::kPitch + chunk * 16, vs + from_row[c], 16);
-            }
-            commit();
-            return;
-          }
-#pragma unroll
-          for (int c = 0; c < kCopies; ++c) {
-            const int idx = c * 32 + lane, row = idx / kChunks, chunk = idx % kChunks;
-            const int row_page = __shfl_sync(0xffffffffu, page, row), row_off = __shfl_sync(0xffffffffu, off, row);
-            const bool read = row_page >= 0 && chunk * 8 < D;
-            const T* ks = kc;
-            const T* vs = vc;
-            if (read) {
-              ks += row_page * j.k_page_stride + row_off * j.k_token_stride + chunk * 8;
-              vs += row_page * j.v_page_stride + row_off * j.v_token_stride + chunk * 8;
-              if (pos0 + uint32_t(i) * kTile + row == newest) {
-                // the new token: read from its own tensors, and written to the cache by the first group
-                if (hb == 0) {
-                  *reinterpret_cast<uint4*>(const_cast<T*>(ks)) = *reinterpret_cast<const uint4*>(nk + chunk * 8);
-                  *reinterpret_cast<uint4*>(const_cast<T*>(vs)) = *reinterpret_cast<const uint4*>(nv + chunk * 8);
-                }
-                ks = nk + chunk * 8;
-                vs = nv + chunk * 8;
+              const int row_page = __shfl_sync(0xffffffffu, page, row), row_off = __shfl_sync(0xffffffffu, off, row);
+              const bool read = row_page >= 0 && chunk * 8 < D;
+              const T* ks = kc;
+              const T* vs = vc;
+              if (read) {
+                ks = row == new_row ? nk + chunk * 8 : ks + (row_page * j.k_page_stride + row_off * j.k_token_stride + chunk * 8);
+                vs = row == new_row ? nv + chunk * 8 : vs + (row_page * j.v_page_stride + row_off * j.v_token_stride + chunk * 8);
               }
+              copy16(kdst + row * S::kPitch + chunk * 16, ks, read ? 16 : 0);
+              copy16(vdst + row * S::kPitch + chunk * 16, vs, read ? 16 : 0);
             }
-            const uint32_t at = row * S::kPitch + chunk * 16;
-            copy16(kdst + at, ks, read ? 16 : 0);
-            copy16(vdst + at, vs, read ? 16 : 0);
           }
+        } else if (i < n_slices && lane == 0) {
+          live_of[warp][i % S::kStages] = 0;
         }
         commit();
       };
@@ -603,6 +621,7 @@ cudaError_t launch(const pm_paged_attention& j, void* scratch, int sms, cudaStre
   AttnArgs a{};
   a.j = j;
   a.share = j.q_heads / j.kv_heads;
+  a.page_shift = j.page_size & (j.page_size - 1) ? -1 : 31 - __builtin_clz(unsigned(j.page_size));
   uint8_t* f = static_cast<uint8_t*>(scratch);
   const int nt = tiles_of_heads(a.share, j.head_dim);
   if (j.head_dim > 64 && j.head_dim <= 80) return nt == 2 ? launch_shape<T, 80, 2>(a, f, sms, s) : launch_shape<T, 80, 1>(a, f, sms, s);
