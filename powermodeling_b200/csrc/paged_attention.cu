@@ -37,12 +37,14 @@ namespace {
 
 constexpr int kMaxRuns = 148 * 4;        // CTAs of the first kernel at most: sizes the scratch
 constexpr int kSeam = 2;                 // what the start of a segment counts for, in tiles
+constexpr int kWhole = 4;                // room for so many tiles at most, and a run for each segment: none is cut
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kSlice = 16, kTile = kSlice * kWarps;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
   pm_paged_attention j;
   int page_shift;                        // log2 of the page size, -1: no power of two
+  int whole;                             // runs end between segments: none is cut
   int share, blocks;                     // query heads per key head; groups of them that one pass serves
   float* part;                           // [2 * CTAs, kHeads, head_dim] weighted values of split segments
   float2* stat;                          // [2 * CTAs, kHeads] (maximum, sum), base 2
@@ -101,16 +103,16 @@ __device__ __forceinline__ Span span_of(const pm_paged_attention& j, int b) {
   s.tiles = s.to > s.from ? int((s.to + kTile - 1) / kTile - s.first) : 0;
   return s;
 }
-// What one key head of a sequence takes on the line.
-__device__ __forceinline__ int length_of(int tiles) { return tiles ? tiles + kSeam : 0; }
+// What one key head of a sequence takes on the line; all the same where segments stay whole.
+__device__ __forceinline__ int length_of(int tiles, int whole) { return tiles == 0 ? 0 : whole ? 1 : tiles + kSeam; }
 
 // The sequences' lengths on the line, of one key head each, summed over the batch: thread t has the sum over the
 // sequences before its `per` consecutive ones, prefix[Threads] all of them.
 template <int Threads>
-__device__ __forceinline__ int64_t scan_line(const pm_paged_attention& j, int per, int64_t* prefix) {
+__device__ __forceinline__ int64_t scan_line(const pm_paged_attention& j, int whole, int per, int64_t* prefix) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   int64_t own = 0;
-  for (int b = t * per; b < min(j.batch, (t + 1) * per); ++b) own += length_of(span_of(j, b).tiles);
+  for (int b = t * per; b < min(j.batch, (t + 1) * per); ++b) own += length_of(span_of(j, b).tiles, whole);
   int64_t sum = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int D = j.head_dim, heads = j.kv_heads * a.blocks;
   const int per = (j.batch + kThreads - 1) / kThreads;
-  const int64_t total = scan_line<kThreads>(j, per, prefix) * heads;
+  const int64_t total = scan_line<kThreads>(j, a.whole, per, prefix) * heads;
 
   // sequences without a live position: zeros
   for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
     int64_t before = prefix[threadIdx.x];
     int b = threadIdx.x * per;
     for (;; ++b) {
-      const int n = length_of(span_of(j, b).tiles);
+      const int n = length_of(span_of(j, b).tiles, a.whole);
       if (cur < (before + n) * heads) break;
       before += n;
     }
@@ -213,14 +215,14 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   const float scale2 = j.scale * kLog2e;
 
   while (cur < end) {
-    const int length = length_of(sp.tiles);
+    const int length = length_of(sp.tiles, a.whole);
     const uint64_t into = uint64_t(cur - base);
     // key head and group of query heads; a 64-bit division only where it takes one
     const int which = into >> 32 ? int(into / uint64_t(length)) : int(uint32_t(into) / uint32_t(length));
     const int kvh = which / a.blocks, hb = which - kvh * a.blocks;
     const int64_t s0 = base + int64_t(which) * length;   // the segment, and this run's part of it
     const int part0 = int(cur - s0), part1 = int(min(int64_t(length), part0 + (end - cur)));
-    const int t0 = max(part0 - kSeam, 0), t1 = max(part1 - kSeam, 0);
+    const int t0 = a.whole ? 0 : max(part0 - kSeam, 0), t1 = a.whole ? sp.tiles : max(part1 - kSeam, 0);
     const int h0 = kvh * a.share + hb * S::kHeads, nh = min(S::kHeads, a.share - hb * S::kHeads);
     if (t1 > t0) {
       const int n_slices = t1 - t0;                        // one slice of this warp in each tile
@@ -592,18 +594,22 @@ cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s)
   }
   const pm_paged_attention& j = a.j;
   a.blocks = (a.share + S::kHeads - 1) / S::kHeads;
-  // no more runs than tiles at the tables' full length, which bounds the lengths
-  const int64_t room = (int64_t(j.table_columns) * j.page_size + kTile - 1) / kTile;
-  const int64_t most = int64_t(j.batch) * j.kv_heads * a.blocks * (room < (1 << 20) ? (room > 1 ? room : 1) : (1 << 20));
   int64_t runs = int64_t(sms) * occ;
   if (runs > kMaxRuns) runs = kMaxRuns;
+  // The tables' full length bounds the lengths.  Where every segment has a run to itself and few tiles, none is cut:
+  // the join's launch costs more than the tiles in turn (us whole and cut: 8 sequences x 8 heads with 128 positions
+  // 7.6 and 10.6, with 256 9.7 and 11.0, with 512 13.8 and 11.9; 128 x 8 segments of 256, more than runs, 31.7 and 28.3).
+  const int64_t room = (int64_t(j.table_columns) * j.page_size + kTile - 1) / kTile;
+  const int64_t segments = int64_t(j.batch) * j.kv_heads * a.blocks;
+  a.whole = room <= 1 || (room <= kWhole && segments <= runs);
+  const int64_t most = segments * (a.whole ? 1 : room < (1 << 20) ? room : (1 << 20));   // no more runs than work
   if (runs > most) runs = most;
   a.cuts = reinterpret_cast<Cut*>(scratch);
   a.stat = reinterpret_cast<float2*>(scratch + kMaxRuns * sizeof(Cut));
   a.part = reinterpret_cast<float*>(scratch + kMaxRuns * sizeof(Cut) + size_t(2) * kMaxRuns * S::kHeads * sizeof(float2));
   kernel<<<unsigned(runs), kThreads, S::kSmem, s>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || room <= 1 || runs <= 1) return e;   // one tile at most, or one run: nothing is ever cut
+  if (e != cudaSuccess || a.whole || runs <= 1) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(runs - 1), unsigned(a.share < S::kHeads ? a.share : S::kHeads));
   cfg.blockDim = dim3(kJoinThreads);
