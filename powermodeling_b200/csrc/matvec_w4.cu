@@ -26,6 +26,7 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "blocks.cuh"
@@ -39,22 +40,34 @@ namespace {
 constexpr int kWarps = 8, kRows = 32;                    // warps that multiply; rows of a warp's tile
 constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait; a result that it poisons is NaN
 
-// Up to 8 tokens: tiles of 256 k, which halves what a stage costs besides its
-// products; up to 16: of 128 k, as the tokens' values take the room.
+// Rows lie in shared memory 256 k (128 bytes) wide, as a copy brings them: 64
+// bytes a row and copy took 42 us where 128 took 27 (8192 x 28672).  Up to 8
+// tokens a warp has all of its rows' 256 k, up to 16 half of them, as the
+// tokens' values take the room.
+constexpr int kBoxK = 256, kPitch = kBoxK / 2, kPieces = kPitch / 16;           // a row, in 16-byte pieces
+constexpr int kRoom = 111 * 1024;                        // of a CTA's stages, two CTAs to an SM
 template <int NT>
 struct Tile {
-  static constexpr int kK = NT == 1 ? 256 : 128, kStages = NT == 1 ? 3 : 4;
-  static constexpr int kPitch = kK / 2, kPieces = kPitch / 16;                 // a row, in 16-byte pieces
-  static constexpr int kBytes = kRows * kPitch, kStageBytes = kWarps * kBytes;
-  // Pieces lie in an order of the row's own, so that 8 rows x 4 words meet all 32 banks.
-  static __device__ __forceinline__ int turn(int row) { return kPieces == 8 ? row & 7 : row >> 1 & 3; }
+  static constexpr int kK = NT == 1 ? 256 : 128, kShare = kBoxK / kK, kStages = NT == 1 ? 3 : 4;   // kShare: warps of a row
+  static constexpr int kStageBytes = kWarps * kRows * kK / 2;
 };
+// Pieces lie in an order of the row's own, so that 8 rows x 4 words meet all 32 banks.
+__device__ __forceinline__ int turn(int row) { return row & 7; }
 
-// Bytes of a stage with the values of `tokens` tokens, a multiple of the
-// swizzle's 1 KB: per warp along k its weights, then per warp along k its tokens' values.
+// A stage: the weights (whole KBs, as their order wants), the tokens' values, and scales and zero points where copies
+// bring them: `scale_box` and `zero_box` bytes a row.
+struct Stage {
+  int x, scales, zeros, bytes;
+};
 template <int NT>
-__host__ __device__ inline int stage_size(int tokens, int warps_k) {
-  return Tile<NT>::kStageBytes + (warps_k * tokens * Tile<NT>::kK * 2 + 1023) / 1024 * 1024;
+__host__ __device__ inline Stage stage_of(int tokens, int warps_n, int scale_box, int zero_box) {
+  const int boxes = kWarps / warps_n / Tile<NT>::kShare, rows = kRows * warps_n;
+  Stage s;
+  s.x = Tile<NT>::kStageBytes;
+  s.scales = s.x + boxes * tokens * kBoxK * 2;
+  s.zeros = s.scales + rows * scale_box;
+  s.bytes = (s.zeros + rows * zero_box + 1023) / 1024 * 1024;
+  return s;
 }
 
 struct W4Args {
@@ -66,19 +79,14 @@ struct W4Args {
   const uint8_t* zeros;
   void* y;
   int warps_n;                                           // warps along n; the others along k
-  int vector_scales;                                     // scales 16-byte, zeros 8-byte aligned
+  int scale_box, zero_box;                               // bytes of a row's scales and zero points in a stage, 0: not copied
   int group_shift;                                       // log2 of the 32-k blocks of a group, -1: no power of two
+  int places;                                            // stages in shared memory
   int stages;                                            // stages of a row block: its k over the stage's
   int ranks;                                             // CTAs of a cluster, which share each row block's stages
   float* part;                                           // ranks == 1: sums of cut row blocks, [2 * CTAs][rows][8 NT]
 };
 
-// (a & b) | c in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
 // The pairs (0,4), (1,5), (2,6), (3,7) of a word's nibbles, less the zero
 // point and over kScale, as exact 16-bit floats.  Integer instructions are
 // what the kernel has least of, so two nibble positions of a half are taken
@@ -91,8 +99,10 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
 template <class T> struct Nibbles;
 template <> struct Nibbles<bf16> {
   static constexpr float kScale = 64.0f;
-  static __device__ __forceinline__ uint32_t zero(uint32_t z) {
-    const __nv_bfloat162 v = __float2bfloat162_rn(float(z) * -0.015625f);
+  // of byte `at` of a word
+  static __device__ __forceinline__ uint32_t zero(uint32_t word, int at) {
+    const uint32_t bits = __byte_perm(word, 0u, 0x4040u + 0x0101u * at), high = 0xff00ff00u;   // -2^127
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), *reinterpret_cast<const __nv_bfloat162*>(&high));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
@@ -109,19 +119,20 @@ template <> struct Nibbles<bf16> {
   }
 };
 template <> struct Nibbles<fp16> {
-  static constexpr float kScale = 1.0f;
-  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | z * 0x10001u; }   // 1024 + z
+  static constexpr float kScale = 512.0f;
+  static __device__ __forceinline__ uint32_t zero(uint32_t word, int at) {
+    const uint32_t bits = __byte_perm(word, 0u, 0x4040u + 0x0101u * at), high = 0xf800f800u;   // -2^15
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&bits), *reinterpret_cast<const __half2*>(&high));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
   static __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&p)[4]) {
+    const uint32_t low = 0x78007800u, high = 0x68006800u;                      // 2^15, 2^11
     const __half2 z = *reinterpret_cast<const __half2*>(&zero);
-    const uint32_t high = and_or(zero << 4, 0x00f000f0u, 0xd400d400u);                                  // -(64 + z)
-    const uint32_t sixteenth = 0x2c002c00u;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t u = i ? w >> 8 : w;
-      const uint32_t a = and_or(u, 0x000f000fu, 0x64006400u), b = and_or(u, 0x00f000f0u, 0x64006400u);
-      const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), z);
-      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&sixteenth),
-                                *reinterpret_cast<const __half2*>(&high));
+      const uint32_t u = i ? w >> 8 : w, a = u & 0x000f000fu, b = u & 0x00f000f0u;
+      const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&low), z);
+      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&high), z);
       p[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
       p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
     }
@@ -146,6 +157,35 @@ __device__ __forceinline__ uint4 load_any(const uint8_t* p, int bytes) {
   r.z = __funnelshift_r(v[2], v[3], 8 * skew);
   r.w = __funnelshift_r(v[3], v[4], 8 * skew);
   return r;
+}
+
+// Keeps what is done with a loaded value from moving up to the load, which it would wait for there.
+__device__ __forceinline__ uint32_t late(uint32_t v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+// A half of a word as a float.
+template <class T>
+__device__ __forceinline__ float half_of(uint32_t word, int high) {
+  const uint16_t bits = uint16_t(high ? word >> 16 : word);
+  return to_float(*reinterpret_cast<const T*>(&bits));
+}
+// 1 to 16 bytes of shared memory, a power of two and so aligned.
+template <int Bytes>
+__device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* from) {
+  if constexpr (Bytes == 16) {
+    const uint4 v = *reinterpret_cast<const uint4*>(from);
+    to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+  } else if constexpr (Bytes == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(from);
+    to[0] = v.x, to[1] = v.y;
+  } else if constexpr (Bytes == 4) {
+    *to = *reinterpret_cast<const uint32_t*>(from);
+  } else if constexpr (Bytes == 2) {
+    *to = *reinterpret_cast<const uint16_t*>(from);
+  } else {
+    *to = *from;
+  }
 }
 
 // The first `count` of eight 16-bit values, zeros after them.
@@ -190,12 +230,14 @@ __device__ __forceinline__ void multipliers_sync() { asm volatile("bar.sync 1, 2
 
 // GB: blocks of 32 k per scale within a tile (1 to all of them); 1 also serves
 // the group sizes that the tile's k is no multiple of, or no divisor.
-// Copies: rows of weights and tokens start on 16-byte boundaries, and one lane
+// Boxes: rows of weights and tokens start on 16-byte boundaries, and one lane
 // of one warp copies boxes; else four warps copy words.
+// Side: scales and zero points come with the stage too.
 constexpr int kBoxThreads = 32, kWordThreads = 128;
-template <class T, int NT, int GB, bool Boxes>
+template <class T, int NT, int GB, bool Boxes, bool Side>
 __global__ void __launch_bounds__(32 * kWarps + (Boxes ? kBoxThreads : kWordThreads), Boxes ? 2 : 1)
-w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+          const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_z) {
   extern __shared__ uint8_t smem_raw[];
   using L = Tile<NT>;
   constexpr int kStages = L::kStages, kGroups = L::kK / 32 / GB, kCols = 8 * NT;
@@ -203,9 +245,9 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
-  const int stage_k = warps_k * L::kK, rows = a.warps_n * kRows;
+  const int stage_k = warps_k * L::kK, boxes = warps_k / L::kShare, rows = a.warps_n * kRows;
   const int m0 = blockIdx.z * kCols, held = min(a.tokens, kCols), tokens = min(a.tokens - m0, kCols);
-  const int stage_bytes = stage_size<NT>(held, warps_k);
+  const Stage at = stage_of<NT>(held, a.warps_n, a.scale_box, a.zero_box);
   // The work is a line of stages, row block after row block.  A cluster's CTAs
   // each take a share of one block's; without clusters the line is cut into
   // equal runs.
@@ -224,55 +266,64 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   int block = int(first / a.stages), s = int(first - int64_t(block) * a.stages);
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), read = full + 8 * kStages;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < a.places; ++i) {
       barrier_init(full + 8 * i, Boxes ? 1 : kWordThreads);
       barrier_init(read + 8 * i, kWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  // the first scale and zero point of a stage: their boxes start on 16-byte boundaries
+  auto first_scale = [&](int at_s) { return (at_s * stage_k / 32 >> a.group_shift) & ~7; };
+  auto first_zero = [&](int at_s) { return (at_s * stage_k / 32 >> a.group_shift) & ~15; };
 
   if (warp >= kWarps) {
     // ------------------------------------------------ the copies
     const int me = threadIdx.x - 32 * kWarps;
     bool ok = true;
+    int place = 0;
+    uint32_t parity = 1;
     for (int i = 0; i < count && ok; ++i) {
-      const int place = i % kStages;
-      const uint32_t stage = ring + place * stage_bytes, bar = full + 8 * place;
+      const uint32_t stage = ring + place * at.bytes, bar = full + 8 * place;
       const int k0 = s * stage_k;
       if (Boxes ? me == 0 : true) {
-        if (i >= kStages) ok = barrier_wait(read + 8 * place, (i / kStages - 1) & 1);
+        if (i >= a.places) ok = barrier_wait(read + 8 * place, parity);
         if (!ok) break;
         if constexpr (Boxes) {
-          barrier_expect(bar, L::kStageBytes + warps_k * held * L::kK * 2);
-          for (int w = 0; w < warps_k; ++w) {
-            copy_box(stage + w * rows * L::kPitch, &map_w, (k0 + w * L::kK) / 2, block * rows, bar);
-            copy_box(stage + L::kStageBytes + w * held * L::kK * 2, &map_x, k0 + w * L::kK, m0, bar);
+          barrier_expect(bar, L::kStageBytes + boxes * held * kBoxK * 2 + rows * (a.scale_box + a.zero_box));
+          for (int w = 0; w < boxes; ++w) {
+            copy_box(stage + w * rows * kPitch, &map_w, (k0 + w * kBoxK) / 2, block * rows, bar);
+            copy_box(stage + at.x + w * held * kBoxK * 2, &map_x, k0 + w * kBoxK, m0, bar);
+          }
+          if constexpr (Side) {
+            copy_box(stage + at.scales, &map_s, first_scale(s), block * rows, bar);
+            if (a.zero_box) copy_box(stage + at.zeros, &map_z, first_zero(s), block * rows, bar);
           }
         } else {
-          constexpr int kPieces = L::kStageBytes / 16 / kWordThreads;          // of a thread
+          constexpr int kOwn = L::kStageBytes / 16 / kWordThreads;             // pieces of a thread
 #pragma unroll 16
-          for (int c = 0; c < kPieces; ++c) {
-            const int p = c * kWordThreads + me, tile = p / (kRows * L::kPieces), row = p / L::kPieces % kRows, piece = p % L::kPieces;
-            const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * L::kK + piece * 32;
+          for (int c = 0; c < kOwn; ++c) {
+            const int p = c * kWordThreads + me, tile = p / (kRows * kPieces), row = p / kPieces % kRows, piece = p % kPieces;
+            const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * kBoxK + piece * 32;
             const int bytes = n < a.n ? min(max((a.k - k + 1) >> 1, 0), 16) : 0;
             const uint8_t* src = a.weight + (bytes ? int64_t(n) * a.weight_stride + (k >> 1) : 0);
-            sts128(stage + tile * L::kBytes + row * L::kPitch + ((piece ^ L::turn(row)) * 16), load_any(src, bytes));
+            sts128(stage + (tile * kRows + row) * kPitch + ((piece ^ turn(row)) * 16), load_any(src, bytes));
           }
-          for (int p = me; p < warps_k * tokens * (L::kK / 8); p += kWordThreads) {
-            const int piece = p % (L::kK / 8), m = p / (L::kK / 8) % tokens, w = p / (L::kK / 8) / tokens;
-            const int k = k0 + w * L::kK + piece * 8, left = min(max(a.k - k, 0), 8);
+          for (int p = me; p < boxes * tokens * (kBoxK / 8); p += kWordThreads) {
+            const int piece = p % (kBoxK / 8), m = p / (kBoxK / 8) % tokens, w = p / (kBoxK / 8) / tokens;
+            const int k = k0 + w * kBoxK + piece * 8, left = min(max(a.k - k, 0), 8);
             const T* src = static_cast<const T*>(a.x) + (left ? int64_t(m0 + m) * a.x_stride + k : 0);
-            sts128(stage + L::kStageBytes + ((w * held + m) * (L::kK / 8) + piece) * 16,
+            sts128(stage + at.x + ((w * held + m) * (kBoxK / 8) + piece) * 16,
                    keep(load_any(reinterpret_cast<const uint8_t*>(src), 2 * left), left));
           }
           barrier_arrive(bar);
         }
       }
       if (++s == a.stages) s = 0, ++block;
+      if (++place == a.places) place = 0, parity ^= 1;
     }
     if (Boxes && me == 0 && !ok)                         // copies under way land before the CTA goes
-      for (int i = 0; i < kStages; ++i) barrier_wait(full + 8 * i, 0), barrier_wait(full + 8 * i, 1);
+      for (int i = 0; i < a.places; ++i) barrier_wait(full + 8 * i, 0), barrier_wait(full + 8 * i, 1);
     if (a.ranks > 1) {
       cg::this_cluster().sync();
       cg::this_cluster().sync();
@@ -281,43 +332,20 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   }
 
   // -------------------------------------------------- the products
-  // Scales and zero points of row `lane`, one stage ahead of their use and as
-  // they are in memory: converting them here would wait for them here.  A
-  // tile's lie side by side, one access where that is aligned.
-  constexpr int kZeroWords = kGroups > 4 ? 2 : 1;
-  uint32_t scale_next[kGroups], zero_next[kGroups];
-  const int per = a.group / 32;
-  const bool side_by_side = kGroups > 1 && per == GB && a.groups % kGroups == 0 && a.vector_scales;
+  // Scales and zero points that no copy brings: row `lane`'s, one by one, one
+  // stage ahead of their use and as they are in memory, as converting them
+  // here would wait for them here.
+  constexpr int kScaleWords = (kGroups + 1) / 2, kZeroWords = (kGroups + 3) / 4;
+  uint32_t scale_next[Side ? 1 : kGroups], zero_next[Side ? 1 : kGroups];
   auto fetch_scales = [&](int at_block, int at_s) {
-    const int block0 = (at_s * stage_k + wk * L::kK) / 32;
+    const int block0 = (at_s * stage_k + wk * L::kK) / 32, per = a.group / 32;
     const int64_t scale_row = int64_t(min(at_block * rows + wn * kRows + lane, a.n - 1)) * a.groups;
-    if (side_by_side) {
-      const int64_t at = scale_row + min(block0 / GB, a.groups - kGroups);
-      auto words = [&](const void* from, uint32_t* to, int bytes) {
-        if (bytes == 32) {
-          *reinterpret_cast<uint4*>(to) = __ldg(static_cast<const uint4*>(from));
-          *reinterpret_cast<uint4*>(to + 4) = __ldg(static_cast<const uint4*>(from) + 1);
-        } else if (bytes == 16) {
-          *reinterpret_cast<uint4*>(to) = __ldg(static_cast<const uint4*>(from));
-        } else if (bytes == 8) {
-          *reinterpret_cast<uint2*>(to) = __ldg(static_cast<const uint2*>(from));
-        } else if (bytes == 4) {
-          *to = __ldg(static_cast<const uint32_t*>(from));
-        } else {
-          *to = __ldg(static_cast<const uint16_t*>(from));
-        }
-      };
-      if (a.scales32) words(static_cast<const float*>(a.scales) + at, scale_next, 4 * kGroups);
-      else words(static_cast<const T*>(a.scales) + at, scale_next, 2 * kGroups);
-      if (a.zeros) words(a.zeros + at, zero_next, kGroups);
-    } else {
 #pragma unroll
-      for (int e = 0; e < kGroups; ++e) {
-        const int at_k = block0 + e * GB, group = a.group_shift >= 0 ? at_k >> a.group_shift : at_k / per;
-        const int64_t at = scale_row + min(group, a.groups - 1);
-        scale_next[e] = a.scales32 ? __ldg(static_cast<const uint32_t*>(a.scales) + at) : __ldg(static_cast<const uint16_t*>(a.scales) + at);
-        if (a.zeros) zero_next[e] = __ldg(a.zeros + at);
-      }
+    for (int e = 0; e < (Side ? 0 : kGroups); ++e) {
+      const int at_k = block0 + e * GB, group = a.group_shift >= 0 ? at_k >> a.group_shift : at_k / per;
+      const int64_t i = scale_row + min(group, a.groups - 1);
+      scale_next[e] = a.scales32 ? __ldg(static_cast<const uint32_t*>(a.scales) + i) : __ldg(static_cast<const uint16_t*>(a.scales) + i);
+      zero_next[e] = a.zeros ? __ldg(a.zeros + i) : 8u;
     }
   };
 
@@ -328,33 +356,50 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   float* red = nullptr;                                  // [wk][row][token], in the place of a row block's last stage
   // this lane's words of its tile (rows g + 8 r), and its tokens' values; columns beyond the tokens repeat the last one:
   // nothing reads their sums
-  const int w_lane = warp * L::kBytes + g * L::kPitch + L::turn(g) * 16 + t * 4;
+  const int box = wk / L::kShare, half = wk % L::kShare;
+  const int w_lane = (box * rows + wn * kRows + g) * kPitch + ((half * (L::kK / 32)) ^ turn(g)) * 16 + t * 4;
   int x_lane[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) x_lane[n] = L::kStageBytes + (wk * held + min(n * 8 + g, tokens - 1)) * (L::kK * 2) + t * 16;
-  if (count) fetch_scales(block, s);
+  for (int n = 0; n < NT; ++n) x_lane[n] = at.x + (box * held + min(n * 8 + g, tokens - 1)) * (kBoxK * 2) + half * (L::kK * 2) + t * 16;
+  if (!Side && count) fetch_scales(block, s);
   for (int left = count; left > 0; --left) {
-    float scale[kGroups];
-    uint32_t zero[kGroups];
+    uint32_t scale[Side ? 4 : 1][Side ? kScaleWords : kGroups], zero[Side ? 4 : 1][Side ? kZeroWords : kGroups];
+    if constexpr (!Side) {
 #pragma unroll
-    for (int e = 0; e < kGroups; ++e) {
-      const uint16_t half = uint16_t(side_by_side ? scale_next[e / 2] >> (16 * (e & 1)) : scale_next[e]);
-      scale[e] = Nibbles<T>::kScale * (a.scales32 ? __uint_as_float(scale_next[e]) : to_float(*reinterpret_cast<const T*>(&half)));
-      zero[e] = a.zeros ? (side_by_side ? zero_next[kZeroWords == 2 ? e / 4 : 0] >> (8 * (e & 3)) : zero_next[e]) & 15u : 8u;
+      for (int e = 0; e < kGroups; ++e) scale[0][e] = late(scale_next[e]), zero[0][e] = late(zero_next[e]) & 15u;
     }
     const bool last = s + 1 == a.stages || left == 1;    // of this CTA in this row block
-    if (left > 1) fetch_scales(s + 1 == a.stages ? block + 1 : block, s + 1 == a.stages ? 0 : s + 1);
+    if (!Side && left > 1) fetch_scales(s + 1 == a.stages ? block + 1 : block, s + 1 == a.stages ? 0 : s + 1);
     ok = ok && barrier_wait(full + 8 * place, parity);
-    const int stage = place * stage_bytes;
+    const int stage = place * at.bytes;
+    if constexpr (Side) {
+      const int group = (s * stage_k + wk * L::kK) / 32 >> a.group_shift;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = wn * kRows + g + 8 * r;
+        load_words<2 * kGroups>(scale[r], smem + stage + at.scales + row * a.scale_box + (group - first_scale(s)) * 2);
+        if (a.zero_box) {
+          load_words<kGroups>(zero[r], smem + stage + at.zeros + row * a.zero_box + (group - first_zero(s)));
+#pragma unroll
+          for (int e = 0; e < kZeroWords; ++e) zero[r][e] &= 0x0f0f0f0fu;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kZeroWords; ++e) zero[r][e] = 0x08080808u;
+        }
+      }
+    }
     const int w_at = stage + w_lane;
 #pragma unroll
     for (int e = 0; e < kGroups; ++e) {
       float part[2][NT][4];
       uint32_t z[4];
-      {
-        const uint32_t own = Nibbles<T>::zero(zero[e]);
+      if constexpr (Side) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = a.zeros ? __shfl_sync(0xffffffffu, own, g + 8 * r) : own;
+        for (int r = 0; r < 4; ++r) z[r] = Nibbles<T>::zero(zero[r][e / 4], e & 3);
+      } else {
+        const uint32_t own = Nibbles<T>::zero(zero[0][e], 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = __shfl_sync(0xffffffffu, own, g + 8 * r);
       }
 #pragma unroll
       for (int b = e * GB; b < (e + 1) * GB; ++b) {
@@ -370,9 +415,9 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           uint32_t p0[4], p1[4];
-          const uint8_t* at = smem + (w_at ^ (b * 16)) + 16 * r * L::kPitch;
-          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(at), z[2 * r], p0);
-          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(at + 8 * L::kPitch), z[2 * r + 1], p1);
+          const uint8_t* word = smem + (w_at ^ (b * 16)) + 16 * r * kPitch;
+          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(word), z[2 * r], p0);
+          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(word + 8 * kPitch), z[2 * r + 1], p1);
           const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -384,7 +429,14 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float s0 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r), s1 = __shfl_sync(0xffffffffu, scale[e], g + 16 * r + 8);
+        float s0, s1;
+        if constexpr (Side) {
+          s0 = Nibbles<T>::kScale * half_of<T>(scale[2 * r][e / 2], e & 1);
+          s1 = Nibbles<T>::kScale * half_of<T>(scale[2 * r + 1][e / 2], e & 1);
+        } else {
+          const float own = Nibbles<T>::kScale * (a.scales32 ? __uint_as_float(scale[0][e]) : half_of<T>(scale[0][e], 0));
+          s0 = __shfl_sync(0xffffffffu, own, g + 16 * r), s1 = __shfl_sync(0xffffffffu, own, g + 16 * r + 8);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           acc[r][n][0] += s0 * part[r][n][0];
@@ -403,11 +455,11 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float* at = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
-          at[0] = ok ? acc[r][n][0] : NAN;
-          at[1] = ok ? acc[r][n][1] : NAN;
-          at[8 * kCols] = ok ? acc[r][n][2] : NAN;
-          at[8 * kCols + 1] = ok ? acc[r][n][3] : NAN;
+          float* to = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
+          to[0] = ok ? acc[r][n][0] : NAN;
+          to[1] = ok ? acc[r][n][1] : NAN;
+          to[8 * kCols] = ok ? acc[r][n][2] : NAN;
+          to[8 * kCols + 1] = ok ? acc[r][n][3] : NAN;
           acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.0f;
         }
       multipliers_sync();
@@ -431,7 +483,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     }
     __syncwarp();
     if (lane == 0) barrier_arrive(read + 8 * place);
-    if (++place == kStages) place = 0, parity ^= 1;
+    if (++place == a.places) place = 0, parity ^= 1;
   }
   if (a.ranks == 1) return;
 
@@ -494,7 +546,7 @@ struct Plan {
 template <int NT>
 Plan plan_for(int tokens, int n, int k, int sms) {
   constexpr int kK = Tile<NT>::kK;
-  Plan p{NT, 8, 1, 0, 0, false};
+  Plan p{NT, kWarps / Tile<NT>::kShare, 1, 0, 0, false};
   const int held = tokens < 8 * NT ? tokens : 8 * NT;
   // Rows of a CTA (32 to 256): few, as long as the warps along k all have some
   // and the tokens' values, read again by every CTA, stay within 4 (8) KB of a
@@ -544,7 +596,7 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swi
                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int NT, int GB, bool Boxes>
+template <class T, int NT, int GB, bool Boxes, bool Side>
 cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   using L = Tile<NT>;
   const int held = a.tokens < 8 * NT ? a.tokens : 8 * NT, warps_k = kWarps / p.warps_n;
@@ -553,16 +605,28 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   a.ranks = p.ranks;
   const unsigned per = unsigned(a.group / 32);
   a.group_shift = per & (per - 1) ? -1 : 31 - __builtin_clz(per);
-  CUtensorMap map_w{}, map_x{};
+  CUtensorMap map_w{}, map_x{}, map_s{}, map_z{};
   if (Boxes) {
     const int64_t x_stride = a.tokens == 1 ? (int64_t(a.k) + 7) / 8 * 8 : a.x_stride;   // one token has no stride
-    if (!make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, L::kPitch == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                  a.weight, (int64_t(a.k) + 1) / 2, a.n, a.weight_stride, L::kPitch, kRows * p.warps_n) ||
-        !make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_NONE, a.x, a.k, a.tokens, x_stride * 2, L::kK, held))
+    if (!make_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, a.weight, (int64_t(a.k) + 1) / 2, a.n,
+                  a.weight_stride, kPitch, kRows * p.warps_n) ||
+        !make_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_NONE, a.x, a.k, a.tokens, x_stride * 2, kBoxK, held))
       return cudaErrorInvalidValue;
   }
-  const size_t bytes = size_t(L::kStages) * stage_size<NT>(held, warps_k) + 1024;
-  const auto kernel = w4_kernel<T, NT, GB, Boxes>;
+  if (Side) {
+    const int groups = std::max(warps_k * L::kK / a.group, 1);                           // of a stage; a power of two
+    a.scale_box = std::max(2 * groups, 16);
+    a.zero_box = a.zeros ? std::max(groups, 16) : 0;
+    if (!make_map(&map_s, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_NONE, a.scales, a.groups, a.n, int64_t(a.groups) * 2,
+                  a.scale_box / 2, kRows * p.warps_n) ||
+        (a.zeros && !make_map(&map_z, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_NONE, a.zeros, a.groups, a.n, a.groups,
+                              a.zero_box, kRows * p.warps_n)))
+      return cudaErrorInvalidValue;
+  }
+  const int stage = stage_of<NT>(held, p.warps_n, a.scale_box, a.zero_box).bytes;
+  a.places = std::min(L::kStages, kRoom / stage);
+  const size_t bytes = size_t(a.places) * stage + 1024;
+  const auto kernel = w4_kernel<T, NT, GB, Boxes, Side>;
   static std::atomic<int> limits[kMaxDevices];           // of this kernel
   ensure_dynamic_smem(kernel, 1024, bytes, limits);
   cudaLaunchConfig_t cfg{};
@@ -578,7 +642,7 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
   }
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, map_w, map_x);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, map_w, map_x, map_s, map_z);
   if (e != cudaSuccess || !p.cut) return e;
   cfg.gridDim.x = unsigned(p.ctas - 1);
   cfg.gridDim.y = unsigned((kRows * p.warps_n * held + kJoinThreads - 1) / kJoinThreads);
@@ -590,12 +654,20 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, w4_join_kernel<T, NT>, a, int(p.ctas));
 }
 
+template <class T, int NT, int GB, bool Boxes>
+cudaError_t launch_scales(const W4Args& a, const Plan& p, cudaStream_t s) {
+  // copies bring rows of 16 bytes or more from 16-byte boundaries, in the tokens' type, of groups that a tile divides or is divided by
+  const bool side = Boxes && !a.scales32 && (a.group & (a.group - 1)) == 0 && aligned(a.scales, 16) && a.groups % 8 == 0 &&
+                    (!a.zeros || (aligned(a.zeros, 16) && a.groups % 16 == 0));
+  return side ? launch_shape<T, NT, GB, Boxes, Boxes>(a, p, s) : launch_shape<T, NT, GB, Boxes, false>(a, p, s);
+}
+
 template <class T, int NT, bool Boxes>
 cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
-  if (a.group == 64) return launch_shape<T, NT, 2, Boxes>(a, p, s);
-  if (NT == 1 && a.group % 256 == 0) return launch_shape<T, NT, NT == 1 ? 8 : 4, Boxes>(a, p, s);
-  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_shape<T, NT, 4, Boxes>(a, p, s);
-  return launch_shape<T, NT, 1, Boxes>(a, p, s);
+  if (a.group == 64) return launch_scales<T, NT, 2, Boxes>(a, p, s);
+  if (NT == 1 && a.group % 256 == 0) return launch_scales<T, NT, NT == 1 ? 8 : 4, Boxes>(a, p, s);
+  if (a.group == 128 || (NT == 2 && a.group % 128 == 0)) return launch_scales<T, NT, 4, Boxes>(a, p, s);
+  return launch_scales<T, NT, 1, Boxes>(a, p, s);
 }
 
 template <class T>
@@ -643,7 +715,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t 
   if (need && (!scratch || !aligned(scratch, 256) || scratch_bytes < need))
     return fail(PM_E_INVALID, "%s: needs %zu bytes of scratch, 256-byte aligned", who, need);
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->scales, 16) && aligned(j->zeros, 8), 0, 0, 0, static_cast<float*>(scratch)};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, plan, s) : launch<fp16>(a, plan, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");
