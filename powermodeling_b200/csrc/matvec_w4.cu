@@ -286,43 +286,47 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     for (int i = 0; i < count && ok; ++i) {
       const uint32_t stage = ring + place * at.bytes, bar = full + 8 * place;
       const int k0 = s * stage_k;
-      if (Boxes ? me == 0 : true) {
-        if (i >= a.places) ok = barrier_wait(read + 8 * place, parity);
+      if (i >= a.places) ok = barrier_wait(read + 8 * place, parity);
+      if constexpr (Boxes) {
+        // a lane for each box
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if constexpr (Boxes) {
-          barrier_expect(bar, L::kStageBytes + boxes * held * kBoxK * 2 + rows * (a.scale_box + a.zero_box));
-          for (int w = 0; w < boxes; ++w) {
-            copy_box(stage + w * rows * kPitch, &map_w, (k0 + w * kBoxK) / 2, block * rows, bar);
-            copy_box(stage + at.x + w * held * kBoxK * 2, &map_x, k0 + w * kBoxK, m0, bar);
+        if (me == 0) barrier_expect(bar, L::kStageBytes + boxes * held * kBoxK * 2 + rows * (a.scale_box + a.zero_box));
+        __syncwarp();
+        const int w = me & 7;
+        if (me < 16) {
+          if (w < boxes) {
+            if (me < 8) copy_box(stage + w * rows * kPitch, &map_w, (k0 + w * kBoxK) / 2, block * rows, bar);
+            else copy_box(stage + at.x + w * held * kBoxK * 2, &map_x, k0 + w * kBoxK, m0, bar);
           }
-          if constexpr (Side) {
-            copy_box(stage + at.scales, &map_s, first_scale(s), block * rows, bar);
-            if (a.zero_box) copy_box(stage + at.zeros, &map_z, first_zero(s), block * rows, bar);
-          }
-        } else {
-          constexpr int kOwn = L::kStageBytes / 16 / kWordThreads;             // pieces of a thread
-#pragma unroll 16
-          for (int c = 0; c < kOwn; ++c) {
-            const int p = c * kWordThreads + me, tile = p / (kRows * kPieces), row = p / kPieces % kRows, piece = p % kPieces;
-            const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * kBoxK + piece * 32;
-            const int bytes = n < a.n ? min(max((a.k - k + 1) >> 1, 0), 16) : 0;
-            const uint8_t* src = a.weight + (bytes ? int64_t(n) * a.weight_stride + (k >> 1) : 0);
-            sts128(stage + (tile * kRows + row) * kPitch + ((piece ^ turn(row)) * 16), load_any(src, bytes));
-          }
-          for (int p = me; p < boxes * tokens * (kBoxK / 8); p += kWordThreads) {
-            const int piece = p % (kBoxK / 8), m = p / (kBoxK / 8) % tokens, w = p / (kBoxK / 8) / tokens;
-            const int k = k0 + w * kBoxK + piece * 8, left = min(max(a.k - k, 0), 8);
-            const T* src = static_cast<const T*>(a.x) + (left ? int64_t(m0 + m) * a.x_stride + k : 0);
-            sts128(stage + at.x + ((w * held + m) * (kBoxK / 8) + piece) * 16,
-                   keep(load_any(reinterpret_cast<const uint8_t*>(src), 2 * left), left));
-          }
-          barrier_arrive(bar);
+        } else if (Side && w == 0) {
+          if (me == 16) copy_box(stage + at.scales, &map_s, first_scale(s), block * rows, bar);
+          else if (me == 24 && a.zero_box) copy_box(stage + at.zeros, &map_z, first_zero(s), block * rows, bar);
         }
+      } else {
+        if (!ok) break;
+        constexpr int kOwn = L::kStageBytes / 16 / kWordThreads;               // pieces of a thread
+#pragma unroll 16
+        for (int c = 0; c < kOwn; ++c) {
+          const int p = c * kWordThreads + me, tile = p / (kRows * kPieces), row = p / kPieces % kRows, piece = p % kPieces;
+          const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * kBoxK + piece * 32;
+          const int bytes = n < a.n ? min(max((a.k - k + 1) >> 1, 0), 16) : 0;
+          const uint8_t* src = a.weight + (bytes ? int64_t(n) * a.weight_stride + (k >> 1) : 0);
+          sts128(stage + (tile * kRows + row) * kPitch + ((piece ^ turn(row)) * 16), load_any(src, bytes));
+        }
+        for (int p = me; p < boxes * tokens * (kBoxK / 8); p += kWordThreads) {
+          const int piece = p % (kBoxK / 8), m = p / (kBoxK / 8) % tokens, w = p / (kBoxK / 8) / tokens;
+          const int k = k0 + w * kBoxK + piece * 8, left = min(max(a.k - k, 0), 8);
+          const T* src = static_cast<const T*>(a.x) + (left ? int64_t(m0 + m) * a.x_stride + k : 0);
+          sts128(stage + at.x + ((w * held + m) * (kBoxK / 8) + piece) * 16,
+                 keep(load_any(reinterpret_cast<const uint8_t*>(src), 2 * left), left));
+        }
+        barrier_arrive(bar);
       }
       if (++s == a.stages) s = 0, ++block;
       if (++place == a.places) place = 0, parity ^= 1;
     }
-    if (Boxes && me == 0 && !ok)                         // copies under way land before the CTA goes
+    if (Boxes && !ok)                                    // copies under way land before the CTA goes
       for (int i = 0; i < a.places; ++i) barrier_wait(full + 8 * i, 0), barrier_wait(full + 8 * i, 1);
     if (a.ranks > 1) {
       cg::this_cluster().sync();
