@@ -20,6 +20,10 @@ configuration's grid and returns one row per point:
   (capture.capture_trial) and analysed by the GPU analysis: pJ per logical
   byte, per FLOP or, with the paired control, the differential pJ per SFU
   instruction (powermodeling/analysis.py:713-762, 937-946).
+* ``operator_sweep`` - the transformer block operators (blocks.py): norms,
+  4-bit products and paged attention over rows, shapes, batches and lengths,
+  device time of one call inside a CUDA graph, the bytes it cannot do
+  without per second, and board energy per such byte.
 
 ``python -m powermodeling_b200.sweeps --out FILE`` runs every grid and
 writes the rows as JSON.  Clocks are left as the GPU has them.
@@ -36,6 +40,7 @@ from typing import Any
 from . import powerbench
 
 SFU_OPCODES = ("ex2", "lg2", "rcp", "rsqrt", "sqrt", "tanh")
+PARTS = ("hbm", "cache", "sfu", "operators", "energy")
 # A measurement window of a few fixed batches (the engine times them with CUDA events).
 QUICK = ["--seconds", "1", "--warmup-seconds", "0", "--idle-seconds", "0", "--warmup-batches", "1"]
 
@@ -68,9 +73,12 @@ def _clock_stop(handle) -> dict:
         samples = sampler.stop()
     finally:
         device.close()
-    sm = [s["sm_clock_mhz"] for s in samples if s.get("sm_clock_mhz")]
-    mem = [s["memory_clock_mhz"] for s in samples if s.get("memory_clock_mhz")]
-    return {"sm_mhz": statistics.median(sm) if sm else None, "mem_mhz": statistics.median(mem) if mem else None}
+    return {"sm_mhz": _median(samples, "sm_clock_mhz"), "mem_mhz": _median(samples, "memory_clock_mhz")}
+
+
+def _median(samples: list, key: str) -> float | None:
+    values = [s[key] for s in samples if s.get(key)]
+    return statistics.median(values) if values else None
 
 
 # ---------------------------------------------------------------------------- HBM
@@ -241,15 +249,135 @@ def energy_arms(sms: int, sfu: bool = True) -> dict[str, dict]:
     return out
 
 
+# ---------------------------------------------------------------------------- block operators
+def operator_points(quick: bool = False) -> list[dict]:
+    """One row of arguments per measured call of a block operator (bfloat16; lengths count the new token)."""
+    pts = []
+    for width in (4096,) if quick else (1024, 4096, 8192):
+        for rows in (1, 512) if quick else (1, 64, 512, 8192):
+            pts.append({"operator": "block_norm", "rows": rows, "width": width})
+            pts.append({"operator": "block_norm_backward", "rows": rows, "width": width})
+    for n, k in ((4096, 4096),) if quick else ((1024, 1024), (4096, 4096), (14336, 4096), (28672, 8192), (8192, 28672)):
+        for tokens in (1, 16) if quick else (1, 4, 8, 16):
+            pts.append({"operator": "matvec_w4", "tokens": tokens, "n": n, "k": k, "group_size": 128})
+    for batch in (1, 8) if quick else (1, 8, 64, 256):
+        for length in (512,) if quick else (128, 1024, 8192, 32768):
+            if batch * length <= 1 << 20:                 # 4 GiB of cache
+                pts.append({"operator": "paged_attention", "batch": batch, "length": length, "q_heads": 32, "kv_heads": 8,
+                            "head_dim": 128, "page_size": 16})
+    return pts
+
+
+def operator_bytes(point: dict) -> int:
+    """What a call has to read and write: each operand and result once, in its 16-bit type."""
+    p = point
+    if p["operator"] == "block_norm":
+        return 2 * (4 * p["rows"] * p["width"] + 2 * p["width"]) + 8 * p["rows"]
+    if p["operator"] == "block_norm_backward":
+        return 2 * (6 * p["rows"] * p["width"] + 4 * p["width"]) + 8 * p["rows"]
+    if p["operator"] == "matvec_w4":
+        groups = -(-p["k"] // p["group_size"])
+        return p["n"] * ((p["k"] + 1) // 2 + 2 * groups) + 2 * p["tokens"] * (p["n"] + p["k"])
+    row = p["kv_heads"] * p["head_dim"] * 2
+    pages = -(-p["length"] // p["page_size"])
+    # old entries read; the new token's key and value read and written; queries and outputs; lengths and the table
+    return p["batch"] * (2 * row * (p["length"] + 1) + 2 * 2 * p["q_heads"] * p["head_dim"] + 4 + 4 * pages)
+
+
+def operator_call(point: dict, seed: int):
+    """A call of the point's operator on its own random operands, as a function of no arguments."""
+    import torch
+    from . import blocks
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda", dtype=torch.bfloat16)
+
+    p = point
+    if p["operator"].startswith("block_norm"):
+        residual, block = normal(p["rows"], p["width"]), normal(p["rows"], p["width"])
+        pre, post = normal(p["width"]), normal(p["width"])
+        _, _, stats = blocks.block_norm(residual, block, pre, post_weight=post, return_stats=True)
+        if p["operator"] == "block_norm":
+            return lambda: blocks.block_norm(residual, block, pre, post_weight=post, return_stats=True)
+        grad_hidden, grad_normed = normal(p["rows"], p["width"]), normal(p["rows"], p["width"])
+        return lambda: blocks.block_norm_backward(grad_hidden, grad_normed, residual, block, pre, stats, post_weight=post)
+    if p["operator"] == "matvec_w4":
+        n, k, group = p["n"], p["k"], p["group_size"]
+        x = normal(p["tokens"], k)
+        weight = torch.randint(0, 256, (n, (k + 1) // 2), generator=gen, device="cuda", dtype=torch.uint8)
+        scales = normal(n, -(-k // group))
+        return lambda: blocks.matvec_w4(x, weight, scales, group_size=group)
+    pages = -(-p["length"] // p["page_size"])
+    shape = (p["batch"] * pages, p["page_size"], p["kv_heads"], p["head_dim"])
+    k_cache, v_cache = normal(*shape), normal(*shape)
+    table = torch.randperm(p["batch"] * pages, generator=gen, device="cuda").to(torch.int32).view(p["batch"], pages)
+    lengths = torch.full((p["batch"],), p["length"], dtype=torch.int32, device="cuda")
+    q = normal(p["batch"], p["q_heads"], p["head_dim"])
+    new_k, new_v = normal(p["batch"], p["kv_heads"], p["head_dim"]), normal(p["batch"], p["kv_heads"], p["head_dim"])
+    return lambda: blocks.paged_attention(q, k_cache, v_cache, table, lengths, new_k=new_k, new_v=new_v)
+
+
+def operator_sweep(quick: bool = False, seconds: float = 1.0) -> list[dict]:
+    """Device time per call: a graph of calls on operand sets that together exceed twice the L2, replayed
+    for about ``seconds`` (``quick``: 0.05) under the sampler, between two events."""
+    import torch
+    l2 = torch.cuda.get_device_properties(0).L2_cache_size
+    seconds = 0.05 if quick else seconds
+    uuid = describe()["uuid"]
+    rows = []
+    for point in operator_points(quick):
+        need = operator_bytes(point)
+        sets = min(max(2, -(-2 * l2 // need)), 64)
+        calls = [operator_call(point, seed) for seed in range(sets)]
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            for call in calls:
+                call()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for call in calls:
+                call()
+
+        def timed(replays: int) -> float:
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            start.record()
+            for _ in range(replays):
+                graph.replay()
+            end.record()
+            torch.cuda.synchronize()
+            return start.elapsed_time(end) / 1e3 / (replays * sets)
+
+        timed(3)
+        replays = max(3, int(seconds / (timed(3) * sets)))
+        handle = _clock_sampler(uuid)
+        s = timed(replays)
+        board = {}
+        if handle is not None:
+            device, sampler = handle
+            try:
+                samples = sampler.stop()
+            finally:
+                device.close()
+            watts = _median(samples, "power_w")
+            board = {"sm_mhz": _median(samples, "sm_clock_mhz"), "board_power_w": watts,
+                     "total_pj_per_byte": watts * s / need * 1e12 if watts else None}
+        rows.append({**point, "us": s * 1e6, "bytes": need, "gbs": need / s / 1e9, "operand_sets": sets, **board})
+        del graph, calls
+    return rows
+
+
 def main(argv=None) -> int:
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--out", required=True)
     parser.add_argument("--quick", action="store_true")
-    parser.add_argument("--only", choices=("hbm", "cache", "sfu", "energy"), action="append")
+    parser.add_argument("--only", choices=PARTS, action="append")
     a = parser.parse_args(argv)
     dev = describe()
     sms = dev["sm_count"]
-    parts = a.only or ["hbm", "cache", "sfu", "energy"]
+    parts = a.only or PARTS
     result: dict[str, Any] = {"device": {k: dev.get(k) for k in ("name", "uuid", "sm_count", "memory_bus_width_bits")}}
     handle = _clock_sampler(dev["uuid"])
     t0 = time.time()
@@ -260,6 +388,8 @@ def main(argv=None) -> int:
     if "sfu" in parts:
         result["sfu"] = sfu_sweep(sms, ks=(8,) if a.quick else range(1, 9))
         result["sfu_uniform_input"] = sfu_sweep(sms, ks=(8,), uniform_input=True)
+    if "operators" in parts:
+        result["operators"] = operator_sweep(a.quick)
     clock = _clock_stop(handle)
     if "hbm" in result and clock.get("mem_mhz"):
         with_theory(result["hbm"], clock["mem_mhz"])

@@ -224,6 +224,41 @@ def test_norm_captured_backward(gen):
             assert torch.equal(a, b)
 
 
+def test_norm_autograd_of_some_inputs(gen):
+    """Each input alone asks for its gradient; both outputs or one lead back to it."""
+    t = norm_inputs(gen, 12, 96, F32, gate_rows=3)
+    gh, gy = randn(gen, 12, 96, dtype=F32), randn(gen, 12, 96, dtype=F32)
+    for use in ((True, True), (True, False), (False, True)):
+        want = R.norm_grads(gh if use[0] else None, gy if use[1] else None, t["residual"], t["block"], t["pre"], t["post"],
+                            t["gate"], 0.5, 1e-5)
+        for name in t:
+            x = {k: v.clone().requires_grad_(k == name) for k, v in t.items()}
+            out = blocks.block_norm(x["residual"], x["block"], x["pre"], post_weight=x["post"], gate=x["gate"], scale=0.5)
+            torch.autograd.backward([o for o, u in zip(out, use) if u], [g for g, u in zip((gh, gy), use) if u])
+            assert all(x[k].grad is None for k in t if k != name)
+            if name in want:
+                check("grad " + name, x[name].grad, want[name], 3 * (96 / 32 + 64) + 12 + 600)
+            else:
+                assert x[name].grad is None or not x[name].grad.any()
+
+
+def test_norm_autograd_refuses_a_capture(gen):
+    """The engine's backward inside a capture is refused, and the capture goes on without it."""
+    w, x = randn(gen, 64, dtype=F32).requires_grad_(), randn(gen, 4, 64, dtype=F32)
+    out = blocks.block_norm(x, x, w)[1].sum()
+    want = blocks.block_norm(x, x, w.detach())[1]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture block_norm_backward itself"):
+            blocks._BlockNormFunction.backward(None, x, x, None)
+        y = blocks.block_norm(x, x, w.detach())[1]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    out.backward()
+    assert w.grad is not None
+
+
 # ---------------------------------------------------------------- 4-bit weights
 def w4_inputs(gen, tokens, n, k, dtype, group, zeros, scales=None):
     groups = -(-k // group)
@@ -268,6 +303,38 @@ def test_w4_groups_and_scale_types(gen, group, zeros):
 @pytest.mark.parametrize("tokens", [17, 33, 64])
 def test_w4_more_tokens_than_one_pass(gen, tokens):
     w4_check(w4_inputs(gen, tokens, 333, 768, BF, 64, True), 64)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 4, 8, 9, 16, 21])
+@pytest.mark.parametrize("group", [32, 64, 128, 256, 512, 1024])
+def test_w4_scales_in_whole_boxes(gen, group, tokens):
+    """Groups by the sixteen, whose scales and zero points copies bring; with one group less or more they do not."""
+    for groups in (8, 16, 48, 15, 17):
+        for zeros in (False, True):
+            w4_check(w4_inputs(gen, tokens, 97, group * groups, FP, group, zeros), group)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("tokens,n,k,group", [(1, 14336, 4096, 128), (8, 14336, 4096, 32), (16, 10001, 8192, 64), (3, 40000, 1024, 64),
+                                              (16, 9000, 4064, 32), (20, 12288, 2048, 256)])
+def test_w4_line_cut_into_runs(gen, tokens, n, k, group, dtype):
+    """Matrices large enough that runs end within row blocks, aligned and from odd addresses."""
+    t = w4_inputs(gen, tokens, n, k, dtype, group, zeros=True)
+    first = w4_check(t, group)
+    assert torch.equal(first, blocks.matvec_w4(t["x"], t["weight"], t["scales"], t["zeros"], group_size=group))
+    held = torch.full((n, t["weight"].shape[1] + 3), 255, device="cuda", dtype=torch.uint8)
+    held[:, 1:-2] = t["weight"]
+    w4_check(dict(t, weight=held[:, 1:-2]), group)
+
+
+def test_w4_scales_that_start_anywhere(gen):
+    """Scales and zero points from addresses that no copy can start at."""
+    t = w4_inputs(gen, 2, 64, 1024, BF, 64, True)
+    scales, zeros = torch.empty(64 * 16 + 1, device="cuda", dtype=BF), torch.empty(64 * 16 + 1, device="cuda", dtype=torch.uint8)
+    scales[1:], zeros[1:] = t["scales"].view(-1), t["zeros"].view(-1)
+    for s in (t["scales"], scales[1:].view(64, 16)):
+        for z in (t["zeros"], zeros[1:].view(64, 16)):
+            w4_check(dict(t, scales=s, zeros=z), 64)
 
 
 def test_w4_strides_and_alignment(gen):
@@ -366,6 +433,15 @@ def test_attention_long_and_ragged(gen):
     attend(gen, [0, 0, 0], 2, 4, 64, 16, BF)
     attend(gen, [1] * 300, 2, 4, 64, 16, BF)
     attend(gen, [33 * (i % 7) for i in range(200)], 8, 1, 64, 16, BF)
+
+
+@pytest.mark.parametrize("batch,longest", [(1, 256), (5, 128), (18, 256), (60, 256), (130, 200), (300, 64), (700, 130)])
+def test_attention_many_short_sequences(gen, batch, longest):
+    """Tables of one to four tiles, with a run for each segment and with fewer; some sequences are empty."""
+    lens = [0 if i % 7 == 3 else (i * 37) % longest + 1 for i in range(batch)]
+    lens[-1] = longest
+    attend(gen, lens, 4, 4, 64, 16, BF)
+    attend(gen, lens, 4, 4, 64, 16, FP, window=50, new=False)
 
 
 def test_attention_absent_pages_and_short_tables(gen):
