@@ -38,6 +38,7 @@ namespace blk {
 namespace {
 
 constexpr int kWarps = 8, kRows = 32;                    // warps that multiply; rows of a warp's tile
+constexpr int kMaxRanks = 8;                             // CTAs of a cluster
 constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait; a result that it poisons is NaN
 
 // Rows lie in shared memory 256 k (128 bytes) wide, as a copy brings them: 64
@@ -491,7 +492,8 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   }
   if (a.ranks == 1) return;
 
-  // a cluster's sums, through distributed shared memory, in the ranks' order
+  // a cluster's sums, through distributed shared memory, in the ranks' order; each rank has a share of the rows, and
+  // all ranks' values are under way at once
   float* sums = reinterpret_cast<float*>(smem);          // one place for all ranks; red's own, or where no copy is under way
   for (int c = threadIdx.x; c < rows * kCols; c += 32 * kWarps) {
     float v = red[c];
@@ -499,18 +501,24 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     sums[c] = v;
   }
   cg::this_cluster().sync();
-  if (rank == 0) {
-    const int64_t first_row = int64_t(blockIdx.x / a.ranks) * rows;
-    T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + first_row;
-    for (int c = threadIdx.x; c < rows * tokens; c += 32 * kWarps) {
-      const int m = c / rows, row = c - m * rows;
-      if (first_row + row >= a.n) continue;
-      float v = sums[row * kCols + m];
-      for (int r = 1; r < a.ranks; ++r) v += cg::this_cluster().map_shared_rank(sums, r)[row * kCols + m];
-      y[int64_t(m) * a.n + row] = from_float<T>(v);
-    }
+  const int64_t first_row = int64_t(blockIdx.x / a.ranks) * rows;
+  T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + first_row;
+  for (int c = rank * 32 * kWarps + threadIdx.x; c < rows * (kCols / 4); c += a.ranks * 32 * kWarps) {
+    const int q = c / rows, row = c - q * rows;
+    if (first_row + row >= a.n || 4 * q >= tokens) continue;
+    float4 v[kMaxRanks];
+#pragma unroll
+    for (int r = 0; r < kMaxRanks; ++r)
+      if (r < a.ranks) v[r] = *reinterpret_cast<const float4*>(cg::this_cluster().map_shared_rank(sums, r) + row * kCols + 4 * q);
+#pragma unroll
+    for (int r = 1; r < kMaxRanks; ++r)
+      if (r < a.ranks) v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
+    const float value[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      if (4 * q + m < tokens) y[int64_t(4 * q + m) * a.n + row] = from_float<T>(value[m]);
   }
-  cg::this_cluster().sync();                             // a CTA's sums stay until rank 0 has them
+  cg::this_cluster().sync();                             // a CTA's sums stay until every rank has them
 }
 
 // Joins the pieces of the row blocks that runs were cut within: CTA c takes
@@ -567,7 +575,7 @@ Plan plan_for(int tokens, int n, int k, int sms) {
     p.cut = blocks * p.stages % slots != 0 || blocks * p.stages / slots % p.stages != 0;
   } else {
     // a cluster for each row block, as long as the SMs hold more and every CTA has a stage
-    while (p.ranks < 8 && blocks * p.ranks * 2 <= slots && p.ranks * 2 <= p.stages) p.ranks *= 2;
+    while (p.ranks < kMaxRanks && blocks * p.ranks * 2 <= slots && p.ranks * 2 <= p.stages) p.ranks *= 2;
     p.ctas = p.ranks > 1 ? blocks * p.ranks : blocks;
   }
   return p;
