@@ -39,6 +39,7 @@ namespace {
 
 constexpr int kWarps = 8, kRows = 32;                    // warps that multiply; rows of a warp's tile
 constexpr int kMaxRanks = 8;                             // CTAs of a cluster
+constexpr int kLine = 8;                                 // stages of a CTA from which on runs are equal
 constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait; a result that it poisons is NaN
 
 // Rows lie in shared memory 256 k (128 bytes) wide, as a copy brings them: 64
@@ -474,12 +475,21 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
         float* part = a.part + ((int64_t(blockIdx.z) * gridDim.x + blockIdx.x) * 2 + (s_first == 0 ? 1 : 0)) * rows * kCols;
         T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + int64_t(block) * rows;
         const int there = min(rows, a.n - block * rows);
-        for (int c = threadIdx.x; c < rows * tokens; c += 32 * kWarps) {
-          const int m = c / rows, row = c - m * rows;
-          float v = 0.0f;
-          for (int w = 0; w < warps_k; ++w) v += red[(w * rows + row) * kCols + m];
-          if (!whole) part[m * rows + row] = v;
-          else if (row < there) y[int64_t(m) * a.n + row] = from_float<T>(v);
+        for (int c = threadIdx.x; c < rows * (kCols / 4); c += 32 * kWarps) {
+          const int q = c / rows, row = c - q * rows;    // four tokens of a row: 2 lanes to a bank where one would be 8 or 16
+          if (4 * q >= tokens) break;
+          float4 v = *reinterpret_cast<const float4*>(red + row * kCols + 4 * q);
+          for (int w = 1; w < warps_k; ++w) {
+            const float4 u = *reinterpret_cast<const float4*>(red + (w * rows + row) * kCols + 4 * q);
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+          }
+          const float value[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            if (4 * q + m >= tokens) continue;
+            if (!whole) part[(4 * q + m) * rows + row] = value[m];
+            else if (row < there) y[int64_t(4 * q + m) * a.n + row] = from_float<T>(value[m]);
+          }
         }
       }
       asm volatile("fence.proxy.async;" ::: "memory");   // these writes come before the copies that go there next
@@ -565,15 +575,21 @@ Plan plan_for(int tokens, int n, int k, int sms) {
   // stage: a quarter (half) of the weights' bytes, and two CTAs to an SM.
   const int need = NT == 1 ? held : 4;
   while (p.warps_n > 1 && p.warps_n / 2 >= need && kWarps / (p.warps_n / 2) * kK < k + kK) p.warps_n /= 2;
-  const int rows = kRows * p.warps_n, stage_k = kWarps / p.warps_n * kK;
-  const int64_t blocks = (int64_t(n) + rows - 1) / rows;
-  p.stages = (k + stage_k - 1) / stage_k;
   const int64_t slots = 2 * int64_t(sms);                // CTAs resident at once
-  if (blocks * p.stages >= 4 * slots) {
-    // enough for every CTA to have four stages or more: equal runs
+  int64_t blocks;
+  auto share = [&](int warps_n) {
+    p.warps_n = warps_n;
+    blocks = (int64_t(n) + kRows * warps_n - 1) / (kRows * warps_n);
+    p.stages = (k + kWarps / warps_n * kK - 1) / (kWarps / warps_n * kK);
+  };
+  share(p.warps_n);
+  if (blocks * p.stages >= kLine * slots) {
+    // enough for every CTA to have kLine stages or more: equal runs
     p.ctas = slots;
     p.cut = blocks * p.stages % slots != 0 || blocks * p.stages / slots % p.stages != 0;
   } else {
+    if (blocks > slots && p.warps_n < kWarps / Tile<NT>::kShare) share(p.warps_n * 2);
+    else if (p.warps_n > 1 && blocks * kMaxRanks * 2 <= slots && p.stages > kMaxRanks) share(p.warps_n / 2);
     // a cluster for each row block, as long as the SMs hold more and every CTA has a stage
     while (p.ranks < kMaxRanks && blocks * p.ranks * 2 <= slots && p.ranks * 2 <= p.stages) p.ranks *= 2;
     p.ctas = p.ranks > 1 ? blocks * p.ranks : blocks;
