@@ -86,6 +86,8 @@ struct W4Args {
   int places;                                            // stages in shared memory
   int stages;                                            // stages of a row block: its k over the stage's
   int ranks;                                             // CTAs of a cluster, which share each row block's stages
+  int runs, run_rest;                                    // ranks == 1: the line is cut into so many runs;
+  int64_t run;                                           // total / runs and what is left
   float* part;                                           // ranks == 1: sums of cut row blocks, [2 * CTAs][rows][8 NT]
 };
 
@@ -230,6 +232,9 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
 }
 __device__ __forceinline__ void multipliers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
+// Where run `run` starts: total * run / runs without a 64-bit division.
+__device__ __forceinline__ int64_t run_start(const W4Args& a, int run) { return a.run * run + uint32_t(a.run_rest * run) / uint32_t(a.runs); }
+
 // GB: blocks of 32 k per scale within a tile (1 to all of them); 1 also serves
 // the group sizes that the tile's k is no multiple of, or no divisor.
 // Boxes: rows of weights and tokens start on 16-byte boundaries, and one lane
@@ -261,11 +266,10 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     first = int64_t(blockIdx.x / a.ranks) * a.stages + from;
     count = int(int64_t(a.stages) * (rank + 1) / a.ranks) - from;
   } else {
-    const int64_t total = int64_t((a.n + rows - 1) / rows) * a.stages;
-    first = total * blockIdx.x / gridDim.x;
-    count = int(total * (blockIdx.x + 1) / gridDim.x - first);
+    first = run_start(a, blockIdx.x);
+    count = int(run_start(a, blockIdx.x + 1) - first);
   }
-  int block = int(first / a.stages), s = int(first - int64_t(block) * a.stages);
+  int block = int(first >> 32 ? first / a.stages : int64_t(uint32_t(first) / uint32_t(a.stages))), s = int(first - int64_t(block) * a.stages);
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), read = full + 8 * kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.places; ++i) {
@@ -532,29 +536,37 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
 }
 
 // Joins the pieces of the row blocks that runs were cut within: CTA c takes
-// the block in which run c starts, unless an earlier run starts there too.
+// the block in which run c starts, unless an earlier run starts there too.  A
+// thread adds four rows of a token; what it adds is known before the wait.
 constexpr int kJoinThreads = 256;
 template <class T, int NT>
-__global__ void __launch_bounds__(kJoinThreads) w4_join_kernel(const __grid_constant__ W4Args a, int runs) {
+__global__ void __launch_bounds__(kJoinThreads) w4_join_kernel(const __grid_constant__ W4Args a) {
   constexpr int kCols = 8 * NT;
   const int rows = a.warps_n * kRows, c = blockIdx.x + 1;
-  const int64_t total = int64_t((a.n + rows - 1) / rows) * a.stages;
-  auto start = [&](int run) { return total * run / runs; };
-  const int64_t block = start(c) / a.stages;
+  const int64_t from = run_start(a, c);
+  const int64_t block = from >> 32 ? from / a.stages : int64_t(uint32_t(from) / uint32_t(a.stages));
+  const int64_t begin = block * a.stages;
+  const bool first = from != begin && run_start(a, c - 1) <= begin;
+  int last = c;                                          // the runs that start in the block end before this one
+  while (first && last < a.runs && run_start(a, last) < begin + a.stages) ++last;
   asm volatile("griddepcontrol.wait;" ::: "memory");    // in every CTA: this kernel's end has to mean the first one's
-  if (start(c) % a.stages == 0 || (start(c - 1) > block * a.stages)) return;
+  if (!first) return;
   const int m0 = blockIdx.z * kCols, tokens = min(a.tokens - m0, kCols);
-  const float* part = a.part + int64_t(blockIdx.z) * runs * 2 * rows * kCols;
-  T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + block * rows;
+  const int i = 4 * (blockIdx.y * kJoinThreads + threadIdx.x), m = i / rows, row = i - m * rows;
   const int there = int(min(int64_t(rows), a.n - block * rows));
-  const int i = blockIdx.y * kJoinThreads + threadIdx.x, m = i / rows, row = i - m * rows;
   if (m >= tokens || row >= there) return;
-  float v = __ldcg(part + (int64_t(c - 1) * 2 + 1) * rows * kCols + i);
-  int last = c;
-  while (last < runs && start(last) < (block + 1) * a.stages) ++last;
+  const float* part = a.part + int64_t(blockIdx.z) * a.runs * 2 * rows * kCols + i;
+  float4 v = __ldcg(reinterpret_cast<const float4*>(part + (int64_t(c - 1) * 2 + 1) * rows * kCols));
 #pragma unroll 4
-  for (int k = c; k < last; ++k) v += __ldcg(part + int64_t(k) * 2 * rows * kCols + i);
-  y[int64_t(m) * a.n + row] = from_float<T>(v);
+  for (int k = c; k < last; ++k) {
+    const float4 u = __ldcg(reinterpret_cast<const float4*>(part + int64_t(k) * 2 * rows * kCols));
+    v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+  }
+  T* y = static_cast<T*>(a.y) + int64_t(m0 + m) * a.n + block * rows + row;
+  const float value[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (row + r < there) y[r] = from_float<T>(value[r]);
 }
 
 // ---------------------------------------------------------------- launch
@@ -631,6 +643,10 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   a.warps_n = p.warps_n;
   a.stages = p.stages;
   a.ranks = p.ranks;
+  a.runs = int(p.ctas);
+  const int64_t total = (int64_t(a.n) + kRows * p.warps_n - 1) / (kRows * p.warps_n) * p.stages;
+  a.run = total / a.runs;
+  a.run_rest = int(total % a.runs);
   const unsigned per = unsigned(a.group / 32);
   a.group_shift = per & (per - 1) ? -1 : 31 - __builtin_clz(per);
   CUtensorMap map_w{}, map_x{}, map_s{}, map_z{};
@@ -673,13 +689,13 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, map_w, map_x, map_s, map_z);
   if (e != cudaSuccess || !p.cut) return e;
   cfg.gridDim.x = unsigned(p.ctas - 1);
-  cfg.gridDim.y = unsigned((kRows * p.warps_n * held + kJoinThreads - 1) / kJoinThreads);
+  cfg.gridDim.y = unsigned((kRows * p.warps_n * held + 4 * kJoinThreads - 1) / (4 * kJoinThreads));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, w4_join_kernel<T, NT>, a, int(p.ctas));
+  return cudaLaunchKernelEx(&cfg, w4_join_kernel<T, NT>, a);
 }
 
 template <class T, int NT, int GB, bool Boxes>
@@ -743,7 +759,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t 
   if (need && (!scratch || !aligned(scratch, 256) || scratch_bytes < need))
     return fail(PM_E_INVALID, "%s: needs %zu bytes of scratch, 256-byte aligned", who, need);
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, plan, s) : launch<fp16>(a, plan, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");
