@@ -379,6 +379,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
       for (int e = 0; e < kGroups; ++e) scale[0][e] = late(scale_next[e]), zero[0][e] = late(zero_next[e]) & 15u;
     }
     const bool last = s + 1 == a.stages || left == 1;    // of this CTA in this row block
+    if (left == 1 && a.ranks == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join's CTAs come and wait
     if (!Side && left > 1) fetch_scales(s + 1 == a.stages ? block + 1 : block, s + 1 == a.stages ? 0 : s + 1);
     ok = ok && barrier_wait(full + 8 * place, parity);
     const int stage = place * at.bytes;
