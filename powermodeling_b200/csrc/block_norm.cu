@@ -23,7 +23,17 @@
 //    same with single elements, neighbours in neighbouring lanes, the next
 //    row's loaded ahead into registers.  What is wider than that reads its
 //    rows again in each pass (the loop kernels).
+//  * Sums and statistics are 32-bit, h enters the second norm unrounded; only
+//    the outputs are rounded to their type.
+// Measured, bf16 with both weights, inputs out of the L2 (a copy runs at 6.55
+// TB/s): forward 8192 rows x 8192 93.8 us = 5.7 TB/s, x 4096 51.8 us = 5.2
+// TB/s; backward 157.9 us = 5.1 and 81.8 us = 4.9 TB/s.  One row of 4096: 3.0
+// us, and 8.6 us for the backward's two launches.  Beside HBM the issue slots
+// are short (half and two thirds of them busy at 8192 wide): the conversions
+// and the reductions' barriers, not the copies, keep it from the copy's rate.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "blocks.cuh"
 
@@ -168,66 +178,51 @@ __device__ __forceinline__ void factor_piece(const NormArgs<T>& f, int64_t segme
 }
 
 // ---------------------------------------------------------------- forward, a row at a time
-// C pieces of N elements per thread, in registers; WarpRow: one warp per row, else one CTA.
-template <class T, int N, int C, bool WarpRow>
+// Rows that 16-byte pieces do not fit: a CTA each, kSingles elements of a
+// thread in registers.  Bound by the latency of a row's loads and its two sums
+// with a few rows to an SM (20000 rows of 1023 bf16: 1.5 TB/s); the parameters
+// come from the L1 each time.
+template <class T>
 __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ NormArgs<T> a) {
   __shared__ float red[2][32];
-  const int64_t row = WarpRow ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= a.rows) return;                             // whole warps of the last CTA, which has no barrier
-  const int first = WarpRow ? threadIdx.x & 31 : threadIdx.x, step = WarpRow ? 32 : blockDim.x;
-  const int pieces = a.width / N;
+  constexpr int C = kSingles;
+  const int64_t row = blockIdx.x;
   const T* r = a.residual + row * a.residual_stride;
   const T* b = a.block + row * a.block_stride;
   const int64_t segment = a.gate_rows ? row / a.rows_per_gate : 0;
-  float h[C][N], x[C][N];
+  float h[C], x[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p = first + c * step;
-    if (p < pieces) {
-      const Raw<T, N> bv = load_raw<T, N>(b + p * N), rv = load_raw<T, N>(r + p * N);
-      bv.unpack(x[c]);
-      rv.unpack(h[c]);
-    }
+    const int p = threadIdx.x + c * blockDim.x;
+    x[c] = p < a.width ? to_float(__ldcs(b + p)) : 0.0f;
+    h[c] = p < a.width ? to_float(__ldcs(r + p)) : 0.0f;
   }
-  auto total = [&](float v, float* where) { return WarpRow ? warp_sum(v) : cta_sum(v, where); };
   float r1 = 1.0f;
   if (a.post.p) {
     float s = 0.0f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (first + c * step < pieces)
-#pragma unroll
-        for (int i = 0; i < N; ++i) s += x[c][i] * x[c][i];
-    r1 = rsqrtf(total(s, red[0]) / float(a.width) + a.eps);
+    for (int c = 0; c < C; ++c) s += x[c] * x[c];
+    r1 = rsqrtf(cta_sum(s, red[0]) / float(a.width) + a.eps);
   }
   float s = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p = first + c * step;
-    if (p < pieces) {
-      float w[N];
-      factor_piece<T, N>(a, segment, p * N, w);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        h[c][i] += w[i] * (x[c][i] * r1);
-        s += h[c][i] * h[c][i];
-      }
-      store<T, N>(a.hidden + row * a.width + p * N, h[c]);
+    const int p = threadIdx.x + c * blockDim.x;
+    if (p < a.width) {
+      float w[1];
+      factor_piece<T, 1>(a, segment, p, w);
+      h[c] += w[0] * (x[c] * r1);
+      s += h[c] * h[c];
+      __stcs(a.hidden + row * a.width + p, from_float<T>(h[c]));
     }
   }
-  const float r2 = rsqrtf(total(s, red[1]) / float(a.width) + a.eps);
+  const float r2 = rsqrtf(cta_sum(s, red[1]) / float(a.width) + a.eps);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p = first + c * step;
-    if (p < pieces) {
-      float w[N];
-      param_piece<T, N>(a.pre, p * N, w);
-#pragma unroll
-      for (int i = 0; i < N; ++i) h[c][i] *= r2 * w[i];
-      store<T, N>(a.normed + row * a.width + p * N, h[c]);
-    }
+    const int p = threadIdx.x + c * blockDim.x;
+    if (p < a.width) __stcs(a.normed + row * a.width + p, from_float<T>(h[c] * (r2 * a.pre.at(p))));
   }
-  if (a.stats && first == 0) {
+  if (a.stats && threadIdx.x == 0) {
     a.stats[2 * row] = r1;
     a.stats[2 * row + 1] = r2;
   }
@@ -436,8 +431,8 @@ __device__ __forceinline__ Run run_of(int64_t rows, int64_t segments, int chunks
   return {items * part / parts, items * (part + 1) / parts, rows / segments, chunks};
 }
 
-// Whether w_pre lives in shared memory: where 640 threads or a warp with two pieces run out of registers.
-constexpr __host__ __device__ bool pre_shared(int n, int c, bool warps) { return n == 8 && (warps ? c == 2 : c == 1); }
+// Whether w_pre lives in shared memory: where a warp with two pieces runs out of registers.
+constexpr __host__ __device__ bool pre_shared(int n, int c, bool warps) { return n == 8 && warps && c == 2; }
 // Rows in a ring: 512 threads of an SM then hold 192 (EachRow: 160) KB of them.
 constexpr __host__ __device__ int stages_of(bool each_row) { return each_row ? 2 : 3; }
 
@@ -446,7 +441,7 @@ constexpr __host__ __device__ int stages_of(bool each_row) { return each_row ? 2
 // warp, the CTA's warps then taking rows in turn).  EachRow: a gate per row,
 // which streams with the rows; its gradient is complete with the row.
 template <class T, int N, int C, bool Warps, bool EachRow, bool Cluster>
-__global__ void __launch_bounds__(Warps ? 256 : C == 1 ? 640 : 512, Warps ? 2 : 1) grad_row_kernel(const __grid_constant__ GradArgs<T> a) {
+__global__ void __launch_bounds__(Warps ? 256 : 512, Warps ? 2 : 1) grad_row_kernel(const __grid_constant__ GradArgs<T> a) {
   constexpr bool kRing = N > 1;
   constexpr int kArrays = EachRow ? 5 : 4, kStages = stages_of(EachRow);
   constexpr bool kPreShared = pre_shared(N, C, Warps);
@@ -1017,6 +1012,7 @@ cudaError_t launch_norm_stream(const NormArgs<T>& a, int ctas, int ranks, int th
 template <class T, bool EachRow>
 cudaError_t launch_norm_streams(const NormArgs<T>& a, int pieces, int sms, cudaStream_t s) {
   auto of_rows = [&](int64_t per, int most) { return int((a.rows + per - 1) / per < most ? (a.rows + per - 1) / per : most); };
+  // by warps and by CTAs, 65536 rows: 256 bf16 wide 26 and 38 us, 512 wide 50 and 49 (both at HBM's rate)
   if (pieces <= 32) return launch_norm_stream<T, 1, true, EachRow, false>(a, of_rows(8, sms * 4), 1, 256, pieces, s);
   if (pieces <= 64) return launch_norm_stream<T, 2, true, EachRow, false>(a, of_rows(8, sms * 2), 1, 256, pieces, s);
   // one piece a thread (64 registers, 1024 threads an SM); of more than 768, two (512 threads of 128): 4.5 against 3.6
@@ -1038,8 +1034,9 @@ cudaError_t launch_forward(const pm_block_norm* j, int sms, cudaStream_t s) {
   const int pieces = a.width / kWide<T>;
   if (wide(a, true) && fits && pieces <= 8192 && aligned(a.stats, 8))
     return each_row ? launch_norm_streams<T, true>(a, pieces, sms, s) : launch_norm_streams<T, false>(a, pieces, sms, s);
+  // 20000 rows of 1023 bf16: 89 us, by the loops 162 (backward included 214 and 884)
   if (fits && a.width <= 1024 * kSingles) {
-    norm_row_kernel<T, 1, kSingles, false><<<unsigned(a.rows), threads_for(a.width, kSingles), 0, s>>>(a);
+    norm_row_kernel<T><<<unsigned(a.rows), threads_for(a.width, kSingles), 0, s>>>(a);
     return cudaGetLastError();
   }
   const int64_t most = int64_t(sms) * 8;
@@ -1052,8 +1049,7 @@ cudaError_t launch_grad_rows(const GradArgs<T>& a, int parts, int ranks, int thr
   size_t bytes = 0;
   if (N > 1) {
     bytes = size_t(stages_of(EachRow)) * (EachRow ? 5 : 4) * C * threads * 16 + (pre_shared(N, C, Warps) ? size_t(C) * threads * N * 4 : 0);
-    const size_t sums = Warps ? size_t(2) * (threads / 32) * a.f.width * 4 : 0;
-    if (sums > bytes) bytes = sums;
+    if constexpr (Warps) bytes = std::max(bytes, size_t(2) * (threads / 32) * a.f.width * 4);
   }
   static std::atomic<int> limits[kMaxDevices];           // of this kernel
   return launch_rows(grad_row_kernel<T, N, C, Warps, EachRow, Cluster>, parts, ranks, threads, bytes, limits, s, a);
@@ -1068,8 +1064,7 @@ cudaError_t launch_grad_streams(const GradArgs<T>& a, bool rows16, bool by_warps
     return per == 1 ? launch_grad_rows<T, N, 1, true, EachRow, false>(a, parts, 1, 256, s)
                     : launch_grad_rows<T, N, 2, true, EachRow, false>(a, parts, 1, 256, s);
   if (ranks > 1) return launch_grad_rows<T, N, 2, false, EachRow, true>(a, parts, ranks, threads, s);
-  return per == 1 ? launch_grad_rows<T, N, 1, false, EachRow, false>(a, parts, 1, threads, s)
-                  : launch_grad_rows<T, N, 2, false, EachRow, false>(a, parts, 1, threads, s);
+  return launch_grad_rows<T, N, 2, false, EachRow, false>(a, parts, 1, threads, s);
 }
 
 template <class T>
@@ -1088,12 +1083,14 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
   const bool rows16 = wide(a.f, false) && aligned(a.grad_residual, 16) && aligned(a.grad_block, 16) && aligned(d->grad_gate, 16) &&
                       (!a.grad_hidden || (aligned(a.grad_hidden, 16) && a.grad_hidden_stride % N == 0)) &&
                       (!a.grad_normed || (aligned(a.grad_normed, 16) && a.grad_normed_stride % N == 0));
-  // pieces of 16 bytes, or single elements; 512 threads of a CTA at most, with one or two pieces or kSingles elements each
+  // pieces of 16 bytes, or single elements; 512 threads of a CTA at most, with two pieces or kSingles elements each (one
+  // piece and up to 640 threads took 386 us instead of 348 for forward and backward of 16384 rows x 5120 bf16)
   const int pieces = rows16 ? j->width / N : j->width;
   const int ranks = ranks_for(pieces, rows16 ? 1024 : 512 * kSingles);
   bool streamed = j->rows <= 0x7fffffff && aligned(a.f.stats, 8) && pieces <= 8 * (rows16 ? 1024 : 512 * kSingles);
   a.slice = (pieces + ranks - 1) / ranks;
-  // rows of up to 64 pieces go by warps, 8 of them a CTA, where a CTA stays in one segment or every row has its gate
+  // Rows of up to 64 pieces go by warps, 8 of them a CTA, where a CTA stays in one segment or every row has its gate
+  // (forward and backward of 65536 rows, by warps and by CTAs: 256 bf16 wide 69 and 184 us, 512 wide 137 and 207).
   const bool by_warps = streamed && rows16 && pieces <= 64;
   int per = rows16 ? 2 : kSingles, row_threads = 256, want = 2 * sms;
   if (by_warps) {
@@ -1101,15 +1098,7 @@ cudaError_t launch_backward(const pm_block_norm* j, const pm_block_norm_grads* d
     want = 2 * sms;
   } else if (streamed) {
     row_threads = threads_for(a.slice, per);
-    int held = share_of_sm(row_threads, 512);
-    // one piece a thread where its 640 threads (of 96 registers) are more than an SM holds with two
-    const int ones = threads_for(a.slice, 1);
-    if (rows16 && ranks == 1 && ones <= 640 && ones > held * row_threads) {
-      per = 1;
-      row_threads = ones;
-      held = 1;
-    }
-    want = sms * held / ranks;
+    want = sms * share_of_sm(row_threads, 512) / ranks;
   }
   if (want > kMaxParts) want = kMaxParts;
   if (want < 1) want = 1;

@@ -2,14 +2,15 @@
 // (and a zero point) per group:
 //   y[m, n] = sum_g s[n, g] sum_{k in g} x[m, k] (q[n, k] - z[n, g]).
 //
-// The weights are read once and bound it.
+// The weights are read once; for one token their bytes bound it, beside a few
+// tokens the instructions that unpack and scale them.
 //  * A warp owns 32 rows of weights and 256 (128) values of k at a time, a
-//    tile of 4 KB.  8 such warps stand side by side along n or along k, so a
-//    stage is 32 KB whatever the matrix's shape: with three stages and two
-//    CTAs an SM enough bytes are in flight.  A ninth warp fills the stages by
-//    tensor copies, the tokens' values beside the weights (rows that start at
-//    any byte: four warps that shift words into place), so the others do
-//    nothing but unpack and multiply: issue slots, not bytes, are short.
+//    tile of 4 (2) KB.  8 such warps stand side by side along n or along k, so
+//    a stage is 32 (16) KB whatever the matrix's shape, and with two CTAs an
+//    SM enough bytes are in flight.  A ninth warp fills the stages by tensor
+//    copies, a box to a lane, the tokens' values, scales and zero points
+//    beside the weights (rows that start at any byte: four warps that shift
+//    words into place), so the others do nothing but unpack and multiply.
 //  * Each token pair serves two tiles of 16 rows in registers.
 //  * A nibble is masked into a 16-bit float's mantissa, exactly.  The matrix
 //    instruction multiplies 16 rows by 8 tokens with exact products and 32-bit
@@ -21,8 +22,15 @@
 //  * 8 tokens (16 in two halves) are the instruction's columns: mma.sync, as
 //    tcgen05's tiles begin at 128 x 8 with both operands in shared memory,
 //    and the unpacked weights come from registers.
-//  * Few rows: the CTAs of a cluster share k and add their sums through
-//    distributed shared memory, in rank order, so results do not vary.
+//  * Few stages: the CTAs of a cluster share k and add their sums through
+//    distributed shared memory, in rank order.  Many: the line of all row
+//    blocks' stages is cut into equal runs, and a second kernel adds the
+//    pieces of the cut blocks in order.  So results do not vary.
+// Measured (a copy runs at 6.55 TB/s): one token x 28672 x 8192 in groups of
+// 128 32.2 us = 3.8 TB/s, 8 tokens 34 us; 16 tokens x 8192 x 28672 in groups
+// of 32 with zero points 51.8 us = 2.7 TB/s; 1024 x 1024 for one token 4.2 us.
+// The copies alone take 27 us of the first; for 16 tokens the issue slots are
+// 60 % busy on the half of the pipes that unpacking needs, with 16 warps an SM.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -578,6 +586,13 @@ struct Plan {
   bool cut;                              // runs end within row blocks: scratch and the second kernel
 };
 
+// Rules, each with what it gained (us): from kLine stages a CTA on, equal runs
+// (one token x 28672 x 8192, 12 stages: 33.2, with row blocks as they come
+// 37.4; below it the second kernel costs more: 16 tokens x 14336 x 4096 28.8
+// by runs, 17.5 by clusters); row blocks of twice the rows where there are more
+// than CTAs at once but less than two rounds (one token x 14336 x 4096 14.0,
+// 11.4), of half where clusters of 8 leave half of the SMs idle (8 tokens x
+// 4096 x 14336 19.6, 13.9).
 template <int NT>
 Plan plan_for(int tokens, int n, int k, int sms) {
   constexpr int kK = Tile<NT>::kK;
@@ -701,12 +716,17 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
 
 template <class T, int NT, int GB, bool Boxes>
 cudaError_t launch_scales(const W4Args& a, const Plan& p, cudaStream_t s) {
-  // copies bring rows of 16 bytes or more from 16-byte boundaries, in the tokens' type, of groups that a tile divides or is divided by
-  const bool side = Boxes && !a.scales32 && (a.group & (a.group - 1)) == 0 && aligned(a.scales, 16) && a.groups % 8 == 0 &&
+  constexpr int kGroups = Tile<NT>::kK / 32 / GB;
+  // copies bring rows of 16 bytes or more from 16-byte boundaries, in the tokens' type; a tile's scales are read as one
+  // word, so they are its kGroups, or the one of a group of several tiles
+  const bool whole = kGroups == 1 ? a.group % (32 * GB) == 0 && (a.group & (a.group - 1)) == 0 : a.group == 32 * GB;
+  const bool side = Boxes && whole && !a.scales32 && aligned(a.scales, 16) && a.groups % 8 == 0 &&
                     (!a.zeros || (aligned(a.zeros, 16) && a.groups % 16 == 0));
   return side ? launch_shape<T, NT, GB, Boxes, Boxes>(a, p, s) : launch_shape<T, NT, GB, Boxes, false>(a, p, s);
 }
 
+// A kernel for each number of groups in a tile.  Scales by copies and by loads of each lane (us): one token x 28672 x
+// 8192 in groups of 128 32.1 and 35.9, 16 tokens in groups of 64 47.6 and 74.3, of 32 (8192 x 28672) 52.2 and 133.
 template <class T, int NT, bool Boxes>
 cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
   if (a.group == 64) return launch_scales<T, NT, 2, Boxes>(a, p, s);
@@ -715,6 +735,7 @@ cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
   return launch_scales<T, NT, 1, Boxes>(a, p, s);
 }
 
+// Copies of boxes need 16-byte rows; by words one token x 28672 x 8192 takes 99 us instead of 32, 16 tokens 178 for 45.
 template <class T>
 cudaError_t launch(const W4Args& a, const Plan& p, cudaStream_t s) {
   const bool aligned_rows = aligned(a.weight, 16) && a.weight_stride % 16 == 0 && aligned(a.x, 16) && (a.x_stride % 8 == 0 || a.tokens == 1);

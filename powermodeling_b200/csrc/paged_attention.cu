@@ -26,6 +26,13 @@
 //  * A weight p enters the product as two 16-bit halves, p = hi + lo, which
 //    keeps 2^-16 of it (16 bits alone would round the output twice); sums
 //    and the running output are 32-bit.
+// Measured (a copy runs at 6.55 TB/s): one sequence of 131072 positions, 8 key
+// heads of 128, 104 us = 5.2 TB/s; 64 ragged sequences up to 8192, 183 us =
+// 5.4 TB/s; 256 of 1024, 194 us = 5.6 TB/s; one of 77 positions 7.2 us, of
+// which a copy's round trip, the reduction over the warps and the launch are
+// nearly all.  At full length the copies' latency with three CTAs an SM bounds
+// it (4.3 of 10 cycles between instructions wait for them), at a few tiles a
+// sequence the start of each segment, about 2 us.
 #include <climits>
 #include <cmath>
 
@@ -572,7 +579,9 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
 
 // ---------------------------------------------------------------- launch
 // Query heads in groups of 8, two groups at once where more than 8 share a
-// key head and their registers allow it (head_dim up to 128).
+// key head and their registers allow it (head_dim up to 128): 32 sequences up
+// to 8192 with 16 query heads a key head of 128 71 us, group after group 87;
+// 12 heads of 64 44 and 49 us.
 int tiles_of_heads(int share, int head_dim) { return share > 8 && head_dim <= 128 ? 2 : 1; }
 
 template <class T, int DP, int NT>
@@ -630,6 +639,8 @@ cudaError_t launch(const pm_paged_attention& j, void* scratch, int sms, cudaStre
   a.page_shift = j.page_size & (j.page_size - 1) ? -1 : 31 - __builtin_clz(unsigned(j.page_size));
   uint8_t* f = static_cast<uint8_t*>(scratch);
   const int nt = tiles_of_heads(a.share, j.head_dim);
+  // a head's own size in shared memory and registers, where it is usual: 32 sequences up to 8192, heads of 80 86 us (by
+  // the kernel for 128 101), of 96 89 (101), of 192 81 (by the kernel for 256 180)
   if (j.head_dim > 64 && j.head_dim <= 80) return nt == 2 ? launch_shape<T, 80, 2>(a, f, sms, s) : launch_shape<T, 80, 1>(a, f, sms, s);
   if (j.head_dim > 80 && j.head_dim <= 96) return nt == 2 ? launch_shape<T, 96, 2>(a, f, sms, s) : launch_shape<T, 96, 1>(a, f, sms, s);
   if (j.head_dim <= 64) return nt == 2 ? launch_shape<T, 64, 2>(a, f, sms, s) : launch_shape<T, 64, 1>(a, f, sms, s);
