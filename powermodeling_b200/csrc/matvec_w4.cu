@@ -48,6 +48,7 @@ namespace {
 constexpr int kWarps = 8, kRows = 32;                    // warps that multiply; rows of a warp's tile
 constexpr int kMaxRanks = 8;                             // CTAs of a cluster
 constexpr int kLine = 8;                                 // stages of a CTA from which on runs are equal
+constexpr int kLinePasses = 8;                           // passes over the tokens up to which they are: scratch is 5 MB a pass
 constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait; a result that it poisons is NaN
 
 // Rows lie in shared memory 256 k (128 bytes) wide, as a copy brings them: 64
@@ -611,7 +612,8 @@ Plan plan_for(int tokens, int n, int k, int sms) {
     p.stages = (k + kWarps / warps_n * kK - 1) / (kWarps / warps_n * kK);
   };
   share(p.warps_n);
-  if (blocks * p.stages >= kLine * slots) {
+  const int64_t passes = (tokens + 8 * NT - 1) / (8 * NT);
+  if (blocks * p.stages >= kLine * slots && passes <= kLinePasses) {
     // enough for every CTA to have kLine stages or more: equal runs
     p.ctas = slots;
     p.cut = blocks * p.stages % slots != 0 || blocks * p.stages / slots % p.stages != 0;

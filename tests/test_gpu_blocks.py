@@ -327,6 +327,14 @@ def test_w4_line_cut_into_runs(gen, tokens, n, k, group, dtype):
     w4_check(dict(t, weight=held[:, 1:-2]), group)
 
 
+@pytest.mark.parametrize("tokens", [128, 129, 300])
+def test_w4_many_passes_over_the_tokens(gen, tokens):
+    """Runs are cut for so many tokens only; beyond, each pass takes whole row blocks and needs no scratch."""
+    w4_check(w4_inputs(gen, tokens, 8200, 16384, BF, 128, zeros=True), 128)
+    need = R.library().pm_matvec_w4_scratch_bytes(tokens, 8200, 16384)
+    assert (need > 0) == (tokens <= 128) and need < 64 << 20
+
+
 def test_w4_scales_that_start_anywhere(gen):
     """Scales and zero points from addresses that no copy can start at."""
     t = w4_inputs(gen, 2, 64, 1024, BF, 64, True)
@@ -629,3 +637,40 @@ def test_graphs_streams_and_repeats(gen):
     for s, o in got:
         for a, b in zip(o, want[0 if s is states[0] else 1]):
             assert torch.equal(a, b)
+
+
+def test_two_graphs_with_second_kernels(gen):
+    """Two graphs whose calls all leave pieces to a second kernel, replayed on two streams at once."""
+    def state(lens, rows):
+        t = norm_inputs(gen, rows, 1024, BF)
+        stats = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"], return_stats=True)[2]
+        kc, vc, table, lengths = cache(gen, lens, 2, 64, 16, BF, fill=0.0)
+        return dict(t=t, stats=stats, g=randn(gen, rows, 1024, dtype=BF), w=w4_inputs(gen, 16, 9000, 8192, BF, 128, True),
+                    q=randn(gen, len(lens), 8, 64, dtype=BF), kc=kc, vc=vc, table=table, lengths=lengths)
+
+    def step(s):
+        t = s["t"]
+        grads = blocks.block_norm_backward(s["g"], s["g"], t["residual"], t["block"], t["pre"], s["stats"], post_weight=t["post"],
+                                           gate=t["gate"])
+        y = blocks.matvec_w4(s["w"]["x"], s["w"]["weight"], s["w"]["scales"], s["w"]["zeros"])
+        return [*grads, y, blocks.paged_attention(s["q"], s["kc"], s["vc"], s["table"], s["lengths"])]
+
+    states = [state([9000, 17, 0, 4000], 300), state([30000], 777)]
+    want = [[x.clone() for x in step(s)] for s in states]
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in states:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(s))
+    for _ in range(30):
+        for x in outs[0] + outs[1]:
+            x.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            for a, b in zip(o, w):
+                assert torch.equal(a, b)
