@@ -178,10 +178,10 @@ __device__ __forceinline__ void factor_piece(const NormArgs<T>& f, int64_t segme
 }
 
 // ---------------------------------------------------------------- forward, a row at a time
-// Rows that 16-byte pieces do not fit: a CTA each, kSingles elements of a
-// thread in registers.  Bound by the latency of a row's loads and its two sums
-// with a few rows to an SM (20000 rows of 1023 bf16: 1.5 TB/s); the parameters
-// come from the L1 each time.
+// Rows that 16-byte pieces do not fit, wider than a thread's registers hold
+// beside the next row's: a CTA each, kSingles elements of a thread.  Bound by
+// the latency of a row's loads and its two sums with two rows to an SM (4000
+// rows of 5001 bf16: 1.1 TB/s); the parameters come from the L1 each time.
 template <class T>
 __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ NormArgs<T> a) {
   __shared__ float red[2][32];
@@ -272,6 +272,78 @@ __device__ __forceinline__ RowSum<Warps, Cluster> row_sum(float (&red)[2][32], f
     }
   }
   return r;
+}
+
+// ---------------------------------------------------------------- forward, rows of single elements
+// Rows that 16-byte pieces do not fit, up to 512 * kSingles wide: a CTA per run
+// of consecutive rows, the parameters in registers, the next row's elements
+// loaded ahead.  Bound by the LSU's instructions, four an element.
+template <class T>
+__global__ void __launch_bounds__(512) norm_singles_kernel(const __grid_constant__ NormArgs<T> a) {
+  constexpr int C = kSingles;
+  __shared__ __align__(16) float red[2][32];
+  __shared__ float shared_sum[2][8];
+  auto total = row_sum<false, false>(red, shared_sum);
+  const float inv = 1.0f / float(a.width);
+  const int64_t from = a.rows * blockIdx.x / gridDim.x, to = a.rows * (blockIdx.x + 1) / gridDim.x;
+  float pre[C], gp[C][1];
+  T next_x[C], next_h[C];                                // beyond the row zeros, which add nothing
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int p = threadIdx.x + c * blockDim.x;
+    pre[c] = p < a.width ? a.pre.at(p) : 0.0f;
+    gp[c][0] = 0.0f;
+    next_x[c] = next_h[c] = from_float<T>(0.0f);
+  }
+  auto fetch = [&](int64_t row) {
+    const T* b = a.block + row * a.block_stride + threadIdx.x;
+    const T* r = a.residual + row * a.residual_stride + threadIdx.x;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (int(threadIdx.x + c * blockDim.x) < a.width) {
+        next_x[c] = __ldcs(b + c * blockDim.x);
+        next_h[c] = __ldcs(r + c * blockDim.x);
+      }
+  };
+  if (from < to) fetch(from);
+  int64_t segment = -1, segment_end = from;
+  for (int64_t row = from; row < to; ++row) {
+    if (row == segment_end) {
+      segment = a.gate_rows ? row / a.rows_per_gate : 0;
+      segment_end = a.gate_rows ? (segment + 1) * a.rows_per_gate : to;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (int(threadIdx.x + c * blockDim.x) < a.width) factor_piece<T, 1>(a, segment, threadIdx.x + c * blockDim.x, gp[c]);
+    }
+    float x[C], h[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) x[c] = to_float(next_x[c]), h[c] = to_float(next_h[c]);
+    if (row + 1 < to) fetch(row + 1);
+    float r1 = 1.0f;
+    if (a.post.p) {
+      float s = 0.0f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) s += x[c] * x[c];
+      r1 = rsqrtf(total(s) * inv + a.eps);
+    }
+    float s = 0.0f;
+    T* hidden = a.hidden + row * a.width + threadIdx.x;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      h[c] += gp[c][0] * (x[c] * r1);
+      s += h[c] * h[c];
+      if (int(threadIdx.x + c * blockDim.x) < a.width) __stcs(hidden + c * blockDim.x, from_float<T>(h[c]));
+    }
+    const float r2 = rsqrtf(total(s) * inv + a.eps);
+    T* normed = a.normed + row * a.width + threadIdx.x;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (int(threadIdx.x + c * blockDim.x) < a.width) __stcs(normed + c * blockDim.x, from_float<T>(h[c] * (r2 * pre[c])));
+    if (a.stats && threadIdx.x == 0) {
+      a.stats[2 * row] = r1;
+      a.stats[2 * row + 1] = r2;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- forward, rows streamed
@@ -1034,7 +1106,14 @@ cudaError_t launch_forward(const pm_block_norm* j, int sms, cudaStream_t s) {
   const int pieces = a.width / kWide<T>;
   if (wide(a, true) && fits && pieces <= 8192 && aligned(a.stats, 8))
     return each_row ? launch_norm_streams<T, true>(a, pieces, sms, s) : launch_norm_streams<T, false>(a, pieces, sms, s);
-  // 20000 rows of 1023 bf16: 89 us, by the loops 162 (backward included 214 and 884)
+  // 20000 rows of 1023 bf16: 60 us, with a CTA for each row 89
+  if (fits && a.width <= 512 * kSingles) {
+    const int threads = threads_for(a.width, kSingles);
+    const int64_t most = int64_t(sms) * std::min(512 / threads, 16);
+    norm_singles_kernel<T><<<unsigned(a.rows < most ? a.rows : most), threads, 0, s>>>(a);
+    return cudaGetLastError();
+  }
+  // a row in registers of 1024 threads; 20000 rows of 1023 so took 89 us and by the loops 162
   if (fits && a.width <= 1024 * kSingles) {
     norm_row_kernel<T><<<unsigned(a.rows), threads_for(a.width, kSingles), 0, s>>>(a);
     return cudaGetLastError();
