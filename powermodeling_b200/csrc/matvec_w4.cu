@@ -9,8 +9,9 @@
 //    a stage is 32 (16) KB whatever the matrix's shape, and with two CTAs an
 //    SM enough bytes are in flight.  A ninth warp fills the stages by tensor
 //    copies, a box to a lane, the tokens' values, scales and zero points
-//    beside the weights (rows that start at any byte: four warps that shift
-//    words into place), so the others do nothing but unpack and multiply.
+//    beside the weights, so the others do nothing but unpack and multiply.
+//    Rows that start at any byte: two warps copy the 16-byte pieces that hold
+//    them, and the readers shift two words into one.
 //  * Each token pair serves two tiles of 16 rows in registers.
 //  * A nibble is masked into a 16-bit float's mantissa, exactly.  The matrix
 //    instruction multiplies 16 rows by 8 tokens with exact products and 32-bit
@@ -62,6 +63,8 @@ struct Tile {
   static constexpr int kK = NT == 1 ? 256 : 128, kShare = kBoxK / kK, kStages = NT == 1 ? 3 : 4;   // kShare: warps of a row
   static constexpr int kStageBytes = kWarps * kRows * kK / 2;
 };
+// Rows that start at any byte: the 16-byte pieces that hold them, as they lie in memory, nine for eight.
+constexpr int kLoosePitch = kPitch + 16, kLoosePieces = kPieces + 1;
 // Pieces lie in an order of the row's own, so that 8 rows x 4 words meet all 32 banks.
 __device__ __forceinline__ int turn(int row) { return row & 7; }
 
@@ -71,10 +74,10 @@ struct Stage {
   int x, scales, zeros, bytes;
 };
 template <int NT>
-__host__ __device__ inline Stage stage_of(int tokens, int warps_n, int scale_box, int zero_box) {
+__host__ __device__ inline Stage stage_of(int pitch, int tokens, int warps_n, int scale_box, int zero_box) {
   const int boxes = kWarps / warps_n / Tile<NT>::kShare, rows = kRows * warps_n;
   Stage s;
-  s.x = Tile<NT>::kStageBytes;
+  s.x = Tile<NT>::kStageBytes / kPitch * pitch;
   s.scales = s.x + boxes * tokens * kBoxK * 2;
   s.zeros = s.scales + rows * scale_box;
   s.bytes = (s.zeros + rows * zero_box + 1023) / 1024 * 1024;
@@ -90,6 +93,7 @@ struct W4Args {
   const uint8_t* zeros;
   void* y;
   int warps_n;                                           // warps along n; the others along k
+  int x_pieces;                                          // tokens start on 16-byte boundaries
   int scale_box, zero_box;                               // bytes of a row's scales and zero points in a stage, 0: not copied
   int group_shift;                                       // log2 of the 32-k blocks of a group, -1: no power of two
   int places;                                            // stages in shared memory
@@ -246,12 +250,13 @@ __device__ __forceinline__ int64_t run_start(const W4Args& a, int run) { return 
 
 // GB: blocks of 32 k per scale within a tile (1 to all of them); 1 also serves
 // the group sizes that the tile's k is no multiple of, or no divisor.
-// Boxes: rows of weights and tokens start on 16-byte boundaries, and one lane
-// of one warp copies boxes; else four warps copy words.
+// Boxes: rows of weights and tokens start on 16-byte boundaries, and a lane
+// copies a box; else the lanes copy 16-byte pieces of the weights as they lie,
+// which the readers shift into place, and the tokens' values by words.
 // Side: scales and zero points come with the stage too.
-constexpr int kBoxThreads = 32, kWordThreads = 128;
+constexpr int kCopyThreads = 32, kLooseThreads = 64;       // copying boxes, pieces
 template <class T, int NT, int GB, bool Boxes, bool Side>
-__global__ void __launch_bounds__(32 * kWarps + (Boxes ? kBoxThreads : kWordThreads), Boxes ? 2 : 1)
+__global__ void __launch_bounds__(32 * kWarps + (Boxes ? kCopyThreads : kLooseThreads), 2)
 w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
           const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_z) {
   extern __shared__ uint8_t smem_raw[];
@@ -263,7 +268,8 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
   const int stage_k = warps_k * L::kK, boxes = warps_k / L::kShare, rows = a.warps_n * kRows;
   const int m0 = blockIdx.z * kCols, held = min(a.tokens, kCols), tokens = min(a.tokens - m0, kCols);
-  const Stage at = stage_of<NT>(held, a.warps_n, a.scale_box, a.zero_box);
+  constexpr int kRowBytes = Boxes ? kPitch : kLoosePitch, kCopies = Boxes ? kCopyThreads : kLooseThreads;
+  const Stage at = stage_of<NT>(kRowBytes, held, a.warps_n, a.scale_box, a.zero_box);
   // The work is a line of stages, row block after row block.  A cluster's CTAs
   // each take a share of one block's; without clusters the line is cut into
   // equal runs.
@@ -282,7 +288,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), read = full + 8 * kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.places; ++i) {
-      barrier_init(full + 8 * i, Boxes ? 1 : kWordThreads);
+      barrier_init(full + 8 * i, Boxes ? 1 : 2 * kCopies);
       barrier_init(read + 8 * i, kWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -320,27 +326,38 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
         }
       } else {
         if (!ok) break;
-        constexpr int kOwn = L::kStageBytes / 16 / kWordThreads;               // pieces of a thread
-#pragma unroll 16
-        for (int c = 0; c < kOwn; ++c) {
-          const int p = c * kWordThreads + me, tile = p / (kRows * kPieces), row = p / kPieces % kRows, piece = p % kPieces;
-          const int n = block * rows + tile % a.warps_n * kRows + row, k = k0 + tile / a.warps_n * kBoxK + piece * 32;
-          const int bytes = n < a.n ? min(max((a.k - k + 1) >> 1, 0), 16) : 0;
-          const uint8_t* src = a.weight + (bytes ? int64_t(n) * a.weight_stride + (k >> 1) : 0);
-          sts128(stage + (tile * kRows + row) * kPitch + ((piece ^ turn(row)) * 16), load_any(src, bytes));
+        // Seven rows at a time, a lane for each piece.  What lies beyond the matrix is left as it is: its tokens' values
+        // are zero, or nothing reads its sums.
+        constexpr int kAtOnce = kCopies / kLoosePieces;
+        const int sub = me / kLoosePieces, piece = me - sub * kLoosePieces, lines = min(rows, a.n - block * rows);
+        for (int w = 0; w < boxes && sub < kAtOnce; ++w) {
+          const int64_t at_byte = (k0 >> 1) + w * kPitch, left = ((int64_t(a.k) + 1) >> 1) - at_byte;
+          const uint8_t* from = a.weight + int64_t(block * rows + sub) * a.weight_stride + at_byte;
+          uint32_t dst = stage + (w * rows + sub) * kLoosePitch + piece * 16;
+#pragma unroll 4
+          for (int line = sub; line < lines; line += kAtOnce) {
+            const int o = 16 * piece - int(reinterpret_cast<uintptr_t>(from) & 15);   // from the row's first byte here
+            if (o < kPitch && o < left) copy16(dst, from + o, int(left - o < 16 ? left - o : 16));
+            from += kAtOnce * a.weight_stride;
+            dst += kAtOnce * kLoosePitch;
+          }
         }
-        for (int p = me; p < boxes * tokens * (kBoxK / 8); p += kWordThreads) {
+        // the tokens' values, zeros beyond k; by words where they lie anywhere
+        for (int p = me; p < boxes * tokens * (kBoxK / 8); p += kCopies) {
           const int piece = p % (kBoxK / 8), m = p / (kBoxK / 8) % tokens, w = p / (kBoxK / 8) / tokens;
           const int k = k0 + w * kBoxK + piece * 8, left = min(max(a.k - k, 0), 8);
           const T* src = static_cast<const T*>(a.x) + (left ? int64_t(m0 + m) * a.x_stride + k : 0);
-          sts128(stage + at.x + ((w * held + m) * (kBoxK / 8) + piece) * 16,
-                 keep(load_any(reinterpret_cast<const uint8_t*>(src), 2 * left), left));
+          const uint32_t to = stage + at.x + ((w * held + m) * (kBoxK / 8) + piece) * 16;
+          if (a.x_pieces) copy16(to, src, 2 * left);
+          else sts128(to, keep(load_any(reinterpret_cast<const uint8_t*>(src), 2 * left), left));
         }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
         barrier_arrive(bar);
       }
       if (++s == a.stages) s = 0, ++block;
       if (++place == a.places) place = 0, parity ^= 1;
     }
+    if (!Boxes) asm volatile("cp.async.wait_all;" ::: "memory");
     if (Boxes && !ok)                                    // copies under way land before the CTA goes
       for (int i = 0; i < a.places; ++i) barrier_wait(full + 8 * i, 0), barrier_wait(full + 8 * i, 1);
     if (a.ranks > 1) {
@@ -376,7 +393,8 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   // this lane's words of its tile (rows g + 8 r), and its tokens' values; columns beyond the tokens repeat the last one:
   // nothing reads their sums
   const int box = wk / L::kShare, half = wk % L::kShare;
-  const int w_lane = (box * rows + wn * kRows + g) * kPitch + ((half * (L::kK / 32)) ^ turn(g)) * 16 + t * 4;
+  const int w_lane = Boxes ? (box * rows + wn * kRows + g) * kPitch + ((half * (L::kK / 32)) ^ turn(g)) * 16 + t * 4
+                           : (box * rows + wn * kRows + g) * kLoosePitch + half * (L::kK / 2) + t * 4;
   int x_lane[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) x_lane[n] = at.x + (box * held + min(n * 8 + g, tokens - 1)) * (kBoxK * 2) + half * (L::kK * 2) + t * 16;
@@ -409,6 +427,15 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
       }
     }
     const int w_at = stage + w_lane;
+    int skew[4];                                         // bytes of a row's start beyond a boundary; the same all along it
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      skew[r] = Boxes ? 0 : int(uint32_t(reinterpret_cast<uintptr_t>(a.weight)) + uint32_t(min(block * rows + wn * kRows + g + 8 * r, a.n - 1)) * uint32_t(a.weight_stride)) & 15;
+    auto word_at = [&](int b, int r) {
+      if constexpr (Boxes) return *reinterpret_cast<const uint32_t*>(smem + (w_at ^ (b * 16)) + 8 * r * kPitch);
+      const uint32_t* at = reinterpret_cast<const uint32_t*>(smem + w_at + 8 * r * kLoosePitch + b * 16 + (skew[r] & 12));
+      return __funnelshift_r(at[0], at[1], 8 * (skew[r] & 3));
+    };
 #pragma unroll
     for (int e = 0; e < kGroups; ++e) {
       float part[2][NT][4];
@@ -435,9 +462,8 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           uint32_t p0[4], p1[4];
-          const uint8_t* word = smem + (w_at ^ (b * 16)) + 16 * r * kPitch;
-          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(word), z[2 * r], p0);
-          Nibbles<T>::unpack(*reinterpret_cast<const uint32_t*>(word + 8 * kPitch), z[2 * r + 1], p1);
+          Nibbles<T>::unpack(word_at(b, 2 * r), z[2 * r], p0);
+          Nibbles<T>::unpack(word_at(b, 2 * r + 1), z[2 * r + 1], p1);
           const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -685,7 +711,7 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
                               a.zero_box, kRows * p.warps_n)))
       return cudaErrorInvalidValue;
   }
-  const int stage = stage_of<NT>(held, p.warps_n, a.scale_box, a.zero_box).bytes;
+  const int stage = stage_of<NT>(Boxes ? kPitch : kLoosePitch, held, p.warps_n, a.scale_box, a.zero_box).bytes;
   a.places = std::min(L::kStages, kRoom / stage);
   const size_t bytes = size_t(a.places) * stage + 1024;
   const auto kernel = w4_kernel<T, NT, GB, Boxes, Side>;
@@ -693,7 +719,7 @@ cudaError_t launch_shape(W4Args a, const Plan& p, cudaStream_t s) {
   ensure_dynamic_smem(kernel, 1024, bytes, limits);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(p.ctas), 1, (a.tokens + 8 * NT - 1) / (8 * NT));
-  cfg.blockDim = dim3(32 * kWarps + (Boxes ? kBoxThreads : kWordThreads));
+  cfg.blockDim = dim3(32 * kWarps + (Boxes ? kCopyThreads : kLooseThreads));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -737,10 +763,11 @@ cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
   return launch_scales<T, NT, 1, Boxes>(a, p, s);
 }
 
-// Copies of boxes need 16-byte rows; by words one token x 28672 x 8192 takes 99 us instead of 32, 16 tokens 178 for 45.
+// Copies of boxes need 16-byte rows; by pieces one token x 28672 x 8190 takes 62 us (8192 in boxes 32), 16 tokens 131 (45),
+// 8 tokens x 4096 x 11006 24 (by four warps that shifted words into place 101, 174 and 48).  What the copying warps have to do for each piece, and two stages at a time, bound it.
 template <class T>
 cudaError_t launch(const W4Args& a, const Plan& p, cudaStream_t s) {
-  const bool aligned_rows = aligned(a.weight, 16) && a.weight_stride % 16 == 0 && aligned(a.x, 16) && (a.x_stride % 8 == 0 || a.tokens == 1);
+  const bool aligned_rows = aligned(a.weight, 16) && a.weight_stride % 16 == 0 && a.x_pieces;
   if (a.tokens <= 8) return aligned_rows ? launch_group<T, 1, true>(a, p, s) : launch_group<T, 1, false>(a, p, s);
   return aligned_rows ? launch_group<T, 2, true>(a, p, s) : launch_group<T, 2, false>(a, p, s);
 }
@@ -783,7 +810,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t 
   if (need && (!scratch || !aligned(scratch, 256) || scratch_bytes < need))
     return fail(PM_E_INVALID, "%s: needs %zu bytes of scratch, 256-byte aligned", who, need);
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->x, 16) && (j->x_stride % 8 == 0 || j->tokens == 1), 0, 0, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, plan, s) : launch<fp16>(a, plan, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");
