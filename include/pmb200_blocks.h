@@ -94,7 +94,9 @@ int pm_block_norm_backward_device(const pm_block_norm* forward, const pm_block_n
  * PM_DT_F16; scales are of that type or PM_DT_F32, [n, ceil(k / group)]
  * contiguous, as are zeros.  group is a multiple of 32; the last may be
  * partial.  y is contiguous [tokens, n].  tokens 0 is allowed and does
- * nothing; the weights are read once for every 16 tokens.
+ * nothing; the weights are read once for every 16 tokens.  A wait for a copy
+ * that does not end within 2 s (a GPU that answers no more) gives up, and what
+ * depends on it is NaN.
  */
 typedef struct {
   int32_t tokens, n, k, group;
