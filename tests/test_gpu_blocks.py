@@ -8,6 +8,9 @@ tree), a norm's square root halves its sum's, and each product adds one.
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -356,6 +359,21 @@ def test_w4_strides_and_alignment(gen):
         w4_check(t, 64)
 
 
+@pytest.mark.parametrize("tokens", [1, 6, 16])
+@pytest.mark.parametrize("k", [500, 1001, 4090, 9001])
+def test_w4_aligned_tokens_beside_loose_weights(gen, k, tokens):
+    """Tokens from 16-byte boundaries with values that are not numbers behind them; weights from every byte."""
+    t = w4_inputs(gen, tokens, 200, k, FP, 64, True)
+    xs = torch.full((tokens, (k + 15) // 8 * 8), float("nan"), device="cuda", dtype=FP)
+    xs[:, :k] = t["x"]
+    t["x"] = xs[:, :k]
+    held = torch.full((200 * ((k + 1) // 2 + 1) + 16,), 255, device="cuda", dtype=torch.uint8)
+    for shift in (0, 1, 2, 7, 15):
+        weight = held[shift:shift + 200 * ((k + 1) // 2 + 1)].view(200, -1)[:, :-1]
+        weight.copy_(t["weight"])
+        w4_check(dict(t, weight=weight), 64)
+
+
 def test_w4_values_that_are_not_numbers(gen):
     """A token with an infinity or a NaN spoils its own row of the result and no other."""
     t = w4_inputs(gen, 4, 64, 300, BF, 32, False)
@@ -674,3 +692,32 @@ def test_two_graphs_with_second_kernels(gen):
         for o, w in zip(outs, want):
             for a, b in zip(o, w):
                 assert torch.equal(a, b)
+
+
+def test_first_call_of_a_process_inside_a_capture(gpu_ready):
+    """Kernels are loaded, their shared memory set and the devices asked on a first call, which may be a captured one."""
+    script = """
+import torch
+from powermodeling_b200 import blocks
+gen = torch.Generator(device="cuda").manual_seed(1)
+def normal(*shape): return torch.randn(*shape, generator=gen, device="cuda").bfloat16()
+r, b, w = normal(64, 2048), normal(64, 2048), normal(2048)
+x, q, s = normal(2, 2048), torch.randint(0, 256, (30000, 1024), generator=gen, device="cuda", dtype=torch.uint8), normal(30000, 16)
+heads, kc, vc = normal(2, 8, 64), normal(40, 16, 2, 64), normal(40, 16, 2, 64)
+table = torch.arange(40, device="cuda", dtype=torch.int32).view(2, 20)
+lengths = torch.tensor([320, 100], device="cuda", dtype=torch.int32)
+def step():
+    h, y, stats = blocks.block_norm(r, b, w, return_stats=True)
+    grads = blocks.block_norm_backward(h, y, r, b, w, stats)
+    return [h, y, stats, *(g for g in grads if g is not None), blocks.matvec_w4(x, q, s), blocks.paged_attention(heads, kc, vc, table, lengths)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0 and done.stdout.strip() == "same", done.stdout + done.stderr
