@@ -422,8 +422,13 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
               ldsm_t(va, at + k * 32);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma<T>(o[n][k], va, hi[n][0], hi[n][1]);
-                mma<T>(o[n][k], va, lo[n][0], lo[n][1]);
+                // the slice's own sum, smallest parts first: the instruction cuts its sums off, which over a long
+                // sequence would add up (2^-15 of the output after 600 slices); the running one is rounded
+                float slice[4];
+                mma_first<T>(slice, va, lo[n][0], lo[n][1]);
+                mma<T>(slice, va, hi[n][0], hi[n][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][k][e] += slice[e];
               }
             }
           }

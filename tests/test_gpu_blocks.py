@@ -541,6 +541,38 @@ def test_attention_values_that_are_not_numbers(gen):
     assert out[0, 4:].isnan().all() and out[0, :4].isfinite().all() and out[1].isfinite().all()
 
 
+def pages_of(gen, x, page):
+    """Rows [batch, length, heads, d] in pages that lie in no order, and the table that finds them."""
+    b, n, hk, d = x.shape
+    table = torch.randperm(b * n // page, generator=gen, device="cuda").to(torch.int32).view(b, -1)
+    pool = torch.empty(b * n // page, page, hk, d, device="cuda", dtype=x.dtype)
+    pool[table.view(-1).long()] = x.view(-1, page, hk, d)
+    return pool, table
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_long_sums_are_rounded(gen, dtype):
+    """Sums of values that are all positive, over 590 tiles a CTA.  A rounded running sum is off by up to 2^-24 of itself
+    in each of 590 slices, either way: six standard deviations are 6 sqrt(590 / 3) = 84 steps; 36 more for a weight and
+    its slice.  Sums that are cut off are all off the same way, by 500 steps and more."""
+    b, n, d, page = 128, 131072, 64, 64
+    k = randn(gen, b, n, 1, d, dtype=dtype, scale=0.03)
+    size = torch.rand(b, 1, 1, d, generator=gen, device="cuda") + 1.0      # outputs at every distance from a rounding's border
+    v = ((torch.rand(b, n, 1, d, generator=gen, device="cuda") + 0.5) * size).to(dtype)
+    kc, table = pages_of(torch.Generator("cuda").manual_seed(7), k, page)
+    vc, _ = pages_of(torch.Generator("cuda").manual_seed(7), v, page)
+    q = randn(gen, b, 1, d, dtype=dtype)
+    out = blocks.paged_attention(q, kc, vc, table, torch.full((b,), n, device="cuda", dtype=torch.int32))
+    del kc, vc
+    for i in range(b):
+        s = (k[i, :, 0].double() * q[i].double()).sum(1) * d ** -0.5
+        largest = (k[i, :, 0].double() * q[i].double()).abs().sum(1).amax() * d ** -0.5
+        want = (torch.softmax(s, 0)[:, None] * v[i, :, 0].double()).sum(0, keepdim=True)
+        half_step = R.HALF[dtype] * 2.0 ** torch.floor(torch.log2(want))
+        off = (out[i].double() - want).abs() - half_step
+        assert bool((off <= 120 * 2.0 ** -24 * want * (1 + 2 * largest)).all()), i
+
+
 def test_attention_offsets_beyond_32_bits(gen):
     """A pool whose last pages lie more than 2^32 elements in."""
     page, hk, d = 64, 8, 128
