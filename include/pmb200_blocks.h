@@ -15,8 +15,8 @@
  * no initialisation, and two calls that may overlap need two.  Outputs do not
  * overlap inputs or scratch.  Elements are row-major with a unit inner
  * stride; the other strides are given in elements (weight rows: bytes).
- * Sums, norms and softmax statistics are held in 32 bits and rounded once, to
- * the nearest even, where a 16-bit output is written.
+ * Sums, norms, softmax statistics and weights are held in 32 bits and rounded
+ * once, to the nearest even, where a 16-bit output is written.
  */
 #ifndef PMB200_BLOCKS_H
 #define PMB200_BLOCKS_H
@@ -128,6 +128,7 @@ int pm_matvec_w4_device(const pm_matvec_w4* job, void* scratch, size_t scratch_b
  * token's own key and value are written to position length - 1 of each
  * sequence (where its page is present) and attended to there; two sequences
  * must not share that entry, and no other sequence may attend to it.
+ * A weight in PM_DT_F16 is held to 2^-39 of the sequence's largest at least.
  * dtype: PM_DT_BF16 or PM_DT_F16 for all of q, the caches, new_k, new_v and
  * out.  head_dim: a multiple of 8 up to 256; q, the caches, new_k and new_v are
  * 16-byte aligned and their strides multiples of 8 elements.  page_size: 1..65536.

@@ -23,9 +23,11 @@
 //    memory.  A group of 8 costs no padding, and its keys are read once.
 //    mma.sync serves because 8 columns are all there is: the tensor core is
 //    idle most of the time and tcgen05's 128-row tiles would be mostly empty.
-//  * A weight p enters the product as two 16-bit halves, p = hi + lo, which
-//    keeps 2^-16 of it (16 bits alone would round the output twice); sums
-//    and the running output are 32-bit.
+//  * A weight enters the product as three 16-bit parts that add up to its 32
+//    bits (fp16: to 2^-39 of the largest weight); sums and the running output
+//    are 32-bit.  One sequence of 131072 positions takes 104.7 us so, 103.1
+//    with two parts (2^-17 of a weight) summed in the instruction; its bf16
+//    outputs are off those of a 32-bit softmax by 5e-6 of their norm, so by 6e-5.
 // Measured (a copy runs at 6.55 TB/s): one sequence of 131072 positions, 8 key
 // heads of 128, 104 us = 5.2 TB/s; 64 ragged sequences up to 8192, 183 us =
 // 5.4 TB/s; 256 of 1024, 194 us = 5.6 TB/s; one of 77 positions 7.2 us, of
@@ -76,18 +78,33 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// Two floats as packed 16-bit values and what their rounding left.
-__device__ __forceinline__ void halves(bf16*, float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  const __nv_bfloat162 l = __floats2bfloat162_rn(x - __bfloat162float(h.x), y - __bfloat162float(h.y));
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+// Weights are held times this: fp16 ends at 2^-24, where a weight then is 2^-39 of the largest.
+template <class T> constexpr float lift = std::is_same<T, fp16>::value ? 32768.0f : 1.0f;
+// Two floats as packed 16-bit values that add up to them: each is cut off where 16 bits end, the next holds what is
+// left, the last one rounded.  bf16: 3 x 8 bits, all of a float's; fp16: 3 x 11, as far as they reach.
+constexpr int kParts = 3;
+__device__ __forceinline__ void split(bf16*, float x, float y, uint32_t (&part)[kParts]) {
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    part[i] = __byte_perm(a, b, 0x7632);
+    x -= __uint_as_float(a & 0xffff0000u);
+    y -= __uint_as_float(b & 0xffff0000u);
+  }
 }
-__device__ __forceinline__ void halves(fp16*, float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+__device__ __forceinline__ void split(fp16*, float x, float y, uint32_t (&part)[kParts]) {
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    __half2 h = __floats2half2_rn(x, y);
+    if (i + 1 < kParts) {
+      asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(part[i]) : "f"(y), "f"(x));
+      h = *reinterpret_cast<const __half2*>(&part[i]);
+      x -= __low2float(h);
+      y -= __high2float(h);
+    } else {
+      part[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -160,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   using S = Shape<T, DP, NT>;
   constexpr int kChunks = DP / 8;                        // 16-byte pieces of a row
   constexpr int kCopies = kSlice * kChunks / 32;         // per lane, for K and for V
-  constexpr float kLift = sizeof(T) == 2 && std::is_same<T, fp16>::value ? 8.0f : 0.0f;   // fp16 halves: weights up to 2^8
+  constexpr float kLift = lift<T>;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int64_t prefix[kThreads + 1];
   __shared__ int64_t found_before;
@@ -374,7 +391,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
               for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + odd[n][e]) * scale2;
           }
           const bool live_a = live >> g & 1, live_b = live >> (g + 8) & 1;
-          uint32_t hi[NT][2], lo[NT][2];
+          uint32_t w[NT][2][kParts];                       // weights of rows g and g + 8
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             if (live != 0xffffu) {
@@ -403,16 +420,17 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
               top[n][0] = m0;
               top[n][1] = m1;
             }
-            const float p0 = exp2_fast(s[n][0] - b0 + kLift), p1 = exp2_fast(s[n][1] - b1 + kLift);
-            const float p2 = exp2_fast(s[n][2] - b0 + kLift), p3 = exp2_fast(s[n][3] - b1 + kLift);
+            const float p0 = exp2_fast(s[n][0] - b0) * kLift, p1 = exp2_fast(s[n][1] - b1) * kLift;
+            const float p2 = exp2_fast(s[n][2] - b0) * kLift, p3 = exp2_fast(s[n][3] - b1) * kLift;
             sum[n][0] += p0 + p2;
             sum[n][1] += p1 + p3;
-            halves(static_cast<T*>(nullptr), p0, p1, hi[n][0], lo[n][0]);
-            halves(static_cast<T*>(nullptr), p2, p3, hi[n][1], lo[n][1]);
-            hi[n][0] = transpose8(hi[n][0]);
-            hi[n][1] = transpose8(hi[n][1]);
-            lo[n][0] = transpose8(lo[n][0]);
-            lo[n][1] = transpose8(lo[n][1]);
+            split(static_cast<T*>(nullptr), p0, p1, w[n][0]);
+            split(static_cast<T*>(nullptr), p2, p3, w[n][1]);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+              w[n][0][i] = transpose8(w[n][0][i]);
+              w[n][1][i] = transpose8(w[n][1][i]);
+            }
           }
           {
             const uint32_t at = vbase + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16;
@@ -425,8 +443,9 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
                 // the slice's own sum, smallest parts first: the instruction cuts its sums off, which over a long
                 // sequence would add up (2^-15 of the output after 600 slices); the running one is rounded
                 float slice[4];
-                mma_first<T>(slice, va, lo[n][0], lo[n][1]);
-                mma<T>(slice, va, hi[n][0], hi[n][1]);
+                mma_first<T>(slice, va, w[n][0][kParts - 1], w[n][1][kParts - 1]);
+#pragma unroll
+                for (int i = kParts - 2; i >= 0; --i) mma<T>(slice, va, w[n][0][i], w[n][1][i]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][k][e] += slice[e];
               }
@@ -485,7 +504,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
         total_of[h] = l;
         if (h < nh) {
           if (!whole) a.stat[slot * S::kHeads + h] = make_float2(m, l);
-          else if (j.lse) j.lse[int64_t(b) * j.q_heads + h0 + h] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+          else if (j.lse) j.lse[int64_t(b) * j.q_heads + h0 + h] = l == 0.0f ? -INFINITY : mb * kLn2 + logf(l / kLift);
         }
       }
       __syncthreads();
@@ -519,7 +538,6 @@ constexpr int kJoinThreads = 256;
 template <class T, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kHeads = 8 * NT;
-  constexpr float kLift = std::is_same<T, fp16>::value ? 8.0f : 0.0f;
   __shared__ float factor[kMaxRuns], partial[8];
   __shared__ float4 sums[kJoinThreads];
   const pm_paged_attention& j = a.j;
@@ -579,7 +597,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     out[2] = from_float<T>(l == 0.0f ? 0.0f : v.z / l);
     out[3] = from_float<T>(l == 0.0f ? 0.0f : v.w / l);
   }
-  if (j.lse && t == 0) j.lse[c.z + row] = l == 0.0f ? -INFINITY : (mb - kLift) * kLn2 + logf(l);
+  if (j.lse && t == 0) j.lse[c.z + row] = l == 0.0f ? -INFINITY : mb * kLn2 + logf(l / lift<T>);
 }
 
 // ---------------------------------------------------------------- launch

@@ -551,6 +551,47 @@ def pages_of(gen, x, page):
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_weights_have_32_bits(gen, dtype):
+    """Values that let three weights cancel to 2^-18 of one of them leave an output as small as a weight's error.
+
+    Steps of 2^-24: 4 of the exponential, 6 of three sums in a matrix instruction, which are cut off, 3 of joining four
+    warps, one of the division; the scores are below 0.1, which the magnitude counts.  Weights of 16 + 1 bits are off by
+    64 steps."""
+    b, n, hk, d = 16, 16, 8, 64
+    q, k = torch.zeros(b, hk, d, device="cuda"), torch.zeros(b, n, hk, d, device="cuda")
+    q[:, :, 0], k[:, :, :, 0] = 1.0, torch.rand(b, n, hk, generator=gen, device="cuda") * -0.1
+    q, k = q.to(dtype), k.to(dtype)
+    w = torch.softmax(k[..., :1].double(), 1).expand(-1, -1, -1, d)      # the scale is 1
+    v = torch.zeros(b, n, hk, d, device="cuda", dtype=dtype)
+    at = torch.argsort(torch.rand(b, n, hk, d, generator=gen, device="cuda"), 1)[:, :3]
+    one, two, three = w.gather(1, at).unbind(1)
+    second = (-one / two).to(dtype)
+    third = (-(one + two * second.double()) / three).to(dtype)
+    v.scatter_(1, at, torch.stack((torch.ones_like(second), second, third), 1))
+    (kc, table), (vc, same) = pages_of(torch.Generator("cuda").manual_seed(7), k, 16), pages_of(torch.Generator("cuda").manual_seed(7), v, 16)
+    assert torch.equal(table, same)
+    lengths = torch.full((b,), n, device="cuda", dtype=torch.int32)
+    want = R.attention(q, kc, vc, table, lengths, None, None, 1.0, 0, "NHD")
+    assert float((want[0].abs() / want[1]).median()) < 2.0 ** -15
+    check("out", blocks.paged_attention(q, kc, vc, table, lengths, scale=1.0), want[:2], 14)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_small_weights_keep_their_bits(gen, dtype):
+    """Two positions, the one with the values a weight of 2^-1 to 2^-24 of the other's."""
+    b = 240
+    q, k, v = (torch.zeros(*shape, device="cuda") for shape in ((b, 1, 64), (b, 16, 1, 64), (b, 16, 1, 64)))
+    q[:, :, :8] = 1.0
+    k[:, 0, :, :8] = torch.linspace(0.1, 24.0, b, device="cuda")[:, None, None] * (math.log(2) / 8)
+    v[:, 1] = torch.rand(b, 1, 64, generator=gen, device="cuda") * 10000 + 50000
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    table = torch.arange(b, device="cuda", dtype=torch.int32)[:, None].contiguous()
+    lengths = torch.full((b,), 2, device="cuda", dtype=torch.int32)
+    want = R.attention(q, k, v, table, lengths, None, None, 1.0, 0, "NHD")
+    check("out", blocks.paged_attention(q, k, v, table, lengths, scale=1.0), want[:2], 24)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
 def test_attention_long_sums_are_rounded(gen, dtype):
     """Sums of values that are all positive, over 590 tiles a CTA.  A rounded running sum is off by up to 2^-24 of itself
     in each of 590 slices, either way: six standard deviations are 6 sqrt(590 / 3) = 84 steps; 36 more for a weight and
