@@ -122,7 +122,9 @@ int pm_matvec_w4_device(const pm_matvec_w4* job, void* scratch, size_t scratch_b
  * page table[b, j / page_size].  A page index outside [0, n_pages), or a
  * position beyond the table, is absent: its positions are not live and
  * nothing there is read.  A sequence without a live position gives zeros and
- * a log sum of -infinity.  Entries that are not live may hold anything.
+ * a log sum of -infinity, and so does one whose scores are all -infinity.
+ * Entries that are not live may hold anything; an infinite value of a live one
+ * makes its element of out infinite, NaN where both signs meet.
  * lse (NULL: not wanted) receives log(sum_j exp(scale * q . K)), [batch, q_heads].
  * With new_k and new_v (both or neither, [batch, kv_heads, head_dim]) the
  * token's own key and value are written to position length - 1 of each

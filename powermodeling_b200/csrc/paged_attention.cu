@@ -112,6 +112,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// What exponents are taken from: the largest score, unless it is infinite (then the sum is infinite, or zero).
+__device__ __forceinline__ float base_of(float top) { return fabsf(top) == INFINITY ? 0.0f : top; }
+
 // Positions [from, to) of a sequence and the tiles that they touch.
 struct Span {
   uint32_t from, to, first;              // first: index of the first tile
@@ -155,6 +158,42 @@ __device__ __forceinline__ int64_t scan_line(const pm_paged_attention& j, int wh
   return prefix[Threads];
 }
 
+// Infinite values.  A weight's parts may be zero, and zero times an infinity is not what the weight times it is; so
+// outputs that are not finite are looked into again: an element is NaN where a live position's value is, where there
+// are infinities of both signs, or where a score is -infinity beside an infinite value; else it has the infinity's sign.
+// Positions [from, to) of one key head, nh query heads at q; a thread to a position.  found: [nh][head_dim], 1 for
+// NaN, 2 and 4 for the infinities.
+template <class T>
+__device__ __noinline__ void look_into_values(const pm_paged_attention& j, int b, int kvh, uint32_t from, uint32_t to, uint32_t newest,
+                                              const T* q, int nh, uint32_t* found) {
+  const int D = j.head_dim;
+  for (int i = threadIdx.x; i < nh * D; i += blockDim.x) found[i] = 0;
+  __syncthreads();
+  const int32_t* table = j.table + b * j.table_stride;
+  for (uint32_t pos = from + threadIdx.x; pos < to; pos += blockDim.x) {
+    const int page = table[pos / uint32_t(j.page_size)], entry = int(pos % uint32_t(j.page_size));
+    if (page < 0 || page >= j.n_pages) continue;
+    const bool is_new = pos == newest;
+    const T* v = is_new ? static_cast<const T*>(j.new_v) + b * j.new_v_stride + kvh * j.new_v_head_stride
+                        : static_cast<const T*>(j.v_cache) + page * j.v_page_stride + entry * j.v_token_stride + kvh * j.v_head_stride;
+    const T* k = is_new ? static_cast<const T*>(j.new_k) + b * j.new_k_stride + kvh * j.new_k_head_stride
+                        : static_cast<const T*>(j.k_cache) + page * j.k_page_stride + entry * j.k_token_stride + kvh * j.k_head_stride;
+    bool any = false;
+    for (int d = 0; d < D; ++d) any |= !(fabsf(to_float(v[d])) < INFINITY);
+    if (!any) continue;
+    for (int h = 0; h < nh; ++h) {
+      float score = 0.0f;
+      for (int d = 0; d < D; ++d) score += to_float(k[d]) * to_float(q[h * j.q_head_stride + d]);
+      const bool nothing = score * j.scale == -INFINITY;
+      for (int d = 0; d < D; ++d) {
+        const float x = to_float(v[d]);
+        if (!(fabsf(x) < INFINITY)) atomicOr(&found[h * D + d], x != x || nothing ? 1u : x > 0.0f ? 2u : 4u);
+      }
+    }
+  }
+  __syncthreads();
+}
+
 // ---------------------------------------------------------------- the runs
 // DP: the head size that the kernel is built for, at least head_dim; NT: groups
 // of 8 query heads served at once.  A row of shared memory is 16 bytes longer
@@ -169,7 +208,7 @@ struct Shape {
   static constexpr int kWarpBytes = kStages * kSliceBytes;
   static constexpr int kOutStride = DP + 4;                                     // floats; 8t + g: no two lanes in a bank
   static constexpr size_t kSmem = size_t(kWarps) * kWarpBytes;
-  static_assert(kHeads * kOutStride * 4 <= kWarpBytes, "a warp's output fits in its ring");
+  static_assert(kHeads * kOutStride * 4 <= kWarpBytes, "a warp's output fits in its ring, and so does what look_into_values finds");
 };
 
 template <class T, int DP, int NT>
@@ -408,7 +447,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
             }
             m0 = fmaxf(m0, top[n][0]);
             m1 = fmaxf(m1, top[n][1]);
-            const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+            const float b0 = base_of(m0), b1 = base_of(m1);
             if (__any_sync(0xffffffffu, m0 != top[n][0] || m1 != top[n][1])) {
               const float c0 = exp2_fast(top[n][0] - b0), c1 = exp2_fast(top[n][1] - b1);
               sum[n][0] *= c0;
@@ -494,7 +533,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_stat[w][h].x);
-        const float mb = m == -INFINITY ? 0.0f : m;
+        const float mb = base_of(m);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float f = exp2_fast(warp_stat[w][h].x - mb);
@@ -508,6 +547,11 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
         }
       }
       __syncthreads();
+      auto put = [&](int h, int d, float v, float l) {
+        if (whole) static_cast<T*>(j.out)[(int64_t(b) * j.q_heads + h0 + h) * D + d] = from_float<T>(l == 0.0f ? 0.0f : v / l);
+        else a.part[(slot * S::kHeads + h) * D + d] = v;
+      };
+      bool odd = false;
       for (int h = 0; h < nh; ++h) {
         const float l = total_of[h];
         for (int d = threadIdx.x; d < D; d += kThreads) {
@@ -515,11 +559,24 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
 #pragma unroll
           for (int w = 0; w < kWarps; ++w)
             v += reinterpret_cast<const float*>(ring + w * S::kWarpBytes)[h * S::kOutStride + d] * factor[w][h];
-          if (whole) static_cast<T*>(j.out)[(int64_t(b) * j.q_heads + h0 + h) * D + d] = from_float<T>(l == 0.0f ? 0.0f : v / l);
-          else a.part[(slot * S::kHeads + h) * D + d] = v;
+          put(h, d, v, l);
+          odd |= !(fabsf(v) < INFINITY);
         }
       }
-      __syncthreads();
+      if (__syncthreads_or(odd)) {
+        uint32_t* found = reinterpret_cast<uint32_t*>(ring);
+        look_into_values<T>(j, b, kvh, max(sp.from, (sp.first + t0) * uint32_t(kTile)), min(sp.to, (sp.first + t1) * uint32_t(kTile)), newest,
+                            static_cast<const T*>(j.q) + b * j.q_stride + h0 * j.q_head_stride, nh, found);
+        for (int h = 0; h < nh; ++h) {
+          const float l = total_of[h];
+          if (!(l > 0.0f)) continue;                       // NaN for every element, or nothing but scores of -infinity
+          for (int d = threadIdx.x; d < D; d += kThreads) {
+            const uint32_t f = found[h * D + d];
+            if (f) put(h, d, f == 2 ? INFINITY : f == 4 ? -INFINITY : NAN, l);
+          }
+        }
+        __syncthreads();
+      }
     }
 
     cur += part1 - part0;
@@ -560,7 +617,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = fmaxf(m, partial[w]);
-  const float mb = m == -INFINITY ? 0.0f : m;
+  const float mb = base_of(m);
   __syncthreads();
   float l = 0.0f;
   for (int i = t; i < n; i += kJoinThreads) {
@@ -581,7 +638,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
     for (int i = t / lanes; i < n; i += groups) {
       const float4 p = __ldcg(reinterpret_cast<const float4*>(a.part + (slot_of(i) * kHeads + row) * D) + lane);
       const float f = factor[i];
-      v.x += p.x * f; v.y += p.y * f; v.z += p.z * f; v.w += p.w * f;
+      auto part = [&](float x) { return fabsf(x) == INFINITY ? x : x * f; };               // f may be zero
+      v.x += part(p.x); v.y += part(p.y); v.z += part(p.z); v.w += part(p.w);
     }
   }
   sums[t] = v;

@@ -530,6 +530,67 @@ def test_attention_scores_far_apart(gen):
     attend(gen, lens, 2, 4, 64, 16, FP, q=torch.zeros(2, 8, 64, dtype=FP, device="cuda"))
 
 
+def like_definition(out, want, magnitude, steps):
+    """Infinities and NaN where the 64-bit form has them, the rest within the tolerance."""
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.isposinf(), want.isposinf()) and torch.equal(out.isneginf(), want.isneginf())
+    fine = want.isfinite()
+    check("out", out[fine], (want[fine], magnitude[fine]), steps)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,hk,share,d,page,layout", [([100, 64, 1, 300], 2, 4, 64, 16, "NHD"), ([1000, 7, 2500], 2, 12, 64, 16, "HND"),
+                                                         ([40000], 2, 3, 128, 64, "NHD"), ([3000, 200], 1, 9, 192, 8, "NHD")])
+def test_attention_infinite_values(gen, lens, hk, share, d, page, layout, dtype):
+    """Live infinities of one sign, of both, and NaN, in whole and cut segments, at every weight there is: each spoils its
+    own element of the heads that share it, with its sign."""
+    kc, vc, table, lengths = cache(gen, lens, hk, d, page, dtype, layout)
+    v = vc if layout == "NHD" else vc.transpose(1, 2)
+    inf, nan = float("inf"), float("nan")
+
+    def put(i, pos, head, element, value):
+        v[table[i, pos // page], pos % page, head, element] = value
+    for i, n in enumerate(lens):
+        put(i, 0, 0, 0, inf)
+        put(i, n // 2, 0, 1, -inf)
+        put(i, n // 3, 0, 2, inf)
+        put(i, n - n // 4 - 1, 0, 2, -inf if n > 1 else inf)
+        put(i, n // 5, hk - 1, 3, nan)
+        for pos in range(0, n, 7):
+            put(i, pos, hk - 1, 5, -inf)
+    q = randn(gen, len(lens), hk * share, d, dtype=dtype)
+    nk, nv = randn(gen, len(lens), hk, d, dtype=dtype), randn(gen, len(lens), hk, d, dtype=dtype)
+    nv[:, 0, 7], nv[0, 0, 4] = inf, -inf
+    for window in (0, 50):
+        for far in (1.0, 12.0):                   # weights down to nothing in 32 bits
+            want = R.attention(q * far, kc, vc, table, lengths, nk, nv, d ** -0.5, window, layout)
+            out = blocks.paged_attention(q * far, kc, vc, table, lengths, new_k=nk, new_v=nv, window=window, layout=layout)
+            assert bool(want[0].isinf().any())
+            like_definition(out, want[0], want[1], d / 8 + 600)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens", [[100, 30], [30000, 4000]])
+def test_attention_infinite_keys(gen, lens, dtype):
+    """A score of infinity makes its row NaN, one of -infinity a weight of nothing, which times an infinity is NaN; the
+    other heads know nothing of it.  Only scores of -infinity give zeros."""
+    kc, vc, table, lengths = cache(gen, lens, 3, 64, 16, dtype)
+    q = randn(gen, 2, 6, 64, dtype=dtype)
+    kc[table[0, 1], 3, 0, 5] = float("inf")       # of the scores' own sign in each head
+    q[0, 0, 5], q[0, 1, 5] = 1.0, -1.0
+    kc[table[1, 0], 2, 1, 6] = float("-inf")
+    q[1, 2, 6], q[1, 3, 6] = 2.0, 0.5
+    vc[table[1, 0], 2, 1, 9] = float("inf")
+    want = R.attention(q, kc, vc, table, lengths, None, None, 0.125, 0, "NHD")
+    out, lse = blocks.paged_attention(q, kc, vc, table, lengths, return_lse=True)
+    assert bool(want[0][0, 0].isnan().all() and want[0][0, 1].isfinite().all() and want[0][1, 2:4, 9].isnan().all())
+    like_definition(out, want[0], want[1].nan_to_num(nan=0.0), 700)
+    assert torch.equal(lse.isnan(), want[2].isnan())
+    out, lse = blocks.paged_attention(torch.ones_like(q), torch.full_like(kc, float("-inf")), torch.ones_like(vc), table, lengths,
+                                      return_lse=True)
+    assert not out.any() and bool(lse.isneginf().all())
+
+
 def test_attention_values_that_are_not_numbers(gen):
     """A live NaN spoils the rows that attend to it and no others; entries that are not live may hold anything
     (every other test's caches are NaN there)."""
