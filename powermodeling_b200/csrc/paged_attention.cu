@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
   for (int b = blockIdx.x; b < j.batch; b += gridDim.x) {
     if (span_of(j, b).tiles) continue;
     T* out = static_cast<T*>(j.out) + int64_t(b) * j.q_heads * D;
-    for (int i = threadIdx.x; i < j.q_heads * D; i += kThreads) out[i] = from_float<T>(0.0f);
+    for (int64_t i = threadIdx.x; i < int64_t(j.q_heads) * D; i += kThreads) out[i] = from_float<T>(0.0f);
     if (j.lse)
       for (int i = threadIdx.x; i < j.q_heads; i += kThreads) j.lse[int64_t(b) * j.q_heads + i] = -INFINITY;
   }

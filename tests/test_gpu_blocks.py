@@ -694,6 +694,25 @@ def test_attention_offsets_beyond_32_bits(gen):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_of_the_most_query_heads(gen, d):
+    """2^24 query heads of one key head: an output of 2^31 and 2^32 elements, of a sequence without and with positions."""
+    heads = 1 << 24
+    q = torch.zeros(1, 1, d, dtype=BF, device="cuda").expand(1, heads, d)
+    kc, vc = randn(gen, 1, 16, 1, d, dtype=BF), randn(gen, 1, 16, 1, d, dtype=BF)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    for n in (0, 5):
+        lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+        held = torch.ones(1, heads, d, dtype=BF, device="cuda")          # what the output's memory held before
+        del held
+        out = blocks.paged_attention(q, kc, vc, table, lengths)
+        want = blocks.paged_attention(q[:, :1], kc, vc, table, lengths)
+        assert torch.equal(want.abs().amax() > 0, lengths[0] > 0)
+        assert all(bool((part == want[:, :1]).all()) for part in out.split(1 << 21, 1))
+        del out
+    torch.cuda.empty_cache()
+
+
 # ---------------------------------------------------------------- together, on streams, in graphs
 def test_decode_layer(gen):
     """A decode layer as it is used: norm, the projections, attention over the cache with its append, norm; three
