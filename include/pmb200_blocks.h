@@ -95,8 +95,8 @@ int pm_block_norm_backward_device(const pm_block_norm* forward, const pm_block_n
  * contiguous, as are zeros.  group is a multiple of 32; the last may be
  * partial.  y is contiguous [tokens, n].  tokens 0 is allowed and does
  * nothing; the weights are read once for every 16 tokens.  A wait for a copy
- * that does not end within 2 s (a GPU that answers no more) gives up, and what
- * depends on it is NaN.
+ * that does not end within the limit (2 s) gives up, and what depends on it is
+ * NaN.
  */
 typedef struct {
   int32_t tokens, n, k, group;
@@ -113,6 +113,8 @@ typedef struct {
 /* Scratch for the current device: 0 where the product needs none (scratch may then be NULL). */
 size_t pm_matvec_w4_scratch_bytes(int32_t tokens, int32_t n, int32_t k);
 int pm_matvec_w4_device(const pm_matvec_w4* job, void* scratch, size_t scratch_bytes, void* stream);
+/* Sets the limit of such a wait for the process's calls from now on, 0 the usual one; returns the limit before. */
+uint64_t pm_matvec_w4_wait_limit(uint64_t nanoseconds);
 
 /*
  * Attention of one query token per sequence over a paged cache:

@@ -50,7 +50,8 @@ constexpr int kWarps = 8, kRows = 32;                    // warps that multiply;
 constexpr int kMaxRanks = 8;                             // CTAs of a cluster
 constexpr int kLine = 8;                                 // stages of a CTA from which on runs are equal
 constexpr int kLinePasses = 8;                           // passes over the tokens up to which they are: scratch is 5 MB a pass
-constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait; a result that it poisons is NaN
+constexpr uint64_t kWaitNs = 2ull * 1000000000ull;       // bound on any single wait, unless the caller sets another
+std::atomic<uint64_t> g_wait_ns{kWaitNs};
 
 // Rows lie in shared memory 256 k (128 bytes) wide, as a copy brings them: 64
 // bytes a row and copy took 42 us where 128 took 27 (8192 x 28672).  Up to 8
@@ -92,6 +93,7 @@ struct W4Args {
   const void* scales;
   const uint8_t* zeros;
   void* y;
+  uint64_t wait_ns;                                      // bound on a wait for a stage
   int warps_n;                                           // warps along n; the others along k
   int x_pieces;                                          // tokens start on 16-byte boundaries
   int scale_box, zero_box;                               // bytes of a row's scales and zero points in a stage, 0: not copied
@@ -220,10 +222,15 @@ __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
 __device__ __forceinline__ void barrier_expect(uint32_t bar, int bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+// Looks once.  The waiting form sleeps for up to milliseconds on its own account: limits that short are kept without it.
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity, uint64_t limit) {
   uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  if (limit < 20000000)
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
 __device__ __forceinline__ uint64_t nanoseconds() {
@@ -231,13 +238,26 @@ __device__ __forceinline__ uint64_t nanoseconds() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// False when the wait runs out.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
-  if (barrier_try(bar, parity)) return true;
-  const uint64_t deadline = nanoseconds() + kWaitNs;
-  while (!barrier_try(bar, parity))
-    if (nanoseconds() > deadline) return false;
+// False when the wait runs out, or has run out elsewhere in the CTA: `failed` says so to all of it.  A CTA that was not
+// running in the meantime looks once more before it gives up.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, uint64_t limit, volatile int* failed) {
+  if (barrier_try(bar, parity, limit)) return true;
+  const uint64_t deadline = nanoseconds() + limit;
+  while (!barrier_try(bar, parity, limit)) {
+    if (*failed) return false;
+    if (nanoseconds() > deadline) {
+      if (barrier_try(bar, parity, limit)) return true;
+      *failed = 1;
+      return false;
+    }
+  }
   return true;
+}
+// The same without a way to give up early, for copies that have to have landed.
+__device__ __forceinline__ void barrier_drain(uint32_t bar, uint32_t parity) {
+  if (barrier_try(bar, parity, kWaitNs)) return;
+  const uint64_t deadline = nanoseconds() + kWaitNs;
+  while (!barrier_try(bar, parity, kWaitNs) && nanoseconds() < deadline) {}
 }
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -263,6 +283,9 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   using L = Tile<NT>;
   constexpr int kStages = L::kStages, kGroups = L::kK / 32 / GB, kCols = 8 * NT;
   __shared__ __align__(8) uint64_t bars[2 * kStages];    // a stage is full; it is read
+  // A wait ran out.  Who gave up goes on without waiting: from then on nothing that this CTA sums counts.  Sums are
+  // looked at only after a barrier that those who gave up come to as well.
+  __shared__ int failed;
   uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
@@ -287,6 +310,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   int block = int(first >> 32 ? first / a.stages : int64_t(uint32_t(first) / uint32_t(a.stages))), s = int(first - int64_t(block) * a.stages);
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), read = full + 8 * kStages;
   if (threadIdx.x == 0) {
+    failed = 0;
     for (int i = 0; i < a.places; ++i) {
       barrier_init(full + 8 * i, Boxes ? 1 : 2 * kCopies);
       barrier_init(read + 8 * i, kWarps);
@@ -302,12 +326,14 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     // ------------------------------------------------ the copies
     const int me = threadIdx.x - 32 * kWarps;
     bool ok = true;
-    int place = 0;
+    int place = 0, filled = 0;
     uint32_t parity = 1;
     for (int i = 0; i < count && ok; ++i) {
       const uint32_t stage = ring + place * at.bytes, bar = full + 8 * place;
       const int k0 = s * stage_k;
-      if (i >= a.places) ok = barrier_wait(read + 8 * place, parity);
+      // A place is filled again only if all eight readers waited for what it held: one that gave up said so before it
+      // arrived.  (Copies to a place whose last ones are still under way would arrive twice in one phase of its barrier.)
+      if (i >= a.places) ok = barrier_wait(read + 8 * place, parity, a.wait_ns, &failed) && !*static_cast<volatile int*>(&failed);
       if constexpr (Boxes) {
         // a lane for each box
         ok = __all_sync(0xffffffffu, ok);
@@ -354,12 +380,15 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
         barrier_arrive(bar);
       }
+      ++filled;
       if (++s == a.stages) s = 0, ++block;
       if (++place == a.places) place = 0, parity ^= 1;
     }
+    // copies under way land before the CTA goes, whether its readers waited for them or not
     if (!Boxes) asm volatile("cp.async.wait_all;" ::: "memory");
-    if (Boxes && !ok)                                    // copies under way land before the CTA goes
-      for (int i = 0; i < a.places; ++i) barrier_wait(full + 8 * i, 0), barrier_wait(full + 8 * i, 1);
+    if (Boxes)
+      for (int i = max(filled - a.places, 0); i < filled; ++i) barrier_drain(full + 8 * (i % a.places), i / a.places & 1);
+    __syncwarp();
     if (a.ranks > 1) {
       cg::this_cluster().sync();
       cg::this_cluster().sync();
@@ -386,7 +415,6 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   };
 
   float acc[2][NT][4] = {};
-  bool ok = true;
   int s_first = s, place = 0;
   uint32_t parity = 0;
   float* red = nullptr;                                  // [wk][row][token], in the place of a row block's last stage
@@ -408,7 +436,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     const bool last = s + 1 == a.stages || left == 1;    // of this CTA in this row block
     if (left == 1 && a.ranks == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join's CTAs come and wait
     if (!Side && left > 1) fetch_scales(s + 1 == a.stages ? block + 1 : block, s + 1 == a.stages ? 0 : s + 1);
-    ok = ok && barrier_wait(full + 8 * place, parity);
+    barrier_wait(full + 8 * place, parity, a.wait_ns, &failed);
     const int stage = place * at.bytes;
     if constexpr (Side) {
       const int group = (s * stage_k + wk * L::kK) / 32 >> a.group_shift;
@@ -502,14 +530,15 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float* to = red + ((wk * rows + wn * kRows + 16 * r + g) * kCols + n * 8 + 2 * t);
-          to[0] = ok ? acc[r][n][0] : NAN;
-          to[1] = ok ? acc[r][n][1] : NAN;
-          to[8 * kCols] = ok ? acc[r][n][2] : NAN;
-          to[8 * kCols + 1] = ok ? acc[r][n][3] : NAN;
+          to[0] = acc[r][n][0];
+          to[1] = acc[r][n][1];
+          to[8 * kCols] = acc[r][n][2];
+          to[8 * kCols + 1] = acc[r][n][3];
           acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.0f;
         }
       multipliers_sync();
       if (a.ranks == 1) {
+        const bool lost = *static_cast<volatile int*>(&failed);
         // a whole block to y, a cut one to scratch: at most one that this run ends within and one that it starts within
         const bool whole = s_first == 0 && s == a.stages;
         float* part = a.part + ((int64_t(blockIdx.z) * gridDim.x + blockIdx.x) * 2 + (s_first == 0 ? 1 : 0)) * rows * kCols;
@@ -523,7 +552,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
             const float4 u = *reinterpret_cast<const float4*>(red + (w * rows + row) * kCols + 4 * q);
             v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
           }
-          const float value[4] = {v.x, v.y, v.z, v.w};
+          const float value[4] = {lost ? NAN : v.x, lost ? NAN : v.y, lost ? NAN : v.z, lost ? NAN : v.w};
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             if (4 * q + m >= tokens) continue;
@@ -551,6 +580,8 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
     sums[c] = v;
   }
   cg::this_cluster().sync();
+  bool lost = false;
+  for (int r = 0; r < a.ranks; ++r) lost |= *static_cast<volatile int*>(cg::this_cluster().map_shared_rank(&failed, r)) != 0;
   const int64_t first_row = int64_t(blockIdx.x / a.ranks) * rows;
   T* y = static_cast<T*>(a.y) + int64_t(m0) * a.n + first_row;
   for (int c = rank * 32 * kWarps + threadIdx.x; c < rows * (kCols / 4); c += a.ranks * 32 * kWarps) {
@@ -563,7 +594,7 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
 #pragma unroll
     for (int r = 1; r < kMaxRanks; ++r)
       if (r < a.ranks) v[0].x += v[r].x, v[0].y += v[r].y, v[0].z += v[r].z, v[0].w += v[r].w;
-    const float value[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+    const float value[4] = {lost ? NAN : v[0].x, lost ? NAN : v[0].y, lost ? NAN : v[0].z, lost ? NAN : v[0].w};
 #pragma unroll
     for (int m = 0; m < 4; ++m)
       if (4 * q + m < tokens) y[int64_t(4 * q + m) * a.n + row] = from_float<T>(value[m]);
@@ -785,6 +816,10 @@ extern "C" size_t pm_matvec_w4_scratch_bytes(int32_t tokens, int32_t n, int32_t 
   return plan_scratch(plan_of(tokens, n, k, sms), tokens);
 }
 
+extern "C" uint64_t pm_matvec_w4_wait_limit(uint64_t nanoseconds) {
+  return g_wait_ns.exchange(nanoseconds ? std::min(nanoseconds, uint64_t(1) << 62) : kWaitNs);   // added to a clock
+}
+
 extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t scratch_bytes, void* stream) {
   const char* who = "pm_matvec_w4_device";
   if (!j) return fail(PM_E_INVALID, "%s: NULL job", who);
@@ -810,7 +845,7 @@ extern "C" int pm_matvec_w4_device(const pm_matvec_w4* j, void* scratch, size_t 
   if (need && (!scratch || !aligned(scratch, 256) || scratch_bytes < need))
     return fail(PM_E_INVALID, "%s: needs %zu bytes of scratch, 256-byte aligned", who, need);
   W4Args a{j->tokens, j->n, j->k, j->group, int((int64_t(j->k) + j->group - 1) / j->group), j->scales_dtype == PM_DT_F32,
-           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, 0, aligned(j->x, 16) && (j->x_stride % 8 == 0 || j->tokens == 1), 0, 0, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
+           j->x_stride, j->weight_stride, j->x, j->weight, j->scales, j->zeros, j->y, g_wait_ns.load(std::memory_order_relaxed), 0, aligned(j->x, 16) && (j->x_stride % 8 == 0 || j->tokens == 1), 0, 0, 0, 0, 0, 0, 0, 0, 0, static_cast<float*>(scratch)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = j->dtype == PM_DT_BF16 ? launch<bf16>(a, plan, s) : launch<fp16>(a, plan, s);
   return e == cudaSuccess ? PM_OK : cuda_fail(e, "pm_matvec_w4_device launch");

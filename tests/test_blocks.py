@@ -195,6 +195,14 @@ def test_c_matvec_refusals(kw, code):
     assert "pm_matvec_w4_device" in N.last_error()
 
 
+def test_c_matvec_wait_limit():
+    limit = K.library().pm_matvec_w4_wait_limit
+    limit.argtypes, limit.restype = [C.c_uint64], C.c_uint64
+    usual = limit(5)
+    assert usual == 2 * 10 ** 9 and limit(2 ** 64 - 1) == 5
+    assert 10 ** 18 < limit(0) < 2 ** 63 and limit(0) == usual       # a limit that a clock in 64 bits can be added to
+
+
 def c_attention(**kw):
     a = dict(batch=2, q_heads=4, kv_heads=2, head_dim=64, page_size=16, n_pages=3, table_columns=2, dtype=1, window=0,
              scale=0.125, q_stride=256, q_head_stride=64, k_page_stride=2048, k_token_stride=128, k_head_stride=64,

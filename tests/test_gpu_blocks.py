@@ -384,6 +384,36 @@ def test_w4_values_that_are_not_numbers(gen):
     assert y[2].isnan().all() and not y[1].isfinite().any()
 
 
+@pytest.mark.parametrize("tokens,n,k,group,loose", [(1, 1024, 1024, 64, 0), (8, 4096, 4096, 128, 0), (16, 1000, 8192, 64, 0),
+                                                    (1, 28672, 8192, 128, 0), (16, 9000, 8192, 32, 0), (40, 9000, 8192, 128, 0),
+                                                    (3, 1001, 4090, 128, 1), (9, 20000, 4096, 64, 1), (1, 70000, 256, 64, 0)])
+def test_w4_waits_that_run_out(gen, tokens, n, k, group, loose):
+    """With limits that a copy's latency passes, every output is right or NaN, whoever gave up; the calls after it are
+    as before."""
+    limit = R.library().pm_matvec_w4_wait_limit
+    limit.argtypes, limit.restype = [R.C.c_uint64], R.C.c_uint64
+    t = w4_inputs(gen, tokens, n, k, BF, group, zeros=True)
+    if loose:
+        held = torch.full((n, t["weight"].shape[1] + 3), 255, device="cuda", dtype=torch.uint8)
+        held[:, 1:-2] = t["weight"]
+        t["weight"] = held[:, 1:-2]
+    args = (t["x"], t["weight"], t["scales"], t["zeros"])
+    before = w4_check(t, group)
+    lost = []
+    try:
+        for ns in (1, 200, 400, 500, 600, 700, 800, 900, 1000, 1200, 1500, 2000, 4000):
+            limit(ns)
+            for _ in range(10):
+                y = blocks.matvec_w4(*args, group_size=group)
+                fine = ~y.isnan()
+                assert torch.equal(y[fine], before[fine]), ns
+                lost.append(int(y.numel() - fine.sum()))
+    finally:
+        limit(0)
+    assert lost[0] > 0
+    assert torch.equal(blocks.matvec_w4(*args, group_size=group), before)
+
+
 # ---------------------------------------------------------------- paged attention
 def cache(gen, lens, hk, d, page, dtype, layout="NHD", columns=None, spare=2, fill=float("nan")):
     """Caches whose pages lie in no order; everything that is not live holds `fill`."""
