@@ -35,6 +35,7 @@ class _BlockNormFunction(torch.autograd.Function):
         hidden, normed, stats = _ops.block_norm(residual, block, pre_weight, post_weight, gate, scale, eps, True)
         ctx.save_for_backward(residual, block, pre_weight, post_weight, gate, stats)
         ctx.scale = scale
+        ctx.captured = torch.cuda.is_current_stream_capturing()
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(stats)
         return hidden, normed, stats
@@ -42,9 +43,9 @@ class _BlockNormFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_hidden, grad_normed, _grad_stats):
-        if torch.cuda.is_current_stream_capturing():
-            # an eager graph of the same leaves would pull its own stream into the capture and end it
-            raise RuntimeError("block_norm: capture block_norm_backward itself, not the autograd engine's call of it")
+        if torch.cuda.is_current_stream_capturing() and not getattr(ctx, "captured", False):
+            # the graph of an eager forward brings its own stream into the capture
+            raise RuntimeError("block_norm: the forward pass was not captured: capture both, or capture block_norm_backward itself")
         residual, block, pre_weight, post_weight, gate, stats = ctx.saved_tensors
         if grad_hidden is None and grad_normed is None:
             return (None,) * 7
@@ -68,11 +69,19 @@ def block_norm(residual, block, pre_weight, *, post_weight=None, gate=None, scal
     [s, width] with s dividing rows (gate row i serves the i-th run of rows / s
     rows; s = rows gates every element), each of that type or float32.  With
     ``return_stats`` a third value, [rows, 2] float32, is returned for
-    ``block_norm_backward``.
+    ``block_norm_backward``.  A training step is captured with its forward and
+    backward together, or by ``block_norm_backward``; a leaf that a living graph
+    of the default stream holds is refused there (``RuntimeError``).
     """
     if torch.is_grad_enabled() and (residual.requires_grad or block.requires_grad or pre_weight.requires_grad
                                     or (post_weight is not None and post_weight.requires_grad)
                                     or (gate is not None and gate.requires_grad)):
+        if torch.cuda.is_current_stream_capturing():
+            held = _ops.held_outside_capture(residual, block, pre_weight, post_weight, gate)
+            if held >= 0:
+                name = ("residual", "block", "pre_weight", "post_weight", "gate")[held]
+                raise RuntimeError(f"block_norm: a graph recorded on the default stream still holds {name}, and a captured "
+                                   "backward would wait for that stream: drop it first, or record it on another stream")
         out = _BlockNormFunction.apply(residual, block, pre_weight, post_weight, gate, scale, eps)
         return out if return_stats else out[:2]
     return _ops.block_norm(residual, block, pre_weight, post_weight, gate, scale, eps, return_stats)

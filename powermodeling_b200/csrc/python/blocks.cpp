@@ -17,7 +17,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 #include <cstdarg>
@@ -391,6 +393,21 @@ PyObject* paged_attention(PyObject* const* args) {
   return Py_BuildValue("(NN)", wrap(out), wrap(lse));
 }
 
+// held_outside_capture(residual, block, pre_weight, post_weight, gate) -> index of the first leaf whose gradient a living
+// graph of the default stream accumulates, -1 without one.  The autograd engine would wait on that stream for a captured
+// backward, which ends the capture.
+PyObject* held_outside_capture(PyObject* const* args) {
+  for (int i = 0; i < 5; ++i) {
+    const at::Tensor t = maybe(args[i], "an input");
+    if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    const std::optional<c10::Stream> stream = node->stream();
+    if (stream && *stream == c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap()) return PyLong_FromLong(i);
+  }
+  return PyLong_FromLong(-1);
+}
+
 template <PyObject* (*Body)(PyObject* const*), int Count>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
@@ -413,7 +430,7 @@ constexpr PyMethodDef method(const char* name) {
 
 PyMethodDef g_methods[] = {method<block_norm, 8>("block_norm"), method<block_norm_backward, 11>("block_norm_backward"),
                            method<matvec_w4, 5>("matvec_w4"), method<paged_attention, 11>("paged_attention"),
-                           {nullptr, nullptr, 0, nullptr}};
+                           method<held_outside_capture, 5>("held_outside_capture"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_blocksnative", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
