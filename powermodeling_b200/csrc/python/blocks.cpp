@@ -59,7 +59,9 @@ void check(int rc, const char* what) {
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse("%s must be a tensor", name);
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t._fw_grad(0).defined()) refuse("%s has a forward-mode tangent, and the block operators have no forward-mode gradient", name);
+  return t;
 }
 // The tensor, or an undefined one for None.
 at::Tensor maybe(PyObject* o, const char* name) { return o == Py_None ? at::Tensor() : tensor(o, name); }

@@ -133,6 +133,25 @@ def test_attention_refusals(kw, message):
         attention(**kw)
 
 
+def operators():
+    """Each operator as a function of one activation, with operands of its own beside it."""
+    w, st = z(32), z(4, 2, dtype=torch.float32)
+    weight, cache, table, lengths = z(8, 16, dtype=torch.uint8), z(3, 16, 2, 32), z(4, 2, dtype=torch.int32), z(4, dtype=torch.int32)
+    return {"block_norm": lambda x: blocks.block_norm(x, x, w)[1],
+            "block_norm_backward": lambda x: blocks.block_norm_backward(x, x, x, x, w, st)[0],
+            "matvec_w4": lambda x: blocks.matvec_w4(x, weight, z(8, 1), group_size=32),
+            "paged_attention": lambda x: blocks.paged_attention(x[:, None], cache[:, :, :1], cache[:, :, :1], table, lengths)}
+
+
+@pytest.mark.parametrize("name", ["block_norm", "block_norm_backward", "matvec_w4", "paged_attention"])
+def test_refusals_of_forward_mode_tangents(name):
+    """There is no forward-mode gradient: a tangent would be lost without an error."""
+    from torch.autograd import forward_ad
+    run, x = operators()[name], z(4, 32)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode tangent"):
+        run(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
 # The C entries refuse the same without touching the (made up) addresses.
 A = 1 << 20
 
