@@ -12,8 +12,10 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -57,11 +59,25 @@ void check(int rc, const char* what) {
   throw NativeFailure{std::string(what) + " failed (" + std::to_string(rc) + "): " + text};
 }
 
+// The calls read memory by themselves, past torch's dispatcher: tensors whose values are not what lies there, or that
+// stand for others, and whatever records or follows the dispatcher's calls would be answered wrongly without an error.
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse("%s must be a tensor", name);
   const at::Tensor& t = THPVariable_Unpack(o);
+  constexpr c10::DispatchKeySet kNotPlain({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                           c10::DispatchKey::Functionalize, c10::DispatchKey::Negative, c10::DispatchKey::Conjugate,
+                                           c10::DispatchKey::ZeroTensor});
+  if (t.layout() != at::kStrided || t.key_set().has_any(kNotPlain))
+    refuse("%s must be a plain strided tensor (not one of vmap, functorch or a dispatch subclass, nor lazily negated)", name);
   if (t._fw_grad(0).defined()) refuse("%s has a forward-mode tangent, and the block operators have no forward-mode gradient", name);
   return t;
+}
+void not_recorded() {
+  using c10::impl::TorchDispatchModeKey;
+  bool recorded = at::tracer::impl::is_dispatch_enabled();
+  for (const TorchDispatchModeKey k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+    recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
+  if (recorded) refuse("the block operators cannot be traced: call them outside torch.jit.trace, make_fx and fake tensors' modes");
 }
 // The tensor, or an undefined one for None.
 at::Tensor maybe(PyObject* o, const char* name) { return o == Py_None ? at::Tensor() : tensor(o, name); }
@@ -415,6 +431,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
   if (count != Count) return PyErr_Format(PyExc_TypeError, "expected %d arguments, got %zd", Count, count);
   try {
+    not_recorded();
     return Body(args);
   } catch (const Refused& r) {
     PyErr_SetString(PyExc_ValueError, r.message.c_str());

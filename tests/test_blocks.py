@@ -152,6 +152,29 @@ def test_refusals_of_forward_mode_tangents(name):
         run(forward_ad.make_dual(x, torch.ones_like(x)))
 
 
+@pytest.mark.parametrize("name", ["block_norm", "block_norm_backward", "matvec_w4", "paged_attention"])
+def test_refusals_of_what_would_go_unseen(name):
+    """What follows or records torch's own calls does not see these: vmap, transforms, traces, fake tensors, values that are
+    negated on reading."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    run, x = operators()[name], z(4, 32)
+    with pytest.raises(ValueError, match="CUDA device"):
+        run(x)
+    with pytest.raises(ValueError, match="plain strided"):
+        torch.vmap(run)(z(2, 4, 32))
+    with pytest.raises(ValueError, match="plain strided"):
+        torch.func.jvp(run, (x,), (x,))
+    with pytest.raises(ValueError, match="plain strided"):
+        run(torch._neg_view(x))
+    with pytest.raises(ValueError, match="traced"):
+        make_fx(run)(x)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises(ValueError, match="traced"):
+        run(mode.from_tensor(x))
+    with pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(run, x, check_trace=False)
+
+
 # The C entries refuse the same without touching the (made up) addresses.
 A = 1 << 20
 
