@@ -73,9 +73,13 @@ def block_norm(residual, block, pre_weight, *, post_weight=None, gate=None, scal
     backward together, or by ``block_norm_backward``; a leaf that a living graph
     of the default stream holds is refused there (``RuntimeError``).
     """
-    if torch.is_grad_enabled() and (residual.requires_grad or block.requires_grad or pre_weight.requires_grad
-                                    or (post_weight is not None and post_weight.requires_grad)
-                                    or (gate is not None and gate.requires_grad)):
+    try:
+        recorded = torch.is_grad_enabled() and (residual.requires_grad or block.requires_grad or pre_weight.requires_grad
+                                                or (post_weight is not None and post_weight.requires_grad)
+                                                or (gate is not None and gate.requires_grad))
+    except AttributeError:                       # no tensor: the native call says which
+        recorded = False
+    if recorded:
         if torch.cuda.is_current_stream_capturing():
             held = _ops.held_outside_capture(residual, block, pre_weight, post_weight, gate)
             if held >= 0:

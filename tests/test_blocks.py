@@ -44,6 +44,9 @@ def norm(**kw):
     (dict(scale=float("nan")), "scale"),
     (dict(eps=-1e-5), "eps"),
     (dict(residual=z(4, 0), block=z(4, 0), pre_weight=z(0)), "empty"),
+    (dict(residual=[[1.0]]), "residual must be a tensor"),
+    (dict(block=None), "block must be a tensor"),
+    (dict(gate=0.5), "gate must be a tensor"),
     (dict(), "CUDA device"),
 ])
 def test_block_norm_refusals(kw, message):
