@@ -83,6 +83,7 @@ void not_recorded() {
 at::Tensor maybe(PyObject* o, const char* name) { return o == Py_None ? at::Tensor() : tensor(o, name); }
 
 double number(PyObject* o) {
+  if (THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad()) refuse("scale and eps are numbers: no gradient goes through them");
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;

@@ -43,6 +43,8 @@ def norm(**kw):
     (dict(gate=z(1, 4, 32)), "gate"),
     (dict(scale=float("nan")), "scale"),
     (dict(eps=-1e-5), "eps"),
+    (dict(scale=torch.tensor(0.5, requires_grad=True)), "no gradient goes through"),
+    (dict(eps=torch.tensor(0.5, requires_grad=True)), "no gradient goes through"),
     (dict(residual=z(4, 0), block=z(4, 0), pre_weight=z(0)), "empty"),
     (dict(residual=[[1.0]]), "residual must be a tensor"),
     (dict(block=None), "block must be a tensor"),
@@ -120,6 +122,7 @@ def attention(**kw):
     (dict(q=z(2, 4, 65)[:, :, :64]), "strides in multiples of 8"),
     (dict(window=-1), "window"),
     (dict(scale=float("inf")), "scale"),
+    (dict(scale=torch.tensor(0.5, requires_grad=True)), "no gradient goes through"),
     (dict(new_k=z(2, 2, 64)), "come together"),
     (dict(new_k=z(2, 2, 64), new_v=z(2, 4, 64)), "new_v"),
     (dict(page_table=z(2, 2, dtype=torch.int64)), "page_table"),
