@@ -106,8 +106,8 @@ def block_norm_backward(grad_hidden, grad_normed, residual, block, pre_weight, s
 def matvec_w4(x, weight, scales, zeros=None, *, group_size=128):
     """``x`` [tokens, k] (bfloat16 or float16, any row stride) times the 4-bit ``weight``: [tokens, n].
 
-    ``weight`` is [n, ceil(k / 2)] uint8 (any row stride), the even k in the
-    low half of a byte; ``scales`` [n, ceil(k / group_size)] of x's type or
+    ``weight`` is [n, ceil(k / 2)] uint8 (any row stride up to 2^23), the even k
+    in the low half of a byte; ``scales`` [n, ceil(k / group_size)] of x's type or
     float32; ``zeros`` the same shape in uint8 (0..15), or None for 8 everywhere.
     Meant for single tokens and small batches: the weights are read once for
     every 16 tokens.  There is no backward.

@@ -109,14 +109,12 @@ std::string shape_text(at::IntArrayRef s) {
   return t + "]";
 }
 
-// Row stride of a 2-D tensor whose rows are contiguous and apart.
+// Row stride of a 2-D tensor whose rows are contiguous and apart; one row has none, whatever the tensor says.
 int64_t rows_of(const char* name, const at::Tensor& t) {
   if (t.dim() != 2) refuse("%s must be two-dimensional, got %s", name, shape_text(t.sizes()).c_str());
   if (t.size(1) > 1 && t.stride(1) != 1) refuse("%s: elements of a row must be contiguous", name);
-  if (t.stride(0) < t.size(1)) {
-    if (t.size(0) > 1) refuse("%s: rows overlap", name);
-    return t.size(1);
-  }
+  if (t.size(0) <= 1) return t.size(1);
+  if (t.stride(0) < t.size(1)) refuse("%s: rows overlap", name);
   return t.stride(0);
 }
 
@@ -279,6 +277,7 @@ PyObject* matvec_w4(PyObject* const* args) {
   if (weight.scalar_type() != at::kByte || weight.dim() != 2 || !k || weight.size(1) != (k + 1) / 2)
     refuse("%s: weight must be uint8 [n, %lld]", who, (long long)((k + 1) / 2));
   j.weight_stride = rows_of("weight", weight);
+  if (j.weight_stride > (1 << 23) && weight.size(0) > 1) refuse("%s: weight rows lie at most 2^23 bytes apart", who);
   const int64_t n = weight.size(0);
   if (group < 32 || group % 32 || group > (1 << 24)) refuse("%s: group_size must be a multiple of 32", who);
   const int64_t groups = (k + group - 1) / group;

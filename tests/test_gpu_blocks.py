@@ -477,6 +477,19 @@ def test_w4_values_that_are_not_numbers(gen):
     assert y[2].isnan().all() and not y[1].isfinite().any()
 
 
+def test_one_row_has_no_stride(gen):
+    """A single row cut from a wider tensor, however far its next one would be: as if it lay alone."""
+    t = w4_inputs(gen, 1, 1, 512, BF, 64, True)
+    far = torch.empty(256, device="cuda", dtype=torch.uint8).as_strided((1, 256), ((1 << 23) + 17, 1))
+    far.copy_(t["weight"])
+    x = torch.empty(1, 513, device="cuda", dtype=BF)[:, :512].copy_(t["x"])
+    assert torch.equal(w4_check(dict(t, weight=far, x=x), 64), w4_check(t, 64))
+    n = norm_inputs(gen, 1, 512, BF)
+    cut = {k: torch.empty(1, 515, device="cuda", dtype=BF)[:, :512].copy_(n[k]) for k in ("residual", "block")}
+    for a, b in zip(norm_both(dict(n, **cut), gen)[:2], norm_both(n, gen)[:2]):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("tokens,n,k,group,loose", [(1, 1024, 1024, 64, 0), (8, 4096, 4096, 128, 0), (16, 1000, 8192, 64, 0),
                                                     (1, 28672, 8192, 128, 0), (16, 9000, 8192, 32, 0), (40, 9000, 8192, 128, 0),
                                                     (3, 1001, 4090, 128, 1), (9, 20000, 4096, 64, 1), (1, 70000, 256, 64, 0)])
