@@ -381,6 +381,25 @@ def test_w4_depths(gen, k, dtype):
             w4_check(w4_inputs(gen, tokens, n, k, dtype, group, zeros=group == 64), group)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("k", [512, 4096, 8190, 8192, 11008, 16384 + 64, 28672])
+def test_w4_depths_closely(gen, k, dtype):
+    """Deep rows, close enough that one weight left out or exchanged would show: the zero point is taken off exactly, so
+    the magnitude is |x| |q - z| |scale|.
+
+    Steps of 2^-24: a group's sum in matrix instructions of 16 values, each cut off (2), one for each group added, 32 for
+    the sums over warps and CTAs.  At 28672 in groups of 128 they are 2^-15.9 of the magnitude, 0.2 % of a typical output,
+    which a single weight makes up 0.6 % of."""
+    for group in (32, 128, 96):
+        for tokens, n in ((1, 160), (7, 96), (16, 64), (1, 30000)):
+            t = w4_inputs(gen, tokens, n, k, dtype, group, zeros=group != 96)
+            x, s = t["x"].double(), t["scales"].double().repeat_interleave(group, 1)[:, :k]
+            zero = t["zeros"].double().repeat_interleave(group, 1)[:, :k] if t["zeros"] is not None else 8.0
+            w = (t["q"].double() - zero) * s
+            y = blocks.matvec_w4(t["x"], t["weight"], t["scales"], t["zeros"], group_size=group)
+            check("y", y, (x @ w.t(), x.abs() @ w.abs().t()), 2 * group / 16 + -(-k // group) + 32)
+
+
 @pytest.mark.parametrize("n", [1, 2, 8, 15, 16, 17, 63, 64, 100, 128, 1001, 4096, 20000])
 @pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 16])
 def test_w4_rows_and_tokens(gen, n, tokens):
