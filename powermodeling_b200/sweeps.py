@@ -331,6 +331,7 @@ def operator_sweep(quick: bool = False, seconds: float = 1.0) -> list[dict]:
         sets = min(max(2, -(-2 * l2 // need)), 64)
         calls = [operator_call(point, seed) for seed in range(sets)]
         side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())      # the operands are made there
         with torch.cuda.stream(side):
             for call in calls:
                 call()

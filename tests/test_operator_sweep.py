@@ -35,6 +35,28 @@ def test_sweep_names_its_parts():
 
 
 @pytest.mark.gpu
+def test_calls_wait_for_their_operands(monkeypatch):
+    import torch
+    seen, flags = torch.zeros(1000, device="cuda"), torch.zeros(1000, device="cuda")
+    with torch.cuda.stream(torch.cuda.Stream()):          # what a first use waits for is done with
+        seen.copy_(flags)
+    torch.cuda.synchronize()
+    count = iter(range(1000))
+
+    def call(point, seed):
+        k = next(count)
+        torch.cuda._sleep(50_000_000)                     # some 25 ms before the operand is there
+        flags[k:k + 1].fill_(1.0)
+        # a call adds what it sees of its operand; nothing is allocated, which would wait
+        return lambda: seen[k:k + 1].add_(flags[k:k + 1]).sub_(1.0)
+    point = {"operator": "matvec_w4", "tokens": 1, "n": 1 << 16, "k": 1 << 14, "group_size": 128}
+    monkeypatch.setattr(sweeps, "operator_points", lambda quick: [point] * 12)        # each on another stream
+    monkeypatch.setattr(sweeps, "operator_call", call)
+    rows = sweeps.operator_sweep(quick=True)
+    assert len(rows) == 12 and not seen.any()
+
+
+@pytest.mark.gpu
 def test_quick_sweep_rows(tmp_path):
     out = tmp_path / "sweep.json"
     assert sweeps.main(["--out", str(out), "--quick", "--only", "operators"]) == 0
