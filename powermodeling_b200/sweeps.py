@@ -320,7 +320,9 @@ def operator_call(point: dict, seed: int):
 
 def operator_sweep(quick: bool = False, seconds: float = 1.0) -> list[dict]:
     """Device time per call: a graph of calls on operand sets that together exceed twice the L2, replayed
-    for about ``seconds`` (``quick``: 0.05) under the sampler, between two events."""
+    for about ``seconds`` (``quick``: 0.05, too short for a power) under the sampler, between two events.
+    ``total_pj_per_byte`` is the board's whole power (the median of samples, idle power included) times
+    the time over the bytes; a trial with its idle phases is what ``energy_arm`` does."""
     import torch
     l2 = torch.cuda.get_device_properties(0).L2_cache_size
     seconds = 0.05 if quick else seconds
@@ -362,7 +364,8 @@ def operator_sweep(quick: bool = False, seconds: float = 1.0) -> list[dict]:
                 samples = sampler.stop()
             finally:
                 device.close()
-            watts = _median(samples, "power_w")
+            # power over fewer than half a second of samples is the ramp's, not the call's
+            watts = _median(samples, "power_w") if len(samples) >= 25 else None
             board = {"sm_mhz": _median(samples, "sm_clock_mhz"), "board_power_w": watts,
                      "total_pj_per_byte": watts * s / need * 1e12 if watts else None}
         rows.append({**point, "us": s * 1e6, "bytes": need, "gbs": need / s / 1e9, "operand_sets": sets, **board})

@@ -66,3 +66,16 @@ def test_quick_sweep_rows(tmp_path):
         assert r["us"] > 0 and math.isfinite(r["us"]) and r["operand_sets"] >= 2
         assert r["gbs"] == pytest.approx(r["bytes"] / r["us"] / 1e3)
         assert r["gbs"] < 20000                           # no call answers without reading its operands
+
+
+@pytest.mark.gpu
+def test_energy_comes_from_windows_that_hold_enough_samples(monkeypatch):
+    """A power from two or three samples is no power: the quick sweep has none, a window of a second has one."""
+    point = {"operator": "matvec_w4", "tokens": 1, "n": 4096, "k": 4096, "group_size": 128}
+    monkeypatch.setattr(sweeps, "operator_points", lambda quick: [point])
+    (quick,), (full,) = sweeps.operator_sweep(quick=True), sweeps.operator_sweep(seconds=1.0)
+    if "board_power_w" not in full:
+        pytest.skip("no power sensor")
+    assert quick["board_power_w"] is None and quick["total_pj_per_byte"] is None
+    assert full["board_power_w"] > 0
+    assert full["total_pj_per_byte"] == pytest.approx(full["board_power_w"] * full["us"] * 1e6 / full["bytes"])
