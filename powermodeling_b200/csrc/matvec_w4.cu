@@ -430,8 +430,13 @@ w4_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap 
   for (int left = count; left > 0; --left) {
     uint32_t scale[Side ? 4 : 1][Side ? kScaleWords : kGroups], zero[Side ? 4 : 1][Side ? kZeroWords : kGroups];
     if constexpr (!Side) {
+      const int blocks_left = (a.k + 31) / 32 - (s * stage_k + wk * L::kK) / 32;         // of 32 k, from the tile's start on
 #pragma unroll
-      for (int e = 0; e < kGroups; ++e) scale[0][e] = late(scale_next[e]), zero[0][e] = late(zero_next[e]) & 15u;
+      for (int e = 0; e < kGroups; ++e) {
+        // beyond the row zero, as the sums there are: an infinite scale is not to meet them
+        scale[0][e] = e * GB < blocks_left ? late(scale_next[e]) : 0u;
+        zero[0][e] = late(zero_next[e]) & 15u;
+      }
     }
     const bool last = s + 1 == a.stages || left == 1;    // of this CTA in this row block
     if (left == 1 && a.ranks == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join's CTAs come and wait

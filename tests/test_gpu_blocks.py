@@ -539,6 +539,22 @@ def test_w4_waits_that_run_out(gen, tokens, n, k, group, loose):
     assert torch.equal(blocks.matvec_w4(*args, group_size=group), before)
 
 
+@pytest.mark.parametrize("dtype,scales", [(BF, BF), (FP, F32)])
+@pytest.mark.parametrize("tokens,n,k,group", [(1, 70, 300, 32), (9, 70, 300, 32), (3, 40, 1000, 128), (1, 64, 4096, 32), (16, 33, 5000, 64)])
+def test_w4_infinite_scales(gen, tokens, n, k, group, dtype, scales):
+    """An infinite scale makes its row infinite, of its group's sum's sign, a NaN not a number; the others know nothing."""
+    t = w4_inputs(gen, tokens, n, k, dtype, group, True, scales)
+    s, groups = t["scales"], t["scales"].shape[1]
+    s[1, groups - 1], s[2, 0], s[3, groups // 2], s[4, groups - 1] = float("inf"), float("-inf"), float("inf"), float("nan")
+    zero = t["zeros"].double().repeat_interleave(group, 1)[:, :k]
+    sums = torch.zeros(tokens, n, groups * group, dtype=torch.float64, device="cuda")
+    sums[:, :, :k] = t["x"].double()[:, None] * (t["q"].double() - zero)
+    want = (sums.view(tokens, n, groups, group).sum(3) * s.double()).sum(2)
+    y = blocks.matvec_w4(t["x"], t["weight"], s, t["zeros"], group_size=group)
+    assert bool(want[:, 1:4].isinf().all())
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isposinf(), want.isposinf()) and torch.equal(y.isneginf(), want.isneginf())
+
+
 # ---------------------------------------------------------------- paged attention
 def cache(gen, lens, hk, d, page, dtype, layout="NHD", columns=None, spare=2, fill=float("nan")):
     """Caches whose pages lie in no order; everything that is not live holds `fill`."""
