@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <c10/core/GradMode.h>
@@ -359,6 +360,10 @@ PyObject* paged_attention(PyObject* const* args) {
     const int64_t shape[3] = {batch, kv_heads, head_dim};
     strided("new_k", nk, shape, nks);
     strided("new_v", nv, shape, nvs);
+    // written in place: every entry has to be its own
+    if (at::has_internal_overlap(kc) == at::MemOverlap::Yes || at::has_internal_overlap(vc) == at::MemOverlap::Yes)
+      refuse("%s: entries of the caches share memory, and the new token's would be written to all of them", who);
+    if (at::get_overlap_status(kc, vc) == at::MemOverlapStatus::Full) refuse("%s: k_cache and v_cache are the same memory", who);
   }
   if (table.dim() != 2 || table.size(0) != batch || table.scalar_type() != at::kInt || (table.size(1) > 1 && table.stride(1) != 1) ||
       table.size(1) > INT32_MAX)

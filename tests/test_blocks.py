@@ -194,6 +194,22 @@ def test_refusals_of_what_would_go_unseen(name):
         torch.jit.trace(run, x, check_trace=False)
 
 
+def test_attention_refuses_an_append_to_shared_memory():
+    new = dict(new_k=z(2, 2, 64), new_v=z(2, 2, 64))
+    cache = z(3, 16, 2, 64)
+    for kw in (dict(k_cache=z(1, 16, 2, 64).expand(3, -1, -1, -1), v_cache=cache),
+               dict(k_cache=cache, v_cache=z(3, 1, 2, 64).expand(-1, 16, -1, -1))):
+        with pytest.raises(ValueError, match="share memory"):
+            attention(**kw, **new)
+        with pytest.raises(ValueError, match="CUDA device"):        # to be read they may
+            attention(**kw)
+    with pytest.raises(ValueError, match="same memory"):
+        attention(k_cache=cache, v_cache=cache, **new)
+    both = z(3, 2, 16, 2, 64)
+    with pytest.raises(ValueError, match="CUDA device"):
+        attention(k_cache=both[:, 0], v_cache=both[:, 1], **new)
+
+
 # The C entries refuse the same without touching the (made up) addresses.
 A = 1 << 20
 

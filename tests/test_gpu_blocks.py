@@ -692,6 +692,43 @@ def test_attention_strides(gen):
     check("out", blocks.paged_attention(order, k, v, table2, lengths, scale=0.2, window=50), want[:2], 700)
 
 
+def test_attention_pages_that_are_shared(gen):
+    """A prefix whose pages several sequences share, a page twice in one table, caches of one memory that are only read."""
+    kc, vc = randn(gen, 12, 16, 2, 64, dtype=BF), randn(gen, 12, 16, 2, 64, dtype=BF)
+    table = torch.tensor([[3, 5, 7, 1], [3, 5, 2, 2], [3, 5, 5, 0]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([50, 33, 64], dtype=torch.int32, device="cuda")
+    attend(gen, [50, 33, 64], 2, 4, 64, 16, BF, made=(kc, vc, table, lengths))
+    attend(gen, [50, 33, 64], 2, 4, 64, 16, BF, made=(kc, kc, table, lengths), new=False)
+    attend(gen, [50, 33, 64], 2, 4, 64, 16, BF, made=(kc, vc[:1].expand(12, -1, -1, -1), table, lengths), new=False)
+
+
+def test_attention_graph_of_a_growing_sequence(gen):
+    """One captured call replayed token by token: lengths, tables, queries and new tokens change in place, from an empty
+    cache over page and tile ends to sequences that are cut."""
+    page, hk, d = 16, 2, 64
+    kc, vc = torch.zeros(1200, page, hk, d, dtype=BF, device="cuda"), torch.zeros(1200, page, hk, d, dtype=BF, device="cuda")
+    table = torch.full((2, 600), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(2, dtype=torch.int32, device="cuda")
+    q, nk, nv = randn(gen, 2, 8, d, dtype=BF), randn(gen, 2, hk, d, dtype=BF), randn(gen, 2, hk, d, dtype=BF)
+    blocks.paged_attention(q, kc, vc, table, lengths, new_k=nk, new_v=nv)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = blocks.paged_attention(q, kc, vc, table, lengths, new_k=nk, new_v=nv, return_lse=True)
+    for lens in ([0, 0], [1, 0], [2, 1], [16, 15], [17, 16], [64, 63], [65, 64], [66, 1000], [9000, 1001], [9600, 3]):
+        for i, n in enumerate(lens):
+            used = -(-n // page)
+            table[i] = -1
+            table[i, :used] = torch.arange(used, device="cuda", dtype=torch.int32) * 2 + i
+        lengths.copy_(torch.tensor(lens, dtype=torch.int32))
+        for x in (kc, vc, q, nk, nv):
+            x.copy_(randn(gen, *x.shape, dtype=BF))
+        want = R.attention(q, kc, vc, table, lengths, nk, nv, d ** -0.5, 0, "NHD")
+        graph.replay()
+        check("out", out, want[:2], 700)
+        assert torch.equal(lse.isneginf(), want[2].isneginf())
+        assert torch.equal(kc, want[4]) and torch.equal(vc, want[5])
+
+
 def test_attention_scores_far_apart(gen):
     """Large scores: weights of one and of nothing; a large negative scale; equal scores."""
     lens = [300, 40]
