@@ -106,6 +106,34 @@ def test_norm_many_rows(gen):
     norm_both(norm_inputs(gen, 5000, 1024, FP, gate_rows=5000), gen)
 
 
+@pytest.mark.parametrize("dtype,width", [(BF, 32776), (BF, 65528), (BF, 65536), (BF, 65544), (F32, 32768), (BF, 32768), (FP, 65535),
+                                         (BF, 1 << 20), (F32, (1 << 20) - 1)])
+@pytest.mark.parametrize("gate_rows", [1, 5])
+def test_norm_widest_rows(gen, dtype, width, gate_rows):
+    """Rows that eight CTAs share, the first that nobody shares, and the widest there are."""
+    norm_both(norm_inputs(gen, 5, width, dtype, gate_rows=gate_rows), gen)
+
+
+def test_norm_offsets_beyond_32_bits(gen):
+    """Rows that lie more than 2^31 elements apart."""
+    held = torch.empty((1 << 32) + 8192, dtype=BF, device="cuda")
+    far = held.as_strided((3, 4096), ((1 << 31) + 8, 1))
+    far.copy_(randn(gen, 3, 4096, dtype=BF))
+    t = norm_inputs(gen, 3, 4096, BF)
+    for name in ("residual", "block"):
+        norm_both(dict(t, **{name: far}), gen)
+    st = blocks.block_norm(t["residual"], t["block"], t["pre"], post_weight=t["post"], gate=t["gate"], return_stats=True)[2]
+    args = (t["residual"], t["block"], t["pre"], st)
+    near = far.contiguous()
+    for gh, gy in ((far, None), (None, far)):
+        got = blocks.block_norm_backward(gh, gy, *args, post_weight=t["post"], gate=t["gate"])
+        want = blocks.block_norm_backward(None if gh is None else near, None if gy is None else near, *args, post_weight=t["post"],
+                                          gate=t["gate"])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del held, far
+    torch.cuda.empty_cache()
+
+
 def test_norm_row_strides_and_alignment(gen):
     for dtype in (BF, F32):
         for width, pad in ((512, 64), (512, 3), (1024, 8), (333, 5)):
@@ -539,6 +567,25 @@ def test_w4_waits_that_run_out(gen, tokens, n, k, group, loose):
     assert torch.equal(blocks.matvec_w4(*args, group_size=group), before)
 
 
+@pytest.mark.parametrize("k", [32768, 32766])
+def test_w4_offsets_beyond_32_bits(gen, k):
+    """Weights of more than 2^32 bytes, rows from 16-byte boundaries and from any byte."""
+    n, group, tail = 290000, 128, 96
+    weight = torch.empty(n, (k + 1) // 2, device="cuda", dtype=torch.uint8)
+    for part in weight.split(20000):
+        part.copy_(torch.randint(0, 256, part.shape, generator=gen, device="cuda", dtype=torch.uint8))
+    assert weight.numel() > 1 << 32
+    scales = randn(gen, n, -(-k // group), scale=0.01, dtype=BF)
+    for tokens in (2, 12):
+        x = randn(gen, tokens, k, dtype=BF)
+        y = blocks.matvec_w4(x, weight, scales, group_size=group)
+        for rows in (slice(0, tail), slice(n // 2, n // 2 + tail), slice(n - tail, n)):
+            q = torch.stack((weight[rows] & 15, weight[rows] >> 4), 2).flatten(1)[:, :k].long()
+            check("y", y[:, rows], R.matvec(x, q, scales[rows], None, group), 400)
+    del weight
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype,scales", [(BF, BF), (FP, F32)])
 @pytest.mark.parametrize("tokens,n,k,group", [(1, 70, 300, 32), (9, 70, 300, 32), (3, 40, 1000, 128), (1, 64, 4096, 32), (16, 33, 5000, 64)])
 def test_w4_infinite_scales(gen, tokens, n, k, group, dtype, scales):
@@ -690,6 +737,27 @@ def test_attention_strides(gen):
     order = randn(gen, 8, 3, 64, dtype=BF).transpose(0, 1)
     want = R.attention(order, k, v, table, lengths, None, None, 0.2, 50, "NHD")
     check("out", blocks.paged_attention(order, k, v, table2, lengths, scale=0.2, window=50), want[:2], 700)
+
+
+def test_attention_of_many_sequences(gen):
+    """100000 sequences of no position or of one, whose value is the answer."""
+    b = 100000
+    lengths = (torch.rand(b, generator=gen, device="cuda") < 0.7).to(torch.int32)
+    table = torch.randperm(b, generator=gen, device="cuda").to(torch.int32)[:, None].contiguous()
+    kc, vc = randn(gen, b, 1, 2, 16, dtype=BF), randn(gen, b, 1, 2, 16, dtype=BF)
+    nk, nv = randn(gen, b, 2, 16, dtype=BF), randn(gen, b, 2, 16, dtype=BF)
+    old = vc.clone()
+    out, lse = blocks.paged_attention(randn(gen, b, 4, 16, dtype=BF), kc, vc, table, lengths, new_k=nk, new_v=nv, return_lse=True)
+    live = lengths.bool()
+    assert torch.equal(out, nv.repeat_interleave(2, 1) * live[:, None, None])
+    assert torch.equal(lse.isneginf(), ~live[:, None].expand(-1, 4))
+    home = table[:, 0].long()
+    assert torch.equal(vc[home[live], 0], nv[live]) and torch.equal(vc[home[~live]], old[home[~live]])
+
+
+def test_attention_largest_pages(gen):
+    attend(gen, [70000, 65536, 3], 1, 2, 16, 65536, BF)
+    attend(gen, [65537], 1, 8, 64, 65536, FP, window=40000, layout="HND")
 
 
 def test_attention_pages_that_are_shared(gen):
