@@ -31,11 +31,11 @@ except ImportError as exc:
 
 class _BlockNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, residual, block, pre_weight, post_weight, gate, scale, eps):
+    def forward(ctx, residual, block, pre_weight, post_weight, gate, scale, eps, captured):
         hidden, normed, stats = _ops.block_norm(residual, block, pre_weight, post_weight, gate, scale, eps, True)
         ctx.save_for_backward(residual, block, pre_weight, post_weight, gate, stats)
         ctx.scale = scale
-        ctx.captured = torch.cuda.is_current_stream_capturing()
+        ctx.captured = captured
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(stats)
         return hidden, normed, stats
@@ -48,13 +48,13 @@ class _BlockNormFunction(torch.autograd.Function):
             raise RuntimeError("block_norm: the forward pass was not captured: capture both, or capture block_norm_backward itself")
         residual, block, pre_weight, post_weight, gate, stats = ctx.saved_tensors
         if grad_hidden is None and grad_normed is None:
-            return (None,) * 7
+            return (None,) * 8
         need = ctx.needs_input_grad
         grads = block_norm_backward(
             None if grad_hidden is None else grad_hidden.contiguous(),
             None if grad_normed is None else grad_normed.contiguous(), residual, block, pre_weight, stats,
             post_weight=post_weight, gate=gate, scale=ctx.scale, weight_grads=need[2] or need[3], gate_grad=need[4])
-        return tuple(g if n else None for g, n in zip(grads, need)) + (None, None)
+        return tuple(g if n else None for g, n in zip(grads, need)) + (None, None, None)
 
 
 def block_norm(residual, block, pre_weight, *, post_weight=None, gate=None, scale=1.0, eps=1e-5, return_stats=False):
@@ -80,13 +80,13 @@ def block_norm(residual, block, pre_weight, *, post_weight=None, gate=None, scal
     except AttributeError:                       # no tensor: the native call says which
         recorded = False
     if recorded:
-        if torch.cuda.is_current_stream_capturing():
-            held = _ops.held_outside_capture(residual, block, pre_weight, post_weight, gate)
-            if held >= 0:
-                name = ("residual", "block", "pre_weight", "post_weight", "gate")[held]
-                raise RuntimeError(f"block_norm: a graph recorded on the default stream still holds {name}, and a captured "
-                                   "backward would wait for that stream: drop it first, or record it on another stream")
-        out = _BlockNormFunction.apply(residual, block, pre_weight, post_weight, gate, scale, eps)
+        held = _ops.held_outside_capture(residual, block, pre_weight, post_weight, gate)
+        captured = held is not None
+        if captured and held >= 0:
+            name = ("residual", "block", "pre_weight", "post_weight", "gate")[held]
+            raise RuntimeError(f"block_norm: a graph recorded on the default stream still holds {name}, and a captured "
+                               "backward would wait for that stream: drop it first, or record it on another stream")
+        out = _BlockNormFunction.apply(residual, block, pre_weight, post_weight, gate, scale, eps, captured)
         return out if return_stats else out[:2]
     return _ops.block_norm(residual, block, pre_weight, post_weight, gate, scale, eps, return_stats)
 

@@ -17,6 +17,7 @@
 #include <ATen/core/Tensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -76,8 +77,9 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
 void not_recorded() {
   using c10::impl::TorchDispatchModeKey;
   bool recorded = at::tracer::impl::is_dispatch_enabled();
-  for (const TorchDispatchModeKey k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
-    recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set())
+    for (const TorchDispatchModeKey k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+      recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(k).has_value();
   if (recorded) refuse("the block operators cannot be traced: call them outside torch.jit.trace, make_fx and fake tensors' modes");
 }
 // The tensor, or an undefined one for None.
@@ -416,10 +418,17 @@ PyObject* paged_attention(PyObject* const* args) {
   return Py_BuildValue("(NN)", wrap(out), wrap(lse));
 }
 
-// held_outside_capture(residual, block, pre_weight, post_weight, gate) -> index of the first leaf whose gradient a living
-// graph of the default stream accumulates, -1 without one.  The autograd engine would wait on that stream for a captured
-// backward, which ends the capture.
+// held_outside_capture(residual, block, pre_weight, post_weight, gate) -> None where the current stream of residual's
+// device is not being captured, else the index of the first leaf whose gradient a living graph of the default stream
+// accumulates, -1 without one.  The autograd engine would wait on that stream for a captured backward, which ends the
+// capture.
 PyObject* held_outside_capture(PyObject* const* args) {
+  const c10::Device device = tensor(args[0], "residual").device();
+  if (!device.is_cuda()) Py_RETURN_NONE;
+  {
+    const c10::cuda::CUDAGuard guard(device);
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) Py_RETURN_NONE;
+  }
   for (int i = 0; i < 5; ++i) {
     const at::Tensor t = maybe(args[i], "an input");
     if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
