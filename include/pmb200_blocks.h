@@ -43,6 +43,8 @@ enum { PM_DT_F32 = 0, PM_DT_BF16 = 1, PM_DT_F16 = 2 };
  * norm); the backward call reads them.  dtype is that of residual, block,
  * hidden and normed; each weight and the gate are of that type or PM_DT_F32.
  * rows 0 is allowed and does nothing.  hidden and normed are contiguous.
+ * Squares are summed in 32 bits: where their sum passes 3.4e38 the row's
+ * reciprocal root mean square is 0.
  */
 typedef struct {
   int64_t rows, gate_rows;
@@ -93,7 +95,8 @@ int pm_block_norm_backward_device(const pm_block_norm* forward, const pm_block_n
  * (0..15, the high half of the byte unread) or 8 where zeros is NULL.  dtype (x and y) is PM_DT_BF16 or
  * PM_DT_F16; scales are of that type or PM_DT_F32, [n, ceil(k / group)]
  * contiguous, as are zeros.  group is a multiple of 32; the last may be
- * partial.  y is contiguous [tokens, n].  tokens 0 is allowed and does
+ * partial.  Weights may be read in aligned pieces of 16 bytes that hold one of
+ * theirs at least.  y is contiguous [tokens, n].  tokens 0 is allowed and does
  * nothing; the weights are read once for every 16 tokens.  A wait for a copy
  * that does not end within the limit (2 s) gives up, and what depends on it is
  * NaN.
@@ -131,7 +134,8 @@ uint64_t pm_matvec_w4_wait_limit(uint64_t nanoseconds);
  * With new_k and new_v (both or neither, [batch, kv_heads, head_dim]) the
  * token's own key and value are written to position length - 1 of each
  * sequence (where its page is present) and attended to there; two sequences
- * must not share that entry, and no other sequence may attend to it.
+ * must not share that entry, and no other position, of this sequence or of
+ * another, may be found there.
  * A weight in PM_DT_F16 is held to 2^-39 of the sequence's largest at least.
  * dtype: PM_DT_BF16 or PM_DT_F16 for all of q, the caches, new_k, new_v and
  * out.  head_dim: a multiple of 8 up to 256; q, the caches, new_k and new_v are

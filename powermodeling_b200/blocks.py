@@ -129,8 +129,8 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, *, new_k=None, new
     keeps the last so many positions (0: all).  ``scale`` defaults to
     head_dim ** -0.5.  With ``new_k`` and ``new_v`` [batch, kv_heads, head_dim]
     the token's own key and value are first written to position length - 1 of
-    the caches, in the same call; no two sequences may share that entry.  A
-    sequence of length 0 gives zeros.  ``return_lse`` adds the logarithm of
+    the caches, in the same call; no other position of any sequence may be found
+    at that entry.  A sequence of length 0 gives zeros.  ``return_lse`` adds the logarithm of
     each row's sum of exponentials, [batch, q_heads] float32.  There is no
     backward.
     """

@@ -11,8 +11,7 @@
 //    arrive meanwhile in a ring of thread-private 16-byte asynchronous copies
 //    (each thread reads what it copied: no barrier but the reductions').  512
 //    threads an SM hold rows of up to 1024 pieces; wider ones are shared by a
-//    cluster (backward) or read by a CTA each (forward), and rows of up to 64
-//    pieces go by warps.
+//    cluster, and rows of up to 64 pieces go by warps.
 //  * Backward: h is recomputed from r, b and the two saved statistics, which
 //    costs no bytes (b is needed anyway) and no rounding.  With gp = scale
 //    gate w_post and bu = b r1 the sums over rows that the parameters need are
@@ -21,8 +20,9 @@
 //    and a second kernel adds the CTAs' in order.
 //  * Rows that 16-byte pieces do not fit (odd widths, strides, addresses): the
 //    same with single elements, neighbours in neighbouring lanes, the next
-//    row's loaded ahead into registers.  What is wider than that reads its
-//    rows again in each pass (the loop kernels).
+//    row's loaded ahead into registers.  What is wider than that, and the
+//    gradients of rows by warps with more gate rows than CTAs, reads its rows
+//    again in each pass (the loop kernels).
 //  * Sums and statistics are 32-bit, h enters the second norm unrounded; only
 //    the outputs are rounded to their type.
 // Measured, bf16 with both weights, inputs out of the L2 (a copy runs at 6.55
@@ -181,7 +181,7 @@ __device__ __forceinline__ void factor_piece(const NormArgs<T>& f, int64_t segme
 // Rows that 16-byte pieces do not fit, wider than a thread's registers hold
 // beside the next row's: a CTA each, kSingles elements of a thread.  Bound by
 // the latency of a row's loads and its two sums with two rows to an SM (4000
-// rows of 5001 bf16: 1.1 TB/s); the parameters come from the L1 each time.
+// rows of 5001 bf16: 1.8 TB/s, 2500 of 8191 1.5); the parameters come from the L1 each time.
 template <class T>
 __global__ void __launch_bounds__(1024) norm_row_kernel(const __grid_constant__ NormArgs<T> a) {
   __shared__ float red[2][32];
@@ -508,7 +508,9 @@ constexpr __host__ __device__ bool pre_shared(int n, int c, bool warps) { return
 // Rows in a ring: 512 threads of an SM then hold 192 (EachRow: 160) KB of them.
 constexpr __host__ __device__ int stages_of(bool each_row) { return each_row ? 2 : 3; }
 
-// N: elements of a piece, 16 bytes of them in the ring, or one in registers.
+// N: elements of a piece, 16 bytes of them in the ring, or one in registers,
+// where two rows of four arrays with kSingles of each pass 128 registers (fp32
+// spills 164 bytes, in a cluster 328).
 // Threads of a row (Warps == false: the CTA, or the cluster's CTAs; true: a
 // warp, the CTA's warps then taking rows in turn).  EachRow: a gate per row,
 // which streams with the rows; its gradient is complete with the row.

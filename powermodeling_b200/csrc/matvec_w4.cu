@@ -20,18 +20,21 @@
 //  * k is summed in an order that suits the nibbles: a lane's word holds k =
 //    0..7 of its eight, and the pairs (0,4), (1,5), (2,6), (3,7) are the
 //    instruction's neighbours, for the weights and for the tokens alike.
-//  * 8 tokens (16 in two halves) are the instruction's columns: mma.sync, as
-//    tcgen05's tiles begin at 128 x 8 with both operands in shared memory,
-//    and the unpacked weights come from registers.
+//  * 8 tokens (16 in two halves) are the instruction's columns: mma.sync, which
+//    takes the unpacked weights from the registers that they are in.  tcgen05
+//    would have them written to tensor memory first, and its sums read back
+//    for each group; that way is not built and not measured.
 //  * Few stages: the CTAs of a cluster share k and add their sums through
 //    distributed shared memory, in rank order.  Many: the line of all row
 //    blocks' stages is cut into equal runs, and a second kernel adds the
 //    pieces of the cut blocks in order.  So results do not vary.
 // Measured (a copy runs at 6.55 TB/s): one token x 28672 x 8192 in groups of
-// 128 32.2 us = 3.8 TB/s, 8 tokens 34 us; 16 tokens x 8192 x 28672 in groups
-// of 32 with zero points 51.8 us = 2.7 TB/s; 1024 x 1024 for one token 4.2 us.
-// The copies alone take 27 us of the first; for 16 tokens the issue slots are
-// 60 % busy on the half of the pipes that unpacking needs, with 16 warps an SM.
+// 128 32.4 us = 3.7 TB/s, 8 tokens 33 us; 16 tokens x 8192 x 28672 in groups
+// of 32 with zero points 50.2 us = 2.8 TB/s; 1024 x 1024 for one token 4.2 us.
+// The copies alone take 27 us of the first, in boxes 128 bytes wide; at the
+// copy's rate its bytes would take 18.5.  For 16 tokens the issue slots are
+// 60 % busy on the half of the pipes that unpacking needs, with 16 warps an SM;
+// at 96 registers a thread these kernels spill up to 28 bytes.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -114,7 +117,7 @@ struct W4Args {
 // bf16: the bits of an integer below 256 are that integer times 2^-133 (the
 // subnormals and the first binade are one even grid), so a nibble at bit 0 or
 // bit 4 is n 2^-133 or n 2^-129, and n - z over 64 is one fma away.
-// fp16: a nibble at bit 0 of 1024's mantissa is 1024 + n, at bit 4 1024 + 16 n.
+// fp16: likewise n 2^-24 and n 2^-20, subnormal, and n - z over 512 is one fma away.
 template <class T> struct Nibbles;
 template <> struct Nibbles<bf16> {
   static constexpr float kScale = 64.0f;
@@ -790,7 +793,7 @@ cudaError_t launch_scales(const W4Args& a, const Plan& p, cudaStream_t s) {
 }
 
 // A kernel for each number of groups in a tile.  Scales by copies and by loads of each lane (us): one token x 28672 x
-// 8192 in groups of 128 32.1 and 35.9, 16 tokens in groups of 64 47.6 and 74.3, of 32 (8192 x 28672) 52.2 and 133.
+// 8192 in groups of 128 32.4 and 36.1, 16 tokens in groups of 64 46.8 and 74.7, of 32 (8192 x 28672) 50.2 and 141.
 template <class T, int NT, bool Boxes>
 cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
   if (a.group == 64) return launch_scales<T, NT, 2, Boxes>(a, p, s);
@@ -799,7 +802,7 @@ cudaError_t launch_group(const W4Args& a, const Plan& p, cudaStream_t s) {
   return launch_scales<T, NT, 1, Boxes>(a, p, s);
 }
 
-// Copies of boxes need 16-byte rows; by pieces one token x 28672 x 8190 takes 62 us (8192 in boxes 32), 16 tokens 131 (45),
+// Copies of boxes need 16-byte rows; by pieces one token x 28672 x 8190 takes 62 us (8192 in boxes 32), 16 tokens 128 (45),
 // 8 tokens x 4096 x 11006 24 (by four warps that shifted words into place 101, 174 and 48).  What the copying warps have to do for each piece, and two stages at a time, bound it.
 template <class T>
 cudaError_t launch(const W4Args& a, const Plan& p, cudaStream_t s) {

@@ -1,8 +1,9 @@
 // Attention of one query token per sequence over a paged key-value cache:
 //   out = softmax(scale q K^T) V over the live positions.
 //
-// The cache is read once and everything else is small, so the bytes of K and
-// V over the memory's rate bound it; what the kernel has to do is to keep
+// The cache is read once for every 8 or 16 query heads of a key head and
+// everything else is small, so the bytes of K and V over the memory's rate
+// bound it; what the kernel has to do is to keep
 // enough bytes in flight on every SM whatever the lengths are.
 //  * Work is counted in tiles of 64 positions of one (sequence, key head).
 //    All tiles of all sequences form one line, on which the start of each
@@ -20,21 +21,22 @@
 //  * The query heads of one key head are the 8 columns of the matrix
 //    instruction: S^T[16 positions x 8 heads] = K Q^T, and O^T[16 dims x 8
 //    heads] += V^T P^T, K and V^T being the row operands straight from shared
-//    memory.  A group of 8 costs no padding, and its keys are read once.
+//    memory.  A group of 8 costs no padding, and its keys are read once; two
+//    groups go together where registers allow, further ones each read again.
 //    mma.sync serves because 8 columns are all there is: the tensor core is
 //    idle most of the time and tcgen05's 128-row tiles would be mostly empty.
 //  * A weight enters the product as three 16-bit parts that add up to its 32
 //    bits (fp16: to 2^-39 of the largest weight); sums and the running output
-//    are 32-bit.  One sequence of 131072 positions takes 104.7 us so, 103.1
-//    with two parts (2^-17 of a weight) summed in the instruction; its bf16
-//    outputs are off those of a 32-bit softmax by 5e-6 of their norm, so by 6e-5.
+//    are 32-bit.  One sequence of 131072 positions takes 105 us so; with two
+//    parts (2^-17 of a weight) summed in the instruction 103, and its bf16
+//    outputs were off a 32-bit softmax's by 6e-5 of their norm, now by 5e-6.
 // Measured (a copy runs at 6.55 TB/s): one sequence of 131072 positions, 8 key
-// heads of 128, 104 us = 5.2 TB/s; 64 ragged sequences up to 8192, 183 us =
-// 5.4 TB/s; 256 of 1024, 194 us = 5.6 TB/s; one of 77 positions 7.2 us, of
+// heads of 128, 105 us = 5.1 TB/s; 64 ragged sequences up to 8192, 186 us =
+// 5.3 TB/s; 256 of 1024, 197 us = 5.5 TB/s; one of 77 positions 7.8 us, of
 // which a copy's round trip, the reduction over the warps and the launch are
 // nearly all.  At full length the copies' latency with three CTAs an SM bounds
-// it (4.3 of 10 cycles between instructions wait for them), at a few tiles a
-// sequence the start of each segment, about 2 us.
+// it (3.0 of 8.6 cycles between a warp's instructions wait for them), at a few
+// tiles a sequence the start of each segment, about 2 us.
 #include <climits>
 #include <cmath>
 
@@ -661,8 +663,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const __gr
 // ---------------------------------------------------------------- launch
 // Query heads in groups of 8, two groups at once where more than 8 share a
 // key head and their registers allow it (head_dim up to 128): 32 sequences up
-// to 8192 with 16 query heads a key head of 128 71 us, group after group 87;
-// 12 heads of 64 44 and 49 us.
+// to 8192, 4 key heads, with 16 query heads a key head of 128 76 us, group
+// after group 94; 12 heads of 64 47 and 56 us.
 int tiles_of_heads(int share, int head_dim) { return share > 8 && head_dim <= 128 ? 2 : 1; }
 
 template <class T, int DP, int NT>
@@ -688,7 +690,7 @@ cudaError_t launch_shape(AttnArgs& a, uint8_t* scratch, int sms, cudaStream_t s)
   if (runs > kMaxRuns) runs = kMaxRuns;
   // The tables' full length bounds the lengths.  Where every segment has a run to itself and few tiles, none is cut:
   // the join's launch costs more than the tiles in turn (us whole and cut: 8 sequences x 8 heads with 128 positions
-  // 7.6 and 10.6, with 256 9.7 and 11.0, with 512 13.8 and 11.9; 128 x 8 segments of 256, more than runs, 31.7 and 28.3).
+  // 7.4 and 8.9, with 256 10.0 and 11.9, with 512 15.1 and 13.1; 128 x 8 segments of 256, more than runs, 38.5 and 36.8).
   const int64_t room = (int64_t(j.table_columns) * j.page_size + kTile - 1) / kTile;
   const int64_t segments = int64_t(j.batch) * j.kv_heads * a.blocks;
   a.whole = room <= 1 || (room <= kWhole && segments <= runs);
@@ -720,8 +722,8 @@ cudaError_t launch(const pm_paged_attention& j, void* scratch, int sms, cudaStre
   a.page_shift = j.page_size & (j.page_size - 1) ? -1 : 31 - __builtin_clz(unsigned(j.page_size));
   uint8_t* f = static_cast<uint8_t*>(scratch);
   const int nt = tiles_of_heads(a.share, j.head_dim);
-  // a head's own size in shared memory and registers, where it is usual: 32 sequences up to 8192, heads of 80 86 us (by
-  // the kernel for 128 101), of 96 89 (101), of 192 81 (by the kernel for 256 180)
+  // a head's own size in shared memory and registers, where it is usual: 32 sequences up to 8192, 8 key heads of 80 97 us
+  // (by the kernel for 128 110), of 96 97 (110), of 192 155 (by the kernel for 256 359)
   if (j.head_dim > 64 && j.head_dim <= 80) return nt == 2 ? launch_shape<T, 80, 2>(a, f, sms, s) : launch_shape<T, 80, 1>(a, f, sms, s);
   if (j.head_dim > 80 && j.head_dim <= 96) return nt == 2 ? launch_shape<T, 96, 2>(a, f, sms, s) : launch_shape<T, 96, 1>(a, f, sms, s);
   if (j.head_dim <= 64) return nt == 2 ? launch_shape<T, 64, 2>(a, f, sms, s) : launch_shape<T, 64, 1>(a, f, sms, s);
