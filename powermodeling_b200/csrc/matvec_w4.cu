@@ -715,8 +715,14 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swi
   if (!encode) return false;
   const cuuint64_t dims[2] = {cuuint64_t(columns), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride_bytes)};
   const cuuint32_t box[2] = {cuuint32_t(box_columns), cuuint32_t(box_rows)}, step[2] = {1, 1};
-  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto made = [&] {
+    return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (made()) return true;
+  // a thread that has called nothing of the runtime yet has no context, and this driver call wants one
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && made();
 }
 
 template <class T, int NT, int GB, bool Boxes, bool Side>

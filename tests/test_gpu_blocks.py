@@ -1123,6 +1123,24 @@ def test_two_graphs_with_second_kernels(gen):
                 assert torch.equal(a, b)
 
 
+def test_calls_from_new_threads(gen):
+    """Each operator as the first thing that a thread does on the GPU, its memory at hand already."""
+    from concurrent.futures import ThreadPoolExecutor
+    s = layer_inputs(gen, [700, 3, 0, 129])
+    t = norm_inputs(gen, 20, 256, BF)
+    st = blocks.block_norm(t["residual"], t["block"], t["pre"], return_stats=True)[2]
+    calls = [lambda: blocks.block_norm(s["x"], s["b"], s["pre"]),
+             lambda: blocks.block_norm_backward(t["block"], t["block"], t["residual"], t["block"], t["pre"], st)[:3],
+             lambda: (blocks.matvec_w4(s["x"], s["w"]["weight"], s["w"]["scales"], group_size=64),),
+             lambda: (blocks.paged_attention(s["x"].view(4, 8, 64), s["kc"], s["vc"], s["table"], s["lengths"]),)]
+    for call in calls:
+        want = call()
+        torch.cuda.synchronize()
+        with ThreadPoolExecutor(1) as pool:
+            got = pool.submit(call).result()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_first_call_of_a_process_inside_a_capture(gpu_ready):
     """Kernels are loaded, their shared memory set and the devices asked on a first call, which may be a captured one."""
     script = """
