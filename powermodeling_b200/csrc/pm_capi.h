@@ -44,9 +44,13 @@ void ensure_dynamic_smem(Kernel kernel, size_t static_bytes, size_t bytes, std::
   if (static_bytes + bytes <= 48 * 1024) return;
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
+  if ((int)bytes <= limits[device].load(std::memory_order_acquire)) return;
+  // one thread at a time, and never down: another's launch may be under way with the larger limit
+  static std::mutex lock;
+  const std::lock_guard<std::mutex> held(lock);
   if ((int)bytes <= limits[device].load(std::memory_order_relaxed)) return;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess)
-    limits[device].store((int)bytes, std::memory_order_relaxed);
+    limits[device].store((int)bytes, std::memory_order_release);
 }
 
 // Grow-only device workspace, pinned staging buffer and private stream of a device.

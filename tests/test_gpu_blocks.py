@@ -1141,6 +1141,44 @@ def test_calls_from_new_threads(gen):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_first_calls_of_a_process_from_many_threads(gpu_ready):
+    """Eight threads make a process's first calls of one kernel at once, each with another size of shared memory."""
+    script = """
+import ctypes as C, sys, threading
+sys.path.insert(0, "tests")
+import torch
+import block_cases as R
+lib, n, k = R.library(), 4096, 4096
+gen = torch.Generator(device="cuda").manual_seed(1)
+q = torch.randint(0, 16, (n, k), generator=gen, device="cuda")
+weight, scales = R.pack(q), (torch.rand(n, k // 128, generator=gen, device="cuda") * 0.01).bfloat16()
+x = [torch.randn(m + 1, k, generator=gen, device="cuda").bfloat16() for m in range(8)]
+y = [torch.empty(m + 1, n, device="cuda", dtype=torch.bfloat16) for m in range(8)]
+scratch = [torch.empty(max(lib.pm_matvec_w4_scratch_bytes(m + 1, n, k), 256), dtype=torch.uint8, device="cuda") for m in range(8)]
+streams = [torch.cuda.Stream() for m in range(8)]
+torch.cuda.synchronize()
+start, codes = threading.Barrier(8), [None] * 8
+def call(m):
+    job = R.MatvecW4(tokens=m + 1, n=n, k=k, group=128, dtype=1, scales_dtype=1, x_stride=k, weight_stride=k // 2, x=x[m].data_ptr(),
+                     weight=weight.data_ptr(), scales=scales.data_ptr(), zeros=None, y=y[m].data_ptr())
+    torch.cuda.current_device()
+    start.wait()
+    codes[m] = [lib.pm_matvec_w4_device(C.byref(job), scratch[m].data_ptr(), scratch[m].numel(), streams[m].cuda_stream) for _ in range(20)]
+threads = [threading.Thread(target=call, args=(m,)) for m in range(8)]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+assert not any(sum(codes, [])), codes
+for m in range(8):
+    want, magnitude = R.matvec(x[m], q, scales, None, 128)
+    assert R.within(y[m], want, magnitude, k / 8 + 64)[0] == 0, m
+print("right")
+"""
+    done = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0 and done.stdout.strip() == "right", done.stdout + done.stderr
+
+
 def test_first_call_of_a_process_inside_a_capture(gpu_ready):
     """Kernels are loaded, their shared memory set and the devices asked on a first call, which may be a captured one."""
     script = """
