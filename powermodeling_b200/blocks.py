@@ -43,10 +43,16 @@ class _BlockNormFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_hidden, grad_normed, _grad_stats):
-        if torch.cuda.is_current_stream_capturing() and not getattr(ctx, "captured", False):
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not getattr(ctx, "captured", False):
             # the graph of an eager forward brings its own stream into the capture
             raise RuntimeError("block_norm: the forward pass was not captured: capture both, or capture block_norm_backward itself")
         residual, block, pre_weight, post_weight, gate, stats = ctx.saved_tensors
+        held = _ops.held_outside_capture(residual, block, pre_weight, post_weight, gate) if capturing else -1
+        if held >= 0:
+            name = ("residual", "block", "pre_weight", "post_weight", "gate")[held]
+            raise RuntimeError(f"block_norm: a graph recorded on the default stream still holds {name}, and its gradient's way "
+                               "out of this capture would wait for that stream: drop that graph first, or record it on another")
         if grad_hidden is None and grad_normed is None:
             return (None,) * 8
         need = ctx.needs_input_grad
@@ -70,8 +76,9 @@ def block_norm(residual, block, pre_weight, *, post_weight=None, gate=None, scal
     rows; s = rows gates every element), each of that type or float32.  With
     ``return_stats`` a third value, [rows, 2] float32, is returned for
     ``block_norm_backward``.  A training step is captured with its forward and
-    backward together, or by ``block_norm_backward``; a leaf that a living graph
-    of the default stream holds is refused there (``RuntimeError``).
+    backward together, or by ``block_norm_backward``; a captured backward to a
+    leaf that a living graph of the default stream holds is refused
+    (``RuntimeError``).
     """
     try:
         recorded = torch.is_grad_enabled() and (residual.requires_grad or block.requires_grad or pre_weight.requires_grad
@@ -80,13 +87,7 @@ def block_norm(residual, block, pre_weight, *, post_weight=None, gate=None, scal
     except AttributeError:                       # no tensor: the native call says which
         recorded = False
     if recorded:
-        held = _ops.held_outside_capture(residual, block, pre_weight, post_weight, gate)
-        captured = held is not None
-        if captured and held >= 0:
-            name = ("residual", "block", "pre_weight", "post_weight", "gate")[held]
-            raise RuntimeError(f"block_norm: a graph recorded on the default stream still holds {name}, and a captured "
-                               "backward would wait for that stream: drop it first, or record it on another stream")
-        out = _BlockNormFunction.apply(residual, block, pre_weight, post_weight, gate, scale, eps, captured)
+        out = _BlockNormFunction.apply(residual, block, pre_weight, post_weight, gate, scale, eps, _ops.captured(residual))
         return out if return_stats else out[:2]
     return _ops.block_norm(residual, block, pre_weight, post_weight, gate, scale, eps, return_stats)
 

@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreads) attention_runs_kernel(const __grid_c
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 // the slice's own sum, smallest parts first: the instruction cuts its sums off, which over a long
-                // sequence would add up (2^-15 of the output after 600 slices); the running one is rounded
+                // sequence would add up (2^-14 of the output after 600 slices); the running one is rounded
                 float slice[4];
                 mma_first<T>(slice, va, w[n][0][kParts - 1], w[n][1][kParts - 1]);
 #pragma unroll

@@ -418,17 +418,18 @@ PyObject* paged_attention(PyObject* const* args) {
   return Py_BuildValue("(NN)", wrap(out), wrap(lse));
 }
 
-// held_outside_capture(residual, block, pre_weight, post_weight, gate) -> None where the current stream of residual's
-// device is not being captured, else the index of the first leaf whose gradient a living graph of the default stream
-// accumulates, -1 without one.  The autograd engine would wait on that stream for a captured backward, which ends the
-// capture.
-PyObject* held_outside_capture(PyObject* const* args) {
+// captured(tensor) -> whether the current stream of the tensor's device is being captured
+PyObject* captured(PyObject* const* args) {
   const c10::Device device = tensor(args[0], "residual").device();
-  if (!device.is_cuda()) Py_RETURN_NONE;
-  {
-    const c10::cuda::CUDAGuard guard(device);
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) Py_RETURN_NONE;
-  }
+  if (!device.is_cuda()) Py_RETURN_FALSE;
+  const c10::cuda::CUDAGuard guard(device);
+  return PyBool_FromLong(c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None);
+}
+
+// held_outside_capture(residual, block, pre_weight, post_weight, gate) -> index of the first leaf whose gradient a living
+// graph of the default stream accumulates, -1 without one.  The autograd engine would wait on that stream for a captured
+// backward's gradients, which ends the capture.
+PyObject* held_outside_capture(PyObject* const* args) {
   for (int i = 0; i < 5; ++i) {
     const at::Tensor t = maybe(args[i], "an input");
     if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
@@ -463,7 +464,7 @@ constexpr PyMethodDef method(const char* name) {
 
 PyMethodDef g_methods[] = {method<block_norm, 8>("block_norm"), method<block_norm_backward, 11>("block_norm_backward"),
                            method<matvec_w4, 5>("matvec_w4"), method<paged_attention, 11>("paged_attention"),
-                           method<held_outside_capture, 5>("held_outside_capture"), {nullptr, nullptr, 0, nullptr}};
+                           method<captured, 1>("captured"), method<held_outside_capture, 5>("held_outside_capture"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_blocksnative", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

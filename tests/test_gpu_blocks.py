@@ -358,8 +358,8 @@ def test_norm_in_graphed_callables(gen):
 
 
 def test_norm_capture_refuses_leaves_held_by_an_eager_graph(gen):
-    """A graph of the default stream over the same leaf: refused by name before anything is captured of it, and the capture goes
-    on; without the graph, or with it on another stream, the step is captured."""
+    """A graph of the default stream over the same leaf: the captured backward to it is refused by name and the capture goes
+    on, the forward is not; without that graph the step is captured."""
     w, x = randn(gen, 64).requires_grad_(), randn(gen, 4, 64)
 
     def step():
@@ -369,7 +369,7 @@ def test_norm_capture_refuses_leaves_held_by_an_eager_graph(gen):
     with torch.cuda.graph(graph):
         with pytest.raises(RuntimeError, match="still holds pre_weight"):
             step()
-        y = blocks.block_norm(x, x, w.detach())[1]
+        y = blocks.block_norm(x, x, w)[1].detach()
     graph.replay()
     assert torch.equal(y, blocks.block_norm(x, x, w.detach())[1])
     held.backward()
